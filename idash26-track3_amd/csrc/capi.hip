@@ -9,6 +9,7 @@
 #include <string>
 
 #include "../../include/mpcx.h"
+#include "attn.h"
 #include "gemm.h"
 #include "kernels.h"
 #include "launch_util.h"
@@ -993,6 +994,311 @@ mpcx_status mpcx_ring_lincomb(mpcx_ctx *c, size_t rows, size_t cols, uint64_t a,
          "ring_lincomb");
   }
   return MPCX_OK;
+}
+
+// ---------------- transformer layers ----------------
+size_t mpcx_ring_gemm_q4_work_bytes(mpcx_ctx *c, int M, int K) {
+  return c && M >= 1 && K >= 1 ? q4_work_bytes(c->bw, M, K) : 0;
+}
+template <typename T>
+static mpcx_status gemm_q4_t(mpcx_ctx *c, int M, int K, int N, int group, const void *a, size_t lda, const uint8_t *q,
+                             const int32_t *scale, void *out, size_t ldc, void *work) {
+  Q4Args<T> g;
+  g.M = M;
+  g.K = K;
+  g.N = N;
+  g.group = group;
+  g.a = static_cast<const T *>(a);
+  g.lda = lda;
+  g.q = q;
+  g.scale = scale;
+  g.c = static_cast<T *>(out);
+  g.ldc = ldc;
+  g.work = work;
+  HIPC(c, launch_gemm_q4<T>(c->L, g), "ring_gemm_q4");
+  return MPCX_OK;
+}
+static bool aligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+mpcx_status mpcx_ring_gemm_q4(mpcx_ctx *c, int M, int K, int N, int group, const void *a, size_t lda, const uint8_t *q,
+                              const int32_t *scale, void *out, size_t ldc, void *work) {
+  CHECK_CTX(c);
+  if (M < 1 || K < 1 || N < 1 || group < 32 || group % 32 != 0 || lda < size_t(K) || ldc < size_t(N))
+    return fail(c, MPCX_EINVAL, "ring_gemm_q4: bad argument");
+  if (!a || !q || !scale || !out || (!work && q4_work_bytes(c->bw, M, K) > 0))
+    return fail(c, MPCX_EINVAL, "ring_gemm_q4: null pointer");
+  if (!aligned(q, 16) || !aligned(work, 16) || !aligned(scale, 4) || !aligned(a, c->bw / 8) || !aligned(out, c->bw / 8))
+    return fail(c, MPCX_EINVAL, "ring_gemm_q4: misaligned pointer");
+  return c->bw == 32 ? gemm_q4_t<uint32_t>(c, M, K, N, group, a, lda, q, scale, out, ldc, work)
+                     : gemm_q4_t<uint64_t>(c, M, K, N, group, a, lda, q, scale, out, ldc, work);
+}
+
+// The cache's sizes are positive and its words countable in 60 bits.
+static bool valid_cache(const mpcx_cache &k) {
+  if (k.n_heads < 1 || k.head_dim < 1 || k.page_size < 1 || k.n_pages < 1) return false;
+  const unsigned __int128 words = (unsigned __int128)(k.n_heads) * k.head_dim * k.page_size * (uint64_t)k.n_pages;
+  return words < (unsigned __int128)1 << 60;
+}
+static CacheDims cache_dims(const mpcx_cache &k) {
+  CacheDims d;
+  d.heads = k.n_heads;
+  d.dim = k.head_dim;
+  d.page = k.page_size;
+  d.n_pages = k.n_pages;
+  return d;
+}
+template <typename T>
+static mpcx_status cache_append_t(mpcx_ctx *c, const mpcx_cache *cache, size_t n_tok, const int64_t *slot,
+                                  const int32_t *pos, const mpcx_rotation *rot, int n_planes,
+                                  const mpcx_cache_plane *planes) {
+  AppendArgs<T> g;
+  g.c = cache_dims(*cache);
+  g.n_tok = n_tok;
+  g.slot = slot;
+  g.pos = pos;
+  if (rot) {
+    g.half = rot->half;
+    g.n_pos = rot->n_pos;
+    g.shift = rot->shift;
+    g.pairs = rot->pairs != 0;
+    g.cos = static_cast<const T *>(rot->d_cos);
+    g.sin = static_cast<const T *>(rot->d_sin);
+  }
+  g.n_planes = n_planes;
+  for (int p = 0; p < n_planes; p++) {
+    g.rows[p] = static_cast<const T *>(planes[p].d_rows);
+    g.ld[p] = planes[p].ld;
+    g.pool[p] = static_cast<T *>(planes[p].d_pool);
+    g.rotate[p] = planes[p].rotate != 0;
+  }
+  HIPC(c, launch_cache_append<T>(c->L, g), "cache_append");
+  return MPCX_OK;
+}
+static_assert(MPCX_MAX_PLANES == kMaxPlanes, "the C API's planes are the library's");
+mpcx_status mpcx_cache_append(mpcx_ctx *c, const mpcx_cache *cache, size_t n_tok, const int64_t *slot,
+                              const int32_t *pos, const mpcx_rotation *rot, int n_planes,
+                              const mpcx_cache_plane *planes) {
+  CHECK_CTX(c);
+  if (!cache || !valid_cache(*cache) || n_planes < 1 || n_planes > MPCX_MAX_PLANES || !planes)
+    return fail(c, MPCX_EINVAL, "cache_append: bad argument");
+  const size_t row = size_t(cache->n_heads) * size_t(cache->head_dim), tb = size_t(c->bw) / 8;
+  if (n_tok > (size_t(1) << 60) / row) return fail(c, MPCX_EINVAL, "cache_append: bad argument");
+  bool turned = false;
+  for (int p = 0; p < n_planes; p++) {
+    if (planes[p].ld < row) return fail(c, MPCX_EINVAL, "cache_append: rows overlap");
+    turned = turned || planes[p].rotate != 0;
+  }
+  if (rot && (rot->half < 1 || rot->half > cache->head_dim / 2 || rot->n_pos < 1 || rot->shift < 0 ||
+              rot->shift >= c->bw))
+    return fail(c, MPCX_EINVAL, "cache_append: bad rotation");
+  if (turned && !rot) return fail(c, MPCX_EINVAL, "cache_append: rotated plane without a rotation");
+  if (n_tok == 0) return MPCX_OK;
+  if (!slot || (turned && (!pos || !rot->d_cos || !rot->d_sin)))
+    return fail(c, MPCX_EINVAL, "cache_append: null pointer");
+  for (int p = 0; p < n_planes; p++) {
+    if (!planes[p].d_rows || !planes[p].d_pool) return fail(c, MPCX_EINVAL, "cache_append: null pointer");
+    if (!aligned(planes[p].d_rows, tb) || !aligned(planes[p].d_pool, tb))
+      return fail(c, MPCX_EINVAL, "cache_append: misaligned pointer");
+  }
+  if (rot && (!aligned(rot->d_cos, tb) || !aligned(rot->d_sin, tb)))
+    return fail(c, MPCX_EINVAL, "cache_append: misaligned pointer");
+  return c->bw == 32 ? cache_append_t<uint32_t>(c, cache, n_tok, slot, pos, rot, n_planes, planes)
+                     : cache_append_t<uint64_t>(c, cache, n_tok, slot, pos, rot, n_planes, planes);
+}
+
+template <typename T>
+static mpcx_status split_mask_t(mpcx_ctx *c, size_t n, const void *mask, uint64_t seed, uint32_t gate, void *s0,
+                                void *s1) {
+  HIPC(c, launch_split<T>(c->L, seed, gate, F_SPLIT + 0, n, static_cast<const T *>(mask), static_cast<T *>(s0),
+                          static_cast<T *>(s1), nullptr),
+       "split_mask");
+  return MPCX_OK;
+}
+mpcx_status mpcx_split_mask(mpcx_ctx *c, size_t n, const void *mask, uint64_t seed, uint32_t gate, void *s0, void *s1) {
+  CHECK_CTX(c);
+  if (n == 0) return MPCX_OK;
+  if (!mask || !s0 || !s1) return fail(c, MPCX_EINVAL, "split_mask: null pointer");
+  return c->bw == 32 ? split_mask_t<uint32_t>(c, n, mask, seed, gate, s0, s1)
+                     : split_mask_t<uint64_t>(c, n, mask, seed, gate, s0, s1);
+}
+
+namespace {
+// The words of an attention gate's left operand (scores: queries; mix: weights)
+// and of its output; false where the batch is not valid.
+bool attn_sizes(const mpcx_attn *a, size_t *rows, size_t *scores) {
+  if (!a || !valid_cache(a->cache) || a->n_heads < 1 || a->n_heads % a->cache.n_heads != 0 || a->n_tok < 0 ||
+      a->n_seq < 0 || a->max_pages < 0 || a->max_q < 1 || a->max_keys < 1 || a->n_scores < 0 ||
+      a->n_scores >= int64_t(1) << 60)
+    return false;
+  const unsigned __int128 n = (unsigned __int128)(a->n_tok) * unsigned(a->n_heads) * unsigned(a->cache.head_dim);
+  if (n >= (unsigned __int128)1 << 60) return false;
+  *rows = size_t(n);
+  *scores = size_t(a->n_scores);
+  return true;
+}
+// Byte offset of a key's second plane, and the key's bytes.
+size_t attn_key_second(const mpcx_ctx *c, size_t first) { return align_up(first * (c->bw / 8)); }
+size_t attn_key_end(const mpcx_ctx *c, size_t first, size_t second) {
+  return align_up(attn_key_second(c, first) + second * (c->bw / 8));
+}
+bool attn_has_tables(const mpcx_attn *a) {
+  return a->d_pages && a->d_qstart && a->d_lo && a->d_hi && a->d_off;
+}
+template <typename T>
+AttnArgs<T> attn_args(const mpcx_attn *a) {
+  AttnArgs<T> g;
+  g.d.c = cache_dims(a->cache);
+  g.d.heads = a->n_heads;
+  g.d.n_tok = a->n_tok;
+  g.d.n_seq = a->n_seq;
+  g.d.max_pages = a->max_pages;
+  g.d.max_q = a->max_q;
+  g.d.max_keys = a->max_keys;
+  g.d.n_scores = a->n_scores;
+  g.d.pages = a->d_pages;
+  g.d.qstart = a->d_qstart;
+  g.d.lo = a->d_lo;
+  g.d.hi = a->d_hi;
+  g.d.off = a->d_off;
+  return g;
+}
+template <typename T>
+hipError_t attn_launch(const Launch &L, bool scores, AttnForm form, const AttnArgs<T> &g) {
+  return scores ? launch_attn_scores<T>(L, form, g) : launch_attn_mix<T>(L, form, g);
+}
+// No words to write: the gate is done (no pointer is read).
+bool attn_empty(const mpcx_attn *a, bool scores) { return a->n_tok == 0 || a->n_seq == 0 || (scores && a->n_scores == 0); }
+
+template <typename T>
+mpcx_status attn_keygen_t(mpcx_ctx *c, bool scores, const mpcx_attn *a, size_t first, size_t second, const void *rx,
+                          const void *b0, const void *b1, void *rz, uint64_t seed, uint32_t gate, void *k0v, void *k1v) {
+  uint8_t *k0 = static_cast<uint8_t *>(k0v), *k1 = static_cast<uint8_t *>(k1v);
+  const size_t at = attn_key_second(c, first);
+  T *A0 = reinterpret_cast<T *>(k0), *A1 = reinterpret_cast<T *>(k1);
+  HIPC(c, launch_split<T>(c->L, seed, gate, F_SPLIT + 0, first, static_cast<const T *>(rx), A0, A1, nullptr), "split");
+  HIPC(c, launch_prf_ring<T>(c->L, seed, gate, F_ROUT, second, static_cast<T *>(rz)), "prf");
+  void *sp = nullptr;
+  HIPC(c, ctx_work(c, second * sizeof(T), &sp), "hipMalloc");
+  T *term = static_cast<T *>(sp);
+  // words of no token's block keep the output mask as their product term
+  HIPC(c, launch_lincomb<T>(c->L, second, 1, T(1), static_cast<const T *>(rz), T(0), nullptr, nullptr, 0, term), "copy");
+  AttnArgs<T> g = attn_args<T>(a);
+  g.x = static_cast<const T *>(rx);
+  g.a1 = A1;
+  g.b0 = static_cast<const T *>(b0);
+  g.b1 = static_cast<const T *>(b1);
+  g.c0 = static_cast<const T *>(rz);
+  g.out = term;
+  if (!attn_empty(a, scores)) HIPC(c, attn_launch<T>(c->L, scores, AttnForm::DEAL, g), "attn_keygen");
+  HIPC(c, launch_split<T>(c->L, seed, gate, F_SPLIT + 2, second, term, reinterpret_cast<T *>(k0 + at),
+                          reinterpret_cast<T *>(k1 + at), nullptr),
+       "split");
+  HIPC(c, hipStreamSynchronize(c->L.stream), "sync");
+  return MPCX_OK;
+}
+mpcx_status attn_keygen(mpcx_ctx *c, bool scores, const mpcx_attn *a, const void *rx, const void *b0, const void *b1,
+                        void *rz, uint64_t seed, uint32_t gate, void *k0, void *k1) {
+  CHECK_CTX(c);
+  size_t rows, wide;
+  if (!attn_sizes(a, &rows, &wide)) return fail(c, MPCX_EINVAL, "attn_keygen: bad batch");
+  const size_t first = scores ? rows : wide, second = scores ? wide : rows;
+  if (second == 0) return MPCX_OK;
+  const size_t tb = size_t(c->bw) / 8;
+  if ((first && !rx) || !b0 || !b1 || !rz || !k0 || !k1 || (!attn_empty(a, scores) && !attn_has_tables(a)))
+    return fail(c, MPCX_EINVAL, "attn_keygen: null pointer");
+  if (!aligned(k0, 16) || !aligned(k1, 16) || !aligned(rx, tb) || !aligned(b0, tb) || !aligned(b1, tb) ||
+      !aligned(rz, tb))
+    return fail(c, MPCX_EINVAL, "attn_keygen: misaligned pointer");
+  return c->bw == 32 ? attn_keygen_t<uint32_t>(c, scores, a, first, second, rx, b0, b1, rz, seed, gate, k0, k1)
+                     : attn_keygen_t<uint64_t>(c, scores, a, first, second, rx, b0, b1, rz, seed, gate, k0, k1);
+}
+
+template <typename T>
+mpcx_status attn_eval_t(mpcx_ctx *c, bool scores, AttnForm form, const mpcx_attn *a, size_t first, size_t second,
+                        const void *k0, const void *k1, const void *x, const void *y, const void *b0, const void *b1,
+                        const void *slope, const int32_t *pos, void *out) {
+  const size_t at = attn_key_second(c, first);
+  AttnArgs<T> g = attn_args<T>(a);
+  g.x = static_cast<const T *>(x);
+  g.y = static_cast<const T *>(y);
+  if (k0) {
+    g.a0 = static_cast<const T *>(k0);
+    g.c0 = reinterpret_cast<const T *>(static_cast<const uint8_t *>(k0) + at);
+    g.b0 = static_cast<const T *>(b0);
+  }
+  if (k1) {
+    g.a1 = static_cast<const T *>(k1);
+    g.c1 = reinterpret_cast<const T *>(static_cast<const uint8_t *>(k1) + at);
+    g.b1 = static_cast<const T *>(b1);
+  }
+  g.slope = static_cast<const T *>(slope);
+  g.pos = pos;
+  g.out = static_cast<T *>(out);
+  HIPC(c, attn_launch<T>(c->L, scores, form, g), "attn_eval");
+  if (form == AttnForm::BOTH) c->counters.msg(second, c->bw);
+  return MPCX_OK;
+}
+mpcx_status attn_eval(mpcx_ctx *c, bool scores, AttnForm form, const mpcx_attn *a, const void *k0, const void *k1,
+                      const void *x, const void *y, const void *b0, const void *b1, const void *slope,
+                      const int32_t *pos, void *out) {
+  CHECK_CTX(c);
+  size_t rows, wide;
+  if (!attn_sizes(a, &rows, &wide)) return fail(c, MPCX_EINVAL, "attn_eval: bad batch");
+  if (attn_empty(a, scores)) return MPCX_OK;
+  const size_t first = scores ? rows : wide, second = scores ? wide : rows, tb = size_t(c->bw) / 8;
+  const bool p0 = form != AttnForm::P1, p1 = form != AttnForm::P0;
+  if ((p0 && (!k0 || !b0)) || (p1 && (!k1 || !b1)) || (first && !x) || !y || !out || (slope && !pos) ||
+      !attn_has_tables(a))
+    return fail(c, MPCX_EINVAL, "attn_eval: null pointer");
+  for (const void *p : {x, y, b0, b1, slope, static_cast<const void *>(out)})
+    if (!aligned(p, tb)) return fail(c, MPCX_EINVAL, "attn_eval: misaligned pointer");
+  if (!aligned(k0, 16) || !aligned(k1, 16)) return fail(c, MPCX_EINVAL, "attn_eval: misaligned pointer");
+  return c->bw == 32
+             ? attn_eval_t<uint32_t>(c, scores, form, a, first, second, k0, k1, x, y, b0, b1, slope, pos, out)
+             : attn_eval_t<uint64_t>(c, scores, form, a, first, second, k0, k1, x, y, b0, b1, slope, pos, out);
+}
+}  // namespace
+
+size_t mpcx_attn_scores_key_bytes(mpcx_ctx *c, const mpcx_attn *a) {
+  size_t rows, wide;
+  return c && attn_sizes(a, &rows, &wide) ? attn_key_end(c, rows, wide) : 0;
+}
+size_t mpcx_attn_mix_key_bytes(mpcx_ctx *c, const mpcx_attn *a) {
+  size_t rows, wide;
+  return c && attn_sizes(a, &rows, &wide) ? attn_key_end(c, wide, rows) : 0;
+}
+mpcx_status mpcx_attn_scores_keygen(mpcx_ctx *c, const mpcx_attn *a, const void *rq, const void *kb0, const void *kb1,
+                                    void *rs, uint64_t seed, uint32_t gate, void *k0, void *k1) {
+  return attn_keygen(c, true, a, rq, kb0, kb1, rs, seed, gate, k0, k1);
+}
+mpcx_status mpcx_attn_mix_keygen(mpcx_ctx *c, const mpcx_attn *a, const void *rp, const void *vb0, const void *vb1,
+                                 void *ro, uint64_t seed, uint32_t gate, void *k0, void *k1) {
+  return attn_keygen(c, false, a, rp, vb0, vb1, ro, seed, gate, k0, k1);
+}
+mpcx_status mpcx_attn_scores_eval(mpcx_ctx *c, const mpcx_attn *a, const void *k0, const void *k1, const void *qhat,
+                                  const void *khat, const void *kb0, const void *kb1, const void *slope,
+                                  const int32_t *pos, void *shat) {
+  return attn_eval(c, true, AttnForm::BOTH, a, k0, k1, qhat, khat, kb0, kb1, slope, pos, shat);
+}
+mpcx_status mpcx_attn_mix_eval(mpcx_ctx *c, const mpcx_attn *a, const void *k0, const void *k1, const void *phat,
+                               const void *vhat, const void *vb0, const void *vb1, void *ohat) {
+  return attn_eval(c, false, AttnForm::BOTH, a, k0, k1, phat, vhat, vb0, vb1, nullptr, nullptr, ohat);
+}
+mpcx_status mpcx_attn_scores_message(mpcx_ctx *c, int party, const mpcx_attn *a, const void *key, const void *qhat,
+                                     const void *khat, const void *kb, const void *slope, const int32_t *pos,
+                                     void *msg) {
+  CHECK_CTX(c);
+  if (party != 0 && party != 1) return fail(c, MPCX_EINVAL, "attn_scores_message: bad party");
+  if (party == 0) return attn_eval(c, true, AttnForm::P0, a, key, nullptr, qhat, khat, kb, nullptr, slope, pos, msg);
+  // the public bias is in party 0's message
+  return attn_eval(c, true, AttnForm::P1, a, nullptr, key, qhat, khat, nullptr, kb, nullptr, nullptr, msg);
+}
+mpcx_status mpcx_attn_mix_message(mpcx_ctx *c, int party, const mpcx_attn *a, const void *key, const void *phat,
+                                  const void *vhat, const void *vb, void *msg) {
+  CHECK_CTX(c);
+  if (party != 0 && party != 1) return fail(c, MPCX_EINVAL, "attn_mix_message: bad party");
+  if (party == 0)
+    return attn_eval(c, false, AttnForm::P0, a, key, nullptr, phat, vhat, vb, nullptr, nullptr, nullptr, msg);
+  return attn_eval(c, false, AttnForm::P1, a, nullptr, key, phat, vhat, nullptr, vb, nullptr, nullptr, msg);
 }
 
 // ---------------- reveal ----------------

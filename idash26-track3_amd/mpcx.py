@@ -6,6 +6,7 @@ without the built library or without a GPU raises.
 """
 import ctypes as C
 import os
+from collections import namedtuple
 
 import numpy as np
 
@@ -23,6 +24,28 @@ class ModelDims(C.Structure):
                 ("prot", C.c_int), ("nfus", C.c_int), ("fus", C.c_int * 4), ("lut_nmax", C.c_int),
                 ("mask_scale", C.c_int), ("slack", C.c_int)]
 
+
+class Cache(C.Structure):
+    _fields_ = [("n_heads", C.c_int), ("head_dim", C.c_int), ("page_size", C.c_int), ("n_pages", C.c_int64)]
+
+
+class _Rotation(C.Structure):
+    _fields_ = [("half", C.c_int), ("pairs", C.c_int), ("n_pos", C.c_int), ("shift", C.c_int),
+                ("d_cos", C.c_void_p), ("d_sin", C.c_void_p)]
+
+
+class _CachePlane(C.Structure):
+    _fields_ = [("d_rows", C.c_void_p), ("ld", C.c_size_t), ("d_pool", C.c_void_p), ("rotate", C.c_int)]
+
+
+class _Attn(C.Structure):
+    _fields_ = [("cache", Cache), ("n_heads", C.c_int), ("n_tok", C.c_int), ("n_seq", C.c_int),
+                ("max_pages", C.c_int), ("max_q", C.c_int), ("max_keys", C.c_int), ("n_scores", C.c_int64),
+                ("d_pages", C.c_void_p), ("d_qstart", C.c_void_p), ("d_lo", C.c_void_p), ("d_hi", C.c_void_p),
+                ("d_off", C.c_void_p)]
+
+
+MAX_PLANES = 8
 
 _SIGS = {
     "mpcx_create": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_void_p]),
@@ -82,6 +105,21 @@ _SIGS = {
                                  C.c_void_p]),
     "mpcx_ring_lincomb": (C.c_int, [C.c_void_p, C.c_size_t, C.c_size_t, C.c_uint64, C.c_void_p, C.c_uint64,
                                     C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+    "mpcx_ring_gemm_q4_work_bytes": (C.c_size_t, [C.c_void_p, C.c_int, C.c_int]),
+    "mpcx_ring_gemm_q4": (C.c_int, [C.c_void_p] + [C.c_int] * 4 + [C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p,
+                                                                  C.c_void_p, C.c_size_t, C.c_void_p]),
+    "mpcx_cache_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
+                                    C.c_void_p]),
+    "mpcx_split_mask": (C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p,
+                                  C.c_void_p]),
+    "mpcx_attn_scores_key_bytes": (C.c_size_t, [C.c_void_p, C.c_void_p]),
+    "mpcx_attn_scores_keygen": (C.c_int, [C.c_void_p] * 6 + [C.c_uint64, C.c_uint32, C.c_void_p, C.c_void_p]),
+    "mpcx_attn_scores_eval": (C.c_int, [C.c_void_p] * 11),
+    "mpcx_attn_scores_message": (C.c_int, [C.c_void_p, C.c_int] + [C.c_void_p] * 8),
+    "mpcx_attn_mix_key_bytes": (C.c_size_t, [C.c_void_p, C.c_void_p]),
+    "mpcx_attn_mix_keygen": (C.c_int, [C.c_void_p] * 6 + [C.c_uint64, C.c_uint32, C.c_void_p, C.c_void_p]),
+    "mpcx_attn_mix_eval": (C.c_int, [C.c_void_p] * 9),
+    "mpcx_attn_mix_message": (C.c_int, [C.c_void_p, C.c_int] + [C.c_void_p] * 6),
     "mpcx_set_adjnorm_lanes": (C.c_int, [C.c_void_p, C.c_int]),
     "mpcx_reveal_key_bytes": (C.c_size_t, [C.c_void_p, C.c_size_t]),
     "mpcx_reveal_keygen": (C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p,
@@ -204,6 +242,17 @@ def dptr(t):
     return C.c_void_p(t.data_ptr()) if t is not None else None
 
 
+# Rotation tables of cache_append: ring tensors (positions, half) at a scale of
+# `shift` bits; pairs: dims (2i, 2i + 1) are turned, else (i, i + half).
+Rotation = namedtuple("Rotation", "cos sin shift pairs", defaults=(False,))
+
+# A batch of attention queries (mpcx_attn): GPU tensors pages (sequences, pages)
+# int32, qstart (sequences + 1) int32, lo and hi (tokens) int32, off (tokens)
+# int64, and the numbers of packed scores and of query heads; max_q and max_keys
+# size the launch.
+AttnBatch = namedtuple("AttnBatch", "pages qstart lo hi off n_scores heads max_q max_keys")
+
+
 class Ctx:
     """A libmpcx context (bw-bit ring, fixed-point scale s) on one GPU."""
 
@@ -235,6 +284,12 @@ class Ctx:
 
     def sync(self):
         self.check(self.lib.mpcx_synchronize(self.h), "synchronize")
+
+    def set_stream(self, stream):
+        """Work on a torch stream from now on (None, or torch's default stream: on
+        the context's own)."""
+        self.check(self.lib.mpcx_set_stream(self.h, stream.cuda_stream if stream is not None else None), "set_stream")
+        self._stream = stream
 
     def set_party_sync(self, sync):
         """Party-mode calls synchronise the stream (True, the default) or return
@@ -526,6 +581,181 @@ class Ctx:
         dv = to_dev(v)
         self.check(self.lib.mpcx_party_reconstruct(self.h, peer.h, v.size, dptr(dv)), "party_reconstruct")
         return self._party_out(dv, v.size)
+
+    # ---------------- transformer layers (GPU tensors in and out) ----------------
+    # Ring words are int32 (bw = 32) or int64 tensors on the context's device.
+    # Where the context works on torch's current stream (set_stream) these calls
+    # only enqueue; elsewhere they wait for torch's stream first and for their own
+    # work at the end, as the methods above do.
+    def _enter(self):
+        cur = _torch().cuda.current_stream()
+        s = getattr(self, "_stream", None)
+        same = s is not None and s.cuda_stream != 0 and s.cuda_stream == cur.cuda_stream
+        if not same:
+            cur.synchronize()
+        return same
+
+    def _leave(self, same):
+        if not same:
+            self.sync()
+
+    def _words(self, t, what, shape=None):
+        """A contiguous ring tensor's address."""
+        torch = _torch()
+        if t.dtype != (torch.int32 if self.bw == 32 else torch.int64) or not t.is_cuda or not t.is_contiguous():
+            raise MpcxError(f"{what}: need a contiguous int{self.bw} tensor on the GPU")
+        if shape is not None and t.shape != shape:
+            raise MpcxError(f"{what}: shape {tuple(t.shape)}, need {tuple(shape)}")
+        return t.data_ptr()
+
+    @staticmethod
+    def _ints(t, what, dtype, shape):
+        if t.dtype != dtype or not t.is_cuda or not t.is_contiguous() or t.shape != shape:
+            raise MpcxError(f"{what}: need a contiguous {dtype} tensor of shape {tuple(shape)} on the GPU")
+        return t.data_ptr()
+
+    def _new(self, shape):
+        torch = _torch()
+        return torch.empty(shape, dtype=torch.int32 if self.bw == 32 else torch.int64, device="cuda")
+
+    def ring_gemm_q4(self, a, q, scale, group, out=None):
+        """mpcx_ring_gemm_q4: a (M, K) ring words (rows may be apart), q (N, rows of
+        whole 32 weights) uint8, scale (groups, N) int32 -> (M, N)."""
+        torch = _torch()
+        M, K = a.shape
+        N = q.shape[0]
+        if out is None:
+            out = self._new((M, N))
+        for t, n in ((a, "a"), (out, "out")):
+            if t.dtype != out.dtype or t.dtype.itemsize * 8 != self.bw or not t.is_cuda or t.dim() != 2 or \
+                    (t.shape[1] > 1 and t.stride(1) != 1):
+                raise MpcxError(f"ring_gemm_q4: {n}: need int{self.bw} rows on the GPU")
+        if out.shape != (M, N):
+            raise MpcxError(f"ring_gemm_q4: out: shape {tuple(out.shape)}, need {(M, N)}")
+        qp = self._ints(q, "ring_gemm_q4: q", torch.uint8, (N, (K + 31) // 32 * 16))
+        sp = self._ints(scale, "ring_gemm_q4: scale", torch.int32, (-(-K // group), N))
+        if M == 0:
+            return out
+        nb = self.lib.mpcx_ring_gemm_q4_work_bytes(self.h, M, K)
+        work = torch.empty(nb, dtype=torch.uint8, device="cuda") if nb else None
+        same = self._enter()
+        self.check(self.lib.mpcx_ring_gemm_q4(self.h, M, K, N, group, a.data_ptr(), a.stride(0) if M > 1 else K, qp, sp,
+                                              out.data_ptr(), out.stride(0) if M > 1 else N,
+                                              work.data_ptr() if nb else None), "ring_gemm_q4")
+        self._leave(same)
+        return out
+
+    @staticmethod
+    def _cache(pool):
+        return Cache(pool.shape[1], pool.shape[3], pool.shape[2], pool.shape[0])
+
+    def cache_append(self, planes, slot, pos=None, rotation=None):
+        """mpcx_cache_append: planes is a list of (rows, pool, rotate), rows (tokens,
+        heads, dim) ring words (tokens may be apart), pool (pages, heads, page size,
+        dim); slot (tokens) int64, pos (tokens) int32, rotation a Rotation."""
+        torch = _torch()
+        n = slot.shape[0]
+        pool = planes[0][1]
+        shape = (n, pool.shape[1], pool.shape[3])
+        sp = self._ints(slot, "cache_append: slot", torch.int64, (n,))
+        pp = self._ints(pos, "cache_append: pos", torch.int32, (n,)) if pos is not None else None
+        arr = (_CachePlane * len(planes))()
+        for i, (r, p, rotate) in enumerate(planes):
+            self._words(p, "cache_append: pool", pool.shape)
+            if r.shape != shape or r.dtype != p.dtype or not r.is_cuda or \
+                    (n and (r[0].stride() != (shape[2], 1) and not r[0].is_contiguous())):
+                raise MpcxError(f"cache_append: rows: need int{self.bw} rows of shape {shape} on the GPU")
+            arr[i] = _CachePlane(r.data_ptr(), r.stride(0) if n > 1 else shape[1] * shape[2], p.data_ptr(), int(rotate))
+        rot = None
+        if rotation is not None:
+            c = rotation.cos
+            rot = _Rotation(c.shape[1], int(rotation.pairs), c.shape[0], rotation.shift,
+                            self._words(c, "cache_append: cos"), self._words(rotation.sin, "cache_append: sin", c.shape))
+        same = self._enter()
+        self.check(self.lib.mpcx_cache_append(self.h, C.byref(self._cache(pool)), n, sp, pp,
+                                              C.byref(rot) if rot is not None else None, len(planes), arr),
+                   "cache_append")
+        self._leave(same)
+
+    def split_mask(self, mask, seed=1, gate=1):
+        """mpcx_split_mask: both parties' shares of a mask tensor."""
+        s0, s1 = self._new(mask.shape), self._new(mask.shape)
+        mp = self._words(mask, "split_mask")
+        same = self._enter()
+        self.check(self.lib.mpcx_split_mask(self.h, mask.numel(), mp, seed, gate, s0.data_ptr(), s1.data_ptr()),
+                   "split_mask")
+        self._leave(same)
+        return s0, s1
+
+    def _attn(self, b, pool):
+        torch = _torch()
+        n, seqs = b.lo.shape[0], b.pages.shape[0]
+        i32 = torch.int32
+        return _Attn(self._cache(pool), b.heads, n, seqs, b.pages.shape[1], b.max_q, b.max_keys, b.n_scores,
+                     self._ints(b.pages, "attn: pages", i32, b.pages.shape),
+                     self._ints(b.qstart, "attn: qstart", i32, (seqs + 1,)), self._ints(b.lo, "attn: lo", i32, (n,)),
+                     self._ints(b.hi, "attn: hi", i32, (n,)), self._ints(b.off, "attn: off", torch.int64, (n,)))
+
+    def _key(self, k, nb, what):
+        if k.numel() * k.element_size() < nb or not k.is_cuda or not k.is_contiguous():
+            raise MpcxError(f"{what}: need {nb} bytes on the GPU")
+        return k.data_ptr()
+
+    def _attn_gate(self, what, scores, b, pool):
+        """The batch, and the shapes of the left operand and of the output."""
+        a = self._attn(b, pool)
+        rows, wide = (a.n_tok, b.heads, pool.shape[3]), (b.n_scores,)
+        nb = (self.lib.mpcx_attn_scores_key_bytes if scores else self.lib.mpcx_attn_mix_key_bytes)(self.h, C.byref(a))
+        return a, nb, (rows if scores else wide), (wide if scores else rows)
+
+    def _attn_keygen(self, what, scores, b, rx, b0, b1, seed, gate):
+        a, nb, left, to = self._attn_gate(what, scores, b, b0)
+        k0, k1, rz = empty_dev(nb), empty_dev(nb), self._new(to)
+        ptrs = [self._words(rx, what, left), self._words(b0, what), self._words(b1, what, b0.shape)]
+        same = self._enter()
+        self.check(getattr(self.lib, "mpcx_" + what)(self.h, C.byref(a), *ptrs, rz.data_ptr(), seed, gate, dptr(k0),
+                                                     dptr(k1)), what)
+        self._leave(same)
+        return k0, k1, rz
+
+    def attn_scores_keygen(self, batch, rq, kb0, kb1, seed=1, gate=1):
+        """Keys of attn_scores_eval and the score mask, from the query mask (tokens,
+        heads, dim) and the share planes of the cache."""
+        return self._attn_keygen("attn_scores_keygen", True, batch, rq, kb0, kb1, seed, gate)
+
+    def attn_mix_keygen(self, batch, rp, vb0, vb1, seed=1, gate=1):
+        return self._attn_keygen("attn_mix_keygen", False, batch, rp, vb0, vb1, seed, gate)
+
+    def attn_scores_eval(self, batch, k0, k1, qhat, khat, kb0, kb1, slope=None, pos=None):
+        """mpcx_attn_scores_eval: queries (tokens, heads, dim) against the cache ->
+        the batch's packed scores."""
+        return self._attn_eval("attn_scores_eval", True, batch, None, (k0, k1), qhat, khat, (kb0, kb1), slope, pos)
+
+    def attn_mix_eval(self, batch, k0, k1, phat, vhat, vb0, vb1):
+        """mpcx_attn_mix_eval: packed weights against the cache -> (tokens, heads, dim)."""
+        return self._attn_eval("attn_mix_eval", False, batch, None, (k0, k1), phat, vhat, (vb0, vb1), None, None)
+
+    def attn_scores_message(self, party, batch, key, qhat, khat, kb, slope=None, pos=None):
+        """One party's message of the scores gate; both messages add up to its output."""
+        return self._attn_eval("attn_scores_message", True, batch, party, (key,), qhat, khat, (kb,), slope, pos)
+
+    def attn_mix_message(self, party, batch, key, phat, vhat, vb):
+        return self._attn_eval("attn_mix_message", False, batch, party, (key,), phat, vhat, (vb,), None, None)
+
+    def _attn_eval(self, what, scores, b, party, keys, x, y, shares, slope, pos):
+        torch = _torch()
+        a, nb, left, to = self._attn_gate(what, scores, b, y)
+        out = self._new(to)
+        args = [self._key(k, nb, what) for k in keys]
+        args += [self._words(x, what, left), self._words(y, what)] + [self._words(s, what, y.shape) for s in shares]
+        if scores:
+            args += [self._words(slope, what, (b.heads,)) if slope is not None else None,
+                     self._ints(pos, what + ": pos", torch.int32, (a.n_tok,)) if pos is not None else None]
+        same = self._enter()
+        self.check(getattr(self.lib, "mpcx_" + what)(self.h, *([] if party is None else [party]), C.byref(a), *args,
+                                                     out.data_ptr()), what)
+        self._leave(same)
+        return out
 
     # ---------------- adjacency normalisation ----------------
     def set_adjnorm_lanes(self, lanes):

@@ -319,6 +319,132 @@ mpcx_status mpcx_ring_gemm(mpcx_ctx *ctx, int M, int K, int N, const void *d_a, 
 mpcx_status mpcx_ring_lincomb(mpcx_ctx *ctx, size_t rows, size_t cols, uint64_t a, const void *d_x, uint64_t b,
                               const void *d_y, const void *d_v, int shift, void *d_out);
 
+/* ---------------- transformer layers ----------------
+ * Secure transformer inference on the same masked-public values: projections
+ * with public 4-bit weights, a paged cache of masked keys and values, and the
+ * two attention products that read it.  GPU-MPC's users reach such layers through
+ * the calls that the reference makes for its own (gpuMatmul, gpu_mpc/ddg_orca_base.h:
+ * 170-271); the reference has no counterpart of these.  Every operator is exact
+ * modulo 2^bw.  All calls of this section but the keygens return with their work
+ * enqueued on the context's stream (see the top of this file); the keygens
+ * synchronize it.  Between the two products a caller uses the truncation and
+ * ReLU gates above on the n_scores words (ReLU attention).  A scale, a table or
+ * a bias is public, so the dealer's masks go through ring_gemm_q4 and
+ * cache_append as the masked values do. */
+
+/* C = A . W mod 2^bw with public 4-bit weights W (K x N) and group scales:
+ *   C[m, n] = sum_g scale[g, n] * sum_{k / group = g} q[n, k] * A[m, k],
+ * no key and no exchange (the output mask is r_A . W, like mpcx_ring_gemm).
+ * d_a: M rows of K ring words, lda >= K words apart.  d_q: N rows of
+ * (K + 31) / 32 * 16 bytes, weight k of a row two's complement (-8..7) in the low
+ * (k even) or high (k odd) half of byte k / 2; the halves past K are not used.
+ * d_scale: ceil(K / group) rows of N int32 steps, at the scale of the weights;
+ * group a multiple of 32.  d_c: M rows of N words, ldc >= N words apart.  d_q is
+ * 16-byte aligned.  d_work: mpcx_ring_gemm_q4_work_bytes bytes, 16-byte aligned,
+ * in use until the stream has reached the call (NULL where that is 0). */
+size_t mpcx_ring_gemm_q4_work_bytes(mpcx_ctx *ctx, int M, int K);
+mpcx_status mpcx_ring_gemm_q4(mpcx_ctx *ctx, int M, int K, int N, int group, const void *d_a, size_t lda,
+                              const uint8_t *d_q, const int32_t *d_scale, void *d_c, size_t ldc, void *d_work);
+
+/* A paged cache: n_pages pages of page_size slots for each of n_heads key /
+ * value heads of head_dim words.  One plane (masked keys, a party's share of
+ * their mask, ...) is an array [n_pages][n_heads][page_size][head_dim] of ring
+ * words; slot s of the cache is slot s % page_size of page s / page_size. */
+typedef struct {
+  int n_heads, head_dim, page_size;
+  int64_t n_pages;
+} mpcx_cache;
+/* Rotation of the first 2 * half dims of a head (2 * half <= head_dim): with
+ * c, s the ring integers of row pos of the tables (n_pos x half) at a scale of
+ * `shift` bits, (x, y) -> (c x - s y, s x + c y) for the dims (i, i + half), or
+ * (2i, 2i + 1) with pairs != 0; the other dims are shifted left by `shift`, so a
+ * rotated row is at one scale. */
+typedef struct {
+  int half, pairs, n_pos, shift;
+  const void *d_cos, *d_sin;
+} mpcx_rotation;
+/* One plane of an append: token t's n_heads * head_dim words at d_rows + t * ld
+ * (ld >= n_heads * head_dim words) go to d_pool, rotated if rotate != 0. */
+typedef struct {
+  const void *d_rows;
+  size_t ld;
+  void *d_pool;
+  int rotate;
+} mpcx_cache_plane;
+#define MPCX_MAX_PLANES 8
+/* Rows of n_tok tokens into slot d_slot[t] of 1..MPCX_MAX_PLANES planes of a
+ * cache, rotated by position d_pos[t] on the way.  Linear, so it is applied
+ * alike to masked rows, to the dealer's masks and to each party's shares of them
+ * (which must go to planes of their own): one call takes a step's keys, values and
+ * shares.  A token whose slot is outside the cache (-1: padding) is not written,
+ * nor are the rotated planes of one whose position is outside the tables.  The
+ * slots of a call are distinct.  rot (host) and d_pos may be NULL where no plane
+ * is rotated; the pools overlap neither each other nor the rows. */
+mpcx_status mpcx_cache_append(mpcx_ctx *ctx, const mpcx_cache *cache, size_t n_tok, const int64_t *d_slot,
+                              const int32_t *d_pos, const mpcx_rotation *rot, int n_planes,
+                              const mpcx_cache_plane *planes);
+/* The dealer's shares of a mask: share0 pseudorandom, share0 + share1 = mask
+ * (n words each): what a party's share plane of the cache is appended from
+ * (writeShares, gpu_mpc/ddg_orca_base.h:394-410). */
+mpcx_status mpcx_split_mask(mpcx_ctx *ctx, size_t n, const void *d_mask, uint64_t seed, uint32_t gate,
+                            void *d_share0, void *d_share1);
+
+/* A batch of attention queries over a cache.  The n_tok tokens are those of
+ * n_seq sequences one after another: sequence b has tokens d_qstart[b] ..
+ * d_qstart[b + 1] - 1 and its key j in slot j % page_size of page
+ * d_pages[b * max_pages + j / page_size] (a page number outside the cache reads
+ * as rows of zeros).  n_heads query heads, a multiple m of the cache's: head h
+ * reads the cache's head h / m.  Token t sees the keys d_lo[t] <= j < d_hi[t]
+ * (causal, prefix, window and document masks; none where lo >= hi), and its
+ * scores are the n_heads * (hi - lo) words from d_off[t] on, head by head, of
+ * n_scores in all.  A token whose range leaves its page row or whose block
+ * leaves the n_scores words is taken to see nothing; tokens of no sequence are
+ * skipped.  max_q and max_keys, about the most tokens of a sequence and keys of a
+ * range, size the launch only. */
+typedef struct {
+  mpcx_cache cache;
+  int n_heads, n_tok, n_seq, max_pages, max_q, max_keys;
+  int64_t n_scores;
+  const int32_t *d_pages, *d_qstart, *d_lo, *d_hi;
+  const int64_t *d_off;
+} mpcx_attn;
+/* Query . key (Beaver): s[t, h, j] = sum_d q[t, h, d] * k[j, h / m, d], plus
+ * slope[h] * (j - pos[t]) where d_slope is not NULL (n_heads public ring words and
+ * n_tok positions).  Queries: n_tok x n_heads x head_dim words.  The cache planes
+ * are the masked keys and both parties' shares of their mask; a key's plane is
+ * used by every later product, so only the query's mask is shared here.  Keygen
+ * takes the query mask and the share planes, writes the score mask and the
+ * parties' keys: the share of the query mask (n_tok * n_heads * head_dim words),
+ * then, from the next multiple of 256 bytes on, the share of the product term
+ * (n_scores words). */
+size_t mpcx_attn_scores_key_bytes(mpcx_ctx *ctx, const mpcx_attn *a);
+mpcx_status mpcx_attn_scores_keygen(mpcx_ctx *ctx, const mpcx_attn *a, const void *d_rq, const void *d_kb0,
+                                    const void *d_kb1, void *d_rs, uint64_t seed, uint32_t gate, void *d_key0,
+                                    void *d_key1);
+mpcx_status mpcx_attn_scores_eval(mpcx_ctx *ctx, const mpcx_attn *a, const void *d_key0, const void *d_key1,
+                                  const void *d_qhat, const void *d_khat, const void *d_kb0, const void *d_kb1,
+                                  const void *d_slope, const int32_t *d_pos, void *d_shat);
+/* Weights . value (Beaver): o[t, h, :] = sum_j p[t, h, j] * v[j, h / m, :] over
+ * the keys that token t sees (zero where it sees none).  Weights: the n_scores
+ * words in the order of the scores.  Keys: the share of the weights' mask
+ * (n_scores words), then, 256-byte aligned, of the product term (n_tok * n_heads *
+ * head_dim words). */
+size_t mpcx_attn_mix_key_bytes(mpcx_ctx *ctx, const mpcx_attn *a);
+mpcx_status mpcx_attn_mix_keygen(mpcx_ctx *ctx, const mpcx_attn *a, const void *d_rp, const void *d_vb0,
+                                 const void *d_vb1, void *d_ro, uint64_t seed, uint32_t gate, void *d_key0,
+                                 void *d_key1);
+mpcx_status mpcx_attn_mix_eval(mpcx_ctx *ctx, const mpcx_attn *a, const void *d_key0, const void *d_key1,
+                               const void *d_phat, const void *d_vhat, const void *d_vb0, const void *d_vb1,
+                               void *d_ohat);
+/* One party's message of the two gates (party 0 or 1, its own key and share
+ * plane): both parties' messages add up to the gate's output, by
+ * mpcx_party_reconstruct. */
+mpcx_status mpcx_attn_scores_message(mpcx_ctx *ctx, int party, const mpcx_attn *a, const void *d_key,
+                                     const void *d_qhat, const void *d_khat, const void *d_kb, const void *d_slope,
+                                     const int32_t *d_pos, void *d_msg);
+mpcx_status mpcx_attn_mix_message(mpcx_ctx *ctx, int party, const mpcx_attn *a, const void *d_key,
+                                  const void *d_phat, const void *d_vhat, const void *d_vb, void *d_msg);
+
 /* ---------------- reveal ----------------
  * Additive shares v0, v1 -> masked public v + r (revealIfLeaf,
  * gpu_mpc/ddg_orca_base.h:72-80; peer->reconstructInPlace,
