@@ -1,40 +1,344 @@
-// q4.hip -- masked activations times public 4-bit weights with group scales.
+// q4.hip -- masked activations times public 4-bit weights with group scales, on
+// the int8 matrix cores.
+//
+// C[m, n] = sum_g scale[g, n] sum_{k in g} q[n, k] A[m, k] mod 2^bw.  A ring word
+// is a sum of bw / 8 balanced digits, A = sum_p 2^(8p) d_p with d_p in [-128, 127],
+// and a 4-bit weight shifted to the high half of a byte is the int8 16 q: one AND
+// (the high halves of a word's bytes) or a shift and an AND (the low ones) turn 8
+// packed weights into 8 operand bytes.  The digits of a word are rows of the MFMA's
+// A operand: its 16 rows are the planes of 4 (Z_2^32) or 2 (Z_2^64) words m, the
+// weights its one B operand, so nothing of the product is computed twice or dropped.
+// Accumulator register r of lane (li, lg) is row 4 lg + r, column li: a lane holds
+// four planes of one word, folds them, and multiplies by the group's scale.
+// A chunk is S = 128, 64 or 32 k, the largest that divides the group; the sums of a
+// chunk are below 2^21, so the fold's shifts stay exact in 32 bits:
+//   sum_p 2^(8p) a_p / 16 = (a_0 >> 4) + (a_1 << 4) + (a_2 << 12) + (a_3 << 20),
+// in Z_2^64 with 64-bit sums of the pairs (a_0, a_1), (a_2, a_3), and the lanes of
+// planes 4..7 (odd lg) shifted up by 32 at the end.
 #include <hip/hip_runtime.h>
 
 #include "attn.h"
+#include "digits.h"
 #include "launch_util.h"
 
 namespace mpcx {
+namespace {
 
-size_t q4_work_bytes(int, int, int) { return 0; }
-
-// One output per thread: the group's sum of weight times word, then its scale.
 template <typename T>
-__global__ __launch_bounds__(256) void k_q4(Q4Args<T> g) {
-  const int n = int(blockIdx.x) * 256 + int(threadIdx.x);
-  if (n >= g.N) return;
-  const uint8_t *q = g.q + size_t(n) * ((size_t(g.K) + 31) / 32 * 16);
-  for (int m = int(blockIdx.y); m < g.M; m += int(gridDim.y)) {
-    const T *a = g.a + size_t(m) * g.lda;
-    T out = 0;
-    for (int k0 = 0, gi = 0; k0 < g.K; k0 += g.group, gi++) {
-      const int k1 = g.K - k0 < g.group ? g.K : k0 + g.group;
-      T v = 0;
-      for (int k = k0; k < k1; k++) {
-        const int w = int((q[k >> 1] >> (4 * (k & 1))) & 15u);
-        v += T(int64_t((w ^ 8) - 8)) * a[k];
-      }
-      out += T(int64_t(g.scale[size_t(gi) * g.N + n])) * v;
-    }
-    g.c[size_t(m) * g.ldc + n] = out;
+constexpr int kRows = 16 / int(sizeof(T));  // words m per MFMA tile
+
+__device__ __forceinline__ v4i_t mfma64(v4i_t a, v4i_t b, v4i_t c) {
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ v4i_t mfma32(long a, long b, v4i_t c) {
+  return __builtin_amdgcn_mfma_i32_16x16x32_i8(a, b, c, 0, 0, 0);
+}
+
+// Operand bytes of a chunk: S / 32 dwords of packed weights per lane (k = chunk S +
+// (S / 4) lg + 8 d + 0..7 in dword d), as even and odd k: dwords lo(d), hi(d).
+// A 64-k operand is lo(2o), lo(2o + 1), hi(2o), hi(2o + 1); a 32-k one lo(0), hi(0).
+__device__ __forceinline__ uint32_t q4_lo(uint32_t w) { return (w << 4) & 0xf0f0f0f0u; }
+__device__ __forceinline__ uint32_t q4_hi(uint32_t w) { return w & 0xf0f0f0f0u; }
+
+// acc of one chunk: a, b are its S / 32 dword pairs (even k, odd k)
+template <int S>
+__device__ __forceinline__ v4i_t q4_product(const uint32_t (&ae)[S / 32], const uint32_t (&ao)[S / 32],
+                                            const uint32_t (&be)[S / 32], const uint32_t (&bo)[S / 32]) {
+  v4i_t acc = {0, 0, 0, 0};
+  if constexpr (S == 32) {
+    acc = mfma32(long(uint64_t(ae[0]) | uint64_t(ao[0]) << 32), long(uint64_t(be[0]) | uint64_t(bo[0]) << 32), acc);
+  } else {
+#pragma unroll
+    for (int o = 0; o < S / 64; o++)
+      acc = mfma64(v4i_t{int(ae[2 * o]), int(ae[2 * o + 1]), int(ao[2 * o]), int(ao[2 * o + 1])},
+                   v4i_t{int(be[2 * o]), int(be[2 * o + 1]), int(bo[2 * o]), int(bo[2 * o + 1])}, acc);
   }
+  return acc;
+}
+// The chunk's sum of the four planes of a lane, divided by 16, times the scale.
+template <typename T>
+__device__ __forceinline__ T q4_fold(v4i_t a, int32_t scale) {
+  if constexpr (sizeof(T) == 4) {
+    return (uint32_t(a[0] >> 4) + (uint32_t(a[1]) << 4) + (uint32_t(a[2]) << 12) + (uint32_t(a[3]) << 20)) *
+           uint32_t(scale);
+  } else {
+    const int32_t t0 = (a[0] >> 4) + (a[1] << 4), t1 = (a[2] >> 4) + (a[3] << 4);
+    return uint64_t(int64_t(t0) * scale) + (uint64_t(int64_t(t1) * scale) << 16);
+  }
+}
+
+// eight words from p on, zero from the `have`-th on
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, int have, bool vec, T (&w)[8]) {
+  if (vec && have >= 8) {
+    const uint4 *v = reinterpret_cast<const uint4 *>(p);
+#pragma unroll
+    for (int i = 0; i < int(sizeof(T)) / 2; i++) {
+      const uint4 x = v[i];
+      __builtin_memcpy(&w[i * 16 / int(sizeof(T))], &x, 16);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) w[i] = i < have ? p[i] : T(0);
+  }
+}
+// Plane p of eight words: the digits of the even and of the odd ones.
+template <typename T>
+__device__ __forceinline__ void plane8(const T (&w)[8], int p, uint32_t *even, uint32_t *odd) {
+  uint32_t y[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    if constexpr (sizeof(T) == 4) {
+      y[i] = w[i] + 0x80808080u;
+    } else {
+      const uint64_t v = w[i] + 0x8080808080808080ull;
+      y[i] = p & 4 ? uint32_t(v >> 32) : uint32_t(v);
+    }
+  }
+  const uint32_t b = uint32_t(p & 3), sel = b | (b + 4) << 8;
+  auto four = [&](uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(a3, a2, sel), __builtin_amdgcn_perm(a1, a0, sel), 0x05040100u) ^
+           0x80808080u;
+  };
+  *even = four(y[0], y[2], y[4], y[6]);
+  *odd = four(y[1], y[3], y[5], y[7]);
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: a workgroup takes 16 columns and MT MFMA tiles of rows; its waves take
+// the chunks of K in turn and add up their sums through LDS.  A lane forms its
+// digits from the words themselves (each word's planes are the rows li of its tile).
+// ---------------------------------------------------------------------------
+template <typename T, int S, int MT>
+__global__ __launch_bounds__(1024) void k_q4_few(Q4Args<T> g, bool vec) {
+  constexpr int R = kRows<T>, NP = int(sizeof(T)), ND = S / 32;
+  __shared__ T red[16][MT][64];
+  const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6, waves = int(blockDim.x) >> 6;
+  const int li = lane & 15, lg = lane >> 4, p = li % NP;
+  const int n = int(blockIdx.x) * 16 + li, nc = n < g.N ? n : g.N - 1;
+  const int m0 = int(blockIdx.y) * MT * R;
+  const size_t qrow = (size_t(g.K) + 31) / 32 * 16;
+  const uint8_t *q = g.q + size_t(nc) * qrow;
+  const int chunks = (g.K + S - 1) / S, per = g.group / S;
+  T out[MT];
+#pragma unroll
+  for (int t = 0; t < MT; t++) out[t] = 0;
+  for (int c = wave; c < chunks; c += waves) {
+    const int kb = c * S + lg * (S / 4);  // this lane's first k
+    uint32_t be[ND], bo[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++) be[d] = 0;
+    if (size_t(kb) < 2 * qrow) __builtin_memcpy(be, q + kb / 2, 4 * ND);
+    const int32_t scale = g.scale[size_t(c / per) * g.N + nc];
+#pragma unroll
+    for (int d = 0; d < ND; d++) bo[d] = q4_hi(be[d]), be[d] = q4_lo(be[d]);
+#pragma unroll
+    for (int t = 0; t < MT; t++) {
+      const int m = m0 + t * R + li / NP;
+      uint32_t ae[ND], ao[ND];
+#pragma unroll
+      for (int d = 0; d < ND; d++) {
+        T w[8];
+        load8<T>(g.a + size_t(m < g.M ? m : 0) * g.lda + kb + 8 * d, m < g.M ? g.K - kb - 8 * d : 0, vec, w);
+        plane8<T>(w, p, &ae[d], &ao[d]);
+      }
+      out[t] += q4_fold<T>(q4_product<S>(ae, ao, be, bo), scale);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < MT; t++) red[wave][t][lane] = out[t];
+  __syncthreads();
+  // word m of tile t, column li: lanes 16 lg.. (Z_2^64: 16 (2 lg).. and the planes above them)
+  for (int e = tid; e < MT * R * 16; e += int(blockDim.x)) {
+    const int t = e / (16 * R), r = e / 16 % R, col = e % 16;
+    const int m = m0 + t * R + r, on = int(blockIdx.x) * 16 + col;
+    T v = 0;
+    for (int w = 0; w < waves; w++) {
+      if constexpr (sizeof(T) == 4) v += red[w][t][16 * r + col];
+      else v += red[w][t][32 * r + col] + (red[w][t][32 * r + 16 + col] << 32);
+    }
+    if (m < g.M && on < g.N) g.c[size_t(m) * g.ldc + on] = v;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows, first step: the words' digits in the order the lanes take them.  The
+// workspace holds, per MFMA tile of rows and step of 128 k, 2 KB of operands:
+// 128 / S chunks of S / 64 operands (64 lanes of 16 bytes; S = 32: one of 8 bytes).
+// ---------------------------------------------------------------------------
+template <typename T, int S>
+__global__ __launch_bounds__(256) void k_q4_digits(Q4Args<T> g, bool vec, int tiles, int steps, uint8_t *work) {
+  constexpr int R = kRows<T>, NP = int(sizeof(T));
+  const size_t per_row = size_t(steps) * 16, n = size_t(tiles) * R * per_row;  // groups of 8 words
+  for (size_t e = size_t(blockIdx.x) * 256 + threadIdx.x; e < n; e += size_t(gridDim.x) * 256) {
+    const int m = int(e / per_row), k = int(e % per_row) * 8;
+    T w[8];
+    load8<T>(g.a + size_t(m < g.M ? m : 0) * g.lda + k, m < g.M ? g.K - k : 0, vec, w);
+    const int c = k / S, lg = k % S / (S / 4), d = k % (S / 4) / 8;
+    uint8_t *tile = work + (size_t(m / R) * steps * (128 / S) + c) * (16 * S);
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+      uint32_t even, odd;
+      plane8<T>(w, p, &even, &odd);
+      const int lane = 16 * lg + m % R * NP + p;
+      if constexpr (S == 32) {
+        *reinterpret_cast<uint2 *>(tile + 8 * lane) = make_uint2(even, odd);
+      } else {
+        uint32_t *o = reinterpret_cast<uint32_t *>(tile + (d / 2) * 1024 + 16 * lane);
+        o[d % 2] = even;
+        o[2 + d % 2] = odd;
+      }
+    }
+  }
+}
+
+// Second step: a workgroup of 2 x 2 waves, each MT tiles of rows by NT of columns;
+// the rows' operands of a step (128 k) are staged in LDS, the weights go straight to
+// the lanes' registers.
+template <typename T, int S, int MT, int NT>
+__global__ __launch_bounds__(256) void k_q4_many(Q4Args<T> g, int steps, const uint8_t *work) {
+  constexpr int R = kRows<T>, ND = S / 32, CH = 128 / S;
+  __shared__ __align__(16) uint4 as[2][2 * MT * 128];  // step, tile, 2 KB
+  const int gx = (g.N + 32 * NT - 1) / (32 * NT);
+  const int lw = xcd_swizzle(int(blockIdx.x), int(gridDim.x));
+  const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6, li = lane & 15, lg = lane >> 4;
+  const int n0 = lw % gx * 32 * NT + (wave & 1) * 16 * NT, t0 = lw / gx * 2 * MT;
+  const size_t qrow = (size_t(g.K) + 31) / 32 * 16;
+  const int per = g.group / S;
+  const uint8_t *q[NT];
+  int nc[NT];
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    const int n = n0 + 16 * t + li;
+    nc[t] = n < g.N ? n : g.N - 1;
+    q[t] = g.q + size_t(nc[t]) * qrow;
+  }
+  T out[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; i++)
+#pragma unroll
+    for (int t = 0; t < NT; t++) out[i][t] = 0;
+  const uint4 *src = reinterpret_cast<const uint4 *>(work);
+  uint4 ra[MT];
+  auto load = [&](int step) {
+#pragma unroll
+    for (int j = 0; j < MT; j++) {  // 256 threads move two tiles at a time
+      const int f = tid + 256 * j;
+      ra[j] = src[(size_t(t0 + f / 128) * steps + step) * 128 + f % 128];
+    }
+  };
+  load(0);
+  for (int step = 0; step < steps; step++) {
+    uint4 *buf = as[step & 1];
+#pragma unroll
+    for (int j = 0; j < MT; j++) buf[tid + 256 * j] = ra[j];
+    __syncthreads();
+    if (step + 1 < steps) load(step + 1);
+#pragma unroll
+    for (int c = 0; c < CH; c++) {
+      const int chunk = step * CH + c, kb = chunk * S + lg * (S / 4);
+      const int gi = min(chunk, (g.K - 1) / S) / per;
+      uint32_t ae[MT][ND], ao[MT][ND];
+#pragma unroll
+      for (int i = 0; i < MT; i++) {
+        const uint4 *a = buf + ((wave >> 1) * MT + i) * 128 + c * S;
+        if constexpr (S == 32) {
+          const uint2 v = reinterpret_cast<const uint2 *>(a)[lane];
+          ae[i][0] = v.x, ao[i][0] = v.y;
+        } else {
+#pragma unroll
+          for (int o = 0; o < ND / 2; o++) {
+            const uint4 v = a[64 * o + lane];
+            ae[i][2 * o] = v.x, ae[i][2 * o + 1] = v.y, ao[i][2 * o] = v.z, ao[i][2 * o + 1] = v.w;
+          }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        uint32_t be[ND], bo[ND];
+#pragma unroll
+        for (int d = 0; d < ND; d++) be[d] = 0;
+        if (size_t(kb) < 2 * qrow) __builtin_memcpy(be, q[t] + kb / 2, 4 * ND);
+        const int32_t scale = g.scale[size_t(gi) * g.N + nc[t]];
+#pragma unroll
+        for (int d = 0; d < ND; d++) bo[d] = q4_hi(be[d]), be[d] = q4_lo(be[d]);
+#pragma unroll
+        for (int i = 0; i < MT; i++) out[i][t] += q4_fold<T>(q4_product<S>(ae[i], ao[i], be, bo), scale);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MT; i++)
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const int n = n0 + 16 * t + li;
+      T v = out[i][t];
+      int r = lg;
+      if constexpr (sizeof(T) == 8) {
+        v += __shfl_xor(v, 16, 64) << 32;  // the planes above, from lane group lg + 1
+        r = lg >> 1;
+        if (lg & 1) continue;
+      }
+      const int m = (t0 + (wave >> 1) * MT + i) * R + r;
+      if (m < g.M && n < g.N) g.c[size_t(m) * g.ldc + n] = v;
+    }
+}
+
+constexpr int kManyMT = 4;
+// rows of MFMA tiles in the workspace: whole workgroups
+template <typename T>
+int many_tiles(int M) {
+  const int wg = 2 * kManyMT * kRows<T>;
+  return (M + wg - 1) / wg * 2 * kManyMT;
+}
+int many_steps(int K) { return (K + 127) / 128; }
+bool few_rows(int M, int) { return M <= 16; }
+
+template <typename T, int S>
+hipError_t launch_at(const Launch &L, const Q4Args<T> &g) {
+  const bool vec = reinterpret_cast<uintptr_t>(g.a) % 16 == 0 && g.lda % (16 / sizeof(T)) == 0;
+  constexpr int R = kRows<T>;
+  if (few_rows(g.M, g.K)) {
+    const int chunks = (g.K + S - 1) / S, waves = chunks < 16 ? chunks : 16;
+    const int tiles = (g.M + R - 1) / R, mt = tiles >= 4 ? 4 : tiles >= 2 ? 2 : 1;
+    const dim3 grid(unsigned((size_t(g.N) + 15) / 16), unsigned((tiles + mt - 1) / mt)), block(64u * unsigned(waves));
+    if (mt == 4) hipLaunchKernelGGL((k_q4_few<T, S, 4>), grid, block, 0, L.stream, g, vec);
+    else if (mt == 2) hipLaunchKernelGGL((k_q4_few<T, S, 2>), grid, block, 0, L.stream, g, vec);
+    else hipLaunchKernelGGL((k_q4_few<T, S, 1>), grid, block, 0, L.stream, g, vec);
+    return hipGetLastError();
+  }
+  const int tiles = many_tiles<T>(g.M), steps = many_steps(g.K);
+  uint8_t *work = static_cast<uint8_t *>(g.work);
+  const size_t groups = size_t(tiles) * R * steps * 16;
+  const size_t want = (groups + 255) / 256, cap = size_t(L.num_cu) * 32;
+  hipLaunchKernelGGL((k_q4_digits<T, S>), dim3(unsigned(want < cap ? want : cap)), dim3(256), 0, L.stream, g, vec, tiles,
+                     steps, work);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  auto many = [&](auto nt) {
+    constexpr int NT = decltype(nt)::value;
+    const size_t wgs = (size_t(g.N) + 32 * NT - 1) / (32 * NT) * size_t(tiles / (2 * kManyMT));
+    if (wgs > size_t(INT32_MAX)) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((k_q4_many<T, S, kManyMT, NT>), dim3(unsigned(wgs)), dim3(256), 0, L.stream, g, steps, work);
+    return hipGetLastError();
+  };
+  const size_t rows = size_t(tiles / (2 * kManyMT));
+  if ((size_t(g.N) + 127) / 128 * rows >= size_t(L.num_cu) * 2) return many(std::integral_constant<int, 4>{});
+  return many(std::integral_constant<int, 1>{});
+}
+
+}  // namespace
+
+size_t q4_work_bytes(int bw, int M, int K) {
+  if (few_rows(M, K)) return 0;
+  return size_t(bw == 32 ? many_tiles<uint32_t>(M) : many_tiles<uint64_t>(M)) * many_steps(K) * 2048;
 }
 
 template <typename T>
 hipError_t launch_gemm_q4(const Launch &L, const Q4Args<T> &g) {
-  const unsigned gy = unsigned(g.M < 65535 ? g.M : 65535);
-  hipLaunchKernelGGL(k_q4<T>, dim3(unsigned((size_t(g.N) + 255) / 256), gy), dim3(256), 0, L.stream, g);
-  return hipGetLastError();
+  if (g.group % 128 == 0) return launch_at<T, 128>(L, g);
+  if (g.group % 64 == 0) return launch_at<T, 64>(L, g);
+  return launch_at<T, 32>(L, g);
 }
 template hipError_t launch_gemm_q4<uint32_t>(const Launch &, const Q4Args<uint32_t> &);
 template hipError_t launch_gemm_q4<uint64_t>(const Launch &, const Q4Args<uint64_t> &);

@@ -204,11 +204,17 @@ class MpcxError(RuntimeError):
     pass
 
 
+_torch_module = None
+
+
 def _torch():
-    import torch
-    if not torch.cuda.is_available():
-        raise MpcxError("no GPU visible: libmpcx has no CPU path")
-    return torch
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        if not torch.cuda.is_available():
+            raise MpcxError("no GPU visible: libmpcx has no CPU path")
+        _torch_module = torch
+    return _torch_module
 
 
 def to_dev(a):
