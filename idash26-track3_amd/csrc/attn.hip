@@ -74,12 +74,21 @@ __device__ __forceinline__ TokenRange token_range(const AttnDims &d, int t) {
     r.lo = r.hi = 0, r.off = 0;
   return r;
 }
-// word index of row `key` of sequence b's kv head in a cache plane, -1 where the
-// page is not in the cache
-__device__ __forceinline__ int64_t cache_row(const AttnDims &d, int b, int head, int key) {
-  const int page = d.pages[int64_t(b) * d.max_pages + key / d.c.page];
-  if (page < 0 || page >= d.c.n_pages) return -1;
-  return ((int64_t(page) * d.c.heads + head) * d.c.page + key % d.c.page) * d.c.dim;
+// Row `key` (inside the page row) of sequence b's kv head in a cache plane: its first
+// word, and whether its page is in the cache (else the word is page 0's).  Loads of
+// rows have no branches around them, so that many are in flight: a row that does not
+// exist is read at a place that does, and its products are left out.
+struct CacheRow {
+  int64_t at;
+  bool in;
+};
+__device__ __forceinline__ CacheRow cache_row(const AttnDims &d, int b, int head, int key) {
+  const uint32_t page = uint32_t(key) / uint32_t(d.c.page), slot = uint32_t(key) - page * uint32_t(d.c.page);
+  const int p = d.pages[int64_t(b) * d.max_pages + page];
+  CacheRow r;
+  r.in = p >= 0 && p < d.c.n_pages;
+  r.at = ((int64_t(r.in ? p : 0) * d.c.heads + head) * d.c.page + slot) * d.c.dim;
+  return r;
 }
 
 // The products of a form, as terms X_t Y_t of a left and a right word (words of the
@@ -116,22 +125,30 @@ __device__ __forceinline__ T attn_start(const AttnArgs<T> &g, size_t i) {
   return g.c0[i];
 }
 // the 16-byte group of words [i, i + 16 / sizeof(T)) of a row of n words at p (VEC:
-// n whole groups, 16-byte aligned rows), zero past the row
+// whole groups, 16-byte aligned rows), some words of the row past its end
 template <typename T, bool VEC>
-__device__ __forceinline__ uint4 row_group(const T *p, int i, int n, bool in) {
+__device__ __forceinline__ uint4 row_group(const T *p, int i, int n) {
   constexpr int G = 16 / int(sizeof(T));
-  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  uint4 v;
   if constexpr (VEC) {
-    if (in && i < n) v = *reinterpret_cast<const uint4 *>(p + i);
+    v = *reinterpret_cast<const uint4 *>(p + (i < n ? i : 0));
   } else {
     T w[G];
 #pragma unroll
-    for (int e = 0; e < G; e++) {
-      w[e] = 0;
-      if (in && i + e < n) w[e] = p[i + e];
-    }
+    for (int e = 0; e < G; e++) w[e] = p[min(i + e, n - 1)];
     __builtin_memcpy(&v, w, 16);
   }
+  return v;
+}
+// the words of a group that lie past n words (or all: !in) set to zero
+template <typename T>
+__device__ __forceinline__ uint4 group_mask(uint4 v, int i, int n, bool in) {
+  constexpr int G = 16 / int(sizeof(T));
+  T w[G];
+  __builtin_memcpy(w, &v, 16);
+#pragma unroll
+  for (int e = 0; e < G; e++) w[e] = in && i + e < n ? w[e] : T(0);
+  __builtin_memcpy(&v, w, 16);
   return v;
 }
 template <typename T>
@@ -220,11 +237,10 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_attn_scores(AttnArgs<T> g,
   auto stage = [&](int s) {
     for (int e = tid; e < 16 * (slab / G); e += 64 * kScoreWaves) {
       const int r = e / (slab / G), q = e % (slab / G), i = s * slab + q * G;
-      const int64_t at = rows.row[r] * d.c.dim;
       const bool in = rows.row[r] >= 0;
-      const uint4 x = row_group<T, VEC>(g.x + at, i, d.c.dim, in);
-      const uint4 a0 = Form<F>::a0 ? row_group<T, VEC>(g.a0 + at, i, d.c.dim, in) : z4;
-      const uint4 a1 = Form<F>::a1 ? row_group<T, VEC>(g.a1 + at, i, d.c.dim, in) : z4;
+      const int64_t at = in ? rows.row[r] * d.c.dim : 0;
+      auto group = [&](const T *p) { return group_mask<T>(row_group<T, VEC>(p + at, i, d.c.dim), i, d.c.dim, in); };
+      const uint4 x = group(g.x), a0 = Form<F>::a0 ? group(g.a0) : z4, a1 = Form<F>::a1 ? group(g.a1) : z4;
 #pragma unroll
       for (int t = 0; t < NT; t++) xs[(t * 16 + r) * sg + q] = left_digits<F, T>(t, x, a0, a1);
     }
@@ -244,7 +260,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_attn_scores(AttnArgs<T> g,
       const int khi = rows.khi;
       for (int64_t kb = rows.klo + int64_t(u.split) * kScoreKeys; kb < khi; kb += int64_t(units.splits) * kScoreKeys) {
         const int64_t key = kb + 16 * wave + li;
-        const int64_t j = key < khi ? cache_row(d, u.b, u.kv, int(key)) : -1;
+        const CacheRow j = cache_row(d, u.b, u.kv, int(min(key, int64_t(khi) - 1)));
         T vs[4] = {0, 0, 0, 0};
         for (int s = 0; s < slabs; s++) {
           if (slabs > 1) {
@@ -260,11 +276,11 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_attn_scores(AttnArgs<T> g,
             uint4 y[CB], b0[CB], b1[CB];
 #pragma unroll
             for (int c = 0; c < CB; c++) {
+              if (c0 + c >= chunks) break;
               const int i = s * slab + ((c0 + c) * 4 + lg) * G;
-              const bool in = j >= 0 && c0 + c < chunks;
-              y[c] = Form<F>::y ? row_group<T, VEC>(g.y + j, i, d.c.dim, in) : z4;
-              b0[c] = Form<F>::b0 ? row_group<T, VEC>(g.b0 + j, i, d.c.dim, in) : z4;
-              b1[c] = Form<F>::b1 ? row_group<T, VEC>(g.b1 + j, i, d.c.dim, in) : z4;
+              y[c] = Form<F>::y ? row_group<T, VEC>(g.y + j.at, i, d.c.dim) : z4;
+              b0[c] = Form<F>::b0 ? row_group<T, VEC>(g.b0 + j.at, i, d.c.dim) : z4;
+              b1[c] = Form<F>::b1 ? row_group<T, VEC>(g.b1 + j.at, i, d.c.dim) : z4;
             }
 #pragma unroll
             for (int c = 0; c < CB; c++) {
@@ -287,7 +303,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_attn_scores(AttnArgs<T> g,
           const int row = 4 * lg + r;
           if (key < rows.lo[row] || key >= rows.hi[row]) continue;
           const size_t o = size_t(rows.base[row] + key);
-          T v = vs[r] + attn_start<F>(g, o);
+          T v = (j.in ? vs[r] : T(0)) + attn_start<F>(g, o);
           if constexpr (F == AttnForm::BOTH || F == AttnForm::P0)
             if (g.slope) v += g.slope[rows.head[row]] * T(key - g.pos[rows.tok[row]]);
           g.out[o] = v;
@@ -342,21 +358,31 @@ __global__ __launch_bounds__(64 * kMixWaves) void k_attn_mix(AttnArgs<T> g, Unit
         for (int it = 0; it < kFlush && kb < khi; it++, kb += step) {
           const int64_t k0 = kb + lg * G;  // this lane's keys k0 .. k0 + G - 1
           uint4 y[G], b0[G], b1[G];
+          CacheRow j[G];
 #pragma unroll
-          for (int i = 0; i < G; i++) {
-            const int64_t j = k0 + i < khi ? cache_row(d, u.b, u.kv, int(k0 + i)) : -1;
-            y[i] = Form<F>::y ? row_group<T, VEC>(g.y + j, col, d.c.dim, j >= 0) : z4;
-            b0[i] = Form<F>::b0 ? row_group<T, VEC>(g.b0 + j, col, d.c.dim, j >= 0) : z4;
-            b1[i] = Form<F>::b1 ? row_group<T, VEC>(g.b1 + j, col, d.c.dim, j >= 0) : z4;
-          }
+          for (int i = 0; i < G; i++) j[i] = cache_row(d, u.b, u.kv, int(min(k0 + i, int64_t(khi) - 1)));
           T xw[G], a0w[G], a1w[G];
+          bool in[G];
 #pragma unroll
           for (int i = 0; i < G; i++) {
-            const bool in = k0 + i >= lo && k0 + i < hi;
-            const int64_t o = base + k0 + i;
-            xw[i] = in ? g.x[o] : T(0);
-            a0w[i] = Form<F>::a0 && in ? g.a0[o] : T(0);
-            a1w[i] = Form<F>::a1 && in ? g.a1[o] : T(0);
+            in[i] = k0 + i >= lo && k0 + i < hi;
+            const int64_t o = in[i] ? base + k0 + i : 0;
+            xw[i] = g.x[o];
+            a0w[i] = Form<F>::a0 ? g.a0[o] : T(0);
+            a1w[i] = Form<F>::a1 ? g.a1[o] : T(0);
+          }
+#pragma unroll
+          for (int i = 0; i < G; i++) {
+            y[i] = Form<F>::y ? row_group<T, VEC>(g.y + j[i].at, col, d.c.dim) : z4;
+            b0[i] = Form<F>::b0 ? row_group<T, VEC>(g.b0 + j[i].at, col, d.c.dim) : z4;
+            b1[i] = Form<F>::b1 ? row_group<T, VEC>(g.b1 + j[i].at, col, d.c.dim) : z4;
+          }
+#pragma unroll
+          for (int i = 0; i < G; i++) {  // a weight outside the range, or of a row that is not there: no product
+            const bool use = in[i] && j[i].in;
+            xw[i] = use ? xw[i] : T(0);
+            a0w[i] = use ? a0w[i] : T(0);
+            a1w[i] = use ? a1w[i] : T(0);
           }
           uint4 x, a0, a1;
           __builtin_memcpy(&x, xw, 16);
