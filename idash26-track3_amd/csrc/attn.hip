@@ -57,8 +57,8 @@ hipError_t launch_cache_append(const Launch &L, const AppendArgs<T> &g) {
 // ---------------------------------------------------------------------------
 // attention products
 // ---------------------------------------------------------------------------
-// What token t sees: keys [lo, hi) and the first word of its block of scores.
-// Ranges and blocks that do not lie inside the bounds see nothing.
+// What a token sees: keys [lo, hi) and the first word of its block of scores.
+// Ranges and blocks that do not lie inside the bounds see nothing (0, 0, 0).
 struct TokenRange {
   int lo, hi;
   int64_t off;
@@ -68,26 +68,12 @@ __device__ __forceinline__ TokenRange token_range(const AttnDims &d, int t) {
   r.lo = d.lo[t];
   r.hi = d.hi[t];
   r.off = d.off[t];
-  const int64_t n = int64_t(r.hi) - r.lo;
-  if (r.lo < 0 || n <= 0 || r.hi > int64_t(d.max_pages) * d.c.page || r.off < 0 || r.off > d.n_scores ||
-      n * d.heads > d.n_scores - r.off)
-    r.lo = r.hi = 0, r.off = 0;
-  return r;
-}
-// Row `key` (inside the page row) of sequence b's kv head in a cache plane: its first
-// word, and whether its page is in the cache (else the word is page 0's).  Loads of
-// rows have no branches around them, so that many are in flight: a row that does not
-// exist is read at a place that does, and its products are left out.
-struct CacheRow {
-  int64_t at;
-  bool in;
-};
-__device__ __forceinline__ CacheRow cache_row(const AttnDims &d, int b, int head, int key) {
-  const uint32_t page = uint32_t(key) / uint32_t(d.c.page), slot = uint32_t(key) - page * uint32_t(d.c.page);
-  const int p = d.pages[int64_t(b) * d.max_pages + page];
-  CacheRow r;
-  r.in = p >= 0 && p < d.c.n_pages;
-  r.at = ((int64_t(r.in ? p : 0) * d.c.heads + head) * d.c.page + slot) * d.c.dim;
+  const int64_t n = int64_t(r.hi) - r.lo;  // below 2^32, times heads below 2^63
+  const bool ok = (r.lo >= 0) & (n > 0) & (r.hi <= int64_t(d.max_pages) * d.c.page) & (r.off >= 0) &
+                  (r.off <= d.n_scores) & (n * d.heads <= d.n_scores - r.off);
+  r.lo = ok ? r.lo : 0;
+  r.hi = ok ? r.hi : 0;
+  r.off = ok ? r.off : 0;
   return r;
 }
 
@@ -156,159 +142,299 @@ __device__ __forceinline__ v4i_t v4(uint4 v) {
   return v4i_t{int(v.x), int(v.y), int(v.z), int(v.w)};
 }
 
-// A tile is 16 rows (token, query head) of one sequence that read one head of the
-// cache.  What its rows see, by lane li of the first 16 threads into LDS:
-struct TileRows {
-  int lo[16], hi[16];
-  int64_t base[16];  // key j's score is word base + j
-  int64_t row[16];   // (token heads + head): the row of queries and outputs, -1: no row
-  int tok[16], head[16];
-  int klo, khi;  // all keys the rows see lie in [klo, khi)
+// Row e of a sequence and a head of the cache is query head e % m of token e / m (m query
+// heads a cache head, below 2^31 rows); a tile is 16 of them.  What a row sees:
+struct TileRow {
+  int lo, hi;
+  int64_t base;  // key j's score is word base + j
+  int tok, head;
 };
-__device__ __forceinline__ void tile_rows(const AttnDims &d, int b, int kv, int64_t e0, TileRows &s) {
-  const int tid = int(threadIdx.x), m = d.heads / d.c.heads;
-  if (tid < 16) {
-    const int t0 = max(d.qstart[b], 0), t1 = min(d.qstart[b + 1], d.n_tok);
-    const int64_t e = e0 + tid;
-    const int64_t t = t0 + e / m;
-    TokenRange r = {0, 0, 0};
-    int64_t row = -1;
-    const int head = kv * m + int(e % m);
-    if (t < t1) {
-      r = token_range(d, int(t));
-      row = t * d.heads + head;
-    }
-    s.lo[tid] = r.lo;
-    s.hi[tid] = r.hi;
-    s.base[tid] = r.off + int64_t(head) * (r.hi - r.lo) - r.lo;
-    s.row[tid] = row;
-    s.tok[tid] = int(t);
-    s.head[tid] = head;
-    int lo = r.hi > r.lo ? r.lo : INT32_MAX, hi = r.hi;
+__device__ __forceinline__ TileRow tile_row(const AttnDims &d, int t0, int t1, int kv, uint32_t m, uint32_t e) {
+  TileRow s;
+  const uint32_t q = e / m;
+  const bool in = int64_t(t0) + q < t1;
+  s.head = kv * int(m) + int(e - q * m);
+  s.tok = in ? t0 + int(q) : t0;
+  const TokenRange r = token_range(d, s.tok);
+  s.lo = in ? r.lo : 0;
+  s.hi = in ? r.hi : 0;
+  s.base = r.off + int64_t(s.head) * (r.hi - r.lo) - r.lo;
+  return s;
+}
+// smallest lo and largest hi of the rows that see something, over N lanes (hi = 0: none)
+template <int N>
+__device__ __forceinline__ void tile_keys(const TileRow &s, int &klo, int &khi) {
+  int lo = s.hi > s.lo ? s.lo : INT32_MAX, hi = s.hi;
 #pragma unroll
-    for (int k = 1; k < 16; k <<= 1) {
-      lo = min(lo, __shfl_xor(lo, k, 16));
-      hi = max(hi, __shfl_xor(hi, k, 16));
-    }
-    s.klo = hi > 0 ? lo : 0;
-    s.khi = hi;
+  for (int k = 1; k < N; k <<= 1) {
+    lo = min(lo, __shfl_xor(lo, k, N));
+    hi = max(hi, __shfl_xor(hi, k, N));
   }
+  klo = __builtin_amdgcn_readfirstlane(lo);
+  khi = __builtin_amdgcn_readfirstlane(hi);
 }
 // A launch's units of work: pair (sequence, cache head) slowest, then tile of rows,
-// column group (mix) and key split; a unit strides over tiles by `tiles` and over
-// keys by `splits`, so the hints they come from do not bound what is computed.
+// column group (mix) and key split: a unit strides over tiles by `tiles` and over keys by
+// `splits` steps of its waves, so the hints that these come from do not bound what is
+// computed, and a short sequence's units have as much less to do each.  Neighbouring
+// units run on different XCDs: an XCD that held whole sequences would be late with the
+// longest.
 struct Units {
-  int64_t n = 0;
-  int tiles = 1, cols = 1, splits = 1;
+  int n = 0, tiles = 1, cols = 1, splits = 1;
+};
+// The steps of `step` keys that wave `wave` of a unit takes, from key `at` on (khi: none
+// are left).
+struct KeySteps {
+  int64_t at, stride;
+  int khi;
+  __device__ __forceinline__ KeySteps(const Units &n, int split, int klo, int khi_, int wave, int waves, int step)
+      : at(int64_t(klo) + (int64_t(split) * waves + wave) * step), stride(int64_t(n.splits) * waves * step), khi(khi_) {}
+  __device__ __forceinline__ void advance() { at += stride; }
+  __device__ __forceinline__ bool any() const { return at < khi; }
 };
 struct Unit {
   int b, kv, tile, col, split;
 };
-__device__ __forceinline__ Unit unit_of(const AttnDims &d, const Units &n, int64_t u) {
+__device__ __forceinline__ Unit unit_of(const AttnDims &d, const Units &n) {
   Unit r;
-  r.split = int(u % n.splits);
-  u /= n.splits;
-  r.col = int(u % n.cols);
-  u /= n.cols;
-  r.tile = int(u % n.tiles);
-  u /= n.tiles;
-  r.kv = int(u % d.c.heads);
-  r.b = int(u / d.c.heads);
+  uint32_t u = blockIdx.x;
+  r.split = int(u % uint32_t(n.splits));
+  u /= uint32_t(n.splits);
+  r.col = int(u % uint32_t(n.cols));
+  u /= uint32_t(n.cols);
+  r.tile = int(u % uint32_t(n.tiles));
+  u /= uint32_t(n.tiles);
+  r.kv = int(u % uint32_t(d.c.heads));
+  r.b = int(u / uint32_t(d.c.heads));
   return r;
 }
 
+// Bytes of four ring words by digit: o[p] holds digit p of the words (Z_2^32: digits 0..3
+// of the words w; the two halves of Z_2^64 words are digits 0..3 and 4..7).
+__device__ __forceinline__ void digit_planes(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, uint32_t (&o)[4]) {
+  const uint32_t a = __builtin_amdgcn_perm(w1, w0, 0x05010400u), b = __builtin_amdgcn_perm(w1, w0, 0x07030602u);
+  const uint32_t c = __builtin_amdgcn_perm(w3, w2, 0x05010400u), d = __builtin_amdgcn_perm(w3, w2, 0x07030602u);
+  o[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+  o[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+  o[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+  o[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
+// The same of whole words as 16-byte groups of digits: one group of Z_2^32, two of Z_2^64
+template <typename T>
+__device__ __forceinline__ void group_planes(uint4 u, uint4 v, uint32_t (&o)[sizeof(T)]) {
+  if constexpr (sizeof(T) == 4) {
+    digit_planes(u.x, u.y, u.z, u.w, o);
+  } else {
+    uint32_t lo[4], hi[4];
+    digit_planes(u.x, u.z, v.x, v.z, lo);
+    digit_planes(u.y, u.w, v.y, v.w, hi);
+#pragma unroll
+    for (int p = 0; p < 4; p++) o[p] = lo[p], o[4 + p] = hi[p];
+  }
+}
+
 // ---------------------------------------------------------------------------
-// Scores.  A workgroup holds a tile's queries in LDS as digits, one plane per term;
-// each of its four waves takes 16 keys at a time, whose rows go from memory straight
-// to the lanes that feed them to the matrix cores (lane (li, lg): key li, 16-byte
-// group lg of every 64 bytes).
+// Scores.  Digits by plane: a 64-word step of the product is bw / 8 planes of 16 bytes
+// a lane on either side, and sum_{p + q < bw / 8} 2^(8(p + q)) A_p B_q takes 10 (Z_2^32)
+// or 36 (Z_2^64) MFMAs.  A workgroup holds the planes of RT tiles of queries in LDS;
+// each of its waves takes 16 keys at a time, whose rows go from memory to the lanes that
+// feed them to the matrix cores: lane (li, lg) holds of key li the 16-byte groups 4 c + lg
+// (c: the row's 64-byte chunks), so every load reads 64 bytes of each row.  A step's rows
+// and the words its products are added to are asked for as soon as the last step's are
+// used up, the first ones before the queries are staged, and the page numbers of the
+// next keys one tile ahead: no load waits for another.  The words of a launch are dims
+// [k0, k0 + kn) of the heads, as many as LDS holds of the queries; `more`: the sums so
+// far are in out.
 // ---------------------------------------------------------------------------
-constexpr int kScoreWaves = 4, kScoreKeys = 16 * kScoreWaves;
-template <AttnForm F, typename T, bool VEC>
-__global__ __launch_bounds__(64 * kScoreWaves) void k_attn_scores(AttnArgs<T> g, Units units, int slab) {
-  constexpr int G = 16 / int(sizeof(T)), NQ = int(sizeof(T)), NT = Form<F>::terms, CB = 4;
-  extern __shared__ __align__(16) uint4 xs[];  // [term][16][groups of the slab + 1]
-  __shared__ TileRows rows;
+template <AttnForm F, typename T, bool VEC, int RT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, sizeof(T) == 4 ? 2 : 1) void k_attn_scores(AttnArgs<T> g, Units units, int k0, int kn, bool more) {
+  constexpr int G = 16 / int(sizeof(T)), NQ = int(sizeof(T)), NT = Form<F>::terms;
+  constexpr int CH = int(sizeof(T)), PAIR = CH / 4;  // chunks of a step; those of four words
+  constexpr bool bias = F == AttnForm::BOTH || F == AttnForm::P0;
+  extern __shared__ __align__(16) uint4 xs[];  // [tile][step][term][plane][lane]
+  __shared__ int rlo[16 * RT], rhi[16 * RT], rpos[16 * RT];
+  __shared__ int slo[16 * RT], shi[16 * RT];
+  __shared__ int64_t rbase[16 * RT], sbase[16 * RT];
+  __shared__ T rslope[16 * RT];
   const AttnDims &d = g.d;
-  const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6, li = lane & 15, lg = lane >> 4;
-  const int sg = slab / G + 1;  // groups of an LDS row
-  const int slabs = (d.c.dim + slab - 1) / slab;
+  const int tid = int(threadIdx.x), lane = tid & 63, li = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int steps = (kn + 63) / 64, kend = k0 + kn;
   const uint4 z4 = make_uint4(0u, 0u, 0u, 0u);
-  auto stage = [&](int s) {
-    for (int e = tid; e < 16 * (slab / G); e += 64 * kScoreWaves) {
-      const int r = e / (slab / G), q = e % (slab / G), i = s * slab + q * G;
-      const bool in = rows.row[r] >= 0;
-      const int64_t at = in ? rows.row[r] * d.c.dim : 0;
-      auto group = [&](const T *p) { return group_mask<T>(row_group<T, VEC>(p + at, i, d.c.dim), i, d.c.dim, in); };
-      const uint4 x = group(g.x), a0 = Form<F>::a0 ? group(g.a0) : z4, a1 = Form<F>::a1 ? group(g.a1) : z4;
-#pragma unroll
-      for (int t = 0; t < NT; t++) xs[(t * 16 + r) * sg + q] = left_digits<F, T>(t, x, a0, a1);
-    }
+  const Unit u = unit_of(d, units);
+  const uint32_t m = uint32_t(d.heads) / uint32_t(d.c.heads);
+  const int t0 = max(d.qstart[u.b], 0), t1 = min(d.qstart[u.b + 1], d.n_tok);
+  const uint32_t n_rows = t1 > t0 ? uint32_t(t1 - t0) * m : 0u;
+  const int32_t *table = d.pages + int64_t(u.b) * d.max_pages;
+  const uint32_t psize = uint32_t(d.c.page);
+
+  struct Query {
+    uint4 x[PAIR], a0[PAIR], a1[PAIR];
   };
-  for (int64_t w = blockIdx.x; w < units.n; w += gridDim.x) {
-    const Unit u = unit_of(d, units, w);
-    const int64_t m = d.heads / d.c.heads;
-    const int64_t n_rows = int64_t(min(d.qstart[u.b + 1], d.n_tok) - max(d.qstart[u.b], 0)) * m;
-    for (int64_t e0 = int64_t(u.tile) * 16; e0 < n_rows; e0 += int64_t(units.tiles) * 16) {
-      __syncthreads();
-      tile_rows(d, u.b, u.kv, e0, rows);
-      __syncthreads();
-      if (slabs == 1) {
-        stage(0);
-        __syncthreads();
+  // a step of 16 keys' rows, and what their products are added to
+  uint4 y[CH], b0[CH], b1[CH];
+  T c0[RT][4], c1[RT][4];
+  int64_t kb = 0, at = 0;  // the keys, this lane's key's row
+  int step = 0;
+  bool in = false;  // its page is in the cache
+  v4i_t acc[RT][NQ];
+  for (int64_t eb = int64_t(u.tile) * (16 * RT); eb < n_rows; eb += int64_t(units.tiles) * (16 * RT)) {
+    const uint32_t e0 = uint32_t(eb);
+    // Queries, four words of a row at a time: lane group l's dword c of step s is words of
+    // chunk c (Z_2^32) or of chunks 2 c, 2 c + 1 (Z_2^64).  The first are asked for
+    // before anything else.
+    auto get = [&](int e, Query &q) {
+      const int r = e % (16 * RT), l = e / (16 * RT) % 4, c = e / (64 * RT) % 4, s = e / (256 * RT);
+      const int i = k0 + 64 * s + 16 * c + l * G;
+      const uint32_t qr = e0 + uint32_t(r), qt = qr < n_rows ? qr / m : 0u;
+      const bool there = qr < n_rows;
+      const int64_t row = (int64_t(t0 + int(qt)) * d.heads + u.kv * int64_t(m) + (there ? qr - qt * m : 0u)) * d.c.dim;
+#pragma unroll
+      for (int h = 0; h < PAIR; h++) {
+        auto group = [&](const T *p) {
+          return group_mask<T>(row_group<T, VEC>(p + row, i + 4 * G * h, d.c.dim), i + 4 * G * h, kend, there);
+        };
+        q.x[h] = group(g.x);
+        q.a0[h] = Form<F>::a0 ? group(g.a0) : z4;
+        q.a1[h] = Form<F>::a1 ? group(g.a1) : z4;
       }
-      const int khi = rows.khi;
-      for (int64_t kb = rows.klo + int64_t(u.split) * kScoreKeys; kb < khi; kb += int64_t(units.splits) * kScoreKeys) {
-        const int64_t key = kb + 16 * wave + li;
-        const CacheRow j = cache_row(d, u.b, u.kv, int(min(key, int64_t(khi) - 1)));
-        T vs[4] = {0, 0, 0, 0};
-        for (int s = 0; s < slabs; s++) {
-          if (slabs > 1) {
-            __syncthreads();
-            stage(s);
-            __syncthreads();
-          }
-          v4i_t acc[NQ];
+    };
+    auto put = [&](int e, const Query &q) {
+      const int r = e % (16 * RT), l = e / (16 * RT) % 4, c = e / (64 * RT) % 4, s = e / (256 * RT);
+      if (s >= steps) return;
 #pragma unroll
-          for (int q = 0; q < NQ; q++) acc[q] = v4i_t{0, 0, 0, 0};
-          const int words = min(slab, d.c.dim - s * slab), chunks = (words + 4 * G - 1) / (4 * G);
-          for (int c0 = 0; c0 < chunks; c0 += CB) {
-            uint4 y[CB], b0[CB], b1[CB];
+      for (int t = 0; t < NT; t++) {
+        uint32_t o[NQ];
+        group_planes<T>(left_digits<F, T>(t, q.x[0], q.a0[0], q.a1[0]),
+                        left_digits<F, T>(t, q.x[PAIR - 1], q.a0[PAIR - 1], q.a1[PAIR - 1]), o);
+        uint32_t *to = reinterpret_cast<uint32_t *>(
+            xs + (size_t(r / 16 * steps + s) * NT + t) * NQ * 64 + 16 * l + r % 16);
 #pragma unroll
-            for (int c = 0; c < CB; c++) {
-              if (c0 + c >= chunks) break;
-              const int i = s * slab + ((c0 + c) * 4 + lg) * G;
-              y[c] = Form<F>::y ? row_group<T, VEC>(g.y + j.at, i, d.c.dim) : z4;
-              b0[c] = Form<F>::b0 ? row_group<T, VEC>(g.b0 + j.at, i, d.c.dim) : z4;
-              b1[c] = Form<F>::b1 ? row_group<T, VEC>(g.b1 + j.at, i, d.c.dim) : z4;
-            }
-#pragma unroll
-            for (int c = 0; c < CB; c++) {
-              if (c0 + c >= chunks) break;
-#pragma unroll
-              for (int t = 0; t < NT; t++) {
-                v4i_t as[NQ];
-                digit_shifts<T>(xs[(t * 16 + li) * sg + (c0 + c) * 4 + lg], as);
-                const v4i_t bv = v4<T>(right_digits<F, T>(t, y[c], b0[c], b1[c]));
-#pragma unroll
-                for (int q = 0; q < NQ; q++) acc[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(as[q], bv, acc[q], 0, 0, 0);
-              }
-            }
-          }
-#pragma unroll
-          for (int r = 0; r < 4; r++) vs[r] += digit_fold<T>(acc, r);
+        for (int p = 0; p < NQ; p++) to[p * 256 + c] = o[p];
+      }
+    };
+    Query first;
+    get(tid, first);
+    const TileRow mine = tile_row(d, t0, t1, u.kv, m, e0 + uint32_t(lane % (16 * RT)));
+    int klo, khi;
+    tile_keys<16 * RT>(mine, klo, khi);
+    KeySteps ahead(units, u.split, klo, khi, wave, WAVES, 16);  // the tile after the one asked for
+    const int last = khi > 0 ? khi - 1 : 0;  // keys past the range read the last one's row
+    auto page_of = [&](int64_t kb) {
+      const uint32_t key = min(uint32_t(kb) + uint32_t(li), uint32_t(last));
+      return table[min(key / psize, uint32_t(d.max_pages - 1))];
+    };
+    __syncthreads();  // the last tile's queries and rows are done with
+    if (tid < 16 * RT) {
+      rlo[tid] = mine.lo;
+      rhi[tid] = mine.hi;
+      rbase[tid] = mine.base;
+      // where a word is read for a row and key without one: some word of a row that has
+      // (a place that others read too, not one that all the GPU reads)
+      const uint64_t some = __ballot(mine.hi > mine.lo);
+      const int from = mine.hi > mine.lo ? tid : some ? __ffsll((unsigned long long)some) - 1 : tid;
+      slo[tid] = __shfl(mine.lo, from);
+      shi[tid] = __shfl(mine.hi, from);
+      sbase[tid] = __shfl(mine.base, from);
+      rslope[tid] = 0;
+      rpos[tid] = 0;
+      if constexpr (bias)
+        if (g.slope && !more) {
+          rslope[tid] = g.slope[mine.head];
+          rpos[tid] = g.pos[mine.tok];
         }
+    }
+    int page = ahead.any() ? page_of(ahead.at) : 0;
+    __syncthreads();
+
+    auto load = [&]() {
+      if (step == 0) {
+        const uint32_t key = min(uint32_t(kb) + uint32_t(li), uint32_t(last));
+        in = page >= 0 && page < d.c.n_pages;
+        at = ((int64_t(in ? page : 0) * d.c.heads + u.kv) * psize + key % psize) * d.c.dim;
+        ahead.advance();
+        if (ahead.any()) page = page_of(ahead.at);
+      }
+#pragma unroll
+      for (int c = 0; c < CH; c++) {
+        const int w = step * 64 + 4 * G * c;  // first word of the chunk
+        if (w < kn) {
+          const int i = k0 + w + lg * G;
+          if constexpr (Form<F>::y) y[c] = row_group<T, VEC>(g.y + at, i, d.c.dim);
+          if constexpr (Form<F>::b0) b0[c] = row_group<T, VEC>(g.b0 + at, i, d.c.dim);
+          if constexpr (Form<F>::b1) b1[c] = row_group<T, VEC>(g.b1 + at, i, d.c.dim);
+        }
+      }
+      if (step == steps - 1) {
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const int row = 16 * t + 4 * lg + r;
+            const uint32_t key = uint32_t(kb) + uint32_t(li);
+            const size_t o = size_t(sbase[row] + max(min(key, uint32_t(shi[row] - 1)), uint32_t(slo[row])));
+            c0[t][r] = more ? g.out[o] : F == AttnForm::P1 ? g.c1[o] : g.c0[o];
+            c1[t][r] = F == AttnForm::BOTH && !more ? g.c1[o] : T(0);
+          }
+      }
+    };
+    auto multiply = [&]() {
+      if (step == 0) {
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+          for (int q = 0; q < NQ; q++) acc[t][q] = v4i_t{0, 0, 0, 0};
+      }
+      const uint4 *x = xs + step * (NT * NQ * 64) + lane;
+#pragma unroll
+      for (int e = 0; e < NT; e++) {
+        v4i_t bp[NQ];  // the step's planes of the keys
+#pragma unroll
+        for (int c = 0; c < 4; c++) {  // one dword of every plane from a group of four words
+          uint32_t o[NQ];
+          const int c0 = c * PAIR, c1 = c0 + PAIR - 1;
+          group_planes<T>(right_digits<F, T>(e, y[c0], b0[c0], b1[c0]), right_digits<F, T>(e, y[c1], b0[c1], b1[c1]), o);
+#pragma unroll
+          for (int q = 0; q < NQ; q++) bp[q][c] = int(o[q]);
+        }
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+          for (int p = 0; p < NQ; p++) {
+            const v4i_t a = v4<T>(x[(t * steps * NT + e) * NQ * 64 + p * 64]);
+#pragma unroll
+            for (int q = 0; q + p < NQ; q++)
+              acc[t][p + q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, bp[q], acc[t][p + q], 0, 0, 0);
+          }
+      }
+      if (step + 1 < steps) return;
+      const uint32_t key = uint32_t(kb) + uint32_t(li);
+#pragma unroll
+      for (int t = 0; t < RT; t++)
 #pragma unroll
         for (int r = 0; r < 4; r++) {  // accumulator register r of lane (li, lg): row 4 lg + r, key li
-          const int row = 4 * lg + r;
-          if (key < rows.lo[row] || key >= rows.hi[row]) continue;
-          const size_t o = size_t(rows.base[row] + key);
-          T v = (j.in ? vs[r] : T(0)) + attn_start<F>(g, o);
-          if constexpr (F == AttnForm::BOTH || F == AttnForm::P0)
-            if (g.slope) v += g.slope[rows.head[row]] * T(key - g.pos[rows.tok[row]]);
-          g.out[o] = v;
+          const int row = 16 * t + 4 * lg + r;
+          if (key < uint32_t(rlo[row]) || key >= uint32_t(rhi[row])) continue;
+          T v = (in ? digit_fold<T>(acc[t], r) : T(0)) + c0[t][r];
+          if constexpr (F == AttnForm::BOTH) v += c1[t][r];
+          if constexpr (bias) v += rslope[row] * T(int64_t(key) - rpos[row]);
+          g.out[size_t(rbase[row] + key)] = v;
         }
-      }
+    };
+    kb = ahead.at;
+    step = 0;
+    if (kb < khi) load();
+    put(tid, first);
+    for (int e = tid + 64 * WAVES; e < 16 * RT * steps * 16; e += 64 * WAVES) {
+      Query q;
+      get(e, q);
+      put(e, q);
+    }
+    __syncthreads();
+    while (kb < khi) {
+      multiply();
+      if (++step == steps) step = 0, kb = ahead.at;
+      if (kb < khi) load();
     }
   }
 }
@@ -321,120 +447,152 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_attn_scores(AttnArgs<T> g,
 // the keys out; their sums meet in LDS and in integer additions to the output, whose
 // order does not matter.
 // ---------------------------------------------------------------------------
-constexpr int kMixWaves = 4;
+constexpr int kMixWaves = 8;
 template <AttnForm F, typename T, bool VEC>
 __global__ __launch_bounds__(64 * kMixWaves) void k_attn_mix(AttnArgs<T> g, Units units) {
   constexpr int G = 16 / int(sizeof(T)), NQ = int(sizeof(T)), NT = Form<F>::terms, CK = 4 * G;
-  constexpr int kFlush = 4096 / CK;  // chunks whose digit sums stay exact (3 terms, Z_2^64)
-  __shared__ TileRows rows;
+  // chunks whose digit sums stay exact (Z_2^64, 3 terms); Z_2^32 needs them modulo 2^32 only
+  constexpr int kFlush = sizeof(T) == 4 ? INT32_MAX : 4096 / CK;
   __shared__ T red[kMixWaves][G * 4][64];
   const AttnDims &d = g.d;
-  const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6, li = lane & 15, lg = lane >> 4;
+  const int tid = int(threadIdx.x), lane = tid & 63, li = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint4 z4 = make_uint4(0u, 0u, 0u, 0u);
-  for (int64_t w = blockIdx.x; w < units.n; w += gridDim.x) {
-    const Unit u = unit_of(d, units, w);
-    const int64_t m = d.heads / d.c.heads;
-    const int64_t n_rows = int64_t(min(d.qstart[u.b + 1], d.n_tok) - max(d.qstart[u.b], 0)) * m;
-    const int col = u.col * 16 * G + li * G;  // this lane's columns
-    for (int64_t e0 = int64_t(u.tile) * 16; e0 < n_rows; e0 += int64_t(units.tiles) * 16) {
-      __syncthreads();
-      tile_rows(d, u.b, u.kv, e0, rows);
-      __syncthreads();
-      const int khi = rows.khi, lo = rows.lo[li], hi = rows.hi[li];
-      const int64_t base = rows.base[li];
-      v4i_t acc[G][NQ];
-      T vs[G][4];
+  const Unit u = unit_of(d, units);
+  const uint32_t m = uint32_t(d.heads) / uint32_t(d.c.heads);
+  const int t0 = max(d.qstart[u.b], 0), t1 = min(d.qstart[u.b + 1], d.n_tok);
+  const uint32_t n_rows = t1 > t0 ? uint32_t(t1 - t0) * m : 0u;
+  const int col = u.col * 16 * G + li * G;  // this lane's columns
+  const int32_t *table = d.pages + int64_t(u.b) * d.max_pages;
+  const uint32_t psize = uint32_t(d.c.page);
+  for (int64_t eb = int64_t(u.tile) * 16; eb < n_rows; eb += int64_t(units.tiles) * 16) {
+    const uint32_t e0 = uint32_t(eb);
+    const TileRow mine = tile_row(d, t0, t1, u.kv, m, e0 + uint32_t(li));
+    int klo, khi;
+    tile_keys<16>(mine, klo, khi);
+    const int lo = mine.lo, hi = mine.hi;
+    // where a weight is read for a row or key without one: some weight of a row that has
+    // (a place that others read too, not one that all the GPU reads)
+    const uint64_t some = __ballot(hi > lo);
+    const int from = hi > lo || !some ? lane : __ffsll((unsigned long long)some) - 1;
+    const int slo = __shfl(lo, from), shi = __shfl(hi, from);
+    const int64_t sbase = __shfl(mine.base, from);
+    KeySteps keys(units, u.split, klo, khi, wave, kMixWaves, CK);
+    // a chunk's rows and weights, and the page numbers of the next one
+    uint4 y[G], b0[G], b1[G];
+    T xw[G], a0w[G], a1w[G];
+    uint32_t used = 0;  // bit i: key i of the chunk counts for this lane's row
+    int page[G];
+    auto pages = [&]() {
+#pragma unroll
+      for (int i = 0; i < G; i++) {
+        const uint32_t key = min(uint32_t(keys.at) + uint32_t(lg * G + i), uint32_t(khi - 1));
+        page[i] = table[key / psize];
+      }
+    };
+    auto load = [&]() {
+      const uint32_t k0 = uint32_t(keys.at) + uint32_t(lg * G);  // this lane's keys k0 .. k0 + G - 1
+      used = 0;
+#pragma unroll
+      for (int i = 0; i < G; i++) {
+        const uint32_t key = min(k0 + i, uint32_t(khi - 1));
+        const bool in = page[i] >= 0 && page[i] < d.c.n_pages;
+        const int64_t at = ((int64_t(in ? page[i] : 0) * d.c.heads + u.kv) * psize + key % psize) * d.c.dim;
+        if constexpr (Form<F>::y) y[i] = row_group<T, VEC>(g.y + at, col, d.c.dim);
+        if constexpr (Form<F>::b0) b0[i] = row_group<T, VEC>(g.b0 + at, col, d.c.dim);
+        if constexpr (Form<F>::b1) b1[i] = row_group<T, VEC>(g.b1 + at, col, d.c.dim);
+        // a weight outside the range, or of a row that is not there: no product
+        if (in && k0 + i >= uint32_t(lo) && k0 + i < uint32_t(hi)) used |= 1u << i;
+      }
+#pragma unroll
+      for (int i = 0; i < G; i++) {
+        const int64_t o = sbase + max(min(k0 + i, uint32_t(shi - 1)), uint32_t(slo));
+        xw[i] = g.x[o];
+        a0w[i] = Form<F>::a0 ? g.a0[o] : T(0);
+        a1w[i] = Form<F>::a1 ? g.a1[o] : T(0);
+      }
+      keys.advance();
+      if (keys.any()) pages();
+    };
+    v4i_t acc[G][NQ];
+    T vs[G][4];
+#pragma unroll
+    for (int q = 0; q < G; q++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) vs[q][r] = 0;
+    bool more = keys.any();
+    if (more) {
+      pages();
+      load();
+    }
+    while (more) {
 #pragma unroll
       for (int q = 0; q < G; q++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) vs[q][r] = 0;
-      int64_t kb = rows.klo + (int64_t(u.split) * kMixWaves + wave) * CK;
-      const int64_t step = int64_t(units.splits) * kMixWaves * CK;
-      while (kb < khi) {
+        for (int s = 0; s < NQ; s++) acc[q][s] = v4i_t{0, 0, 0, 0};
+      for (int it = 0; it < kFlush && more; it++) {
+        uint4 x, a0, a1;
 #pragma unroll
-        for (int q = 0; q < G; q++)
+        for (int i = 0; i < G; i++) {
+          const bool use = used >> i & 1u;
+          xw[i] = use ? xw[i] : T(0);
+          a0w[i] = use ? a0w[i] : T(0);
+          a1w[i] = use ? a1w[i] : T(0);
+        }
+        __builtin_memcpy(&x, xw, 16);
+        __builtin_memcpy(&a0, a0w, 16);
+        __builtin_memcpy(&a1, a1w, 16);
 #pragma unroll
-          for (int s = 0; s < NQ; s++) acc[q][s] = v4i_t{0, 0, 0, 0};
-        for (int it = 0; it < kFlush && kb < khi; it++, kb += step) {
-          const int64_t k0 = kb + lg * G;  // this lane's keys k0 .. k0 + G - 1
-          uint4 y[G], b0[G], b1[G];
-          CacheRow j[G];
-#pragma unroll
-          for (int i = 0; i < G; i++) j[i] = cache_row(d, u.b, u.kv, int(min(k0 + i, int64_t(khi) - 1)));
-          T xw[G], a0w[G], a1w[G];
-          bool in[G];
-#pragma unroll
-          for (int i = 0; i < G; i++) {
-            in[i] = k0 + i >= lo && k0 + i < hi;
-            const int64_t o = in[i] ? base + k0 + i : 0;
-            xw[i] = g.x[o];
-            a0w[i] = Form<F>::a0 ? g.a0[o] : T(0);
-            a1w[i] = Form<F>::a1 ? g.a1[o] : T(0);
-          }
+        for (int t = 0; t < NT; t++) {
+          v4i_t as[NQ];
+          digit_shifts<T>(left_digits<F, T>(t, x, a0, a1), as);
+          uint32_t dig[G][4];
 #pragma unroll
           for (int i = 0; i < G; i++) {
-            y[i] = Form<F>::y ? row_group<T, VEC>(g.y + j[i].at, col, d.c.dim) : z4;
-            b0[i] = Form<F>::b0 ? row_group<T, VEC>(g.b0 + j[i].at, col, d.c.dim) : z4;
-            b1[i] = Form<F>::b1 ? row_group<T, VEC>(g.b1 + j[i].at, col, d.c.dim) : z4;
+            const uint4 v = right_digits<F, T>(t, y[i], b0[i], b1[i]);
+            dig[i][0] = v.x, dig[i][1] = v.y, dig[i][2] = v.z, dig[i][3] = v.w;
           }
 #pragma unroll
-          for (int i = 0; i < G; i++) {  // a weight outside the range, or of a row that is not there: no product
-            const bool use = in[i] && j[i].in;
-            xw[i] = use ? xw[i] : T(0);
-            a0w[i] = use ? a0w[i] : T(0);
-            a1w[i] = use ? a1w[i] : T(0);
-          }
-          uint4 x, a0, a1;
-          __builtin_memcpy(&x, xw, 16);
-          __builtin_memcpy(&a0, a0w, 16);
-          __builtin_memcpy(&a1, a1w, 16);
+          for (int q = 0; q < G; q++) {
+            v4i_t bv;
+            if constexpr (sizeof(T) == 4) bv = v4i_t{int(dig[0][q]), int(dig[1][q]), int(dig[G - 2][q]), int(dig[G - 1][q])};
+            else bv = v4i_t{int(dig[0][2 * q]), int(dig[0][2 * q + 1]), int(dig[1][2 * q]), int(dig[1][2 * q + 1])};
 #pragma unroll
-          for (int t = 0; t < NT; t++) {
-            v4i_t as[NQ];
-            digit_shifts<T>(left_digits<F, T>(t, x, a0, a1), as);
-            uint32_t dig[G][4];
-#pragma unroll
-            for (int i = 0; i < G; i++) {
-              const uint4 v = right_digits<F, T>(t, y[i], b0[i], b1[i]);
-              dig[i][0] = v.x, dig[i][1] = v.y, dig[i][2] = v.z, dig[i][3] = v.w;
-            }
-#pragma unroll
-            for (int q = 0; q < G; q++) {
-              v4i_t bv;
-              if constexpr (sizeof(T) == 4) bv = v4i_t{int(dig[0][q]), int(dig[1][q]), int(dig[G - 2][q]), int(dig[G - 1][q])};
-              else bv = v4i_t{int(dig[0][2 * q]), int(dig[0][2 * q + 1]), int(dig[1][2 * q]), int(dig[1][2 * q + 1])};
-#pragma unroll
-              for (int s = 0; s < NQ; s++)
-                acc[q][s] = __builtin_amdgcn_mfma_i32_16x16x64_i8(as[s], bv, acc[q][s], 0, 0, 0);
-            }
+            for (int s = 0; s < NQ; s++)
+              acc[q][s] = __builtin_amdgcn_mfma_i32_16x16x64_i8(as[s], bv, acc[q][s], 0, 0, 0);
           }
         }
-#pragma unroll
-        for (int q = 0; q < G; q++)
-#pragma unroll
-          for (int r = 0; r < 4; r++) vs[q][r] += digit_fold<T>(acc[q], r);
+        more = keys.any();
+        if (more) load();
       }
 #pragma unroll
       for (int q = 0; q < G; q++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) red[wave][q * 4 + r][lane] = vs[q][r];
-      __syncthreads();
-      for (int e = tid; e < G * 4 * 64; e += 64 * kMixWaves) {
-        // words in the order of the output: row, column (G a lane)
-        const int row = e / (16 * G), c = e % (16 * G), q = c % G, l = 16 * (row / 4) + c / G, at = q * 4 + row % 4;
-        const int oc = u.col * 16 * G + c;
-        if (rows.row[row] < 0 || oc >= d.c.dim) continue;
-        T v = 0;
+        for (int r = 0; r < 4; r++) vs[q][r] += digit_fold<T>(acc[q], r);
+    }
+    __syncthreads();  // the last tile's sums are read
 #pragma unroll
-        for (int k = 0; k < kMixWaves; k++) v += red[k][at][l];
-        const size_t o = size_t(rows.row[row]) * d.c.dim + oc;
-        if (units.splits == 1) {
-          g.out[o] = v + attn_start<F>(g, o);
-        } else if constexpr (sizeof(T) == 4) {
-          atomicAdd(reinterpret_cast<unsigned int *>(&g.out[o]), static_cast<unsigned int>(v));
-        } else {
-          atomicAdd(reinterpret_cast<unsigned long long *>(&g.out[o]), static_cast<unsigned long long>(v));
-        }
+    for (int q = 0; q < G; q++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) red[wave][q * 4 + r][lane] = vs[q][r];
+    __syncthreads();
+    for (int e = tid; e < G * 4 * 64; e += 64 * kMixWaves) {
+      // words in the order of the output: row, column (G a lane)
+      const int row = e / (16 * G), c = e % (16 * G), q = c % G, l = 16 * (row / 4) + c / G, at = q * 4 + row % 4;
+      const int oc = u.col * 16 * G + c;
+      const uint32_t er = e0 + uint32_t(row);
+      if (er >= n_rows || oc >= d.c.dim) continue;
+      const uint32_t qt = er / m;
+      T v = 0;
+#pragma unroll
+      for (int k = 0; k < kMixWaves; k++) v += red[k][at][l];
+      const size_t o = size_t((int64_t(t0 + int(qt)) * d.heads + u.kv * int64_t(m) + (er - qt * m)) * d.c.dim + oc);
+      if (units.splits == 1) {
+        g.out[o] = v + attn_start<F>(g, o);
+      } else if constexpr (sizeof(T) == 4) {
+        atomicAdd(reinterpret_cast<unsigned int *>(&g.out[o]), static_cast<unsigned int>(v));
+      } else {
+        atomicAdd(reinterpret_cast<unsigned long long *>(&g.out[o]), static_cast<unsigned long long>(v));
       }
     }
   }
@@ -456,39 +614,61 @@ bool vec_rows(const AttnArgs<T> &g, bool left) {
       ok = ok && reinterpret_cast<uintptr_t>(p) % 16 == 0;
   return ok;
 }
-// about `want` units, at least one tile and one split each
-Units units_for(const AttnDims &d, int cols, int64_t want, int64_t keys_per_split) {
+// About `want` units, at least one tile and one split for each pair and column group;
+// none (n = 0) where the pairs alone are too many for a launch.
+Units units_for(const AttnDims &d, int cols, int rows, int64_t want, int64_t keys_per_split) {
   Units u;
+  const int64_t m = d.heads / d.c.heads, base = int64_t(d.n_seq) * d.c.heads;
+  constexpr int64_t kMost = 1 << 30;
+  if (base > kMost / cols) return u;
   u.cols = cols;
-  const int64_t m = d.heads / d.c.heads, pairs = int64_t(d.n_seq) * d.c.heads;
-  const int64_t tiles = std::min<int64_t>((int64_t(d.max_q) * m + 15) / 16, 1 << 20);
-  const int64_t base = pairs * cols * tiles, most = (int64_t(d.max_keys) + keys_per_split - 1) / keys_per_split;
-  u.tiles = int(tiles);
-  u.splits = int(std::max<int64_t>(1, std::min<int64_t>((want + base - 1) / base, std::min<int64_t>(most, 1 << 16))));
-  u.n = base * u.splits;
+  u.tiles = int(std::max<int64_t>(1, std::min((int64_t(d.max_q) * m + rows - 1) / rows, kMost / (base * cols))));
+  const int64_t one = base * cols * u.tiles, keys = (int64_t(d.max_keys) + keys_per_split - 1) / keys_per_split;
+  u.splits = int(std::max<int64_t>(1, std::min((want + one - 1) / one, std::min(keys, kMost / one))));
+  u.n = int(one * u.splits);
   return u;
 }
-unsigned grid_of(const Units &u) { return unsigned(std::min<int64_t>(u.n, 1 << 24)); }
 
+// LDS of a launch's queries: 1 KB a plane and step
+template <AttnForm F, typename T>
+constexpr size_t kStepLds = size_t(Form<F>::terms) * sizeof(T) * 1024;
+constexpr size_t kScoreLds = 62 * 1024;
+
+template <AttnForm F, typename T, int RT, int WAVES>
+hipError_t scores_rows(const Launch &L, const AttnArgs<T> &g, int dims, int64_t want) {
+  const Units u = units_for(g.d, 1, 16 * RT, want, 16 * WAVES);
+  if (u.n == 0) return hipErrorInvalidValue;
+  const bool vec = vec_rows(g, true);
+  for (int k0 = 0; k0 < g.d.c.dim; k0 += dims) {
+    const int kn = std::min(dims, g.d.c.dim - k0);
+    const size_t lds = kStepLds<F, T> * RT * size_t((kn + 63) / 64);
+    if (vec)
+      hipLaunchKernelGGL((k_attn_scores<F, T, true, RT, WAVES>), dim3(unsigned(u.n)), dim3(64 * WAVES), lds, L.stream, g, u,
+                         k0, kn, k0 > 0);
+    else
+      hipLaunchKernelGGL((k_attn_scores<F, T, false, RT, WAVES>), dim3(unsigned(u.n)), dim3(64 * WAVES), lds, L.stream, g, u,
+                         k0, kn, k0 > 0);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
 template <AttnForm F, typename T>
 hipError_t scores_at(const Launch &L, const AttnArgs<T> &g) {
-  constexpr int G = 16 / int(sizeof(T));
-  // the tile's queries in at most 64 KB: slabs of whole 64-byte groups
-  const int most = 64 * 1024 / (Form<F>::terms * 16 * int(sizeof(T))) / (4 * G) * (4 * G) - 4 * G;
-  const int slab = std::min((g.d.c.dim + 4 * G - 1) / (4 * G) * (4 * G), most);
-  const size_t lds = size_t(Form<F>::terms) * 16 * (slab / G + 1) * 16;
-  const Units u = units_for(g.d, 1, int64_t(L.num_cu) * 8, kScoreKeys);
-  if (vec_rows(g, true))
-    hipLaunchKernelGGL((k_attn_scores<F, T, true>), dim3(grid_of(u)), dim3(64 * kScoreWaves), lds, L.stream, g, u, slab);
-  else
-    hipLaunchKernelGGL((k_attn_scores<F, T, false>), dim3(grid_of(u)), dim3(64 * kScoreWaves), lds, L.stream, g, u, slab);
-  return hipGetLastError();
+  const int m = g.d.heads / g.d.c.heads;
+  const size_t steps = size_t(g.d.c.dim + 63) / 64;
+  // two tiles of rows to a workgroup where a sequence has them and LDS holds them
+  if (int64_t(g.d.max_q) * m >= 32 && steps * kStepLds<F, T> * 2 <= kScoreLds)
+    return scores_rows<F, T, 2, 8>(L, g, g.d.c.dim, int64_t(L.num_cu) * 2);
+  const int dims = int(std::min(steps, kScoreLds / kStepLds<F, T>)) * 64;
+  return scores_rows<F, T, 1, 4>(L, g, dims, int64_t(L.num_cu) * 2);
 }
 template <AttnForm F, typename T>
 hipError_t mix_at(const Launch &L, const AttnArgs<T> &g) {
   constexpr int G = 16 / int(sizeof(T));
   const Units u =
-      units_for(g.d, (g.d.c.dim + 16 * G - 1) / (16 * G), int64_t(L.num_cu) * 4, int64_t(kMixWaves) * 4 * G * 4);
+      units_for(g.d, (g.d.c.dim + 16 * G - 1) / (16 * G), 16, int64_t(L.num_cu), int64_t(kMixWaves) * 4 * G * 4);
+  if (u.n == 0) return hipErrorInvalidValue;
   if (u.splits > 1) {
     const size_t n = size_t(g.d.n_tok) * g.d.heads * g.d.c.dim, want = (n + 255) / 256, cap = size_t(L.num_cu) * 32;
     hipLaunchKernelGGL((k_mix_init<F, T>), dim3(unsigned(want < cap ? want : cap)), dim3(256), 0, L.stream, g, n);
@@ -496,9 +676,9 @@ hipError_t mix_at(const Launch &L, const AttnArgs<T> &g) {
     if (e != hipSuccess) return e;
   }
   if (vec_rows(g, false))
-    hipLaunchKernelGGL((k_attn_mix<F, T, true>), dim3(grid_of(u)), dim3(64 * kMixWaves), 0, L.stream, g, u);
+    hipLaunchKernelGGL((k_attn_mix<F, T, true>), dim3(unsigned(u.n)), dim3(64 * kMixWaves), 0, L.stream, g, u);
   else
-    hipLaunchKernelGGL((k_attn_mix<F, T, false>), dim3(grid_of(u)), dim3(64 * kMixWaves), 0, L.stream, g, u);
+    hipLaunchKernelGGL((k_attn_mix<F, T, false>), dim3(unsigned(u.n)), dim3(64 * kMixWaves), 0, L.stream, g, u);
   return hipGetLastError();
 }
 

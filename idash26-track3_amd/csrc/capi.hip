@@ -1130,7 +1130,8 @@ bool attn_sizes(const mpcx_attn *a, size_t *rows, size_t *scores) {
       a->n_scores >= int64_t(1) << 60)
     return false;
   const unsigned __int128 n = (unsigned __int128)(a->n_tok) * unsigned(a->n_heads) * unsigned(a->cache.head_dim);
-  if (n >= (unsigned __int128)1 << 60) return false;
+  if (n >= (unsigned __int128)1 << 60 || int64_t(a->n_tok) * (a->n_heads / a->cache.n_heads) >= int64_t(1) << 31)
+    return false;
   *rows = size_t(n);
   *scores = size_t(a->n_scores);
   return true;

@@ -393,8 +393,8 @@ mpcx_status mpcx_split_mask(mpcx_ctx *ctx, size_t n, const void *d_mask, uint64_
  * n_seq sequences one after another: sequence b has tokens d_qstart[b] ..
  * d_qstart[b + 1] - 1 and its key j in slot j % page_size of page
  * d_pages[b * max_pages + j / page_size] (a page number outside the cache reads
- * as rows of zeros).  n_heads query heads, a multiple m of the cache's: head h
- * reads the cache's head h / m.  Token t sees the keys d_lo[t] <= j < d_hi[t]
+ * as rows of zeros).  n_heads query heads, a multiple m of the cache's (n_tok * m
+ * below 2^31): head h reads the cache's head h / m.  Token t sees the keys d_lo[t] <= j < d_hi[t]
  * (causal, prefix, window and document masks; none where lo >= hi), and its
  * scores are the n_heads * (hi - lo) words from d_off[t] on, head by head, of
  * n_scores in all.  A token whose range leaves its page row or whose block
