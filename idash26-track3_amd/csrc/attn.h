@@ -10,6 +10,7 @@ namespace mpcx {
 // C[m, n] = sum_g scale[g, n] sum_{k in group g} q[n, k] A[m, k] mod 2^bw.
 // q: N rows of q4_row_bytes(K) bytes, weight k of a row in the low (k even) or
 // high half of byte k / 2, two's complement; scale: ceil(K / group) x N.
+constexpr int kQ4MaxK = 1 << 24;  // a tile's weights lie within 32 bits
 inline size_t q4_row_bytes(int K) { return (size_t(K) + 31) / 32 * 16; }
 template <typename T>
 struct Q4Args {

@@ -1022,7 +1022,7 @@ static bool aligned(const void *p, size_t to) { return reinterpret_cast<uintptr_
 mpcx_status mpcx_ring_gemm_q4(mpcx_ctx *c, int M, int K, int N, int group, const void *a, size_t lda, const uint8_t *q,
                               const int32_t *scale, void *out, size_t ldc, void *work) {
   CHECK_CTX(c);
-  if (M < 1 || K < 1 || N < 1 || group < 32 || group % 32 != 0 || lda < size_t(K) || ldc < size_t(N))
+  if (M < 1 || K < 1 || K > kQ4MaxK || N < 1 || group < 32 || group % 32 != 0 || lda < size_t(K) || ldc < size_t(N))
     return fail(c, MPCX_EINVAL, "ring_gemm_q4: bad argument");
   if (!a || !q || !scale || !out || (!work && q4_work_bytes(c->bw, M, K) > 0))
     return fail(c, MPCX_EINVAL, "ring_gemm_q4: null pointer");

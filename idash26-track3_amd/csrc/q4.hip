@@ -17,6 +17,8 @@
 // planes 4..7 (odd lg) shifted up by 32 at the end.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "attn.h"
 #include "digits.h"
 #include "launch_util.h"
@@ -192,64 +194,132 @@ __global__ __launch_bounds__(256) void k_q4_digits(Q4Args<T> g, bool vec, int ti
   }
 }
 
-// Second step: a workgroup of 2 x 2 waves, each MT tiles of rows by NT of columns;
-// the rows' operands of a step (128 k) are staged in LDS, the weights go straight to
-// the lanes' registers.
+// Sums over chunks of plane sums times scales.  Z_2^32: one 24-bit multiply-add a plane
+// (a chunk's plane sums are below 2^21, divided by 16 in plane 0 so that no bit of the
+// word is lost; the planes above need 4 fewer bits), the planes folded at the end; a
+// scale past 24 bits is its low 12 bits and, in a second pass, the others.  Z_2^64:
+// 64-bit sums of the plane pairs.
+template <typename T>
+struct Q4Sum;
+template <>
+struct Q4Sum<uint32_t> {
+  int32_t w[4];
+  static __device__ __forceinline__ int32_t high(int32_t s) {
+    return (uint32_t(s) + (1u << 23)) >> 24 ? s >> 12 : 0;
+  }
+  __device__ __forceinline__ void add(v4i_t a, int32_t s) {
+    w[0] += __mul24(a[0] >> 4, s);
+#pragma unroll
+    for (int p = 1; p < 4; p++) w[p] += __mul24(a[p], s);
+  }
+  __device__ __forceinline__ void add_high(v4i_t a, int32_t s) {
+#pragma unroll
+    for (int p = 0; p < 4; p++) {
+      int32_t x;  // (not __mul24, whose sign extensions would move to where every scale passes)
+      asm("v_mul_i32_i24_e32 %0, %1, %2" : "=v"(x) : "v"(p ? a[p] : a[0] >> 4), "v"(s));
+      w[p] += int32_t(uint32_t(x) << 12);
+    }
+  }
+  __device__ __forceinline__ uint32_t word() const {
+    return uint32_t(w[0]) + (uint32_t(w[1]) << 4) + (uint32_t(w[2]) << 12) + (uint32_t(w[3]) << 20);
+  }
+};
+template <>
+struct Q4Sum<uint64_t> {
+  int64_t w[2];
+  __device__ __forceinline__ void add(v4i_t a, int32_t s) {
+    w[0] += int64_t((a[0] >> 4) + (a[1] << 4)) * s;
+    w[1] += int64_t((a[2] >> 4) + (a[3] << 4)) * s;
+  }
+  static __device__ __forceinline__ int32_t high(int32_t) { return 0; }
+  __device__ __forceinline__ void add_high(v4i_t, int32_t) {}
+  __device__ __forceinline__ uint64_t word() const { return uint64_t(w[0]) + (uint64_t(w[1]) << 16); }
+};
+
+// Second step: a workgroup of 2 x 2 waves, each MT tiles of rows by NT of columns.  The
+// rows' operands of a step (128 k) go through LDS, the weights and scales straight to the
+// lanes' registers; all are asked for a step ahead.
 template <typename T, int S, int MT, int NT>
-__global__ __launch_bounds__(256) void k_q4_many(Q4Args<T> g, int steps, const uint8_t *work) {
+__global__ __launch_bounds__(256, 2) void k_q4_many(Q4Args<T> g, int steps, const uint8_t *work) {
   constexpr int R = kRows<T>, ND = S / 32, CH = 128 / S;
-  __shared__ __align__(16) uint4 as[2][2 * MT * 128];  // step, tile, 2 KB
+  __shared__ __align__(16) v4i_t as0[2 * MT * 128], as1[2 * MT * 128];  // even and odd steps: tile, 2 KB
   const int gx = (g.N + 32 * NT - 1) / (32 * NT);
   const int lw = xcd_swizzle(int(blockIdx.x), int(gridDim.x));
-  const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6, li = lane & 15, lg = lane >> 4;
+  const int tid = int(threadIdx.x), lane = tid & 63, li = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n0 = lw % gx * 32 * NT + (wave & 1) * 16 * NT, t0 = lw / gx * 2 * MT;
-  const size_t qrow = (size_t(g.K) + 31) / 32 * 16;
-  const int per = g.group / S;
-  const uint8_t *q[NT];
-  int nc[NT];
+  const uint32_t qrow = uint32_t((size_t(g.K) + 31) / 32 * 16);
+  const int per = g.group / S, last = (g.K - 1) / S;
+  // places in 32 bits from bases that a wave shares (launch_gemm_q4 bounds K)
+  const int nw = min(n0, g.N - 1);
+  const uint8_t *qw = g.q + size_t(nw) * qrow;
+  const int32_t *sw = g.scale + nw;
+  uint32_t qo[NT], so[NT];
 #pragma unroll
   for (int t = 0; t < NT; t++) {
-    const int n = n0 + 16 * t + li;
-    nc[t] = n < g.N ? n : g.N - 1;
-    q[t] = g.q + size_t(nc[t]) * qrow;
+    so[t] = uint32_t(min(16 * t + li, g.N - 1 - nw));
+    qo[t] = so[t] * qrow;
   }
-  T out[MT][NT];
-#pragma unroll
-  for (int i = 0; i < MT; i++)
-#pragma unroll
-    for (int t = 0; t < NT; t++) out[i][t] = 0;
-  const uint4 *src = reinterpret_cast<const uint4 *>(work);
-  uint4 ra[MT];
-  auto load = [&](int step) {
-#pragma unroll
-    for (int j = 0; j < MT; j++) {  // 256 threads move two tiles at a time
-      const int f = tid + 256 * j;
-      ra[j] = src[(size_t(t0 + f / 128) * steps + step) * 128 + f % 128];
-    }
+  Q4Sum<T> out[MT][NT] = {};
+  // 256 threads move two tiles of rows at a time
+  const v4i_t *src = reinterpret_cast<const v4i_t *>(work) + size_t(t0) * steps * 128;
+  const uint32_t ro = uint32_t(tid / 128 * steps * 128 + tid % 128);
+  // a step's weights and scales
+  struct Ahead {
+    uint32_t b[CH][NT][ND];
+    int32_t s[CH][NT];
   };
-  load(0);
-  for (int step = 0; step < steps; step++) {
-    uint4 *buf = as[step & 1];
+  auto load = [&](v4i_t *as, int step, Ahead &h) __attribute__((always_inline)) {
+    step = min(step, steps - 1);
+    // the rows' operands straight into LDS: a wave moves 64 groups of 16 bytes to
+    // consecutive places
 #pragma unroll
-    for (int j = 0; j < MT; j++) buf[tid + 256 * j] = ra[j];
-    __syncthreads();
-    if (step + 1 < steps) load(step + 1);
+    for (int j = 0; j < MT; j++)
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void *)(src + (size_t(2 * j) * steps + step) * 128 + ro),
+          (__attribute__((address_space(3))) void *)(as + 256 * j + 64 * wave), 16, 0, 0);
+    // weights past the end of a row meet rows' zeros
 #pragma unroll
     for (int c = 0; c < CH; c++) {
-      const int chunk = step * CH + c, kb = chunk * S + lg * (S / 4);
-      const int gi = min(chunk, (g.K - 1) / S) / per;
+      const int chunk = step * CH + c;
+      const uint32_t at = min(uint32_t(chunk) * (S / 2) + uint32_t(lg) * (S / 8), qrow - S / 8);
+      const int32_t *sg = sw + size_t(min(chunk, last) / per) * g.N;
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        __builtin_memcpy(h.b[c][t], __builtin_assume_aligned(qw + (qo[t] + at), S / 8), 4 * ND);
+        h.s[c][t] = sg[so[t]];
+      }
+    }
+  };
+  // Every wave's loads have landed, those into LDS (which the compiler does not wait for
+  // at a barrier) among them, and the last step's operands are done with.
+  auto arrived = [&](Ahead &h) __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int c = 0; c < CH; c++)
+#pragma unroll
+      for (int t = 0; t < NT; t++) {  // here, so that their use does not wait for the loads that leave next
+        asm volatile("" : "+v"(h.s[c][t]));
+#pragma unroll
+        for (int d = 0; d < ND; d++) asm volatile("" : "+v"(h.b[c][t][d]));
+      }
+  };
+  auto compute = [&](const v4i_t *as, const Ahead &h) __attribute__((always_inline)) {
+    const v4i_t *buf = as + (wave >> 1) * MT * 128;
+#pragma unroll
+    for (int c = 0; c < CH; c++) {
       uint32_t ae[MT][ND], ao[MT][ND];
 #pragma unroll
       for (int i = 0; i < MT; i++) {
-        const uint4 *a = buf + ((wave >> 1) * MT + i) * 128 + c * S;
+        const v4i_t *a = buf + i * 128 + c * S;
         if constexpr (S == 32) {
           const uint2 v = reinterpret_cast<const uint2 *>(a)[lane];
           ae[i][0] = v.x, ao[i][0] = v.y;
         } else {
 #pragma unroll
           for (int o = 0; o < ND / 2; o++) {
-            const uint4 v = a[64 * o + lane];
-            ae[i][2 * o] = v.x, ae[i][2 * o + 1] = v.y, ao[i][2 * o] = v.z, ao[i][2 * o + 1] = v.w;
+            const v4i_t v = a[64 * o + lane];
+            ae[i][2 * o] = v[0], ae[i][2 * o + 1] = v[1], ao[i][2 * o] = v[2], ao[i][2 * o + 1] = v[3];
           }
         }
       }
@@ -257,22 +327,37 @@ __global__ __launch_bounds__(256) void k_q4_many(Q4Args<T> g, int steps, const u
       for (int t = 0; t < NT; t++) {
         uint32_t be[ND], bo[ND];
 #pragma unroll
-        for (int d = 0; d < ND; d++) be[d] = 0;
-        if (size_t(kb) < 2 * qrow) __builtin_memcpy(be, q[t] + kb / 2, 4 * ND);
-        const int32_t scale = g.scale[size_t(gi) * g.N + nc[t]];
+        for (int d = 0; d < ND; d++) be[d] = q4_lo(h.b[c][t][d]), bo[d] = q4_hi(h.b[c][t][d]);
+        v4i_t acc[MT];
 #pragma unroll
-        for (int d = 0; d < ND; d++) bo[d] = q4_hi(be[d]), be[d] = q4_lo(be[d]);
+        for (int i = 0; i < MT; i++) acc[i] = q4_product<S>(ae[i], ao[i], be, bo);
+        const int32_t high = Q4Sum<T>::high(h.s[c][t]), low = h.s[c][t] - int32_t(uint32_t(high) << 12);
 #pragma unroll
-        for (int i = 0; i < MT; i++) out[i][t] += q4_fold<T>(q4_product<S>(ae[i], ao[i], be, bo), scale);
+        for (int i = 0; i < MT; i++) out[i][t].add(acc[i], low);
+        if (__any(high)) {
+#pragma unroll
+          for (int i = 0; i < MT; i++) out[i][t].add_high(acc[i], high);
+        }
       }
     }
+  };
+  Ahead x, y;
+  load(as0, 0, x);
+  for (int step = 0; step < steps; step += 2) {
+    arrived(x);
+    load(as1, step + 1, y);
+    compute(as0, x);
+    if (step + 1 >= steps) break;
+    arrived(y);
+    load(as0, step + 2, x);
+    compute(as1, y);
   }
 #pragma unroll
   for (int i = 0; i < MT; i++)
 #pragma unroll
     for (int t = 0; t < NT; t++) {
       const int n = n0 + 16 * t + li;
-      T v = out[i][t];
+      T v = out[i][t].word();
       int r = lg;
       if constexpr (sizeof(T) == 8) {
         v += __shfl_xor(v, 16, 64) << 32;  // the planes above, from lane group lg + 1
@@ -292,7 +377,7 @@ int many_tiles(int M) {
   return (M + wg - 1) / wg * 2 * kManyMT;
 }
 int many_steps(int K) { return (K + 127) / 128; }
-bool few_rows(int M, int) { return M <= 16; }
+bool few_rows(int M, int) { return M <= 64; }
 
 template <typename T, int S>
 hipError_t launch_at(const Launch &L, const Q4Args<T> &g) {
@@ -323,7 +408,9 @@ hipError_t launch_at(const Launch &L, const Q4Args<T> &g) {
     return hipGetLastError();
   };
   const size_t rows = size_t(tiles / (2 * kManyMT));
-  if ((size_t(g.N) + 127) / 128 * rows >= size_t(L.num_cu) * 2) return many(std::integral_constant<int, 4>{});
+  constexpr int kWideNT = S == 32 ? 2 : 4;
+  if ((size_t(g.N) + 32 * kWideNT - 1) / (32 * kWideNT) * rows >= size_t(L.num_cu) * 2)
+    return many(std::integral_constant<int, kWideNT>{});
   return many(std::integral_constant<int, 1>{});
 }
 
@@ -336,6 +423,7 @@ size_t q4_work_bytes(int bw, int M, int K) {
 
 template <typename T>
 hipError_t launch_gemm_q4(const Launch &L, const Q4Args<T> &g) {
+  if (g.K > kQ4MaxK) return hipErrorInvalidValue;
   if (g.group % 128 == 0) return launch_at<T, 128>(L, g);
   if (g.group % 64 == 0) return launch_at<T, 64>(L, g);
   return launch_at<T, 32>(L, g);

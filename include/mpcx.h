@@ -339,7 +339,7 @@ mpcx_status mpcx_ring_lincomb(mpcx_ctx *ctx, size_t rows, size_t cols, uint64_t 
  * (K + 31) / 32 * 16 bytes, weight k of a row two's complement (-8..7) in the low
  * (k even) or high (k odd) half of byte k / 2; the halves past K are not used.
  * d_scale: ceil(K / group) rows of N int32 steps, at the scale of the weights;
- * group a multiple of 32.  d_c: M rows of N words, ldc >= N words apart.  d_q is
+ * group a multiple of 32; K up to 2^24.  d_c: M rows of N words, ldc >= N words apart.  d_q is
  * 16-byte aligned.  d_work: mpcx_ring_gemm_q4_work_bytes bytes, 16-byte aligned,
  * in use until the stream has reached the call (NULL where that is 0). */
 size_t mpcx_ring_gemm_q4_work_bytes(mpcx_ctx *ctx, int M, int K);
