@@ -108,41 +108,58 @@ __device__ __forceinline__ void plane8(const T (&w)[8], int p, uint32_t *even, u
 
 // ---------------------------------------------------------------------------
 // Few rows: a workgroup takes 16 columns and MT MFMA tiles of rows; its waves take
-// the chunks of K in turn and add up their sums through LDS.  A lane forms its
-// digits from the words themselves (each word's planes are the rows li of its tile).
+// the chunks of K in turn and add up their sums through LDS.  DIRECT: a lane forms its
+// digits from the words themselves (a word's planes are the rows li of its tile, so each
+// word is taken apart once for every plane and column tile); else from the workspace.
 // ---------------------------------------------------------------------------
-template <typename T, int S, int MT>
-__global__ __launch_bounds__(1024) void k_q4_few(Q4Args<T> g, bool vec) {
+template <typename T, int S, int MT, bool DIRECT>
+__global__ __launch_bounds__(1024) void k_q4_few(Q4Args<T> g, bool vec, int steps) {
   constexpr int R = kRows<T>, NP = int(sizeof(T)), ND = S / 32;
   __shared__ T red[16][MT][64];
-  const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6, waves = int(blockDim.x) >> 6;
+  const int tid = int(threadIdx.x), lane = tid & 63, waves = int(blockDim.x) >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int li = lane & 15, lg = lane >> 4, p = li % NP;
   const int n = int(blockIdx.x) * 16 + li, nc = n < g.N ? n : g.N - 1;
   const int m0 = int(blockIdx.y) * MT * R;
   const size_t qrow = (size_t(g.K) + 31) / 32 * 16;
-  const uint8_t *q = g.q + size_t(nc) * qrow;
+  const uint8_t *q = g.q + size_t(nc) * qrow + lg * (S / 8);
   const int chunks = (g.K + S - 1) / S, per = g.group / S;
   T out[MT];
 #pragma unroll
   for (int t = 0; t < MT; t++) out[t] = 0;
+  const uint8_t *frag = static_cast<const uint8_t *>(g.work) + size_t(blockIdx.y) * MT * steps * 2048;
+#pragma unroll 2
   for (int c = wave; c < chunks; c += waves) {
     const int kb = c * S + lg * (S / 4);  // this lane's first k
     uint32_t be[ND], bo[ND];
-#pragma unroll
-    for (int d = 0; d < ND; d++) be[d] = 0;
-    if (size_t(kb) < 2 * qrow) __builtin_memcpy(be, q + kb / 2, 4 * ND);
+    // weights past the end of a row meet rows' zeros
+    __builtin_memcpy(be, __builtin_assume_aligned(q + min(size_t(c) * (S / 2), qrow - S / 8 - lg * (S / 8)), S / 8), 4 * ND);
     const int32_t scale = g.scale[size_t(c / per) * g.N + nc];
 #pragma unroll
     for (int d = 0; d < ND; d++) bo[d] = q4_hi(be[d]), be[d] = q4_lo(be[d]);
 #pragma unroll
     for (int t = 0; t < MT; t++) {
-      const int m = m0 + t * R + li / NP;
       uint32_t ae[ND], ao[ND];
+      if constexpr (DIRECT) {
+        const int m = m0 + t * R + li / NP;
 #pragma unroll
-      for (int d = 0; d < ND; d++) {
-        T w[8];
-        load8<T>(g.a + size_t(m < g.M ? m : 0) * g.lda + kb + 8 * d, m < g.M ? g.K - kb - 8 * d : 0, vec, w);
-        plane8<T>(w, p, &ae[d], &ao[d]);
+        for (int d = 0; d < ND; d++) {
+          T w[8];
+          load8<T>(g.a + size_t(m < g.M ? m : 0) * g.lda + kb + 8 * d, m < g.M ? g.K - kb - 8 * d : 0, vec, w);
+          plane8<T>(w, p, &ae[d], &ao[d]);
+        }
+      } else {
+        const uint8_t *f = frag + size_t(t) * steps * 2048 + size_t(c) * (16 * S);
+        if constexpr (S == 32) {
+          const uint2 v = reinterpret_cast<const uint2 *>(f)[lane];
+          ae[0] = v.x, ao[0] = v.y;
+        } else {
+#pragma unroll
+          for (int o = 0; o < ND / 2; o++) {
+            const v4i_t v = reinterpret_cast<const v4i_t *>(f)[64 * o + lane];
+            ae[2 * o] = v[0], ae[2 * o + 1] = v[1], ao[2 * o] = v[2], ao[2 * o + 1] = v[3];
+          }
+        }
       }
       out[t] += q4_fold<T>(q4_product<S>(ae, ao, be, bo), scale);
     }
@@ -370,36 +387,50 @@ __global__ __launch_bounds__(256, 2) void k_q4_many(Q4Args<T> g, int steps, cons
 }
 
 constexpr int kManyMT = 4;
-// rows of MFMA tiles in the workspace: whole workgroups
 template <typename T>
-int many_tiles(int M) {
-  const int wg = 2 * kManyMT * kRows<T>;
-  return (M + wg - 1) / wg * 2 * kManyMT;
+int row_tiles(int M) {
+  return (M + kRows<T> - 1) / kRows<T>;
+}
+// tiles in the workspace: whole workgroups of either kernel
+template <typename T>
+int work_tiles(int M) {
+  return (row_tiles<T>(M) + 2 * kManyMT - 1) / (2 * kManyMT) * 2 * kManyMT;
 }
 int many_steps(int K) { return (K + 127) / 128; }
-bool few_rows(int M, int) { return M <= 64; }
+constexpr int kFewM = 64;
+template <typename T>
+bool direct_rows(int M, int K, int N) {
+  return M <= kFewM && size_t(row_tiles<T>(M)) * K * ((size_t(N) + 15) / 16) <= (sizeof(T) == 4 ? size_t(1) << 20 : size_t(1) << 19);
+}
 
 template <typename T, int S>
 hipError_t launch_at(const Launch &L, const Q4Args<T> &g) {
   const bool vec = reinterpret_cast<uintptr_t>(g.a) % 16 == 0 && g.lda % (16 / sizeof(T)) == 0;
-  constexpr int R = kRows<T>;
-  if (few_rows(g.M, g.K)) {
-    const int chunks = (g.K + S - 1) / S, waves = chunks < 16 ? chunks : 16;
-    const int tiles = (g.M + R - 1) / R, mt = tiles >= 4 ? 4 : tiles >= 2 ? 2 : 1;
-    const dim3 grid(unsigned((size_t(g.N) + 15) / 16), unsigned((tiles + mt - 1) / mt)), block(64u * unsigned(waves));
-    if (mt == 4) hipLaunchKernelGGL((k_q4_few<T, S, 4>), grid, block, 0, L.stream, g, vec);
-    else if (mt == 2) hipLaunchKernelGGL((k_q4_few<T, S, 2>), grid, block, 0, L.stream, g, vec);
-    else hipLaunchKernelGGL((k_q4_few<T, S, 1>), grid, block, 0, L.stream, g, vec);
-    return hipGetLastError();
-  }
-  const int tiles = many_tiles<T>(g.M), steps = many_steps(g.K);
+  const bool direct = direct_rows<T>(g.M, g.K, g.N);
+  const int tiles = work_tiles<T>(g.M), steps = many_steps(g.K);
   uint8_t *work = static_cast<uint8_t *>(g.work);
-  const size_t groups = size_t(tiles) * R * steps * 16;
-  const size_t want = (groups + 255) / 256, cap = size_t(L.num_cu) * 32;
-  hipLaunchKernelGGL((k_q4_digits<T, S>), dim3(unsigned(want < cap ? want : cap)), dim3(256), 0, L.stream, g, vec, tiles,
-                     steps, work);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  if (!direct) {
+    const size_t groups = size_t(tiles) * kRows<T> * steps * 16;
+    const size_t want = (groups + 255) / 256, cap = size_t(L.num_cu) * 32;
+    hipLaunchKernelGGL((k_q4_digits<T, S>), dim3(unsigned(want < cap ? want : cap)), dim3(256), 0, L.stream, g, vec, tiles,
+                       steps, work);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  if (g.M <= kFewM) {
+    const int chunks = (g.K + S - 1) / S, waves = chunks < 16 ? chunks : 16;
+    const int rt = row_tiles<T>(g.M);
+    auto few = [&](auto mt) {
+      constexpr int MT = decltype(mt)::value;
+      const dim3 grid(unsigned((size_t(g.N) + 15) / 16), unsigned((rt + MT - 1) / MT)), block(64u * unsigned(waves));
+      if (direct) hipLaunchKernelGGL((k_q4_few<T, S, MT, true>), grid, block, 0, L.stream, g, vec, steps);
+      else hipLaunchKernelGGL((k_q4_few<T, S, MT, false>), grid, block, 0, L.stream, g, vec, steps);
+      return hipGetLastError();
+    };
+    if (rt >= 3) return few(std::integral_constant<int, 4>{});
+    if (rt == 2) return few(std::integral_constant<int, 2>{});
+    return few(std::integral_constant<int, 1>{});
+  }
   auto many = [&](auto nt) {
     constexpr int NT = decltype(nt)::value;
     const size_t wgs = (size_t(g.N) + 32 * NT - 1) / (32 * NT) * size_t(tiles / (2 * kManyMT));
@@ -417,8 +448,7 @@ hipError_t launch_at(const Launch &L, const Q4Args<T> &g) {
 }  // namespace
 
 size_t q4_work_bytes(int bw, int M, int K) {
-  if (few_rows(M, K)) return 0;
-  return size_t(bw == 32 ? many_tiles<uint32_t>(M) : many_tiles<uint64_t>(M)) * many_steps(K) * 2048;
+  return size_t(bw == 32 ? work_tiles<uint32_t>(M) : work_tiles<uint64_t>(M)) * many_steps(K) * 2048;
 }
 
 template <typename T>
