@@ -11,47 +11,110 @@
 namespace mpcx {
 
 // ---------------------------------------------------------------------------
-// Rows into the cache: workgroup row y = plane, one thread per pair of words.
+// Rows into the cache: one thread per group of G words of a token's row (16 bytes where
+// every row and table is aligned to them), one row of workgroups per plane.  A rotated
+// word needs its partner too, which the neighbouring thread or one half a rotation away
+// reads as its own: the second read is served by the caches.
 // ---------------------------------------------------------------------------
-template <typename T>
+template <typename T, int G>
+struct Words {
+  T w[G];
+};
+template <typename T, int G>
+__device__ __forceinline__ Words<T, G> load_words(const T *p) {
+  Words<T, G> r;
+  __builtin_memcpy(r.w, __builtin_assume_aligned(p, sizeof(T) * G), sizeof(T) * G);
+  return r;
+}
+template <typename T, int G>
 __global__ __launch_bounds__(256) void k_cache_append(AppendArgs<T> g) {
   const int p = int(blockIdx.y);
   const T *rows = g.rows[p];
   T *pool = g.pool[p];
+  const size_t ld = g.ld[p];
   const bool rot = g.rotate[p];
-  const size_t row = size_t(g.c.heads) * g.c.dim, n = g.n_tok * row;
-  for (size_t e = size_t(blockIdx.x) * 256 + threadIdx.x; e < n; e += size_t(gridDim.x) * 256) {
-    const size_t t = e / row;
-    const int h = int(e % row) / g.c.dim, i = int(e % row) % g.c.dim;
-    const int64_t slot = g.slot[t];
-    if (slot < 0 || slot >= g.c.n_pages * g.c.page) continue;
-    const T *x = rows + t * g.ld[p] + size_t(h) * g.c.dim;
-    T v = x[i];
+  const uint32_t per_head = uint32_t(g.c.dim) / G, row = per_head * uint32_t(g.c.heads);
+  const uint64_t slots = uint64_t(g.c.n_pages) * uint64_t(g.c.page);
+  // this thread's place (token, group of the row), and the grid's stride as one
+  const size_t first = size_t(blockIdx.x) * 256 + threadIdx.x, stride = size_t(gridDim.x) * 256;
+  size_t t = first / row;
+  uint32_t r = uint32_t(first - t * row);
+  const size_t step_t = stride / row;
+  const uint32_t step_r = uint32_t(stride - step_t * row);
+  for (; t < g.n_tok; t += step_t, r += step_r) {
+    if (r >= row) {
+      r -= row;
+      if (++t >= g.n_tok) break;
+    }
+    const uint64_t slot = uint64_t(g.slot[t]);
+    if (slot >= slots) continue;  // a negative slot, too
+    const uint32_t h = r / per_head;
+    const int i = int(r - h * per_head) * G;
+    const T *x = rows + t * ld + size_t(h) * g.c.dim;
+    Words<T, G> v = load_words<T, G>(x + i);
     if (rot) {
       const int at = g.pos[t];
       if (at < 0 || at >= g.n_pos) continue;
+      const T *ct = g.cos + size_t(at) * g.half, *st = g.sin + size_t(at) * g.half;
       if (i >= 2 * g.half) {
-        v <<= g.shift;
+#pragma unroll
+        for (int k = 0; k < G; k++) v.w[k] <<= g.shift;
+      } else if (g.pairs) {
+        if constexpr (G == 1) {
+          const T o = x[i ^ 1], c = ct[i / 2], s = st[i / 2];
+          v.w[0] = i & 1 ? T(s * o + c * v.w[0]) : T(c * v.w[0] - s * o);
+        } else {
+          const Words<T, G / 2> c = load_words<T, G / 2>(ct + i / 2), s = load_words<T, G / 2>(st + i / 2);
+#pragma unroll
+          for (int k = 0; k < G; k += 2) {
+            const T a = v.w[k], b = v.w[k + 1];
+            v.w[k] = c.w[k / 2] * a - s.w[k / 2] * b;
+            v.w[k + 1] = s.w[k / 2] * a + c.w[k / 2] * b;
+          }
+        }
       } else {
-        const bool second = g.pairs ? (i & 1) : i >= g.half;
-        const int f = g.pairs ? i >> 1 : (second ? i - g.half : i);
-        const T c = g.cos[size_t(at) * g.half + f], s = g.sin[size_t(at) * g.half + f];
-        const T o = x[g.pairs ? i ^ 1 : (second ? i - g.half : i + g.half)];
-        v = second ? T(s * o + c * v) : T(c * v - s * o);
+        const bool second = i >= g.half;
+        const int f = second ? i - g.half : i;
+        const Words<T, G> c = load_words<T, G>(ct + f), s = load_words<T, G>(st + f);
+        const Words<T, G> o = load_words<T, G>(x + (second ? f : f + g.half));
+#pragma unroll
+        for (int k = 0; k < G; k++)
+          v.w[k] = second ? T(s.w[k] * o.w[k] + c.w[k] * v.w[k]) : T(c.w[k] * v.w[k] - s.w[k] * o.w[k]);
       }
     }
-    const size_t page = size_t(slot / g.c.page), in = size_t(slot % g.c.page);
-    pool[((page * g.c.heads + h) * g.c.page + in) * g.c.dim + i] = v;
+    const uint64_t page = slots >> 32 ? slot / uint64_t(g.c.page) : uint64_t(uint32_t(slot) / uint32_t(g.c.page));
+    const uint64_t in = slot - page * uint64_t(g.c.page);
+    T *to = pool + ((page * g.c.heads + h) * g.c.page + in) * g.c.dim + i;
+    __builtin_memcpy(__builtin_assume_aligned(to, sizeof(T) * G), v.w, sizeof(T) * G);
   }
 }
 
-template <typename T>
-hipError_t launch_cache_append(const Launch &L, const AppendArgs<T> &g) {
-  const size_t n = g.n_tok * g.c.heads * g.c.dim;
-  const size_t want = (n + 255) / 256, cap = size_t(L.num_cu) * 64;
-  hipLaunchKernelGGL(k_cache_append<T>, dim3(unsigned(want < cap ? want : cap), unsigned(g.n_planes)), dim3(256), 0,
+template <typename T, int G>
+hipError_t append_at(const Launch &L, const AppendArgs<T> &g) {
+  const size_t n = g.n_tok * size_t(g.c.heads) * (size_t(g.c.dim) / G);
+  const size_t want = (n + 255) / 256, cap = size_t(L.num_cu) * 32;
+  hipLaunchKernelGGL((k_cache_append<T, G>), dim3(unsigned(want < cap ? want : cap), unsigned(g.n_planes)), dim3(256), 0,
                      L.stream, g);
   return hipGetLastError();
+}
+template <typename T>
+hipError_t launch_cache_append(const Launch &L, const AppendArgs<T> &g) {
+  constexpr int G = 16 / int(sizeof(T));
+  bool vec = g.c.dim % G == 0;
+  auto check = [&](const void *p) { vec = vec && reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  bool rot = false;
+  for (int p = 0; p < g.n_planes; p++) {
+    check(g.rows[p]);
+    check(g.pool[p]);
+    vec = vec && g.ld[p] % G == 0;
+    rot = rot || g.rotate[p];
+  }
+  if (rot) {  // a table row starts at a whole group, or half of one
+    vec = vec && g.half % (g.pairs ? G / 2 : G) == 0;
+    check(g.cos);
+    check(g.sin);
+  }
+  return vec ? append_at<T, G>(L, g) : append_at<T, 1>(L, g);
 }
 
 // ---------------------------------------------------------------------------

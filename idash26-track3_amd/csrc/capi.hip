@@ -1032,11 +1032,11 @@ mpcx_status mpcx_ring_gemm_q4(mpcx_ctx *c, int M, int K, int N, int group, const
                      : gemm_q4_t<uint64_t>(c, M, K, N, group, a, lda, q, scale, out, ldc, work);
 }
 
-// The cache's sizes are positive and its words countable in 60 bits.
+// The cache's sizes are positive, a token's words countable in 31 bits and all in 60.
 static bool valid_cache(const mpcx_cache &k) {
   if (k.n_heads < 1 || k.head_dim < 1 || k.page_size < 1 || k.n_pages < 1) return false;
   const unsigned __int128 words = (unsigned __int128)(k.n_heads) * k.head_dim * k.page_size * (uint64_t)k.n_pages;
-  return words < (unsigned __int128)1 << 60;
+  return words < (unsigned __int128)1 << 60 && int64_t(k.n_heads) * k.head_dim < int64_t(1) << 31;
 }
 static CacheDims cache_dims(const mpcx_cache &k) {
   CacheDims d;

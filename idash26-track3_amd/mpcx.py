@@ -596,19 +596,22 @@ class Ctx:
     def _enter(self):
         cur = _torch().cuda.current_stream()
         s = getattr(self, "_stream", None)
-        same = s is not None and s.cuda_stream != 0 and s.cuda_stream == cur.cuda_stream
-        if not same:
-            cur.synchronize()
-        return same
+        if s is not None and s.cuda_stream == cur.cuda_stream != 0:
+            return True
+        cur.synchronize()
+        return False
 
     def _leave(self, same):
         if not same:
             self.sync()
 
+    @property
+    def _word(self):
+        return _torch().int32 if self.bw == 32 else _torch().int64
+
     def _words(self, t, what, shape=None):
         """A contiguous ring tensor's address."""
-        torch = _torch()
-        if t.dtype != (torch.int32 if self.bw == 32 else torch.int64) or not t.is_cuda or not t.is_contiguous():
+        if t.dtype is not self._word or not t.is_cuda or not t.is_contiguous():
             raise MpcxError(f"{what}: need a contiguous int{self.bw} tensor on the GPU")
         if shape is not None and t.shape != shape:
             raise MpcxError(f"{what}: shape {tuple(t.shape)}, need {tuple(shape)}")
@@ -616,26 +619,29 @@ class Ctx:
 
     @staticmethod
     def _ints(t, what, dtype, shape):
-        if t.dtype != dtype or not t.is_cuda or not t.is_contiguous() or t.shape != shape:
+        if t.dtype is not dtype or t.shape != shape or not t.is_cuda or not t.is_contiguous():
             raise MpcxError(f"{what}: need a contiguous {dtype} tensor of shape {tuple(shape)} on the GPU")
         return t.data_ptr()
 
     def _new(self, shape):
-        torch = _torch()
-        return torch.empty(shape, dtype=torch.int32 if self.bw == 32 else torch.int64, device="cuda")
+        return _torch().empty(shape, dtype=self._word, device="cuda")
+
+    def _rows(self, t, what):
+        """A matrix of ring words whose rows may be apart: its address and row stride."""
+        if t.dtype is not self._word or not t.is_cuda or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+            raise MpcxError(f"{what}: need int{self.bw} rows on the GPU")
+        return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
     def ring_gemm_q4(self, a, q, scale, group, out=None):
         """mpcx_ring_gemm_q4: a (M, K) ring words (rows may be apart), q (N, rows of
         whole 32 weights) uint8, scale (groups, N) int32 -> (M, N)."""
         torch = _torch()
+        ap, lda = self._rows(a, "ring_gemm_q4: a")
         M, K = a.shape
         N = q.shape[0]
         if out is None:
             out = self._new((M, N))
-        for t, n in ((a, "a"), (out, "out")):
-            if t.dtype != out.dtype or t.dtype.itemsize * 8 != self.bw or not t.is_cuda or t.dim() != 2 or \
-                    (t.shape[1] > 1 and t.stride(1) != 1):
-                raise MpcxError(f"ring_gemm_q4: {n}: need int{self.bw} rows on the GPU")
+        op, ldc = self._rows(out, "ring_gemm_q4: out")
         if out.shape != (M, N):
             raise MpcxError(f"ring_gemm_q4: out: shape {tuple(out.shape)}, need {(M, N)}")
         qp = self._ints(q, "ring_gemm_q4: q", torch.uint8, (N, (K + 31) // 32 * 16))
@@ -645,15 +651,15 @@ class Ctx:
         nb = self.lib.mpcx_ring_gemm_q4_work_bytes(self.h, M, K)
         work = torch.empty(nb, dtype=torch.uint8, device="cuda") if nb else None
         same = self._enter()
-        self.check(self.lib.mpcx_ring_gemm_q4(self.h, M, K, N, group, a.data_ptr(), a.stride(0) if M > 1 else K, qp, sp,
-                                              out.data_ptr(), out.stride(0) if M > 1 else N,
+        self.check(self.lib.mpcx_ring_gemm_q4(self.h, M, K, N, group, ap, lda, qp, sp, op, ldc,
                                               work.data_ptr() if nb else None), "ring_gemm_q4")
         self._leave(same)
         return out
 
     @staticmethod
     def _cache(pool):
-        return Cache(pool.shape[1], pool.shape[3], pool.shape[2], pool.shape[0])
+        n, heads, page, dim = pool.shape
+        return Cache(heads, dim, page, n)
 
     def cache_append(self, planes, slot, pos=None, rotation=None):
         """mpcx_cache_append: planes is a list of (rows, pool, rotate), rows (tokens,
@@ -661,26 +667,28 @@ class Ctx:
         dim); slot (tokens) int64, pos (tokens) int32, rotation a Rotation."""
         torch = _torch()
         n = slot.shape[0]
-        pool = planes[0][1]
-        shape = (n, pool.shape[1], pool.shape[3])
+        pool = planes[0][1].shape
+        shape, near = (n, pool[1], pool[3]), (pool[3], 1)
         sp = self._ints(slot, "cache_append: slot", torch.int64, (n,))
         pp = self._ints(pos, "cache_append: pos", torch.int32, (n,)) if pos is not None else None
         arr = (_CachePlane * len(planes))()
-        for i, (r, p, rotate) in enumerate(planes):
-            self._words(p, "cache_append: pool", pool.shape)
-            if r.shape != shape or r.dtype != p.dtype or not r.is_cuda or \
-                    (n and (r[0].stride() != (shape[2], 1) and not r[0].is_contiguous())):
+        for a, (r, p, rotate) in zip(arr, planes):
+            a.d_pool = self._words(p, "cache_append: pool", pool)
+            if r.shape != shape or r.dtype is not p.dtype or not r.is_cuda or \
+                    (r.stride()[1:] != near and not r.is_contiguous()):
                 raise MpcxError(f"cache_append: rows: need int{self.bw} rows of shape {shape} on the GPU")
-            arr[i] = _CachePlane(r.data_ptr(), r.stride(0) if n > 1 else shape[1] * shape[2], p.data_ptr(), int(rotate))
+            a.d_rows = r.data_ptr()
+            a.ld = r.stride(0) if n > 1 else shape[1] * shape[2]
+            a.rotate = rotate
         rot = None
         if rotation is not None:
             c = rotation.cos
-            rot = _Rotation(c.shape[1], int(rotation.pairs), c.shape[0], rotation.shift,
-                            self._words(c, "cache_append: cos"), self._words(rotation.sin, "cache_append: sin", c.shape))
+            rot = C.byref(_Rotation(c.shape[1], int(rotation.pairs), c.shape[0], rotation.shift,
+                                    self._words(c, "cache_append: cos"),
+                                    self._words(rotation.sin, "cache_append: sin", c.shape)))
         same = self._enter()
-        self.check(self.lib.mpcx_cache_append(self.h, C.byref(self._cache(pool)), n, sp, pp,
-                                              C.byref(rot) if rot is not None else None, len(planes), arr),
-                   "cache_append")
+        self.check(self.lib.mpcx_cache_append(self.h, C.byref(Cache(pool[1], pool[3], pool[2], pool[0])), n, sp, pp, rot,
+                                              len(planes), arr), "cache_append")
         self._leave(same)
 
     def split_mask(self, mask, seed=1, gate=1):

@@ -349,7 +349,8 @@ mpcx_status mpcx_ring_gemm_q4(mpcx_ctx *ctx, int M, int K, int N, int group, con
 /* A paged cache: n_pages pages of page_size slots for each of n_heads key /
  * value heads of head_dim words.  One plane (masked keys, a party's share of
  * their mask, ...) is an array [n_pages][n_heads][page_size][head_dim] of ring
- * words; slot s of the cache is slot s % page_size of page s / page_size. */
+ * words; slot s of the cache is slot s % page_size of page s / page_size.
+ * n_heads * head_dim is below 2^31. */
 typedef struct {
   int n_heads, head_dim, page_size;
   int64_t n_pages;
