@@ -691,6 +691,28 @@ class Ctx:
                                               len(planes), arr), "cache_append")
         self._leave(same)
 
+    def gate_keygen(self, kind, mask, seed=1, gate=1):
+        """tr_keygen on a mask tensor: the parties' keys and the output mask, shaped as
+        the input's."""
+        n = mask.numel()
+        nb = self.lib.mpcx_tr_key_bytes(self.h, kind, n)
+        k0, k1, out = empty_dev(nb), empty_dev(nb), self._new(mask.shape)
+        mp = self._words(mask, "gate_keygen")
+        same = self._enter()
+        self.check(self.lib.mpcx_tr_keygen(self.h, kind, n, mp, out.data_ptr(), seed, gate, dptr(k0), dptr(k1)),
+                   "tr_keygen")
+        self._leave(same)
+        return k0, k1, out
+
+    def gate_eval(self, kind, k0, k1, xhat):
+        """tr_eval on a tensor of masked words."""
+        out, xp = self._new(xhat.shape), self._words(xhat, "gate_eval")
+        same = self._enter()
+        self.check(self.lib.mpcx_tr_eval(self.h, kind, xhat.numel(), dptr(k0), dptr(k1), xp, None, 0, out.data_ptr()),
+                   "tr_eval")
+        self._leave(same)
+        return out
+
     def split_mask(self, mask, seed=1, gate=1):
         """mpcx_split_mask: both parties' shares of a mask tensor."""
         s0, s1 = self._new(mask.shape), self._new(mask.shape)

@@ -618,3 +618,63 @@ def test_binding_refusals(ctx):
                        ([(rows, pool.to(other), False)], slot), ([(rows, pool, True)], slot)):
         with pytest.raises(mpcx.MpcxError):
             ctx.cache_append(planes, at)
+
+
+# ---------------- together, and one party at a time ----------------
+@pytest.mark.parametrize("bw", [32, 64])
+def test_attention_layer(bw):
+    """The operators in one layer, prompt and single tokens, with the framework's
+    truncation and ReLU gates between: the plain fixed-point layer bit for bit."""
+    import attention
+    said = []
+    assert attention.run(bw, say=said.append), said
+    assert len(said) == 5
+
+
+def test_parties_reconstruct_the_gates(ctx):
+    """Each party's message from its own key and shares, exchanged over a channel:
+    both hold the gate's output."""
+    import threading
+    torch = _torch()
+    B = Batch(ctx.bw, 2, 5, 30, 4, 2, 24, 8, "prefix", seed=8)
+    g, planes = B.gpu(), [dev(v) for v in (B.y, B.b0, B.b1)]
+    q, p = dev(words(B.rng, (B.tokens, 4, 24), ctx.bw)), dev(words(B.rng, (B.n,), ctx.bw))
+    slope, pos = dev(words(B.rng, (4,), ctx.bw)), dev(B.pos)
+    ks = ctx.attn_scores_keygen(g, q, planes[1], planes[2])
+    km = ctx.attn_mix_keygen(g, p, planes[1], planes[2])
+    want = [host(ctx.attn_scores_eval(g, ks[0], ks[1], q, *planes, slope=slope, pos=pos), ctx.bw),
+            host(ctx.attn_mix_eval(g, km[0], km[1], p, *planes), ctx.bw).reshape(-1)]
+    peers, got, errors = mpcx.Peer.pair(), {}, []
+
+    def party(i):
+        try:
+            c = mpcx.Ctx(bw=ctx.bw, scale=12)
+            s = c.attn_scores_message(i, g, ks[i], q, planes[0], planes[1 + i], slope=slope, pos=pos)
+            o = c.attn_mix_message(i, g, km[i], p, planes[0], planes[1 + i])
+            got[i] = [c.party_reconstruct(peers[i], host(v, ctx.bw).reshape(-1)) for v in (s, o)]
+            c.close()
+        except Exception as e:  # a thread's failure is the test's
+            errors.append(e)
+
+    threads = [threading.Thread(target=party, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not errors and len(got) == 2, errors
+    for i in (0, 1):
+        assert all(np.array_equal(a, b) for a, b in zip(got[i], want))
+    for peer in peers:
+        peer.close()
+    torch.cuda.synchronize()
+
+
+def test_sizes_past_the_bounds_are_refused(ctx):
+    L, h = ctx.lib, ctx.h
+    d = _torch().zeros(64, dtype=_torch().int64, device="cuda").data_ptr()
+    assert L.mpcx_ring_gemm_q4(h, 1, (1 << 24) + 1, 1, 32, d, (1 << 24) + 1, d, d, d, 1, d) == 1
+    a = mpcx._Attn(mpcx.Cache(1, 8, 4, 3), 1 << 16, 1 << 16, 1, 1, 1, 1, 0, d, d, d, d, d)
+    assert L.mpcx_attn_mix_eval(h, C.byref(a), d, d, d, d, d, d, d) == 1  # 2^32 rows
+    big = mpcx.Cache(1 << 16, 1 << 16, 1, 1)
+    plane = (mpcx._CachePlane * 1)(mpcx._CachePlane(d, 1 << 32, d, 0))
+    assert L.mpcx_cache_append(h, C.byref(big), 1, d, None, None, 1, plane) == 1
