@@ -722,7 +722,7 @@ hipError_t scores_at(const Launch &L, const AttnArgs<T> &g) {
   const size_t steps = size_t(g.d.c.dim + 63) / 64;
   // two tiles of rows to a workgroup where a sequence has them and LDS holds them
   if (int64_t(g.d.max_q) * m >= 32 && steps * kStepLds<F, T> * 2 <= kScoreLds)
-    return scores_rows<F, T, 2, 8>(L, g, g.d.c.dim, int64_t(L.num_cu) * 2);
+    return scores_rows<F, T, 2, sizeof(T) == 4 ? 8 : 4>(L, g, g.d.c.dim, int64_t(L.num_cu) * 2);
   const int dims = int(std::min(steps, kScoreLds / kStepLds<F, T>)) * 64;
   return scores_rows<F, T, 1, 4>(L, g, dims, int64_t(L.num_cu) * 2);
 }

@@ -220,37 +220,37 @@ template <typename T>
 struct Q4Sum;
 template <>
 struct Q4Sum<uint32_t> {
-  int32_t w[4];
+  uint32_t w[4];
   static __device__ __forceinline__ int32_t high(int32_t s) {
     return (uint32_t(s) + (1u << 23)) >> 24 ? s >> 12 : 0;
   }
   __device__ __forceinline__ void add(v4i_t a, int32_t s) {
-    w[0] += __mul24(a[0] >> 4, s);
+    w[0] += uint32_t(__mul24(a[0] >> 4, s));
 #pragma unroll
-    for (int p = 1; p < 4; p++) w[p] += __mul24(a[p], s);
+    for (int p = 1; p < 4; p++) w[p] += uint32_t(__mul24(a[p], s));
   }
   __device__ __forceinline__ void add_high(v4i_t a, int32_t s) {
 #pragma unroll
     for (int p = 0; p < 4; p++) {
       int32_t x;  // (not __mul24, whose sign extensions would move to where every scale passes)
       asm("v_mul_i32_i24_e32 %0, %1, %2" : "=v"(x) : "v"(p ? a[p] : a[0] >> 4), "v"(s));
-      w[p] += int32_t(uint32_t(x) << 12);
+      w[p] += uint32_t(x) << 12;
     }
   }
   __device__ __forceinline__ uint32_t word() const {
-    return uint32_t(w[0]) + (uint32_t(w[1]) << 4) + (uint32_t(w[2]) << 12) + (uint32_t(w[3]) << 20);
+    return w[0] + (w[1] << 4) + (w[2] << 12) + (w[3] << 20);
   }
 };
 template <>
 struct Q4Sum<uint64_t> {
-  int64_t w[2];
+  uint64_t w[2];
   __device__ __forceinline__ void add(v4i_t a, int32_t s) {
-    w[0] += int64_t((a[0] >> 4) + (a[1] << 4)) * s;
-    w[1] += int64_t((a[2] >> 4) + (a[3] << 4)) * s;
+    w[0] += uint64_t(int64_t((a[0] >> 4) + (a[1] << 4)) * s);
+    w[1] += uint64_t(int64_t((a[2] >> 4) + (a[3] << 4)) * s);
   }
   static __device__ __forceinline__ int32_t high(int32_t) { return 0; }
   __device__ __forceinline__ void add_high(v4i_t, int32_t) {}
-  __device__ __forceinline__ uint64_t word() const { return uint64_t(w[0]) + (uint64_t(w[1]) << 16); }
+  __device__ __forceinline__ uint64_t word() const { return w[0] + (w[1] << 16); }
 };
 
 // Second step: a workgroup of 2 x 2 waves, each MT tiles of rows by NT of columns.  The
