@@ -520,7 +520,6 @@ __global__ __launch_bounds__(64 * kMixWaves) void k_attn_mix(AttnArgs<T> g, Unit
   const AttnDims &d = g.d;
   const int tid = int(threadIdx.x), lane = tid & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint4 z4 = make_uint4(0u, 0u, 0u, 0u);
   const Unit u = unit_of(d, units);
   const uint32_t m = uint32_t(d.heads) / uint32_t(d.c.heads);
   const int t0 = max(d.qstart[u.b], 0), t1 = min(d.qstart[u.b + 1], d.n_tok);
@@ -716,21 +715,35 @@ hipError_t scores_rows(const Launch &L, const AttnArgs<T> &g, int dims, int64_t 
   }
   return hipSuccess;
 }
+// Two tiles of rows to a workgroup, where LDS holds them: the keys' planes are formed once
+// for both.  Z_2^32: from about one workgroup a CU on (4 prompts of 512 tokens, 8 heads of
+// 64: 45.0 us, one tile 50.4; 4 of 64 tokens against 1024 keys: 23.1, one 20.8); Z_2^64,
+// where a key's planes cost more: from 64 rows on (4 of 16 tokens, 4 heads a key: 18.1 us,
+// one 22.2; 4 of 8 tokens: 17.1, one 13.2).
+template <typename T>
+bool two_tiles(const AttnDims &d, int num_cu) {
+  const int64_t rows = int64_t(d.max_q) * (d.heads / d.c.heads);
+  if (sizeof(T) == 8) return rows >= 64;
+  return int64_t(d.n_seq) * d.c.heads * ((rows + 31) / 32) >= num_cu;
+}
 template <AttnForm F, typename T>
 hipError_t scores_at(const Launch &L, const AttnArgs<T> &g) {
-  const int m = g.d.heads / g.d.c.heads;
   const size_t steps = size_t(g.d.c.dim + 63) / 64;
-  // two tiles of rows to a workgroup where a sequence has them and LDS holds them
-  if (int64_t(g.d.max_q) * m >= 32 && steps * kStepLds<F, T> * 2 <= kScoreLds)
-    return scores_rows<F, T, 2, sizeof(T) == 4 ? 8 : 4>(L, g, g.d.c.dim, int64_t(L.num_cu) * 2);
+  const int64_t want = int64_t(L.num_cu) * 2;
+  if (steps * kStepLds<F, T> * 2 <= kScoreLds && two_tiles<T>(g.d, L.num_cu))
+    return scores_rows<F, T, 2, sizeof(T) == 4 ? 8 : 4>(L, g, g.d.c.dim, want);
   const int dims = int(std::min(steps, kScoreLds / kStepLds<F, T>)) * 64;
-  return scores_rows<F, T, 1, 4>(L, g, dims, int64_t(L.num_cu) * 2);
+  return scores_rows<F, T, 1, 4>(L, g, dims, want);
 }
 template <AttnForm F, typename T>
 hipError_t mix_at(const Launch &L, const AttnArgs<T> &g) {
   constexpr int G = 16 / int(sizeof(T));
-  const Units u =
-      units_for(g.d, (g.d.c.dim + 16 * G - 1) / (16 * G), 16, int64_t(L.num_cu), int64_t(kMixWaves) * 4 * G * 4);
+  // Keys are split down to one step a wave, but not those of four steps at most, where the
+  // second launch costs more (one token, 8 heads of 64 in Z_2^32: 2000 keys 12.4 us, split
+  // to four steps 18.8; 300 keys 10.7, split 11.9).
+  constexpr int64_t kStepKeys = int64_t(kMixWaves) * 4 * G;
+  const int64_t part = g.d.max_keys > 4 * kStepKeys ? kStepKeys : 4 * kStepKeys;
+  const Units u = units_for(g.d, (g.d.c.dim + 16 * G - 1) / (16 * G), 16, int64_t(L.num_cu), part);
   if (u.n == 0) return hipErrorInvalidValue;
   if (u.splits > 1) {
     const size_t n = size_t(g.d.n_tok) * g.d.heads * g.d.c.dim, want = (n + 255) / 256, cap = size_t(L.num_cu) * 32;

@@ -397,10 +397,14 @@ int work_tiles(int M) {
   return (row_tiles<T>(M) + 2 * kManyMT - 1) / (2 * kManyMT) * 2 * kManyMT;
 }
 int many_steps(int K) { return (K + 127) / 128; }
-constexpr int kFewM = 64;
+constexpr int kFewTiles = 16;
+template <typename T>
+bool few_rows(int M) {
+  return row_tiles<T>(M) <= kFewTiles;
+}
 template <typename T>
 bool direct_rows(int M, int K, int N) {
-  return M <= kFewM && size_t(row_tiles<T>(M)) * K * ((size_t(N) + 15) / 16) <= (sizeof(T) == 4 ? size_t(1) << 20 : size_t(1) << 19);
+  return few_rows<T>(M) && size_t(row_tiles<T>(M)) * K * ((size_t(N) + 15) / 16) <= (sizeof(T) == 4 ? size_t(1) << 20 : size_t(1) << 19);
 }
 
 template <typename T, int S>
@@ -417,7 +421,7 @@ hipError_t launch_at(const Launch &L, const Q4Args<T> &g) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  if (g.M <= kFewM) {
+  if (few_rows<T>(g.M)) {
     const int chunks = (g.K + S - 1) / S, waves = chunks < 16 ? chunks : 16;
     const int rt = row_tiles<T>(g.M);
     auto few = [&](auto mt) {
