@@ -444,7 +444,7 @@ hipError_t launch_at(const Launch &L, const Q4Args<T> &g) {
   };
   const size_t rows = size_t(tiles / (2 * kManyMT));
   constexpr int kWideNT = S == 32 ? 2 : 4;
-  if ((size_t(g.N) + 32 * kWideNT - 1) / (32 * kWideNT) * rows >= size_t(L.num_cu) * 2)
+  if ((size_t(g.N) + 32 * kWideNT - 1) / (32 * kWideNT) * rows >= size_t(L.num_cu) * (sizeof(T) == 4 ? 1 : 2))
     return many(std::integral_constant<int, kWideNT>{});
   return many(std::integral_constant<int, 1>{});
 }
