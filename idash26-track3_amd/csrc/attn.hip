@@ -14,7 +14,10 @@ namespace mpcx {
 // Rows into the cache: one thread per group of G words of a token's row (16 bytes where
 // every row and table is aligned to them), one row of workgroups per plane.  A rotated
 // word needs its partner too, which the neighbouring thread or one half a rotation away
-// reads as its own: the second read is served by the caches.
+// reads as its own: the second read is served by the caches.  Bound by the bytes, each
+// read and written once: 6000 tokens of 4 heads of 80 in Z_2^64, six planes, 47.7 us, 186
+// MB at 3.9 TB/s (a large copy reaches 4.7); word by word 76.5.  A few tokens are bound by
+// the launch (48 of 8 heads of 128: 3.7 us).
 // ---------------------------------------------------------------------------
 template <typename T, int G>
 struct Words {
@@ -308,6 +311,12 @@ __device__ __forceinline__ void group_planes(uint4 u, uint4 v, uint32_t (&o)[siz
 // next keys one tile ahead: no load waits for another.  The words of a launch are dims
 // [k0, k0 + kn) of the heads, as many as LDS holds of the queries; `more`: the sums so
 // far are in out.
+// One token a sequence is bound by the cache's bytes: 8 sequences of up to 4096 keys, 8
+// cache heads of 128 in Z_2^32: 76.8 us for 296 MB, 3.9 TB/s (equal lengths: 72 us; the
+// start, some 10 us from the first page number to the first product, and the longest
+// sequence's end are what is left).  Prompts are bound by the digits' vector instructions,
+// about as many cycles as the MFMAs at two waves a SIMD: 4 x 512 tokens, 8 heads of 64:
+// 42.2 us.
 // ---------------------------------------------------------------------------
 template <AttnForm F, typename T, bool VEC, int RT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 4 ? 2 : 1) void k_attn_scores(AttnArgs<T> g, Units units, int k0, int kn, bool more) {
@@ -506,9 +515,20 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 4 ? 2 : 1) void k_attn_sco
 // Weighted sums.  A wave takes 64 bytes of keys at a time (16 or 8): their weights as
 // the 16 rows' operand, and 256 bytes of columns of the values' rows, lane (li, lg)
 // loading group li of the rows lg G .. + G - 1, so that word q of its groups is the
-// operand of column tile q.  The waves of a workgroup and the launch's splits share
-// the keys out; their sums meet in LDS and in integer additions to the output, whose
-// order does not matter.
+// operand of column tile q.  A value's digits go to the matrix cores as its word holds
+// them, each word's bytes beside one another, and the weights' digits shifted against them
+// (digit p - s of a weight meets digit s of a value): 16 or 64 MFMAs where planes would
+// take 10 or 36, but planes would have to gather a column's bytes from four keys' rows,
+// and the MFMAs do not bound it.  The waves of a workgroup and the launch's splits share
+// the keys out; their sums meet in LDS and in integer additions to the output, whose order
+// does not matter.
+// One token a sequence is bound by the cache's bytes: 8 sequences of up to 4096 keys, 8
+// heads of 128 in Z_2^32: 68.2 us for 296 MB, 4.3 TB/s; one of 50000 keys, 4 heads: 63.1
+// us, 317 MB at 5.0 TB/s.  Prompts are bound by the digits' vector instructions, which
+// every tile of rows repeats: 3 of up to 301 tokens, 6 heads of 72 in Z_2^64: 40.2 us.
+// (Values' planes staged in LDS for eight tiles of rows were slower, for their longer
+// start: 86.8 us against 72.8 for 597 tokens and 1061 keys, 16.4 against 7.3 for 26.)
+// Eight waves: four take 94.6 us for the 8 sequences, 58.6 for the prompts.
 // ---------------------------------------------------------------------------
 constexpr int kMixWaves = 8;
 template <AttnForm F, typename T, bool VEC>
@@ -729,6 +749,8 @@ bool two_tiles(const AttnDims &d, int num_cu) {
 template <AttnForm F, typename T>
 hipError_t scores_at(const Launch &L, const AttnArgs<T> &g) {
   const size_t steps = size_t(g.d.c.dim + 63) / 64;
+  // two workgroups a CU: one takes 97.5 us for 8 tokens against up to 4096 keys each, 8
+  // cache heads of 128, two 79.5, four 78.6 but 26.2 for 21.3 for 4 x 64 against 1024
   const int64_t want = int64_t(L.num_cu) * 2;
   if (steps * kStepLds<F, T> * 2 <= kScoreLds && two_tiles<T>(g.d, L.num_cu))
     return scores_rows<F, T, 2, sizeof(T) == 4 ? 8 : 4>(L, g, g.d.c.dim, want);
@@ -738,6 +760,8 @@ hipError_t scores_at(const Launch &L, const AttnArgs<T> &g) {
 template <AttnForm F, typename T>
 hipError_t mix_at(const Launch &L, const AttnArgs<T> &g) {
   constexpr int G = 16 / int(sizeof(T));
+  // One workgroup a CU, which its registers allow: half as many take 42.0 us for 4 tokens
+  // against 6000 keys, 4 cache heads of 80 (one a CU 28.6), twice as many 32.1.
   // Keys are split down to one step a wave, but not those of four steps at most, where the
   // second launch costs more (one token, 8 heads of 64 in Z_2^32: 2000 keys 12.4 us, split
   // to four steps 18.8; 300 keys 10.7, split 11.9).

@@ -15,6 +15,12 @@
 //   sum_p 2^(8p) a_p / 16 = (a_0 >> 4) + (a_1 << 4) + (a_2 << 12) + (a_3 << 20),
 // in Z_2^64 with 64-bit sums of the pairs (a_0, a_1), (a_2, a_3), and the lanes of
 // planes 4..7 (odd lg) shifted up by 32 at the end.
+//
+// What it costs: bw / 8 int8 multiply-adds a weight and word, half a byte a weight, a
+// scale a group.  Few rows are bound by the weights' bytes and, below some 10 MB of
+// them, by a launch's start; many by the matrix cores and, beside them, by the scales'
+// multiply-adds, 5 vector instructions a chunk and tile.  The figures below are of one
+// MI355X; "rows x K x N", groups of 128 unless said.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -107,10 +113,13 @@ __device__ __forceinline__ void plane8(const T (&w)[8], int p, uint32_t *even, u
 }
 
 // ---------------------------------------------------------------------------
-// Few rows: a workgroup takes 16 columns and MT MFMA tiles of rows; its waves take
-// the chunks of K in turn and add up their sums through LDS.  DIRECT: a lane forms its
+// Few rows: a workgroup takes 16 columns and MT MFMA tiles of rows; its (up to 16) waves
+// take the chunks of K in turn and add up their sums through LDS, so that 4096 columns are
+// 4096 waves, each with a few loads of the weights in flight.  DIRECT: a lane forms its
 // digits from the words themselves (a word's planes are the rows li of its tile, so each
 // word is taken apart once for every plane and column tile); else from the workspace.
+// 1 x 4096 x 4096 in Z_2^32: 6.8 us, 9 MB of weights and scales at 1.3 TB/s, of which an
+// empty kernel is 3; 5 x 8192 x 2047 in Z_2^64, groups of 64: 12.2 us and the digits' 4.8.
 // ---------------------------------------------------------------------------
 template <typename T, int S, int MT, bool DIRECT>
 __global__ __launch_bounds__(1024) void k_q4_few(Q4Args<T> g, bool vec, int steps) {
@@ -181,9 +190,10 @@ __global__ __launch_bounds__(1024) void k_q4_few(Q4Args<T> g, bool vec, int step
 }
 
 // ---------------------------------------------------------------------------
-// Many rows, first step: the words' digits in the order the lanes take them.  The
-// workspace holds, per MFMA tile of rows and step of 128 k, 2 KB of operands:
-// 128 / S chunks of S / 64 operands (64 lanes of 16 bytes; S = 32: one of 8 bytes).
+// Digits once for all columns, in the order the lanes take them.  The workspace holds,
+// per MFMA tile of rows and step of 128 k, 2 KB of operands: 128 / S chunks of S / 64
+// operands (64 lanes of 16 bytes; S = 32: one of 8 bytes).  768 x 4096 words of Z_2^32:
+// 10.6 us, 25 MB in and out at 2.4 TB/s.
 // ---------------------------------------------------------------------------
 template <typename T, int S>
 __global__ __launch_bounds__(256) void k_q4_digits(Q4Args<T> g, bool vec, int tiles, int steps, uint8_t *work) {
@@ -253,9 +263,15 @@ struct Q4Sum<uint64_t> {
   __device__ __forceinline__ uint64_t word() const { return w[0] + (w[1] << 16); }
 };
 
-// Second step: a workgroup of 2 x 2 waves, each MT tiles of rows by NT of columns.  The
-// rows' operands of a step (128 k) go through LDS, the weights and scales straight to the
-// lanes' registers; all are asked for a step ahead.
+// Many rows: a workgroup of 2 x 2 waves, each MT tiles of rows by NT of columns.  The
+// rows' operands of a step (128 k), which every column tile shares, go straight into LDS,
+// the weights and scales, which only two waves share, to the lanes' registers (through
+// LDS, too, they took as long); all are asked for a step ahead (two ahead: as long).  Two
+// waves a SIMD (256 registers each), so that one's scales run beside the other's MFMAs.
+// 768 x 4096 x 4096 in Z_2^32: 79.9 us, 1.29 POP/s of digits against 1.8 of a large int8
+// product: vector instructions issue 44% of the time and MFMAs 26%, each waiting for the
+// other in a wave (all of a step's products in one block of code, the rare scales done over:
+// 84), and 768 workgroups at two a CU are one and a half rounds.
 template <typename T, int S, int MT, int NT>
 __global__ __launch_bounds__(256, 2) void k_q4_many(Q4Args<T> g, int steps, const uint8_t *work) {
   constexpr int R = kRows<T>, ND = S / 32, CH = 128 / S;
@@ -397,14 +413,22 @@ int work_tiles(int M) {
   return (row_tiles<T>(M) + 2 * kManyMT - 1) / (2 * kManyMT) * 2 * kManyMT;
 }
 int many_steps(int K) { return (K + 127) / 128; }
+// Up to 16 tiles of rows take the first kernel.  4096 x 4096: 64 rows of Z_2^32 21.7 us,
+// by the other 27.1; 128 rows 35.2, by the other 29.0; Z_2^64 in groups of 64: 32 rows
+// 27.5, by the other 36.6; 64 rows 45.1, by the other 39.8.
 constexpr int kFewTiles = 16;
 template <typename T>
 bool few_rows(int M) {
   return row_tiles<T>(M) <= kFewTiles;
 }
+// Its lanes form the digits themselves while that is little work, which the launch that
+// forms them in the workspace costs more than: 64 x 1024 x 1024 7.2 us, with it 9.8; 1 x
+// 4096 x 4096 8.4, with it 10.0; 16 x 4096 x 4096 14.6, with it 12.0; Z_2^64: 4 x 4096 x
+// 4096 15.5, with it 12.2.
 template <typename T>
 bool direct_rows(int M, int K, int N) {
-  return few_rows<T>(M) && size_t(row_tiles<T>(M)) * K * ((size_t(N) + 15) / 16) <= (sizeof(T) == 4 ? size_t(1) << 20 : size_t(1) << 19);
+  constexpr size_t most = size_t(sizeof(T) == 4 ? 1 << 20 : 1 << 19);  // words by column tile
+  return few_rows<T>(M) && size_t(row_tiles<T>(M)) * K * ((size_t(N) + 15) / 16) <= most;
 }
 
 template <typename T, int S>
@@ -442,10 +466,15 @@ hipError_t launch_at(const Launch &L, const Q4Args<T> &g) {
     hipLaunchKernelGGL((k_q4_many<T, S, kManyMT, NT>), dim3(unsigned(wgs)), dim3(256), 0, L.stream, g, steps, work);
     return hipGetLastError();
   };
-  const size_t rows = size_t(tiles / (2 * kManyMT));
-  constexpr int kWideNT = S == 32 ? 2 : 4;
-  if ((size_t(g.N) + 32 * kWideNT - 1) / (32 * kWideNT) * rows >= size_t(L.num_cu) * (sizeof(T) == 4 ? 1 : 2))
-    return many(std::integral_constant<int, kWideNT>{});
+  // The widest column tiles that give every CU its two workgroups: 512 x 4096 x 4096 by 4
+  // tiles 57.6 us, by 2 66.0; 256 rows by 4 40.0, by 2 35.8; 128 rows by 4 38.5, by 2 31.0,
+  // by 1 28.1.  Groups of 32 hold twice the scales, too many for the registers of 4 tiles
+  // (512 rows 438 us, by 2 161).
+  const size_t rows = size_t(tiles / (2 * kManyMT)), enough = size_t(L.num_cu) * 2;
+  auto wgs = [&](int nt) { return (size_t(g.N) + 32 * nt - 1) / (32 * nt) * rows; };
+  if constexpr (S != 32)
+    if (wgs(4) >= enough) return many(std::integral_constant<int, 4>{});
+  if (wgs(2) >= enough) return many(std::integral_constant<int, 2>{});
   return many(std::integral_constant<int, 1>{});
 }
 

@@ -399,8 +399,8 @@ mpcx_status mpcx_split_mask(mpcx_ctx *ctx, size_t n, const void *d_mask, uint64_
  * (causal, prefix, window and document masks; none where lo >= hi), and its
  * scores are the n_heads * (hi - lo) words from d_off[t] on, head by head, of
  * n_scores in all.  A token whose range leaves its page row or whose block
- * leaves the n_scores words is taken to see nothing; tokens of no sequence are
- * skipped.  max_q and max_keys, about the most tokens of a sequence and keys of a
+ * leaves the n_scores words is taken to see nothing; tokens of no sequence get no
+ * scores, and their rows of a weighted sum are unspecified.  max_q and max_keys, about the most tokens of a sequence and keys of a
  * range, size the launch only. */
 typedef struct {
   mpcx_cache cache;
