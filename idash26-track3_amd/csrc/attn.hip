@@ -314,12 +314,18 @@ __device__ __forceinline__ void group_planes(uint4 u, uint4 v, uint32_t (&o)[siz
 // One token a sequence is bound by the cache's bytes: 8 sequences of up to 4096 keys, 8
 // cache heads of 128 in Z_2^32: 76.8 us for 296 MB, 3.9 TB/s (equal lengths: 72 us; the
 // start, some 10 us from the first page number to the first product, and the longest
-// sequence's end are what is left).  Prompts are bound by the digits' vector instructions,
-// about as many cycles as the MFMAs at two waves a SIMD: 4 x 512 tokens, 8 heads of 64:
-// 42.2 us.
+// sequence's end are what is left).  Prompts are bound by a wave's own order: 6 us of start
+// and then 4 us a step, of which at two waves a SIMD half is issue (two thirds of that
+// vector instructions, most of them the digits', one third MFMAs), the rest what the waves
+// wait for one another, LDS and the rows (asked for before the products instead of after
+// them: no faster).  4 x 512 tokens, 8 heads of 64 in Z_2^32: 47.1 us.
+// Four waves, so that one workgroup's start runs beside another's products: with calls and
+// launches eight take 55.2 us for 4 x 256 tokens against 1024 keys, four 46.6; 62.7 for
+// 3 x 400 of 16 heads of 128, four 53.6; but 44.9 for the 4 x 512, four 49.8.
 // ---------------------------------------------------------------------------
-template <AttnForm F, typename T, bool VEC, int RT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, sizeof(T) == 4 ? 2 : 1) void k_attn_scores(AttnArgs<T> g, Units units, int k0, int kn, bool more) {
+constexpr int kScoreWaves = 4;
+template <AttnForm F, typename T, bool VEC, int RT>
+__global__ __launch_bounds__(64 * kScoreWaves, sizeof(T) == 4 ? 2 : 1) void k_attn_scores(AttnArgs<T> g, Units units, int k0, int kn, bool more) {
   constexpr int G = 16 / int(sizeof(T)), NQ = int(sizeof(T)), NT = Form<F>::terms;
   constexpr int CH = int(sizeof(T)), PAIR = CH / 4;  // chunks of a step; those of four words
   constexpr bool bias = F == AttnForm::BOTH || F == AttnForm::P0;
@@ -390,7 +396,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 4 ? 2 : 1) void k_attn_sco
     const TileRow mine = tile_row(d, t0, t1, u.kv, m, e0 + uint32_t(lane % (16 * RT)));
     int klo, khi;
     tile_keys<16 * RT>(mine, klo, khi);
-    KeySteps ahead(units, u.split, klo, khi, wave, WAVES, 16);  // the tile after the one asked for
+    KeySteps ahead(units, u.split, klo, khi, wave, kScoreWaves, 16);  // the tile after the one asked for
     const int last = khi > 0 ? khi - 1 : 0;  // keys past the range read the last one's row
     auto page_of = [&](int64_t kb) {
       const uint32_t key = min(uint32_t(kb) + uint32_t(li), uint32_t(last));
@@ -497,7 +503,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 4 ? 2 : 1) void k_attn_sco
     step = 0;
     if (kb < khi) load();
     put(tid, first);
-    for (int e = tid + 64 * WAVES; e < 16 * RT * steps * 16; e += 64 * WAVES) {
+    for (int e = tid + 64 * kScoreWaves; e < 16 * RT * steps * 16; e += 64 * kScoreWaves) {
       Query q;
       get(e, q);
       put(e, q);
@@ -716,19 +722,19 @@ template <AttnForm F, typename T>
 constexpr size_t kStepLds = size_t(Form<F>::terms) * sizeof(T) * 1024;
 constexpr size_t kScoreLds = 62 * 1024;
 
-template <AttnForm F, typename T, int RT, int WAVES>
+template <AttnForm F, typename T, int RT>
 hipError_t scores_rows(const Launch &L, const AttnArgs<T> &g, int dims, int64_t want) {
-  const Units u = units_for(g.d, 1, 16 * RT, want, 16 * WAVES);
+  const Units u = units_for(g.d, 1, 16 * RT, want, 16 * kScoreWaves);
   if (u.n == 0) return hipErrorInvalidValue;
   const bool vec = vec_rows(g, true);
   for (int k0 = 0; k0 < g.d.c.dim; k0 += dims) {
     const int kn = std::min(dims, g.d.c.dim - k0);
     const size_t lds = kStepLds<F, T> * RT * size_t((kn + 63) / 64);
     if (vec)
-      hipLaunchKernelGGL((k_attn_scores<F, T, true, RT, WAVES>), dim3(unsigned(u.n)), dim3(64 * WAVES), lds, L.stream, g, u,
+      hipLaunchKernelGGL((k_attn_scores<F, T, true, RT>), dim3(unsigned(u.n)), dim3(64 * kScoreWaves), lds, L.stream, g, u,
                          k0, kn, k0 > 0);
     else
-      hipLaunchKernelGGL((k_attn_scores<F, T, false, RT, WAVES>), dim3(unsigned(u.n)), dim3(64 * WAVES), lds, L.stream, g, u,
+      hipLaunchKernelGGL((k_attn_scores<F, T, false, RT>), dim3(unsigned(u.n)), dim3(64 * kScoreWaves), lds, L.stream, g, u,
                          k0, kn, k0 > 0);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -736,8 +742,8 @@ hipError_t scores_rows(const Launch &L, const AttnArgs<T> &g, int dims, int64_t 
   return hipSuccess;
 }
 // Two tiles of rows to a workgroup, where LDS holds them: the keys' planes are formed once
-// for both.  Z_2^32: from about one workgroup a CU on (4 prompts of 512 tokens, 8 heads of
-// 64: 45.0 us, one tile 50.4; 4 of 64 tokens against 1024 keys: 23.1, one 20.8); Z_2^64,
+// for both.  Z_2^32: from about one workgroup a CU on (4 prompts of 256 tokens against 1024
+// keys, 8 heads of 64: 46.6 us, one tile 60.5; 4 of 64 tokens: 23.1, one 20.8); Z_2^64,
 // where a key's planes cost more: from 64 rows on (4 of 16 tokens, 4 heads a key: 18.1 us,
 // one 22.2; 4 of 8 tokens: 17.1, one 13.2).
 template <typename T>
@@ -753,9 +759,9 @@ hipError_t scores_at(const Launch &L, const AttnArgs<T> &g) {
   // cache heads of 128, two 79.5, four 78.6 but 26.2 for 21.3 for 4 x 64 against 1024
   const int64_t want = int64_t(L.num_cu) * 2;
   if (steps * kStepLds<F, T> * 2 <= kScoreLds && two_tiles<T>(g.d, L.num_cu))
-    return scores_rows<F, T, 2, sizeof(T) == 4 ? 8 : 4>(L, g, g.d.c.dim, want);
+    return scores_rows<F, T, 2>(L, g, g.d.c.dim, want);
   const int dims = int(std::min(steps, kScoreLds / kStepLds<F, T>)) * 64;
-  return scores_rows<F, T, 1, 4>(L, g, dims, want);
+  return scores_rows<F, T, 1>(L, g, dims, want);
 }
 template <AttnForm F, typename T>
 hipError_t mix_at(const Launch &L, const AttnArgs<T> &g) {
