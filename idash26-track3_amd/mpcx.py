@@ -263,10 +263,12 @@ class Ctx:
     """A libmpcx context (bw-bit ring, fixed-point scale s) on one GPU."""
 
     def __init__(self, bw=32, scale=12, device=0):
-        _torch()
+        torch = _torch()
         self.lib = load()
         self.bw, self.s = bw, scale
         self.T = np.uint32 if bw == 32 else np.uint64
+        self._word = torch.int32 if bw == 32 else torch.int64
+        self._device, self._stream, self._stream_id = device, None, 0
         h = C.c_void_p()
         st = self.lib.mpcx_create(bw, scale, device, C.byref(h))
         if st != 0:
@@ -294,8 +296,9 @@ class Ctx:
     def set_stream(self, stream):
         """Work on a torch stream from now on (None, or torch's default stream: on
         the context's own)."""
-        self.check(self.lib.mpcx_set_stream(self.h, stream.cuda_stream if stream is not None else None), "set_stream")
-        self._stream = stream
+        handle = stream.cuda_stream if stream is not None else 0
+        self.check(self.lib.mpcx_set_stream(self.h, handle or None), "set_stream")
+        self._stream, self._stream_id = stream, handle
 
     def set_party_sync(self, sync):
         """Party-mode calls synchronise the stream (True, the default) or return
@@ -594,9 +597,8 @@ class Ctx:
     # only enqueue; elsewhere they wait for torch's stream first and for their own
     # work at the end, as the methods above do.
     def _enter(self):
-        cur = _torch().cuda.current_stream()
-        s = getattr(self, "_stream", None)
-        if s is not None and s.cuda_stream == cur.cuda_stream != 0:
+        cur = _torch_module.cuda.current_stream(self._device)
+        if self._stream_id == cur.cuda_stream != 0:
             return True
         cur.synchronize()
         return False
@@ -604,10 +606,6 @@ class Ctx:
     def _leave(self, same):
         if not same:
             self.sync()
-
-    @property
-    def _word(self):
-        return _torch().int32 if self.bw == 32 else _torch().int64
 
     def _words(self, t, what, shape=None):
         """A contiguous ring tensor's address."""
@@ -624,7 +622,7 @@ class Ctx:
         return t.data_ptr()
 
     def _new(self, shape):
-        return _torch().empty(shape, dtype=self._word, device="cuda")
+        return _torch_module.empty(shape, dtype=self._word, device=self._device)
 
     def _rows(self, t, what):
         """A matrix of ring words whose rows may be apart: its address and row stride."""
@@ -649,7 +647,7 @@ class Ctx:
         if M == 0:
             return out
         nb = self.lib.mpcx_ring_gemm_q4_work_bytes(self.h, M, K)
-        work = torch.empty(nb, dtype=torch.uint8, device="cuda") if nb else None
+        work = torch.empty(nb, dtype=torch.uint8, device=self._device) if nb else None
         same = self._enter()
         self.check(self.lib.mpcx_ring_gemm_q4(self.h, M, K, N, group, ap, lda, qp, sp, op, ldc,
                                               work.data_ptr() if nb else None), "ring_gemm_q4")
@@ -671,15 +669,13 @@ class Ctx:
         shape, near = (n, pool[1], pool[3]), (pool[3], 1)
         sp = self._ints(slot, "cache_append: slot", torch.int64, (n,))
         pp = self._ints(pos, "cache_append: pos", torch.int32, (n,)) if pos is not None else None
-        arr = (_CachePlane * len(planes))()
-        for a, (r, p, rotate) in zip(arr, planes):
-            a.d_pool = self._words(p, "cache_append: pool", pool)
-            if r.shape != shape or r.dtype is not p.dtype or not r.is_cuda or \
-                    (r.stride()[1:] != near and not r.is_contiguous()):
+        arr = []
+        for r, p, rotate in planes:
+            to, st = self._words(p, "cache_append: pool", pool), r.stride()
+            if r.shape != shape or r.dtype is not self._word or not r.is_cuda or \
+                    (st[1:] != near and not r.is_contiguous()):
                 raise MpcxError(f"cache_append: rows: need int{self.bw} rows of shape {shape} on the GPU")
-            a.d_rows = r.data_ptr()
-            a.ld = r.stride(0) if n > 1 else shape[1] * shape[2]
-            a.rotate = rotate
+            arr.append(_CachePlane(r.data_ptr(), st[0] if n > 1 else shape[1] * shape[2], to, rotate))
         rot = None
         if rotation is not None:
             c = rotation.cos
@@ -688,7 +684,7 @@ class Ctx:
                                     self._words(rotation.sin, "cache_append: sin", c.shape)))
         same = self._enter()
         self.check(self.lib.mpcx_cache_append(self.h, C.byref(Cache(pool[1], pool[3], pool[2], pool[0])), n, sp, pp, rot,
-                                              len(planes), arr), "cache_append")
+                                              len(arr), (_CachePlane * len(arr))(*arr)), "cache_append")
         self._leave(same)
 
     def gate_keygen(self, kind, mask, seed=1, gate=1):
