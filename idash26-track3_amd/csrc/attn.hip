@@ -325,7 +325,8 @@ __device__ __forceinline__ void group_planes(uint4 u, uint4 v, uint32_t (&o)[siz
 // ---------------------------------------------------------------------------
 constexpr int kScoreWaves = 4;
 template <AttnForm F, typename T, bool VEC, int RT>
-__global__ __launch_bounds__(64 * kScoreWaves, sizeof(T) == 4 ? 2 : 1) void k_attn_scores(AttnArgs<T> g, Units units, int k0, int kn, bool more) {
+__global__ __launch_bounds__(64 * kScoreWaves, sizeof(T) == 4 ? 2 : 1) void k_attn_scores(AttnArgs<T> g, Units units,
+                                                                                          int k0, int kn, bool more) {
   constexpr int G = 16 / int(sizeof(T)), NQ = int(sizeof(T)), NT = Form<F>::terms;
   constexpr int CH = int(sizeof(T)), PAIR = CH / 4;  // chunks of a step; those of four words
   constexpr bool bias = F == AttnForm::BOTH || F == AttnForm::P0;

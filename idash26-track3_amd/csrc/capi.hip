@@ -1022,7 +1022,8 @@ static bool aligned(const void *p, size_t to) { return reinterpret_cast<uintptr_
 mpcx_status mpcx_ring_gemm_q4(mpcx_ctx *c, int M, int K, int N, int group, const void *a, size_t lda, const uint8_t *q,
                               const int32_t *scale, void *out, size_t ldc, void *work) {
   CHECK_CTX(c);
-  if (M < 1 || K < 1 || K > kQ4MaxK || N < 1 || group < 32 || group % 32 != 0 || lda < size_t(K) || ldc < size_t(N))
+  constexpr int kMost = INT32_MAX - 255;  // rows and columns are counted to the end of their last tile
+  if (M < 1 || M > kMost || K < 1 || K > kQ4MaxK || N < 1 || N > kMost || group < 32 || group % 32 != 0 || lda < size_t(K) || ldc < size_t(N))
     return fail(c, MPCX_EINVAL, "ring_gemm_q4: bad argument");
   if (!a || !q || !scale || !out || (!work && q4_work_bytes(c->bw, M, K) > 0))
     return fail(c, MPCX_EINVAL, "ring_gemm_q4: null pointer");
@@ -1253,6 +1254,12 @@ mpcx_status attn_eval(mpcx_ctx *c, bool scores, AttnForm form, const mpcx_attn *
   for (const void *p : {x, y, b0, b1, slope, static_cast<const void *>(out)})
     if (!aligned(p, tb)) return fail(c, MPCX_EINVAL, "attn_eval: misaligned pointer");
   if (!aligned(k0, 16) || !aligned(k1, 16)) return fail(c, MPCX_EINVAL, "attn_eval: misaligned pointer");
+  const size_t nb = second * tb, key = attn_key_end(c, first, second);
+  const size_t plane = size_t(a->cache.n_pages) * a->cache.n_heads * a->cache.page_size * a->cache.head_dim * tb;
+  if (!bytes_apart(out, nb, x, first * tb) || (p0 && !bytes_apart(out, nb, k0, key)) ||
+      (p1 && !bytes_apart(out, nb, k1, key)) || !bytes_apart(out, nb, y, plane) ||
+      (p0 && !bytes_apart(out, nb, b0, plane)) || (p1 && !bytes_apart(out, nb, b1, plane)))
+    return fail(c, MPCX_EINVAL, "attn_eval: the output overlaps an input");
   return c->bw == 32
              ? attn_eval_t<uint32_t>(c, scores, form, a, first, second, k0, k1, x, y, b0, b1, slope, pos, out)
              : attn_eval_t<uint64_t>(c, scores, form, a, first, second, k0, k1, x, y, b0, b1, slope, pos, out);

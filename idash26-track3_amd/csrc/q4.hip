@@ -130,7 +130,7 @@ __global__ __launch_bounds__(1024) void k_q4_few(Q4Args<T> g, bool vec, int step
   const int li = lane & 15, lg = lane >> 4, p = li % NP;
   const int n = int(blockIdx.x) * 16 + li, nc = n < g.N ? n : g.N - 1;
   const int m0 = int(blockIdx.y) * MT * R;
-  const size_t qrow = (size_t(g.K) + 31) / 32 * 16;
+  const size_t qrow = q4_row_bytes(g.K);
   const uint8_t *q = g.q + size_t(nc) * qrow + lg * (S / 8);
   const int chunks = (g.K + S - 1) / S, per = g.group / S;
   T out[MT];
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(256, 2) void k_q4_many(Q4Args<T> g, int steps, cons
   const int tid = int(threadIdx.x), lane = tid & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n0 = lw % gx * 32 * NT + (wave & 1) * 16 * NT, t0 = lw / gx * 2 * MT;
-  const uint32_t qrow = uint32_t((size_t(g.K) + 31) / 32 * 16);
+  const uint32_t qrow = uint32_t(q4_row_bytes(g.K));
   const int per = g.group / S, last = (g.K - 1) / S;
   // places in 32 bits from bases that a wave shares (launch_gemm_q4 bounds K)
   const int nw = min(n0, g.N - 1);

@@ -339,8 +339,8 @@ mpcx_status mpcx_ring_lincomb(mpcx_ctx *ctx, size_t rows, size_t cols, uint64_t 
  * (K + 31) / 32 * 16 bytes, weight k of a row two's complement (-8..7) in the low
  * (k even) or high (k odd) half of byte k / 2; the halves past K are not used.
  * d_scale: ceil(K / group) rows of N int32 steps, at the scale of the weights;
- * group a multiple of 32; K up to 2^24.  d_c: M rows of N words, ldc >= N words apart.  d_q is
- * 16-byte aligned.  d_work: mpcx_ring_gemm_q4_work_bytes bytes, 16-byte aligned,
+ * group a multiple of 32; K up to 2^24.  d_c: M rows of N words, ldc >= N words
+ * apart, none of them a word of d_a.  d_q is 16-byte aligned.  d_work: mpcx_ring_gemm_q4_work_bytes bytes, 16-byte aligned,
  * in use until the stream has reached the call (NULL where that is 0). */
 size_t mpcx_ring_gemm_q4_work_bytes(mpcx_ctx *ctx, int M, int K);
 mpcx_status mpcx_ring_gemm_q4(mpcx_ctx *ctx, int M, int K, int N, int group, const void *d_a, size_t lda,
@@ -401,7 +401,7 @@ mpcx_status mpcx_split_mask(mpcx_ctx *ctx, size_t n, const void *d_mask, uint64_
  * n_scores in all.  A token whose range leaves its page row or whose block
  * leaves the n_scores words is taken to see nothing; tokens of no sequence get no
  * scores, and their rows of a weighted sum are unspecified.  max_q and max_keys, about the most tokens of a sequence and keys of a
- * range, size the launch only. */
+ * range, size the launch only.  A gate's output overlaps none of its inputs. */
 typedef struct {
   mpcx_cache cache;
   int n_heads, n_tok, n_seq, max_pages, max_q, max_keys;

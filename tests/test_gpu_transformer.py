@@ -678,3 +678,19 @@ def test_sizes_past_the_bounds_are_refused(ctx):
     big = mpcx.Cache(1 << 16, 1 << 16, 1, 1)
     plane = (mpcx._CachePlane * 1)(mpcx._CachePlane(d, 1 << 32, d, 0))
     assert L.mpcx_cache_append(h, C.byref(big), 1, d, None, None, 1, plane) == 1
+
+
+def test_outputs_over_inputs_are_refused(ctx):
+    B = Batch(ctx.bw, 1, 4, 20, 2, 2, 16, 4, "causal", seed=9)
+    g, planes = B.gpu(), [dev(v) for v in (B.y, B.b0, B.b1)]
+    q, p = dev(words(B.rng, (B.tokens, 2, 16), ctx.bw)), dev(words(B.rng, (B.n,), ctx.bw))
+    ks, km = ctx.attn_scores_keygen(g, q, *planes[1:]), ctx.attn_mix_keygen(g, p, *planes[1:])
+    L, h, a = ctx.lib, ctx.h, ctx._attn(g, planes[0])
+    y, b0, b1 = (t.data_ptr() for t in planes)
+    for out in (q, ks[0], ks[1], *planes):
+        assert L.mpcx_attn_scores_eval(h, C.byref(a), ks[0].data_ptr(), ks[1].data_ptr(), q.data_ptr(), y, b0, b1, None,
+                                       None, out.data_ptr()) == 1
+    for out in (p, km[0], km[1], *planes):
+        assert L.mpcx_attn_mix_eval(h, C.byref(a), km[0].data_ptr(), km[1].data_ptr(), p.data_ptr(), y, b0, b1,
+                                    out.data_ptr()) == 1
+    assert b"overlaps" in L.mpcx_last_error(h)
