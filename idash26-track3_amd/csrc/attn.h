@@ -3,6 +3,7 @@
 // that read it (attn.hip).
 #pragma once
 #include "kernels.h"
+#include "q4_layout.h"
 
 namespace mpcx {
 
@@ -11,7 +12,6 @@ namespace mpcx {
 // q: N rows of q4_row_bytes(K) bytes, weight k of a row in the low (k even) or
 // high half of byte k / 2, two's complement; scale: ceil(K / group) x N.
 constexpr int kQ4MaxK = 1 << 24;  // a tile's weights lie within 32 bits
-__host__ __device__ inline size_t q4_row_bytes(int K) { return (size_t(K) + 31) / 32 * 16; }
 template <typename T>
 struct Q4Args {
   int M = 0, K = 0, N = 0, group = 0;

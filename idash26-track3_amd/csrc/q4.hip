@@ -130,8 +130,8 @@ __global__ __launch_bounds__(1024) void k_q4_few(Q4Args<T> g, bool vec, int step
   const int li = lane & 15, lg = lane >> 4, p = li % NP;
   const int n = int(blockIdx.x) * 16 + li, nc = n < g.N ? n : g.N - 1;
   const int m0 = int(blockIdx.y) * MT * R;
-  const size_t qrow = q4_row_bytes(g.K);
-  const uint8_t *q = g.q + size_t(nc) * qrow + lg * (S / 8);
+  const uint32_t qrow = uint32_t(q4_row_bytes(g.K));
+  const uint8_t *q = g.q + size_t(nc) * qrow;
   const int chunks = (g.K + S - 1) / S, per = g.group / S;
   T out[MT];
 #pragma unroll
@@ -142,7 +142,7 @@ __global__ __launch_bounds__(1024) void k_q4_few(Q4Args<T> g, bool vec, int step
     const int kb = c * S + lg * (S / 4);  // this lane's first k
     uint32_t be[ND], bo[ND];
     // weights past the end of a row meet rows' zeros
-    __builtin_memcpy(be, __builtin_assume_aligned(q + min(size_t(c) * (S / 2), qrow - S / 8 - lg * (S / 8)), S / 8), 4 * ND);
+    __builtin_memcpy(be, __builtin_assume_aligned(q + q4_place(qrow, S, c, lg), S / 8), 4 * ND);
     const int32_t scale = g.scale[size_t(c / per) * g.N + nc];
 #pragma unroll
     for (int d = 0; d < ND; d++) bo[d] = q4_hi(be[d]), be[d] = q4_lo(be[d]);
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(256, 2) void k_q4_many(Q4Args<T> g, int steps, cons
 #pragma unroll
     for (int c = 0; c < CH; c++) {
       const int chunk = step * CH + c;
-      const uint32_t at = min(uint32_t(chunk) * (S / 2) + uint32_t(lg) * (S / 8), qrow - S / 8);
+      const uint32_t at = q4_place(qrow, S, chunk, lg);
       const int32_t *sg = sw + size_t(min(chunk, last) / per) * g.N;
 #pragma unroll
       for (int t = 0; t < NT; t++) {

@@ -1,0 +1,35 @@
+"""The transformer operators where sizes, launches and buffers meet their ends, and
+the kernel instances that small shapes do not choose, against the definitions in
+64-bit integers.  All results are ring words, so every comparison is of all bits."""
+import numpy as np
+import pytest
+
+import mpcx
+from test_gpu_transformer import dev, host, q4_pack, q4_plain, words
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", params=[32, 64])
+def ctx(request):
+    c = mpcx.Ctx(bw=request.param, scale=12)
+    yield c
+    c.close()
+
+
+def q4_case(ctx, M, K, N, group, seed=0):
+    rng = np.random.default_rng(seed + M * 7 + K * 3 + N)
+    a, w = words(rng, (M, K), ctx.bw), rng.integers(-8, 8, (N, K))
+    scale = rng.integers(-(1 << 31), 1 << 31, (-(-K // group), N)).astype(np.int32)
+    scale.flat[0], scale.flat[-1] = -(1 << 31), (1 << 31) - 1
+    return a, w, scale
+
+
+# ---------------- 4-bit weights ----------------
+@pytest.mark.parametrize("M", [1, 2, 40, 90])
+@pytest.mark.parametrize("K,N,group", [(1, 1, 128), (31, 16, 64), (32, 5, 64), (32, 17, 128), (33, 5, 128), (64, 5, 128),
+                                       (65, 3, 128), (96, 5, 128), (97, 18, 256), (127, 16, 128), (40, 9, 192)])
+def test_q4_rows_shorter_than_a_chunk(ctx, M, K, N, group):
+    a, w, scale = q4_case(ctx, M, K, N, group)
+    got = host(ctx.ring_gemm_q4(dev(a), dev(q4_pack(w)), dev(scale), group), ctx.bw)
+    assert np.array_equal(got, q4_plain(a, w, scale, group).astype(ctx.T))
