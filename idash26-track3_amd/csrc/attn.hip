@@ -703,17 +703,20 @@ bool vec_rows(const AttnArgs<T> &g, bool left) {
       ok = ok && reinterpret_cast<uintptr_t>(p) % 16 == 0;
   return ok;
 }
-// About `want` units, at least one tile and one split for each pair and column group;
-// none (n = 0) where the pairs alone are too many for a launch.
-Units units_for(const AttnDims &d, int cols, int rows, int64_t want, int64_t keys_per_split) {
+// Rows of a sequence and a cache head by the caller's hint; no sequence has more tokens
+// than the batch.
+int64_t rows_hint(const AttnDims &d) { return int64_t(std::min(d.max_q, d.n_tok)) * (d.heads / d.c.heads); }
+// About `want` units of `threads`, at least one tile and one split for each pair and column
+// group, and no more threads than a launch may have; none (n = 0) where the pairs alone
+// are too many.
+Units units_for(const AttnDims &d, int threads, int cols, int rows, int64_t want, int64_t keys_per_split) {
   Units u;
-  const int64_t m = d.heads / d.c.heads, base = int64_t(d.n_seq) * d.c.heads;
-  constexpr int64_t kMost = 1 << 30;
-  if (base > kMost / cols) return u;
+  const int64_t base = int64_t(d.n_seq) * d.c.heads, most = int64_t(kMostThreads / unsigned(threads));
+  if (base > most / cols) return u;
   u.cols = cols;
-  u.tiles = int(std::max<int64_t>(1, std::min((int64_t(d.max_q) * m + rows - 1) / rows, kMost / (base * cols))));
+  u.tiles = int(std::max<int64_t>(1, std::min((rows_hint(d) + rows - 1) / rows, most / (base * cols))));
   const int64_t one = base * cols * u.tiles, keys = (int64_t(d.max_keys) + keys_per_split - 1) / keys_per_split;
-  u.splits = int(std::max<int64_t>(1, std::min((want + one - 1) / one, std::min(keys, kMost / one))));
+  u.splits = int(std::max<int64_t>(1, std::min((want + one - 1) / one, std::min(keys, most / one))));
   u.n = int(one * u.splits);
   return u;
 }
@@ -725,7 +728,7 @@ constexpr size_t kScoreLds = 62 * 1024;
 
 template <AttnForm F, typename T, int RT>
 hipError_t scores_rows(const Launch &L, const AttnArgs<T> &g, int dims, int64_t want) {
-  const Units u = units_for(g.d, 1, 16 * RT, want, 16 * kScoreWaves);
+  const Units u = units_for(g.d, 64 * kScoreWaves, 1, 16 * RT, want, 16 * kScoreWaves);
   if (u.n == 0) return hipErrorInvalidValue;
   const bool vec = vec_rows(g, true);
   for (int k0 = 0; k0 < g.d.c.dim; k0 += dims) {
@@ -749,7 +752,7 @@ hipError_t scores_rows(const Launch &L, const AttnArgs<T> &g, int dims, int64_t 
 // one 22.2; 4 of 8 tokens: 17.1, one 13.2).
 template <typename T>
 bool two_tiles(const AttnDims &d, int num_cu) {
-  const int64_t rows = int64_t(d.max_q) * (d.heads / d.c.heads);
+  const int64_t rows = rows_hint(d);
   if (sizeof(T) == 8) return rows >= 64;
   return int64_t(d.n_seq) * d.c.heads * ((rows + 31) / 32) >= num_cu;
 }
@@ -774,7 +777,7 @@ hipError_t mix_at(const Launch &L, const AttnArgs<T> &g) {
   // to four steps 18.8; 300 keys 10.7, split 11.9).
   constexpr int64_t kStepKeys = int64_t(kMixWaves) * 4 * G;
   const int64_t part = g.d.max_keys > 4 * kStepKeys ? kStepKeys : 4 * kStepKeys;
-  const Units u = units_for(g.d, (g.d.c.dim + 16 * G - 1) / (16 * G), 16, int64_t(L.num_cu), part);
+  const Units u = units_for(g.d, 64 * kMixWaves, (g.d.c.dim + 16 * G - 1) / (16 * G), 16, int64_t(L.num_cu), part);
   if (u.n == 0) return hipErrorInvalidValue;
   if (u.splits > 1) {
     const size_t n = size_t(g.d.n_tok) * g.d.heads * g.d.c.dim, want = (n + 255) / 256, cap = size_t(L.num_cu) * 32;

@@ -36,6 +36,9 @@ inline int variant_block(const Launch &L) {
   return (L.aes_variant >= 0 && L.aes_variant < n) ? v[L.aes_variant].block : 256;
 }
 
+// HIP's limit on the threads of a launch along one dimension
+constexpr size_t kMostThreads = UINT32_MAX;
+
 template <typename K>
 inline int grid_for(K kernel, int block, size_t n, int num_cu) {
   int occ = 0;

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import mpcx
-from test_gpu_transformer import dev, host, q4_pack, q4_plain, words
+from test_gpu_transformer import Batch, dev, host, q4_pack, q4_plain, words
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +33,21 @@ def test_q4_rows_shorter_than_a_chunk(ctx, M, K, N, group):
     a, w, scale = q4_case(ctx, M, K, N, group)
     got = host(ctx.ring_gemm_q4(dev(a), dev(q4_pack(w)), dev(scale), group), ctx.bw)
     assert np.array_equal(got, q4_plain(a, w, scale, group).astype(ctx.T))
+
+
+# ---------------- launches ----------------
+@pytest.mark.parametrize("max_q,max_keys", [(1 << 20, 1), (1 << 20, 60), ((1 << 31) - 1, (1 << 31) - 1)])
+def test_launch_hints_of_any_size(ctx, max_q, max_keys):
+    """8 sequences of 8 cache heads: 2^20 tokens a sequence, taken at their word, are
+    more threads than a launch may have."""
+    B = Batch(ctx.bw, 8, 3, 60, 32, 8, 16, 16, "causal", seed=3)
+    g, planes = B.gpu()._replace(max_q=max_q, max_keys=max_keys), [dev(v) for v in (B.y, B.b0, B.b1)]
+    rq, q = words(B.rng, (B.tokens, 32, 16), ctx.bw), words(B.rng, (B.tokens, 32, 16), ctx.bw)
+    rp, p = words(B.rng, (B.n,), ctx.bw), words(B.rng, (B.n,), ctx.bw)
+    with np.errstate(over="ignore"):
+        k0, k1, rs = ctx.attn_scores_keygen(g, dev(rq), *planes[1:])
+        got = host(ctx.attn_scores_eval(g, k0, k1, dev(q), *planes), ctx.bw)
+        assert np.array_equal(got, B.scores(q - rq, B.y - B.b0 - B.b1) + host(rs, ctx.bw))
+        k0, k1, ro = ctx.attn_mix_keygen(g, dev(rp), *planes[1:])
+        got = host(ctx.attn_mix_eval(g, k0, k1, dev(p), *planes), ctx.bw)
+        assert np.array_equal(got, B.mix(p - rp, B.y - B.b0 - B.b1) + host(ro, ctx.bw))
