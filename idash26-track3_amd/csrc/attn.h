@@ -19,6 +19,7 @@ struct Q4Args {
   size_t lda = 0;
   const uint8_t *q = nullptr;
   const int32_t *scale = nullptr;
+  int lds = 0;  // words between the scales' rows (N, or more for some columns of a product)
   T *c = nullptr;
   size_t ldc = 0;
   void *work = nullptr;  // q4_work_bytes

@@ -1012,6 +1012,7 @@ static mpcx_status gemm_q4_t(mpcx_ctx *c, int M, int K, int N, int group, const 
   g.lda = lda;
   g.q = q;
   g.scale = scale;
+  g.lds = N;
   g.c = static_cast<T *>(out);
   g.ldc = ldc;
   g.work = work;

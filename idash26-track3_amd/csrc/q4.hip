@@ -23,6 +23,7 @@
 // MI355X; "rows x K x N", groups of 128 unless said.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "attn.h"
@@ -143,7 +144,7 @@ __global__ __launch_bounds__(1024) void k_q4_few(Q4Args<T> g, bool vec, int step
     uint32_t be[ND], bo[ND];
     // weights past the end of a row meet rows' zeros
     __builtin_memcpy(be, __builtin_assume_aligned(q + q4_place(qrow, S, c, lg), S / 8), 4 * ND);
-    const int32_t scale = g.scale[size_t(c / per) * g.N + nc];
+    const int32_t scale = g.scale[size_t(c / per) * g.lds + nc];
 #pragma unroll
     for (int d = 0; d < ND; d++) bo[d] = q4_hi(be[d]), be[d] = q4_lo(be[d]);
 #pragma unroll
@@ -316,7 +317,7 @@ __global__ __launch_bounds__(256, 2) void k_q4_many(Q4Args<T> g, int steps, cons
     for (int c = 0; c < CH; c++) {
       const int chunk = step * CH + c;
       const uint32_t at = q4_place(qrow, S, chunk, lg);
-      const int32_t *sg = sw + size_t(min(chunk, last) / per) * g.N;
+      const int32_t *sg = sw + size_t(min(chunk, last) / per) * g.lds;
 #pragma unroll
       for (int t = 0; t < NT; t++) {
         __builtin_memcpy(h.b[c][t], __builtin_assume_aligned(qw + (qo[t] + at), S / 8), 4 * ND);
@@ -431,6 +432,21 @@ bool direct_rows(int M, int K, int N) {
   return few_rows<T>(M) && size_t(row_tiles<T>(M)) * K * ((size_t(N) + 15) / 16) <= most;
 }
 
+// launch(g) on as many columns at a time as `most` allows
+template <typename T, class Fn>
+hipError_t by_columns(const Q4Args<T> &g, size_t most, Fn &&launch) {
+  for (size_t n = 0; n < size_t(g.N); n += most) {
+    Q4Args<T> part = g;
+    part.N = int(std::min(most, size_t(g.N) - n));
+    part.q += n * q4_row_bytes(g.K);
+    part.scale += n;
+    part.c += n;
+    const hipError_t e = launch(part);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
 template <typename T, int S>
 hipError_t launch_at(const Launch &L, const Q4Args<T> &g) {
   const bool vec = reinterpret_cast<uintptr_t>(g.a) % 16 == 0 && g.lda % (16 / sizeof(T)) == 0;
@@ -450,27 +466,32 @@ hipError_t launch_at(const Launch &L, const Q4Args<T> &g) {
     const int rt = row_tiles<T>(g.M);
     auto few = [&](auto mt) {
       constexpr int MT = decltype(mt)::value;
-      const dim3 grid(unsigned((size_t(g.N) + 15) / 16), unsigned((rt + MT - 1) / MT)), block(64u * unsigned(waves));
-      if (direct) hipLaunchKernelGGL((k_q4_few<T, S, MT, true>), grid, block, 0, L.stream, g, vec, steps);
-      else hipLaunchKernelGGL((k_q4_few<T, S, MT, false>), grid, block, 0, L.stream, g, vec, steps);
-      return hipGetLastError();
+      return by_columns(g, kMostThreads / (64u * unsigned(waves)) * 16, [&](const Q4Args<T> &p) {
+        const dim3 grid(unsigned((size_t(p.N) + 15) / 16), unsigned((rt + MT - 1) / MT)), block(64u * unsigned(waves));
+        if (direct) hipLaunchKernelGGL((k_q4_few<T, S, MT, true>), grid, block, 0, L.stream, p, vec, steps);
+        else hipLaunchKernelGGL((k_q4_few<T, S, MT, false>), grid, block, 0, L.stream, p, vec, steps);
+        return hipGetLastError();
+      });
     };
     if (rt >= 3) return few(std::integral_constant<int, 4>{});
     if (rt == 2) return few(std::integral_constant<int, 2>{});
     return few(std::integral_constant<int, 1>{});
   }
+  const size_t rows = size_t(tiles / (2 * kManyMT)), enough = size_t(L.num_cu) * 2;
   auto many = [&](auto nt) {
     constexpr int NT = decltype(nt)::value;
-    const size_t wgs = (size_t(g.N) + 32 * NT - 1) / (32 * NT) * size_t(tiles / (2 * kManyMT));
-    if (wgs > size_t(INT32_MAX)) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_q4_many<T, S, kManyMT, NT>), dim3(unsigned(wgs)), dim3(256), 0, L.stream, g, steps, work);
-    return hipGetLastError();
+    const size_t most = kMostThreads / 256 / rows;  // workgroups along the columns
+    if (most == 0) return hipErrorInvalidValue;
+    return by_columns(g, most * 32 * NT, [&](const Q4Args<T> &p) {
+      const size_t wgs = (size_t(p.N) + 32 * NT - 1) / (32 * NT) * rows;
+      hipLaunchKernelGGL((k_q4_many<T, S, kManyMT, NT>), dim3(unsigned(wgs)), dim3(256), 0, L.stream, p, steps, work);
+      return hipGetLastError();
+    });
   };
   // The widest column tiles that give every CU its two workgroups: 512 x 4096 x 4096 by 4
   // tiles 57.6 us, by 2 66.0; 256 rows by 4 40.0, by 2 35.8; 128 rows by 4 38.5, by 2 31.0,
   // by 1 28.1.  Groups of 32 hold twice the scales, too many for the registers of 4 tiles
   // (512 rows 438 us, by 2 161).
-  const size_t rows = size_t(tiles / (2 * kManyMT)), enough = size_t(L.num_cu) * 2;
   auto wgs = [&](int nt) { return (size_t(g.N) + 32 * nt - 1) / (32 * nt) * rows; };
   if constexpr (S != 32)
     if (wgs(4) >= enough) return many(std::integral_constant<int, 4>{});

@@ -36,6 +36,28 @@ def test_q4_rows_shorter_than_a_chunk(ctx, M, K, N, group):
 
 
 # ---------------- launches ----------------
+def test_q4_columns_past_one_launch(ctx):
+    """16 waves a column tile: columns past 2^26 are more threads than a launch may have."""
+    import torch
+    M, K, N, group = 1, 512, (1 << 26) + 37, 544
+    gen = torch.Generator(device="cuda").manual_seed(ctx.bw)
+    q = torch.empty((N, K // 2), dtype=torch.uint8, device="cuda")
+    for i in range(0, N, 1 << 24):
+        q[i:i + (1 << 24)].random_(0, 256, generator=gen)
+    scale = torch.randint(-(1 << 31), 1 << 31, (1, N), dtype=torch.int64, device="cuda", generator=gen).int()
+    rng = np.random.default_rng(5)
+    a = words(rng, (M, K), ctx.bw)
+    out = ctx.ring_gemm_q4(dev(a), q, scale, group)
+    at = np.unique(np.concatenate([np.arange(64), np.arange(N - 128, N), rng.integers(0, N, 4000)]))
+    t = torch.from_numpy(at).cuda()
+    byte = q[t].cpu().numpy().astype(np.int64)
+    w = np.stack([byte & 15, byte >> 4], -1).reshape(at.size, K)
+    want = q4_plain(a, (w ^ 8) - 8, scale[:, t].cpu().numpy(), group).astype(ctx.T)
+    assert np.array_equal(host(out[:, t], ctx.bw), want)
+    del q, scale, out
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("max_q,max_keys", [(1 << 20, 1), (1 << 20, 60), ((1 << 31) - 1, (1 << 31) - 1)])
 def test_launch_hints_of_any_size(ctx, max_q, max_keys):
     """8 sequences of 8 cache heads: 2^20 tokens a sequence, taken at their word, are
