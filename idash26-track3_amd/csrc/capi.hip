@@ -1,6 +1,7 @@
 // capi.hip -- extern "C" entry points of libmpcx (declared in include/mpcx.h).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -1020,6 +1021,11 @@ static mpcx_status gemm_q4_t(mpcx_ctx *c, int M, int K, int N, int group, const 
   return MPCX_OK;
 }
 static bool aligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+// rows of ring words, ld words apart (no further than addresses can be)
+static ByteRows word_rows(const mpcx_ctx *c, const void *p, size_t rows, size_t ld, size_t width) {
+  const size_t tb = size_t(c->bw) / 8;
+  return {p, rows, std::min(ld, size_t(1) << 59) * tb, width * tb};
+}
 mpcx_status mpcx_ring_gemm_q4(mpcx_ctx *c, int M, int K, int N, int group, const void *a, size_t lda, const uint8_t *q,
                               const int32_t *scale, void *out, size_t ldc, void *work) {
   CHECK_CTX(c);
@@ -1030,6 +1036,12 @@ mpcx_status mpcx_ring_gemm_q4(mpcx_ctx *c, int M, int K, int N, int group, const
     return fail(c, MPCX_EINVAL, "ring_gemm_q4: null pointer");
   if (!aligned(q, 16) || !aligned(work, 16) || !aligned(scale, 4) || !aligned(a, c->bw / 8) || !aligned(out, c->bw / 8))
     return fail(c, MPCX_EINVAL, "ring_gemm_q4: misaligned pointer");
+  const ByteRows ra = word_rows(c, a, size_t(M), lda, size_t(K)), rc = word_rows(c, out, size_t(M), ldc, size_t(N));
+  const size_t nq = size_t(N) * q4_row_bytes(K), ns = (size_t(K) + size_t(group) - 1) / size_t(group) * size_t(N) * 4;
+  const size_t nw = q4_work_bytes(c->bw, M, K);
+  if (!rows_apart(rc, ra) || !rows_apart(rc, q, nq) || !rows_apart(rc, scale, ns) || !rows_apart(rc, work, nw) ||
+      !rows_apart(ra, work, nw) || !bytes_apart(work, nw, q, nq) || !bytes_apart(work, nw, scale, ns))
+    return fail(c, MPCX_EINVAL, "ring_gemm_q4: the output or the workspace overlaps another buffer");
   return c->bw == 32 ? gemm_q4_t<uint32_t>(c, M, K, N, group, a, lda, q, scale, out, ldc, work)
                      : gemm_q4_t<uint64_t>(c, M, K, N, group, a, lda, q, scale, out, ldc, work);
 }

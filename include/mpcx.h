@@ -340,8 +340,10 @@ mpcx_status mpcx_ring_lincomb(mpcx_ctx *ctx, size_t rows, size_t cols, uint64_t 
  * (k even) or high (k odd) half of byte k / 2; the halves past K are not used.
  * d_scale: ceil(K / group) rows of N int32 steps, at the scale of the weights;
  * group a multiple of 32; K up to 2^24.  d_c: M rows of N words, ldc >= N words
- * apart, none of them a word of d_a.  d_q is 16-byte aligned.  d_work: mpcx_ring_gemm_q4_work_bytes bytes, 16-byte aligned,
- * in use until the stream has reached the call (NULL where that is 0). */
+ * apart.  d_q is 16-byte aligned.  d_work: mpcx_ring_gemm_q4_work_bytes bytes,
+ * 16-byte aligned, in use until the stream has passed the call.  The output and the
+ * workspace overlap no other buffer (refused; d_a and d_c may be columns of one
+ * larger matrix). */
 size_t mpcx_ring_gemm_q4_work_bytes(mpcx_ctx *ctx, int M, int K);
 mpcx_status mpcx_ring_gemm_q4(mpcx_ctx *ctx, int M, int K, int N, int group, const void *d_a, size_t lda,
                               const uint8_t *d_q, const int32_t *d_scale, void *d_c, size_t ldc, void *d_work);

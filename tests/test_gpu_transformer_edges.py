@@ -1,6 +1,8 @@
 """The transformer operators where sizes, launches and buffers meet their ends, and
 the kernel instances that small shapes do not choose, against the definitions in
 64-bit integers.  All results are ring words, so every comparison is of all bits."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -73,3 +75,42 @@ def test_launch_hints_of_any_size(ctx, max_q, max_keys):
         k0, k1, ro = ctx.attn_mix_keygen(g, dev(rp), *planes[1:])
         got = host(ctx.attn_mix_eval(g, k0, k1, dev(p), *planes), ctx.bw)
         assert np.array_equal(got, B.mix(p - rp, B.y - B.b0 - B.b1) + host(ro, ctx.bw))
+
+
+# ---------------- buffers ----------------
+EINVAL = 1
+
+
+def test_q4_output_or_workspace_over_another_buffer(ctx):
+    import torch
+    M, K, N, group, tb = 6, 64, 40, 32, ctx.bw // 8
+    nb = ctx.lib.mpcx_ring_gemm_q4_work_bytes(ctx.h, M, K)
+    buf = torch.zeros(5 * (1 << 16), dtype=torch.uint8, device="cuda")
+    a, q, s, c, w = (buf.data_ptr() + (i << 16) for i in range(5))
+    assert nb < 1 << 16
+    torch.cuda.synchronize()
+
+    def call(a=a, lda=K, q=q, s=s, c=c, ldc=N, w=w):
+        return ctx.lib.mpcx_ring_gemm_q4(ctx.h, M, K, N, group, a, lda, q, s, c, ldc, w)
+
+    assert call() == 0
+    for bad in (dict(c=a), dict(c=a + K * tb - tb), dict(c=a + ((M - 1) * K + K - 1) * tb), dict(c=q), dict(c=q + N * 32 - tb),
+                dict(c=s), dict(c=s + 2 * N * 4 - tb), dict(c=w), dict(c=w + nb - tb), dict(w=a), dict(w=q), dict(w=s),
+                dict(w=c), dict(a=w + nb - 8), dict(lda=K + N, c=a + (K - 1) * tb, ldc=K + N),
+                dict(lda=K + N, c=a + (K + 1) * tb, ldc=K + N), dict(lda=K + N, c=a + K * tb, ldc=K + N + 1)):
+        assert call(**bad) == EINVAL, bad
+        assert b"overlaps" in ctx.lib.mpcx_last_error(ctx.h)
+    ctx.sync()
+
+
+@pytest.mark.parametrize("M", [3, 70])
+def test_q4_into_columns_of_its_operand(ctx, M):
+    """Input and output side by side in one matrix."""
+    K, N, group = 96, 50, 32
+    a, w, scale = q4_case(ctx, M, K, N, group)
+    big = words(np.random.default_rng(M), (M, K + N + 3), ctx.bw)
+    big[:, :K] = a
+    d = dev(big)
+    ctx.ring_gemm_q4(d[:, :K], dev(q4_pack(w)), dev(scale), group, out=d[:, K + 1:K + 1 + N])
+    big[:, K + 1:K + 1 + N] = q4_plain(a, w, scale, group)
+    assert np.array_equal(host(d, ctx.bw), big)
