@@ -1052,6 +1052,9 @@ static bool valid_cache(const mpcx_cache &k) {
   const unsigned __int128 words = (unsigned __int128)(k.n_heads) * k.head_dim * k.page_size * (uint64_t)k.n_pages;
   return words < (unsigned __int128)1 << 60 && int64_t(k.n_heads) * k.head_dim < int64_t(1) << 31;
 }
+static size_t cache_plane_bytes(const mpcx_ctx *c, const mpcx_cache &k) {
+  return size_t(k.n_pages) * size_t(k.n_heads) * size_t(k.page_size) * size_t(k.head_dim) * (size_t(c->bw) / 8);
+}
 static CacheDims cache_dims(const mpcx_cache &k) {
   CacheDims d;
   d.heads = k.n_heads;
@@ -1115,6 +1118,20 @@ mpcx_status mpcx_cache_append(mpcx_ctx *c, const mpcx_cache *cache, size_t n_tok
   }
   if (rot && (!aligned(rot->d_cos, tb) || !aligned(rot->d_sin, tb)))
     return fail(c, MPCX_EINVAL, "cache_append: misaligned pointer");
+  const size_t pool = cache_plane_bytes(c, *cache);
+  for (int p = 0; p < n_planes; p++) {
+    const void *to = planes[p].d_pool;
+    bool ok = bytes_apart(to, pool, slot, n_tok * sizeof *slot);
+    if (turned) {
+      const size_t table = size_t(rot->n_pos) * size_t(rot->half) * tb;
+      ok = ok && bytes_apart(to, pool, pos, n_tok * sizeof *pos) && bytes_apart(to, pool, rot->d_cos, table) &&
+           bytes_apart(to, pool, rot->d_sin, table);
+    }
+    for (int q = 0; q < n_planes; q++)
+      ok = ok && rows_apart(word_rows(c, planes[q].d_rows, n_tok, planes[q].ld, row), to, pool) &&
+           (q >= p || bytes_apart(to, pool, planes[q].d_pool, pool));
+    if (!ok) return fail(c, MPCX_EINVAL, "cache_append: a pool overlaps another buffer");
+  }
   return c->bw == 32 ? cache_append_t<uint32_t>(c, cache, n_tok, slot, pos, rot, n_planes, planes)
                      : cache_append_t<uint64_t>(c, cache, n_tok, slot, pos, rot, n_planes, planes);
 }
@@ -1268,7 +1285,7 @@ mpcx_status attn_eval(mpcx_ctx *c, bool scores, AttnForm form, const mpcx_attn *
     if (!aligned(p, tb)) return fail(c, MPCX_EINVAL, "attn_eval: misaligned pointer");
   if (!aligned(k0, 16) || !aligned(k1, 16)) return fail(c, MPCX_EINVAL, "attn_eval: misaligned pointer");
   const size_t nb = second * tb, key = attn_key_end(c, first, second);
-  const size_t plane = size_t(a->cache.n_pages) * a->cache.n_heads * a->cache.page_size * a->cache.head_dim * tb;
+  const size_t plane = cache_plane_bytes(c, a->cache);
   if (!bytes_apart(out, nb, x, first * tb) || (p0 && !bytes_apart(out, nb, k0, key)) ||
       (p1 && !bytes_apart(out, nb, k1, key)) || !bytes_apart(out, nb, y, plane) ||
       (p0 && !bytes_apart(out, nb, b0, plane)) || (p1 && !bytes_apart(out, nb, b1, plane)))

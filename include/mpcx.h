@@ -382,7 +382,8 @@ typedef struct {
  * shares.  A token whose slot is outside the cache (-1: padding) is not written,
  * nor are the rotated planes of one whose position is outside the tables.  The
  * slots of a call are distinct.  rot (host) and d_pos may be NULL where no plane
- * is rotated; the pools overlap neither each other nor the rows. */
+ * is rotated.  The pools overlap neither each other nor the rows and tables
+ * (refused). */
 mpcx_status mpcx_cache_append(mpcx_ctx *ctx, const mpcx_cache *cache, size_t n_tok, const int64_t *d_slot,
                               const int32_t *d_pos, const mpcx_rotation *rot, int n_planes,
                               const mpcx_cache_plane *planes);

@@ -114,3 +114,31 @@ def test_q4_into_columns_of_its_operand(ctx, M):
     ctx.ring_gemm_q4(d[:, :K], dev(q4_pack(w)), dev(scale), group, out=d[:, K + 1:K + 1 + N])
     big[:, K + 1:K + 1 + N] = q4_plain(a, w, scale, group)
     assert np.array_equal(host(d, ctx.bw), big)
+
+
+def test_cache_append_pool_over_another_buffer(ctx):
+    import torch
+    tb = ctx.bw // 8
+    cache, n, row = mpcx.Cache(2, 8, 4, 3), 5, 16
+    pool = 2 * 8 * 4 * 3 * tb
+    buf = torch.zeros(8 << 18, dtype=torch.uint8, device="cuda")
+    rows0, rows1, pool0, pool1, slot, pos, cos, sin = (buf.data_ptr() + (i << 18) for i in range(8))
+    buf[4 << 18:(4 << 18) + 8 * n].view(torch.int64).copy_(torch.arange(n))
+    torch.cuda.synchronize()
+
+    def call(rows0=rows0, ld0=row, pool0=pool0, rows1=rows1, pool1=pool1, slot=slot, pos=pos, cos=cos, sin=sin, turn=1):
+        planes = (mpcx._CachePlane * 2)(mpcx._CachePlane(rows0, ld0, pool0, turn), mpcx._CachePlane(rows1, row, pool1, 0))
+        return ctx.lib.mpcx_cache_append(ctx.h, C.byref(cache), n, slot, pos, C.byref(mpcx._Rotation(4, 0, 8, 3, cos, sin)),
+                                         2, planes)
+
+    assert call() == 0
+    for bad in (dict(pool0=rows0), dict(pool0=rows1), dict(pool1=rows0 + (n * row - 1) * tb), dict(pool1=pool0),
+                dict(pool1=pool0 + pool - tb), dict(pool0=pool1 + pool - tb), dict(pool0=slot), dict(pool1=slot + 8 * n - 8),
+                dict(pool0=pos), dict(pool1=cos), dict(pool1=sin + 32 * tb - tb), dict(rows0=pool1 - tb),
+                dict(ld0=4096, pool1=rows0 + 4096 * tb * (n - 1) - tb)):
+        assert call(**bad) == EINVAL, bad
+        assert b"overlaps" in ctx.lib.mpcx_last_error(ctx.h)
+    # between the rows, at a table that no plane uses, and just past the rows
+    assert call(ld0=4096, pool1=rows0 + 4096 * tb + row * tb) == 0
+    assert call(turn=0, pool0=cos) == 0 and call(pool0=rows0 + n * row * tb) == 0
+    ctx.sync()
