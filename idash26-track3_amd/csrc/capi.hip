@@ -1175,6 +1175,14 @@ size_t attn_key_end(const mpcx_ctx *c, size_t first, size_t second) {
 bool attn_has_tables(const mpcx_attn *a) {
   return a->d_pages && a->d_qstart && a->d_lo && a->d_hi && a->d_off;
 }
+// True where n bytes at p overlap none of the batch's tables.
+bool tables_apart(const mpcx_attn *a, const void *p, size_t n) {
+  const size_t toks = size_t(a->n_tok), seqs = size_t(a->n_seq);
+  return bytes_apart(p, n, a->d_pages, seqs * size_t(a->max_pages) * sizeof *a->d_pages) &&
+         bytes_apart(p, n, a->d_qstart, (seqs + 1) * sizeof *a->d_qstart) &&
+         bytes_apart(p, n, a->d_lo, toks * sizeof *a->d_lo) && bytes_apart(p, n, a->d_hi, toks * sizeof *a->d_hi) &&
+         bytes_apart(p, n, a->d_off, toks * sizeof *a->d_off);
+}
 template <typename T>
 AttnArgs<T> attn_args(const mpcx_attn *a) {
   AttnArgs<T> g;
@@ -1284,11 +1292,13 @@ mpcx_status attn_eval(mpcx_ctx *c, bool scores, AttnForm form, const mpcx_attn *
   for (const void *p : {x, y, b0, b1, slope, static_cast<const void *>(out)})
     if (!aligned(p, tb)) return fail(c, MPCX_EINVAL, "attn_eval: misaligned pointer");
   if (!aligned(k0, 16) || !aligned(k1, 16)) return fail(c, MPCX_EINVAL, "attn_eval: misaligned pointer");
-  const size_t nb = second * tb, key = attn_key_end(c, first, second);
-  const size_t plane = cache_plane_bytes(c, a->cache);
+  const size_t nb = second * tb, key = attn_key_end(c, first, second), plane = cache_plane_bytes(c, a->cache);
   if (!bytes_apart(out, nb, x, first * tb) || (p0 && !bytes_apart(out, nb, k0, key)) ||
       (p1 && !bytes_apart(out, nb, k1, key)) || !bytes_apart(out, nb, y, plane) ||
-      (p0 && !bytes_apart(out, nb, b0, plane)) || (p1 && !bytes_apart(out, nb, b1, plane)))
+      (p0 && !bytes_apart(out, nb, b0, plane)) || (p1 && !bytes_apart(out, nb, b1, plane)) ||
+      (slope && (!bytes_apart(out, nb, slope, size_t(a->n_heads) * tb) ||
+                 !bytes_apart(out, nb, pos, size_t(a->n_tok) * sizeof *pos))) ||
+      !tables_apart(a, out, nb))
     return fail(c, MPCX_EINVAL, "attn_eval: the output overlaps an input");
   return c->bw == 32
              ? attn_eval_t<uint32_t>(c, scores, form, a, first, second, k0, k1, x, y, b0, b1, slope, pos, out)

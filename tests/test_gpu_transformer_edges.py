@@ -142,3 +142,50 @@ def test_cache_append_pool_over_another_buffer(ctx):
     assert call(ld0=4096, pool1=rows0 + 4096 * tb + row * tb) == 0
     assert call(turn=0, pool0=cos) == 0 and call(pool0=rows0 + n * row * tb) == 0
     ctx.sync()
+
+
+class Gate:
+    """The buffers of an attention gate, each at a place of its own, as the C calls
+    take them."""
+
+    def __init__(self, ctx, scores):
+        import torch
+        self.ctx, self.scores, self.tb = ctx, scores, ctx.bw // 8
+        names = "pages qstart lo hi off slope pos x y b0 b1 k0 k1 out".split()
+        self.buf = torch.zeros(len(names) << 18, dtype=torch.uint8, device="cuda")
+        self.at = {n: self.buf.data_ptr() + (i << 18) for i, n in enumerate(names)}
+        for name, values in dict(pages=[2, 0], qstart=[0, 3], lo=[0, 0, 1], hi=[2, 3, 5], off=[0, 8, 20, 36],
+                                 pos=[1, 2, 4]).items():
+            t = torch.tensor(values[:3], dtype=torch.int64 if name == "off" else torch.int32)
+            self.buf[self.at[name] - self.buf.data_ptr():][:t.numel() * t.element_size()] = t.view(torch.uint8).cuda()
+        self.rows, self.wide = 3 * 4 * 8, 36
+        self.left, self.to = (self.rows, self.wide) if scores else (self.wide, self.rows)
+        self.bytes = dict(pages=8, qstart=8, lo=12, hi=12, off=24, slope=4 * self.tb, pos=12, x=self.left * self.tb,
+                          y=192 * self.tb, b0=192 * self.tb, b1=192 * self.tb, out=self.to * self.tb)
+        key = (self.left * self.tb + 255) // 256 * 256 + (self.to * self.tb + 255) // 256 * 256
+        self.bytes.update(k0=key, k1=key)
+        torch.cuda.synchronize()
+
+    def batch(self, v):
+        return mpcx._Attn(mpcx.Cache(2, 8, 4, 3), 4, 3, 1, 2, 3, 5, self.wide, v["pages"], v["qstart"], v["lo"], v["hi"],
+                          v["off"])
+
+    def eval(self, **over):
+        v = {**self.at, **over}
+        f = self.ctx.lib.mpcx_attn_scores_eval if self.scores else self.ctx.lib.mpcx_attn_mix_eval
+        extra = [v["slope"], v["pos"]] if self.scores else []
+        return f(self.ctx.h, C.byref(self.batch(v)), *[v[n] for n in ("k0", "k1", "x", "y", "b0", "b1")], *extra, v["out"])
+
+
+@pytest.mark.parametrize("scores", [True, False])
+def test_attn_output_over_an_input(ctx, scores):
+    g = Gate(ctx, scores)
+    assert g.eval() == 0
+    for n in g.at:
+        if n == "out" or (not scores and n in ("slope", "pos")):
+            continue
+        for out in (g.at[n], g.at[n] + (g.bytes[n] - 1) // g.tb * g.tb, g.at[n] - g.bytes["out"] + g.tb):
+            assert g.eval(out=out) == EINVAL, (n, out)
+            assert b"overlaps" in ctx.lib.mpcx_last_error(ctx.h)
+        assert g.eval(out=g.at[n] + (g.bytes[n] + g.tb - 1) // g.tb * g.tb) == 0, n
+    ctx.sync()
