@@ -1248,6 +1248,14 @@ mpcx_status attn_keygen(mpcx_ctx *c, bool scores, const mpcx_attn *a, const void
   if (!aligned(k0, 16) || !aligned(k1, 16) || !aligned(rx, tb) || !aligned(b0, tb) || !aligned(b1, tb) ||
       !aligned(rz, tb))
     return fail(c, MPCX_EINVAL, "attn_keygen: misaligned pointer");
+  const size_t nz = second * tb, key = attn_key_end(c, first, second), plane = cache_plane_bytes(c, a->cache);
+  auto apart = [&](const void *p, size_t n) {  // an output and the inputs
+    return bytes_apart(p, n, rx, first * tb) && bytes_apart(p, n, b0, plane) && bytes_apart(p, n, b1, plane) &&
+           tables_apart(a, p, n);
+  };
+  if (!apart(rz, nz) || !apart(k0, key) || !apart(k1, key) || !bytes_apart(rz, nz, k0, key) ||
+      !bytes_apart(rz, nz, k1, key) || !bytes_apart(k0, key, k1, key))
+    return fail(c, MPCX_EINVAL, "attn_keygen: an output overlaps another buffer");
   return c->bw == 32 ? attn_keygen_t<uint32_t>(c, scores, a, first, second, rx, b0, b1, rz, seed, gate, k0, k1)
                      : attn_keygen_t<uint64_t>(c, scores, a, first, second, rx, b0, b1, rz, seed, gate, k0, k1);
 }

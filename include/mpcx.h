@@ -406,8 +406,8 @@ mpcx_status mpcx_split_mask(mpcx_ctx *ctx, size_t n, const void *d_mask, uint64_
  * scores, and their rows of a weighted sum are unspecified.  max_q and max_keys,
  * about the most tokens of a sequence and keys of a range, size the launch only.
  * n_seq times the cache's heads times the groups of 256 bytes of a head is below
- * 2^23.  A gate's output overlaps none of its inputs, these tables included
- * (refused). */
+ * 2^23.  A gate's output, and a keygen's three, overlap no other buffer, these
+ * tables included (refused). */
 typedef struct {
   mpcx_cache cache;
   int n_heads, n_tok, n_seq, max_pages, max_q, max_keys;

@@ -176,6 +176,12 @@ class Gate:
         extra = [v["slope"], v["pos"]] if self.scores else []
         return f(self.ctx.h, C.byref(self.batch(v)), *[v[n] for n in ("k0", "k1", "x", "y", "b0", "b1")], *extra, v["out"])
 
+    def keygen(self, **over):
+        """x is the left operand's mask, out the output's."""
+        v = {**self.at, **over}
+        f = self.ctx.lib.mpcx_attn_scores_keygen if self.scores else self.ctx.lib.mpcx_attn_mix_keygen
+        return f(self.ctx.h, C.byref(self.batch(v)), v["x"], v["b0"], v["b1"], v["out"], 1, 1, v["k0"], v["k1"])
+
 
 @pytest.mark.parametrize("scores", [True, False])
 def test_attn_output_over_an_input(ctx, scores):
@@ -188,4 +194,21 @@ def test_attn_output_over_an_input(ctx, scores):
             assert g.eval(out=out) == EINVAL, (n, out)
             assert b"overlaps" in ctx.lib.mpcx_last_error(ctx.h)
         assert g.eval(out=g.at[n] + (g.bytes[n] + g.tb - 1) // g.tb * g.tb) == 0, n
+    ctx.sync()
+
+
+@pytest.mark.parametrize("scores", [True, False])
+def test_attn_keygen_output_over_another_buffer(ctx, scores):
+    g = Gate(ctx, scores)
+    assert g.keygen() == 0
+    for to in ("out", "k0", "k1"):
+        step = 16 if to != "out" else g.tb  # keys are aligned to 16 bytes
+        for n in g.at:
+            if n == to or n in ("y", "slope", "pos"):
+                continue
+            past = -(-(g.at[n] + g.bytes[n]) // step) * step
+            for at in (g.at[n], past - step, (g.at[n] - g.bytes[to]) // step * step + step):
+                assert g.keygen(**{to: at}) == EINVAL, (to, n, at)
+                assert b"overlaps" in ctx.lib.mpcx_last_error(ctx.h)
+            assert g.keygen(**{to: past}) == 0, (to, n)
     ctx.sync()
