@@ -1148,6 +1148,13 @@ mpcx_status mpcx_split_mask(mpcx_ctx *c, size_t n, const void *mask, uint64_t se
   CHECK_CTX(c);
   if (n == 0) return MPCX_OK;
   if (!mask || !s0 || !s1) return fail(c, MPCX_EINVAL, "split_mask: null pointer");
+  if (n > size_t(1) << 60) return fail(c, MPCX_EINVAL, "split_mask: bad argument");
+  const size_t tb = size_t(c->bw) / 8, nb = n * tb;
+  if (!aligned(mask, tb) || !aligned(s0, tb) || !aligned(s1, tb))
+    return fail(c, MPCX_EINVAL, "split_mask: misaligned pointer");
+  if (!bytes_apart(s0, nb, s1, nb) || (s0 != mask && !bytes_apart(s0, nb, mask, nb)) ||
+      (s1 != mask && !bytes_apart(s1, nb, mask, nb)))
+    return fail(c, MPCX_EINVAL, "split_mask: a share overlaps another buffer");
   return c->bw == 32 ? split_mask_t<uint32_t>(c, n, mask, seed, gate, s0, s1)
                      : split_mask_t<uint64_t>(c, n, mask, seed, gate, s0, s1);
 }

@@ -389,7 +389,8 @@ mpcx_status mpcx_cache_append(mpcx_ctx *ctx, const mpcx_cache *cache, size_t n_t
                               const mpcx_cache_plane *planes);
 /* The dealer's shares of a mask: share0 pseudorandom, share0 + share1 = mask
  * (n words each): what a party's share plane of the cache is appended from
- * (writeShares, gpu_mpc/ddg_orca_base.h:394-410). */
+ * (writeShares, gpu_mpc/ddg_orca_base.h:394-410).  One share may take the mask's
+ * place; other overlaps are refused. */
 mpcx_status mpcx_split_mask(mpcx_ctx *ctx, size_t n, const void *d_mask, uint64_t seed, uint32_t gate,
                             void *d_share0, void *d_share1);
 

@@ -212,3 +212,30 @@ def test_attn_keygen_output_over_another_buffer(ctx, scores):
                 assert b"overlaps" in ctx.lib.mpcx_last_error(ctx.h)
             assert g.keygen(**{to: past}) == 0, (to, n)
     ctx.sync()
+
+
+def test_split_mask_buffers(ctx):
+    import torch
+    n, tb = 300, ctx.bw // 8
+    buf = torch.zeros(3 << 16, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    m, s0, s1 = (buf.data_ptr() + (i << 16) for i in range(3))
+
+    def call(m=m, s0=s0, s1=s1):
+        return ctx.lib.mpcx_split_mask(ctx.h, n, m, 1, 1, s0, s1)
+
+    assert call() == 0
+    for bad in (dict(s0=s1), dict(s0=s1 + (n - 1) * tb), dict(s0=m + tb), dict(s1=m + (n - 1) * tb), dict(m=s0 + tb),
+                dict(m=s0 + 1), dict(s0=m + n * tb + 1), dict(s1=s1 + tb // 2), dict(s0=m, s1=m)):
+        assert call(**bad) == EINVAL, bad
+    ctx.sync()
+    mask = words(np.random.default_rng(3), (n,), ctx.bw)
+    want = [host(s, ctx.bw) for s in ctx.split_mask(dev(mask), seed=5, gate=6)]
+    for place in (0, 1):  # a share in the mask's place
+        d, other = dev(mask), dev(mask)
+        torch.cuda.synchronize()
+        to = [other.data_ptr(), other.data_ptr()]
+        to[place] = d.data_ptr()
+        assert ctx.lib.mpcx_split_mask(ctx.h, n, d.data_ptr(), 5, 6, *to) == 0
+        ctx.sync()
+        assert np.array_equal(host(d, ctx.bw), want[place]) and np.array_equal(host(other, ctx.bw), want[1 - place])
