@@ -1179,8 +1179,8 @@ size_t attn_key_second(const mpcx_ctx *c, size_t first) { return align_up(first 
 size_t attn_key_end(const mpcx_ctx *c, size_t first, size_t second) {
   return align_up(attn_key_second(c, first) + second * (c->bw / 8));
 }
-bool attn_has_tables(const mpcx_attn *a) {
-  return a->d_pages && a->d_qstart && a->d_lo && a->d_hi && a->d_off;
+bool attn_has_tables(const mpcx_attn *a) {  // page rows of no page have no memory
+  return (a->d_pages || a->max_pages == 0) && a->d_qstart && a->d_lo && a->d_hi && a->d_off;
 }
 // True where n bytes at p overlap none of the batch's tables.
 bool tables_apart(const mpcx_attn *a, const void *p, size_t n) {

@@ -239,3 +239,19 @@ def test_split_mask_buffers(ctx):
         assert ctx.lib.mpcx_split_mask(ctx.h, n, d.data_ptr(), 5, 6, *to) == 0
         ctx.sync()
         assert np.array_equal(host(d, ctx.bw), want[place]) and np.array_equal(host(other, ctx.bw), want[1 - place])
+
+
+# ---------------- lengths of zero ----------------
+def test_attn_without_pages(ctx):
+    """Sequences that have no page yet: every token sees nothing."""
+    B = Batch(ctx.bw, 2, 3, 5, 4, 2, 8, 4, "causal", seed=2)
+    i32 = np.int32
+    none = dev(np.zeros(B.tokens, i32))
+    g = mpcx.AttnBatch(dev(np.zeros((2, 0), i32)), dev(B.qstart), none, none, dev(np.zeros(B.tokens, np.int64)), 0, 4, 3, 1)
+    planes = [dev(v) for v in (B.y, B.b0, B.b1)]
+    nothing = dev(np.zeros(0, ctx.T))
+    k0, k1, ro = ctx.attn_mix_keygen(g, nothing, *planes[1:], seed=3)
+    assert np.array_equal(host(ctx.attn_mix_eval(g, k0, k1, nothing, *planes), ctx.bw), host(ro, ctx.bw))
+    q = dev(words(B.rng, (B.tokens, 4, 8), ctx.bw))
+    k0, k1, rs = ctx.attn_scores_keygen(g, q, *planes[1:])
+    assert rs.shape == (0,) and ctx.attn_scores_eval(g, k0, k1, q, *planes).shape == (0,)
