@@ -778,6 +778,8 @@ class Ctx:
         torch = _torch()
         a, nb, left, to = self._attn_gate(what, scores, b, y)
         out = self._new(to)
+        if party is not None:
+            out.zero_()  # words of no token's block are sent, too: nothing of what was in this memory before
         args = [self._key(k, nb, what) for k in keys]
         args += [self._words(x, what, left), self._words(y, what)] + [self._words(s, what, y.shape) for s in shares]
         if scores:

@@ -446,7 +446,9 @@ mpcx_status mpcx_attn_mix_eval(mpcx_ctx *ctx, const mpcx_attn *a, const void *d_
                                void *d_ohat);
 /* One party's message of the two gates (party 0 or 1, its own key and share
  * plane): both parties' messages add up to the gate's output, by
- * mpcx_party_reconstruct. */
+ * mpcx_party_reconstruct.  Scores in no token's block and sums of tokens of no
+ * sequence are not written: a caller who sends a message whole clears it before,
+ * so that what its memory held is not sent. */
 mpcx_status mpcx_attn_scores_message(mpcx_ctx *ctx, int party, const mpcx_attn *a, const void *d_key,
                                      const void *d_qhat, const void *d_khat, const void *d_kb, const void *d_slope,
                                      const int32_t *d_pos, void *d_msg);

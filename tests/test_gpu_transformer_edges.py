@@ -255,3 +255,32 @@ def test_attn_without_pages(ctx):
     q = dev(words(B.rng, (B.tokens, 4, 8), ctx.bw))
     k0, k1, rs = ctx.attn_scores_keygen(g, q, *planes[1:])
     assert rs.shape == (0,) and ctx.attn_scores_eval(g, k0, k1, q, *planes).shape == (0,)
+
+
+# ---------------- what a party sends ----------------
+def test_messages_hold_nothing_of_earlier_memory(ctx):
+    """Words of no token's block and rows of tokens of no sequence go to the other
+    party with the rest."""
+    import torch
+    B = Batch(ctx.bw, 2, 4, 30, 4, 2, 8, 4, "ragged", seed=4, gap=9)
+    B.qstart[-1] -= 1  # the last token is of no sequence
+    last = B.tokens - 1
+    g, planes = B.gpu(), [dev(v) for v in (B.y, B.b0, B.b1)]
+    q, p = dev(words(B.rng, (B.tokens, 4, 8), ctx.bw)), dev(words(B.rng, (B.n,), ctx.bw))
+    ks, km = ctx.attn_scores_keygen(g, q, *planes[1:]), ctx.attn_mix_keygen(g, p, *planes[1:])
+    seen = B.inside()
+    for t, _, _, o in B.blocks():
+        if t == last:
+            seen[o] = False
+    assert (~seen).sum() > 9
+    for i in (0, 1):
+        for scores in (True, False):
+            old = torch.full((B.n,) if scores else tuple(q.shape), 0x5A5A5A5A, dtype=q.dtype, device="cuda")
+            torch.cuda.synchronize()
+            del old  # its memory is the next tensor's of this size
+            if scores:
+                m = host(ctx.attn_scores_message(i, g, ks[i], q, planes[0], planes[1 + i]), ctx.bw)
+                assert (m[~seen] == 0).all() and m[seen].any()
+            else:
+                m = host(ctx.attn_mix_message(i, g, km[i], p, planes[0], planes[1 + i]), ctx.bw)
+                assert (m[last] == 0).all() and m[:last].any()
