@@ -703,9 +703,10 @@ class Ctx:
     def gate_eval(self, kind, k0, k1, xhat):
         """tr_eval on a tensor of masked words."""
         out, xp = self._new(xhat.shape), self._words(xhat, "gate_eval")
+        nb = self.lib.mpcx_tr_key_bytes(self.h, kind, xhat.numel())
+        keys = [self._key(k, nb, "gate_eval") if nb else None for k in (k0, k1)]  # LOCALARS has none
         same = self._enter()
-        self.check(self.lib.mpcx_tr_eval(self.h, kind, xhat.numel(), dptr(k0), dptr(k1), xp, None, 0, out.data_ptr()),
-                   "tr_eval")
+        self.check(self.lib.mpcx_tr_eval(self.h, kind, xhat.numel(), *keys, xp, None, 0, out.data_ptr()), "tr_eval")
         self._leave(same)
         return out
 

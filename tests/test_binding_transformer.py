@@ -1,0 +1,91 @@
+"""What the binding's tensor calls check before they enter the library: on the CPU,
+with stand-ins for the tensors and the library."""
+import math
+import types
+
+import pytest
+
+import mpcx
+
+INT, LONG, BYTE = (types.SimpleNamespace(name=n, size=s) for n, s in (("int32", 4), ("int64", 8), ("uint8", 1)))
+
+
+class Tensor:
+    """Shape, strides and place of a GPU tensor."""
+
+    def __init__(self, shape, dtype=None, device=0, stride=None):
+        self.shape, self.dtype, self.device_index = tuple(shape), dtype or INT, device
+        self.strides = stride or tuple(math.prod(self.shape[i + 1:]) for i in range(len(self.shape)))
+
+    is_cuda = property(lambda self: self.device_index >= 0)
+
+    def get_device(self):
+        return self.device_index
+
+    def is_contiguous(self):
+        want = 1
+        for n, s in zip(reversed(self.shape), reversed(self.strides)):
+            if n != 1 and s != want:
+                return False
+            want *= n
+        return True
+
+    def stride(self, d=None):
+        return self.strides if d is None else self.strides[d]
+
+    def dim(self):
+        return len(self.shape)
+
+    def numel(self):
+        return math.prod(self.shape)
+
+    def element_size(self):
+        return self.dtype.size
+
+    def data_ptr(self):
+        return 4096
+
+    def zero_(self):
+        return self
+
+
+class Lib:
+    """Says that a key or workspace has 1000 bytes; records the other calls."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*a):
+            if name.endswith("_bytes"):
+                return 1000
+            if name != "mpcx_synchronize":
+                self.calls.append((name, a))
+            return 0
+        return call
+
+
+@pytest.fixture
+def ctx(monkeypatch):
+    stream = types.SimpleNamespace(cuda_stream=7, synchronize=lambda: None)
+    torch = types.SimpleNamespace(int32=INT, int64=LONG, uint8=BYTE, empty=lambda shape, dtype=None, device=None: Tensor(
+        shape if isinstance(shape, tuple) else (shape,), dtype, device),
+        zeros=lambda n, dtype=None, device=None: Tensor((n,), dtype, 0 if device == "cuda" else device),
+        cuda=types.SimpleNamespace(current_stream=lambda device=None: stream))
+    monkeypatch.setattr(mpcx, "_torch_module", torch)
+    monkeypatch.setattr(mpcx, "_torch", lambda: torch)
+    c = mpcx.Ctx.__new__(mpcx.Ctx)
+    c.lib, c.h, c.bw, c._word, c._device, c._stream_id = Lib(), None, 32, INT, 0, 7
+    return c
+
+
+@pytest.mark.parametrize("bad", [dict(shape=(999,)), dict(shape=(1000,), device=-1), dict(shape=(1000,), stride=(2,)),
+                                 dict(shape=(0,))])
+def test_gate_eval_checks_its_keys(ctx, bad):
+    key, x = Tensor((1000,), BYTE), Tensor((5,))
+    ctx.gate_eval(mpcx.TR, key, key, x)
+    assert [c[0] for c in ctx.lib.calls] == ["mpcx_tr_eval"]
+    for keys in ((Tensor(dtype=BYTE, **bad), key), (key, Tensor(dtype=BYTE, **bad))):
+        with pytest.raises(mpcx.MpcxError):
+            ctx.gate_eval(mpcx.TR, *keys, x)
+    assert len(ctx.lib.calls) == 1

@@ -284,3 +284,18 @@ def test_messages_hold_nothing_of_earlier_memory(ctx):
             else:
                 m = host(ctx.attn_mix_message(i, g, km[i], p, planes[0], planes[1 + i]), ctx.bw)
                 assert (m[last] == 0).all() and m[:last].any()
+
+
+def test_gate_eval_keys(ctx):
+    """A key of another gate or of fewer words is refused; a gate without keys takes none."""
+    x = dev(words(np.random.default_rng(1), (100,), ctx.bw))
+    k0, k1, _ = ctx.gate_keygen(mpcx.TRRELU, x)
+    short, _, _ = ctx.gate_keygen(mpcx.TRRELU, x[:40].contiguous())
+    other, _, _ = ctx.gate_keygen(mpcx.TR, x)
+    assert other.numel() < k0.numel()
+    ctx.gate_eval(mpcx.TRRELU, k0, k1, x)
+    for a, b in ((short, k1), (k0, short), (other, k1), (k0, k1.cpu()), (k0[1:], k1)):
+        with pytest.raises(mpcx.MpcxError):
+            ctx.gate_eval(mpcx.TRRELU, a, b, x)
+    word = host(x, ctx.bw).view(np.int32 if ctx.bw == 32 else np.int64)
+    assert np.array_equal(host(ctx.gate_eval(mpcx.LOCALARS, None, None, x), ctx.bw).view(word.dtype), word >> 12)
