@@ -634,6 +634,8 @@ class Ctx:
         """mpcx_ring_gemm_q4: a (M, K) ring words (rows may be apart), q (N, rows of
         whole 32 weights) uint8, scale (groups, N) int32 -> (M, N)."""
         torch = _torch()
+        if group < 1:
+            raise MpcxError(f"ring_gemm_q4: groups of {group}")
         ap, lda = self._rows(a, "ring_gemm_q4: a")
         M, K = a.shape
         N = q.shape[0]

@@ -89,3 +89,10 @@ def test_gate_eval_checks_its_keys(ctx, bad):
         with pytest.raises(mpcx.MpcxError):
             ctx.gate_eval(mpcx.TR, *keys, x)
     assert len(ctx.lib.calls) == 1
+
+
+@pytest.mark.parametrize("group", [0, -32])
+def test_q4_groups_of_nothing(ctx, group):
+    with pytest.raises(mpcx.MpcxError):
+        ctx.ring_gemm_q4(Tensor((2, 64)), Tensor((4, 32), BYTE), Tensor((2, 4)), group)
+    assert not ctx.lib.calls
