@@ -244,6 +244,12 @@ def from_dev(t, dtype, count=None):
     return out if count is None else out[:count]
 
 
+def _c_ints(what, *sizes):
+    """Refuses sizes past a C int, which ctypes would cut short."""
+    if max(sizes) > 0x7FFFFFFF:
+        raise MpcxError(f"{what}: a size of {max(sizes)}")
+
+
 def dptr(t):
     return C.c_void_p(t.data_ptr()) if t is not None else None
 
@@ -639,6 +645,7 @@ class Ctx:
         ap, lda = self._rows(a, "ring_gemm_q4: a")
         M, K = a.shape
         N = q.shape[0]
+        _c_ints("ring_gemm_q4", M, K, N, group)
         if out is None:
             out = self._new((M, N))
         op, ldc = self._rows(out, "ring_gemm_q4: out")
@@ -668,6 +675,7 @@ class Ctx:
         torch = _torch()
         n = slot.shape[0]
         pool = planes[0][1].shape
+        _c_ints("cache_append", *pool[1:])
         shape, near = (n, pool[1], pool[3]), (pool[3], 1)
         sp = self._ints(slot, "cache_append: slot", torch.int64, (n,))
         pp = self._ints(pos, "cache_append: pos", torch.int32, (n,)) if pos is not None else None
@@ -681,6 +689,7 @@ class Ctx:
         rot = None
         if rotation is not None:
             c = rotation.cos
+            _c_ints("cache_append", *c.shape, rotation.shift)
             rot = C.byref(_Rotation(c.shape[1], int(rotation.pairs), c.shape[0], rotation.shift,
                                     self._words(c, "cache_append: cos"),
                                     self._words(rotation.sin, "cache_append: sin", c.shape)))
@@ -725,6 +734,7 @@ class Ctx:
     def _attn(self, b, pool):
         torch = _torch()
         n, seqs = b.lo.shape[0], b.pages.shape[0]
+        _c_ints("attn", n, *b.pages.shape, b.heads, b.max_q, b.max_keys, *pool.shape[1:])
         i32 = torch.int32
         return _Attn(self._cache(pool), b.heads, n, seqs, b.pages.shape[1], b.max_q, b.max_keys, b.n_scores,
                      self._ints(b.pages, "attn: pages", i32, b.pages.shape),

@@ -96,3 +96,54 @@ def test_q4_groups_of_nothing(ctx, group):
     with pytest.raises(mpcx.MpcxError):
         ctx.ring_gemm_q4(Tensor((2, 64)), Tensor((4, 32), BYTE), Tensor((2, 4)), group)
     assert not ctx.lib.calls
+
+
+BIG = (1 << 32) + 2  # 2 where a C int is taken
+
+
+@pytest.mark.parametrize("M,K,N", [(BIG, 64, 4), (2, BIG, 4), (2, 64, BIG)])
+def test_q4_sizes_past_a_c_int(ctx, M, K, N):
+    args = Tensor((M, K)), Tensor((N, (K + 31) // 32 * 16), BYTE), Tensor((-(-K // 32), N))
+    with pytest.raises(mpcx.MpcxError):
+        ctx.ring_gemm_q4(*args, 32)
+    assert not ctx.lib.calls
+    ctx.ring_gemm_q4(Tensor((2, 64)), Tensor((4, 32), BYTE), Tensor((2, 4)), 32)
+    assert len(ctx.lib.calls) == 1
+
+
+def batch(seqs=1, tokens=2, pages=3, **kw):
+    v = dict(n_scores=8, heads=2, max_q=2, max_keys=4)
+    v.update(kw)
+    return mpcx.AttnBatch(Tensor((seqs, pages)), Tensor((seqs + 1,)), Tensor((tokens,)), Tensor((tokens,)),
+                          Tensor((tokens,), LONG), **v)
+
+
+def mix(ctx, b, pool=(5, 2, 4, 8)):
+    key = Tensor((1000,), BYTE)
+    return ctx.attn_mix_eval(b, key, key, Tensor((b.n_scores,)), *[Tensor(pool) for _ in range(3)])
+
+
+@pytest.mark.parametrize("over", [dict(tokens=BIG), dict(seqs=BIG), dict(pages=BIG), dict(heads=BIG), dict(max_q=BIG),
+                                  dict(max_keys=BIG)])
+def test_attn_sizes_past_a_c_int(ctx, over):
+    with pytest.raises(mpcx.MpcxError):
+        mix(ctx, batch(**over))
+    assert not ctx.lib.calls
+    assert mix(ctx, batch()).shape == (2, 2, 8)
+
+
+@pytest.mark.parametrize("at", [1, 2, 3])
+def test_cache_sizes_past_a_c_int(ctx, at):
+    pool = [5, 2, 4, 8]
+    pool[at] = BIG
+    with pytest.raises(mpcx.MpcxError):
+        mix(ctx, batch(), tuple(pool))
+    with pytest.raises(mpcx.MpcxError):
+        ctx.cache_append([(Tensor((2, pool[1], pool[3])), Tensor(pool), False)], Tensor((2,), LONG))
+    with pytest.raises(mpcx.MpcxError):  # the table's sizes
+        ctx.cache_append([(Tensor((2, 2, 8)), Tensor((5, 2, 4, 8)), True)], Tensor((2,), LONG), Tensor((2,)),
+                         mpcx.Rotation(Tensor((BIG, 4)), Tensor((BIG, 4)), 12))
+    assert not ctx.lib.calls
+    ctx.cache_append([(Tensor((2, 2, 8)), Tensor((5, 2, 4, 8)), True)], Tensor((2,), LONG), Tensor((2,)),
+                     mpcx.Rotation(Tensor((9, 4)), Tensor((9, 4)), 12))
+    assert len(ctx.lib.calls) == 1
