@@ -226,13 +226,13 @@ def to_dev(a):
     return torch.from_numpy(a.view(view)).cuda()
 
 
-def empty_dev(nbytes):
-    """Zeroed device bytes, zeroed when this returns: the library works on a
-    stream that is not ordered with torch's, so a fill still pending there could
-    land on top of its results."""
+def empty_dev(nbytes, device=None):
+    """Zeroed bytes on a GPU (None: torch's current one), zeroed when this returns:
+    the library works on a stream that is not ordered with torch's, so a fill still
+    pending there could land on top of its results."""
     torch = _torch()
-    t = torch.zeros(max(int(nbytes), 1), dtype=torch.uint8, device="cuda")
-    torch.cuda.current_stream().synchronize()
+    t = torch.zeros(max(int(nbytes), 1), dtype=torch.uint8, device="cuda" if device is None else device)
+    (torch.cuda.current_stream() if device is None else torch.cuda.current_stream(device)).synchronize()
     return t
 
 
@@ -615,16 +615,15 @@ class Ctx:
 
     def _words(self, t, what, shape=None):
         """A contiguous ring tensor's address."""
-        if t.dtype is not self._word or not t.is_cuda or not t.is_contiguous():
-            raise MpcxError(f"{what}: need a contiguous int{self.bw} tensor on the GPU")
+        if t.dtype is not self._word or t.get_device() != self._device or not t.is_contiguous():
+            raise MpcxError(f"{what}: need a contiguous int{self.bw} tensor on GPU {self._device}")
         if shape is not None and t.shape != shape:
             raise MpcxError(f"{what}: shape {tuple(t.shape)}, need {tuple(shape)}")
         return t.data_ptr()
 
-    @staticmethod
-    def _ints(t, what, dtype, shape):
-        if t.dtype is not dtype or t.shape != shape or not t.is_cuda or not t.is_contiguous():
-            raise MpcxError(f"{what}: need a contiguous {dtype} tensor of shape {tuple(shape)} on the GPU")
+    def _ints(self, t, what, dtype, shape):
+        if t.dtype is not dtype or t.shape != shape or t.get_device() != self._device or not t.is_contiguous():
+            raise MpcxError(f"{what}: need a contiguous {dtype} tensor of shape {tuple(shape)} on GPU {self._device}")
         return t.data_ptr()
 
     def _new(self, shape):
@@ -632,8 +631,9 @@ class Ctx:
 
     def _rows(self, t, what):
         """A matrix of ring words whose rows may be apart: its address and row stride."""
-        if t.dtype is not self._word or not t.is_cuda or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-            raise MpcxError(f"{what}: need int{self.bw} rows on the GPU")
+        if t.dtype is not self._word or t.get_device() != self._device or t.dim() != 2 or \
+                (t.shape[1] > 1 and t.stride(1) != 1):
+            raise MpcxError(f"{what}: need int{self.bw} rows on GPU {self._device}")
         return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
     def ring_gemm_q4(self, a, q, scale, group, out=None):
@@ -682,9 +682,9 @@ class Ctx:
         arr = []
         for r, p, rotate in planes:
             to, st = self._words(p, "cache_append: pool", pool), r.stride()
-            if r.shape != shape or r.dtype is not self._word or not r.is_cuda or \
+            if r.shape != shape or r.dtype is not self._word or r.get_device() != self._device or \
                     (st[1:] != near and not r.is_contiguous()):
-                raise MpcxError(f"cache_append: rows: need int{self.bw} rows of shape {shape} on the GPU")
+                raise MpcxError(f"cache_append: rows: need int{self.bw} rows of shape {shape} on GPU {self._device}")
             arr.append(_CachePlane(r.data_ptr(), st[0] if n > 1 else shape[1] * shape[2], to, rotate))
         rot = None
         if rotation is not None:
@@ -703,7 +703,7 @@ class Ctx:
         the input's."""
         n = mask.numel()
         nb = self.lib.mpcx_tr_key_bytes(self.h, kind, n)
-        k0, k1, out = empty_dev(nb), empty_dev(nb), self._new(mask.shape)
+        k0, k1, out = empty_dev(nb, self._device), empty_dev(nb, self._device), self._new(mask.shape)
         mp = self._words(mask, "gate_keygen")
         same = self._enter()
         self.check(self.lib.mpcx_tr_keygen(self.h, kind, n, mp, out.data_ptr(), seed, gate, dptr(k0), dptr(k1)),
@@ -742,8 +742,8 @@ class Ctx:
                      self._ints(b.hi, "attn: hi", i32, (n,)), self._ints(b.off, "attn: off", torch.int64, (n,)))
 
     def _key(self, k, nb, what):
-        if k.numel() * k.element_size() < nb or not k.is_cuda or not k.is_contiguous():
-            raise MpcxError(f"{what}: need {nb} bytes on the GPU")
+        if k.numel() * k.element_size() < nb or k.get_device() != self._device or not k.is_contiguous():
+            raise MpcxError(f"{what}: need {nb} bytes on GPU {self._device}")
         return k.data_ptr()
 
     def _attn_gate(self, what, scores, b, pool):
@@ -755,7 +755,7 @@ class Ctx:
 
     def _attn_keygen(self, what, scores, b, rx, b0, b1, seed, gate):
         a, nb, left, to = self._attn_gate(what, scores, b, b0)
-        k0, k1, rz = empty_dev(nb), empty_dev(nb), self._new(to)
+        k0, k1, rz = empty_dev(nb, self._device), empty_dev(nb, self._device), self._new(to)
         ptrs = [self._words(rx, what, left), self._words(b0, what), self._words(b1, what, b0.shape)]
         same = self._enter()
         self.check(getattr(self.lib, "mpcx_" + what)(self.h, C.byref(a), *ptrs, rz.data_ptr(), seed, gate, dptr(k0),

@@ -147,3 +147,43 @@ def test_cache_sizes_past_a_c_int(ctx, at):
     ctx.cache_append([(Tensor((2, 2, 8)), Tensor((5, 2, 4, 8)), True)], Tensor((2,), LONG), Tensor((2,)),
                      mpcx.Rotation(Tensor((9, 4)), Tensor((9, 4)), 12))
     assert len(ctx.lib.calls) == 1
+
+
+def test_keys_are_made_on_the_contexts_gpu(ctx):
+    ctx._device = 1
+    keys = ctx.gate_keygen(mpcx.TR, Tensor((5,), device=1))
+    b = batch()._replace(**{n: Tensor(getattr(batch(), n).shape, getattr(batch(), n).dtype, 1)
+                            for n in ("pages", "qstart", "lo", "hi", "off")})
+    keys += ctx.attn_mix_keygen(b, Tensor((8,), device=1), Tensor((5, 2, 4, 8), device=1), Tensor((5, 2, 4, 8), device=1))
+    assert [k.get_device() for k in keys] == [1] * 6
+
+
+CALLS = {
+    "ring_gemm_q4": (lambda c, *t: c.ring_gemm_q4(*t, 32), [(2, 64), ((4, 32), BYTE), (2, 4)]),
+    "cache_append": (lambda c, r, p, s, pos, co, si: c.cache_append([(r, p, True)], s, pos, mpcx.Rotation(co, si, 12)),
+                     [(2, 2, 8), (5, 2, 4, 8), ((2,), LONG), (2,), (9, 4), (9, 4)]),
+    "gate_keygen": (lambda c, m: c.gate_keygen(mpcx.TR, m), [(5,)]),
+    "gate_eval": (lambda c, a, b, x: c.gate_eval(mpcx.TR, a, b, x), [((1000,), BYTE), ((1000,), BYTE), (5,)]),
+    "split_mask": (lambda c, m: c.split_mask(m), [(5,)]),
+    "attn_scores_eval": (
+        lambda c, pages, q, lo, hi, off, slope, pos, *t: c.attn_scores_eval(
+            mpcx.AttnBatch(pages, q, lo, hi, off, 8, 2, 2, 4), *t, slope=slope, pos=pos),
+        [(1, 3), (2,), (2,), (2,), ((2,), LONG), (2,), (2,), ((1000,), BYTE), ((1000,), BYTE), (2, 2, 8), (5, 2, 4, 8),
+         (5, 2, 4, 8), (5, 2, 4, 8)]),
+    "attn_mix_message": (
+        lambda c, pages, q, lo, hi, off, *t: c.attn_mix_message(1, mpcx.AttnBatch(pages, q, lo, hi, off, 8, 2, 2, 4), *t),
+        [(1, 3), (2,), (2,), (2,), ((2,), LONG), ((1000,), BYTE), (8,), (5, 2, 4, 8), (5, 2, 4, 8)]),
+}
+
+
+@pytest.mark.parametrize("name", sorted(CALLS))
+def test_tensors_of_another_gpu(ctx, name):
+    call, shapes = CALLS[name]
+    made = [(s if isinstance(s[0], tuple) else (s, INT)) for s in shapes]
+    call(ctx, *[Tensor(*m) for m in made])
+    assert len(ctx.lib.calls) == 1
+    for i in range(len(made)):
+        for device in (1, -1):
+            with pytest.raises(mpcx.MpcxError):
+                call(ctx, *[Tensor(*m, device=device if i == j else 0) for j, m in enumerate(made)])
+    assert len(ctx.lib.calls) == 1
