@@ -683,7 +683,7 @@ class Ctx:
         for r, p, rotate in planes:
             to, st = self._words(p, "cache_append: pool", pool), r.stride()
             if r.shape != shape or r.dtype is not self._word or r.get_device() != self._device or \
-                    (st[1:] != near and not r.is_contiguous()):
+                    (st[1:] != near and not ((shape[1] == 1 or st[1] == shape[2]) and (shape[2] == 1 or st[2] == 1))):
                 raise MpcxError(f"cache_append: rows: need int{self.bw} rows of shape {shape} on GPU {self._device}")
             arr.append(_CachePlane(r.data_ptr(), st[0] if n > 1 else shape[1] * shape[2], to, rotate))
         rot = None

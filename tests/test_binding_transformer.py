@@ -187,3 +187,19 @@ def test_tensors_of_another_gpu(ctx, name):
             with pytest.raises(mpcx.MpcxError):
                 call(ctx, *[Tensor(*m, device=device if i == j else 0) for j, m in enumerate(made)])
     assert len(ctx.lib.calls) == 1
+
+
+@pytest.mark.parametrize("heads,dim,stride,ok", [
+    (1, 8, (24, 24, 1), True), (1, 8, (8, 1, 1), True), (1, 1, (5, 7, 3), True), (3, 1, (9, 1, 4), True),
+    (2, 8, (16, 8, 1), True), (2, 8, (40, 8, 1), True), (2, 8, (40, 9, 1), False), (1, 8, (8, 8, 2), False),
+    (2, 1, (9, 4, 1), False), (2, 8, (8, 16, 1), False)])
+def test_cache_append_strides_of_single_heads_and_dims(ctx, heads, dim, stride, ok):
+    """A stride counts where there is more than one of its dimension."""
+    rows, pool = Tensor((4, heads, dim), stride=stride), Tensor((5, heads, 4, dim))
+    if not ok:
+        with pytest.raises(mpcx.MpcxError):
+            ctx.cache_append([(rows, pool, False)], Tensor((4,), LONG))
+        return
+    ctx.cache_append([(rows, pool, False)], Tensor((4,), LONG))
+    (_, args), = ctx.lib.calls
+    assert args[-1][0].ld == stride[0]

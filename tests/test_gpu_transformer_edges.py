@@ -144,6 +144,22 @@ def test_cache_append_pool_over_another_buffer(ctx):
     ctx.sync()
 
 
+@pytest.mark.parametrize("heads,dim", [(1, 8), (1, 1), (3, 1)])
+def test_cache_append_rows_of_single_heads_and_dims(ctx, heads, dim):
+    """Rows cut out of wider ones."""
+    rng = np.random.default_rng(heads + dim)
+    big, pool = words(rng, (6, heads, dim + 5), ctx.bw), words(rng, (3, heads, 4, dim), ctx.bw)
+    if heads > 1:
+        big = words(rng, (6, dim + 4, heads), ctx.bw)
+    slot = rng.permutation(12)[:6].astype(np.int64)
+    d, p = dev(big), dev(pool)
+    rows = d[:, :, 2:2 + dim] if heads == 1 else d[:, 1:1 + dim].transpose(1, 2)
+    ctx.cache_append([(rows, p, False)], dev(slot))
+    for t, s in enumerate(slot):
+        pool[s // 4, :, s % 4] = big[t, :, 2:2 + dim] if heads == 1 else big[t, 1:1 + dim].T
+    assert np.array_equal(host(p, ctx.bw), pool)
+
+
 class Gate:
     """The buffers of an attention gate, each at a place of its own, as the C calls
     take them."""
