@@ -998,8 +998,11 @@ mpcx_status mpcx_ring_lincomb(mpcx_ctx *c, size_t rows, size_t cols, uint64_t a,
 }
 
 // ---------------- transformer layers ----------------
+// rows and columns are counted to the end of their last tile
+static constexpr int kQ4Most = INT32_MAX - 255;
+static bool q4_sizes(int M, int K) { return M >= 1 && M <= kQ4Most && K >= 1 && K <= kQ4MaxK; }
 size_t mpcx_ring_gemm_q4_work_bytes(mpcx_ctx *c, int M, int K) {
-  return c && M >= 1 && K >= 1 ? q4_work_bytes(c->bw, M, K) : 0;
+  return c && q4_sizes(M, K) ? q4_work_bytes(c->bw, M, K) : 0;
 }
 template <typename T>
 static mpcx_status gemm_q4_t(mpcx_ctx *c, int M, int K, int N, int group, const void *a, size_t lda, const uint8_t *q,
@@ -1029,8 +1032,7 @@ static ByteRows word_rows(const mpcx_ctx *c, const void *p, size_t rows, size_t 
 mpcx_status mpcx_ring_gemm_q4(mpcx_ctx *c, int M, int K, int N, int group, const void *a, size_t lda, const uint8_t *q,
                               const int32_t *scale, void *out, size_t ldc, void *work) {
   CHECK_CTX(c);
-  constexpr int kMost = INT32_MAX - 255;  // rows and columns are counted to the end of their last tile
-  if (M < 1 || M > kMost || K < 1 || K > kQ4MaxK || N < 1 || N > kMost || group < 32 || group % 32 != 0 || lda < size_t(K) || ldc < size_t(N))
+  if (!q4_sizes(M, K) || N < 1 || N > kQ4Most || group < 32 || group % 32 != 0 || lda < size_t(K) || ldc < size_t(N))
     return fail(c, MPCX_EINVAL, "ring_gemm_q4: bad argument");
   if (!a || !q || !scale || !out || (!work && q4_work_bytes(c->bw, M, K) > 0))
     return fail(c, MPCX_EINVAL, "ring_gemm_q4: null pointer");

@@ -341,7 +341,8 @@ mpcx_status mpcx_ring_lincomb(mpcx_ctx *ctx, size_t rows, size_t cols, uint64_t 
  * d_scale: ceil(K / group) rows of N int32 steps, at the scale of the weights;
  * group a multiple of 32; K up to 2^24.  d_c: M rows of N words, ldc >= N words
  * apart.  d_q is 16-byte aligned.  d_work: mpcx_ring_gemm_q4_work_bytes bytes,
- * 16-byte aligned, in use until the stream has passed the call.  The output and the
+ * 16-byte aligned, in use until the stream has passed the call (0 bytes: sizes
+ * that are refused).  The output and the
  * workspace overlap no other buffer (refused; d_a and d_c may be columns of one
  * larger matrix). */
 size_t mpcx_ring_gemm_q4_work_bytes(mpcx_ctx *ctx, int M, int K);

@@ -37,6 +37,20 @@ def test_q4_rows_shorter_than_a_chunk(ctx, M, K, N, group):
     assert np.array_equal(got, q4_plain(a, w, scale, group).astype(ctx.T))
 
 
+def test_q4_work_bytes_at_the_ends_of_the_sizes(ctx):
+    """What the rows' digits take, whole tiles of 32 or 16 rows and steps of 128 words;
+    nothing for sizes that are refused."""
+    def want(M, K):
+        rows = 32 if ctx.bw == 32 else 16
+        return -(-M // rows) * rows * ctx.bw // 8 * (-(-K // 128) * 128)
+
+    top = (1 << 31) - 1
+    for M, K in ((1, 1), (33, 129), (1, 1 << 24), (top - 255, 1), (top - 255, 1 << 24)):
+        assert ctx.lib.mpcx_ring_gemm_q4_work_bytes(ctx.h, M, K) == want(M, K)
+    for M, K in ((0, 1), (1, 0), (-1, 5), (top, 1), (top - 254, 1), (1, top), (1, (1 << 24) + 1)):
+        assert ctx.lib.mpcx_ring_gemm_q4_work_bytes(ctx.h, M, K) == 0
+
+
 # ---------------- launches ----------------
 def test_q4_columns_past_one_launch(ctx):
     """16 waves a column tile: columns past 2^26 are more threads than a launch may have."""
