@@ -59,6 +59,8 @@ class Cache:
 
     def room(self, counts):
         """Slots and positions of the next counts[b] tokens of each sequence."""
+        if max(u + n for u, n in zip(self.used, counts)) > self.table.shape[1] * self.page:
+            raise ValueError("the sequences' pages are full")
         slot, pos, seq = [], [], []
         for b, n in enumerate(counts):
             for i in range(self.used[b], self.used[b] + n):
@@ -88,6 +90,8 @@ class Layer:
     def batch(self, cache, counts):
         """The tokens of a step: where they go and what they see (each its sequence
         up to itself)."""
+        if max(u + n for u, n in zip(cache.used, counts)) > len(self.cos):  # a row without a table row is not written
+            raise ValueError(f"the rotation's tables have {len(self.cos)} positions")
         slot, pos, seq = cache.room(counts)
         start = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
         hi = pos + 1
