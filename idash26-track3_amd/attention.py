@@ -14,6 +14,7 @@ import argparse
 import time
 
 import numpy as np
+import torch
 
 import mpcx
 
@@ -82,6 +83,7 @@ class Layer:
         self.cos, self.sin = np.round(np.cos(angle) * (1 << s)).astype(np.int64), \
             np.round(np.sin(angle) * (1 << s)).astype(np.int64)
         self.slope = np.round(2.0 ** (-np.arange(1, heads + 1)) * (1 << (2 * s)) / 64).astype(np.int64)
+        self.bias = self._dev(self.slope)
         self.rotation = mpcx.Rotation(self._dev(self.cos), self._dev(self.sin), s)
 
     def _dev(self, v):
@@ -106,7 +108,7 @@ class Layer:
         cache of one slot a page."""
         n = rows.shape[0]
         out = self.ctx._new((n, n_heads, 1, self.dim))
-        slot = mpcx.to_dev(np.arange(n, dtype=np.int64))
+        slot = torch.arange(n, device=rows.device)
         self.ctx.cache_append([(rows, out, True)], slot, pos, self.rotation)
         return out.view(n, n_heads, self.dim)
 
@@ -147,7 +149,7 @@ class Layer:
         q = gate("q", mpcx.TR, self._rotated(q, self.heads, pos))
         k = gate("k", mpcx.TR, self._rotated(k, self.kv, pos))
         ctx.cache_append([(k, cache.keys[0], False), (v, cache.values[0], False)], slot)
-        s = ctx.attn_scores_eval(batch, *keys["scores"][:2], q, *cache.keys, slope=self._dev(self.slope), pos=pos)
+        s = ctx.attn_scores_eval(batch, *keys["scores"][:2], q, *cache.keys, slope=self.bias, pos=pos)
         p = gate("p", mpcx.TRRELU, s)
         o = gate("o", mpcx.TR, ctx.attn_mix_eval(batch, *keys["mix"][:2], p, *cache.values))
         return gate("out", mpcx.TR, self.w_out(ctx, o.flatten(1)))

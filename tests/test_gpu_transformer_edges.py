@@ -329,3 +329,22 @@ def test_gate_eval_keys(ctx):
             ctx.gate_eval(mpcx.TRRELU, a, b, x)
     word = host(x, ctx.bw).view(np.int32 if ctx.bw == 32 else np.int64)
     assert np.array_equal(host(ctx.gate_eval(mpcx.LOCALARS, None, None, x), ctx.bw).view(word.dtype), word >> 12)
+
+
+# ---------------- the layer ----------------
+def test_layer_evaluates_without_host_data(monkeypatch):
+    """Weights, tables and the bias are on the GPU before the first step."""
+    import attention
+    took = []
+    evaluate, copy = attention.Layer.evaluate, mpcx.to_dev
+
+    def watched(self, *a):
+        monkeypatch.setattr(mpcx, "to_dev", lambda x: took.append(x.shape) or copy(x))
+        try:
+            return evaluate(self, *a)
+        finally:
+            monkeypatch.setattr(mpcx, "to_dev", copy)
+
+    monkeypatch.setattr(attention.Layer, "evaluate", watched)
+    assert attention.run(32, singles=1, say=lambda line: None)
+    assert took == []
