@@ -599,9 +599,12 @@ class Ctx:
 
     # ---------------- transformer layers (GPU tensors in and out) ----------------
     # Ring words are int32 (bw = 32) or int64 tensors on the context's device.
-    # Where the context works on torch's current stream (set_stream) these calls
-    # only enqueue; elsewhere they wait for torch's stream first and for their own
-    # work at the end, as the methods above do.
+    # Where the context works on torch's current stream (set_stream) ring_gemm_q4,
+    # cache_append, split_mask and the attention evaluations and messages only
+    # enqueue, so a graph can capture them; gate_eval and the keygens wait for the
+    # stream there, too.  Inputs made on another stream are the caller's to order
+    # (Stream.wait_stream).  On any other stream all of them wait for torch's current
+    # stream first and for their own work at the end, as the methods above do.
     def _enter(self):
         cur = _torch_module.cuda.current_stream(self._device)
         if self._stream_id == cur.cuda_stream != 0:

@@ -22,7 +22,8 @@
  * buffers, the null stream's fills and copies included, has to be done, or
  * ordered before that stream, when the call is made.  mpcx_prg_hash, mpcx_prf,
  * mpcx_dcf_*, mpcx_tr_keygen, mpcx_mul_keygen, mpcx_lut8_keygen,
- * mpcx_reveal_keygen, mpcx_ring_gemm, mpcx_ring_lincomb,
+ * mpcx_reveal_keygen, mpcx_ring_gemm, mpcx_ring_lincomb, mpcx_ring_gemm_q4,
+ * mpcx_cache_append, mpcx_split_mask, mpcx_attn_*_eval, mpcx_attn_*_message,
  * mpcx_maxpool_eval_noalloc and, with mpcx_set_party_sync(ctx, 0),
  * mpcx_party_* return with their work enqueued there: their buffers stay in
  * use until the stream has reached it.

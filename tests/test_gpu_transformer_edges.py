@@ -331,6 +331,47 @@ def test_gate_eval_keys(ctx):
     assert np.array_equal(host(ctx.gate_eval(mpcx.LOCALARS, None, None, x), ctx.bw).view(word.dtype), word >> 12)
 
 
+# ---------------- streams ----------------
+def test_which_calls_wait_for_their_stream(ctx):
+    """On the caller's stream the products only enqueue; the gates' evaluations and
+    the keygens wait."""
+    import torch
+    B = Batch(ctx.bw, 1, 2, 20, 2, 1, 16, 4, "causal", seed=6)
+    g, planes = B.gpu(), [dev(v) for v in (B.y, B.b0, B.b1)]
+    q, p = dev(words(B.rng, (B.tokens, 2, 16), ctx.bw)), dev(words(B.rng, (B.n,), ctx.bw))
+    w, scale = dev(q4_pack(B.rng.integers(-8, 8, (50, 32)))), dev(B.rng.integers(1, 99, (1, 50)).astype(np.int32))
+    slot, rows = dev(np.arange(B.tokens)), q[:, :1]
+    stream, big = torch.cuda.Stream(), torch.empty(1 << 30, dtype=torch.uint8, device="cuda")
+    ctx.set_stream(stream)
+    with torch.cuda.stream(stream):
+        ks, km = ctx.attn_scores_keygen(g, q, *planes[1:]), ctx.attn_mix_keygen(g, p, *planes[1:])
+        k0, k1, _ = ctx.gate_keygen(mpcx.TR, q)
+        calls = {
+            "ring_gemm_q4": lambda: ctx.ring_gemm_q4(q.view(-1, 32), w, scale, 32),
+            "cache_append": lambda: ctx.cache_append([(rows, planes[0], False)], slot),
+            "split_mask": lambda: ctx.split_mask(q),
+            "attn_scores_eval": lambda: ctx.attn_scores_eval(g, *ks[:2], q, *planes),
+            "attn_mix_eval": lambda: ctx.attn_mix_eval(g, *km[:2], p, *planes),
+            "attn_scores_message": lambda: ctx.attn_scores_message(0, g, ks[0], q, *planes[:2]),
+            "attn_mix_message": lambda: ctx.attn_mix_message(0, g, km[0], p, *planes[:2]),
+            "gate_eval": lambda: ctx.gate_eval(mpcx.TR, k0, k1, q),
+            "attn_scores_keygen": lambda: ctx.attn_scores_keygen(g, q, *planes[1:]),
+            "attn_mix_keygen": lambda: ctx.attn_mix_keygen(g, p, *planes[1:])}
+        for call in calls.values():
+            call()
+        done = {}
+        for name, call in calls.items():
+            torch.cuda.synchronize()
+            for k in range(64):  # some 20 ms
+                big.fill_(k)
+            call()
+            done[name] = stream.query()
+        torch.cuda.synchronize()
+    ctx.set_stream(None)
+    waits = {"gate_eval", "attn_scores_keygen", "attn_mix_keygen"}
+    assert done == {name: name in waits for name in calls}
+
+
 # ---------------- the layer ----------------
 def test_layer_evaluates_without_host_data(monkeypatch):
     """Weights, tables and the bias are on the GPU before the first step."""
