@@ -10,6 +10,7 @@ import mpcx
 from test_gpu_transformer import Batch, dev, host, q4_pack, q4_plain, words
 
 pytestmark = pytest.mark.gpu
+EINVAL = 1
 
 
 @pytest.fixture(scope="module", params=[32, 64])
@@ -37,6 +38,45 @@ def test_q4_rows_shorter_than_a_chunk(ctx, M, K, N, group):
     assert np.array_equal(got, q4_plain(a, w, scale, group).astype(ctx.T))
 
 
+# Instances by the launch's rules on 256 compute units: a row tile is 4 rows of Z_2^32 or
+# 2 of Z_2^64, so `tiles` of them are the same instance in both rings.
+#   up to 16 tiles: the kernel of few rows, of 1, 2 or 4 tiles a workgroup, from digits in
+#   the workspace where tiles x K x column tiles pass 2^20;
+#   more: column tiles a wave, the most of 4 (groups of 64 and 128), 2 and 1 that give 512
+#   workgroups of 8 row tiles and 32 times as many columns.
+Q4_INSTANCES = [
+    # tiles, K, N, group: few rows, digits in the workspace
+    (1, 4200, 4100, 128), (2, 2111, 4097, 128), (4, 1000, 4500, 128), (16, 900, 2003, 256),
+    (1, 4200, 4100, 64), (2, 2111, 4097, 64), (13, 700, 2600, 192),
+    (1, 4200, 4100, 32), (2, 2111, 4097, 96), (3, 1500, 4200, 32),
+    # many rows: 4, 2 and 1 column tiles a wave
+    (125, 130, 4090, 128), (130, 200, 4095, 64), (126, 257, 2090, 128), (125, 100, 2100, 64),
+    (127, 161, 2081, 32), (250, 95, 1030, 96), (17, 1300, 100, 128), (40, 300, 333, 64), (21, 190, 258, 32)]
+
+
+@pytest.mark.parametrize("scales", ["any", "small", "few large"])
+@pytest.mark.parametrize("tiles,K,N,group", Q4_INSTANCES)
+def test_q4_instances(ctx, tiles, K, N, group, scales):
+    M = tiles * (4 if ctx.bw == 32 else 2) - 1
+    a, w, scale = q4_case(ctx, M, K, N, group, seed=11)
+    if scales != "any":  # scales within 24 bits, and among them some that are not
+        rng = np.random.default_rng(K)
+        small = rng.integers(-(1 << 23), 1 << 23, scale.shape).astype(np.int32)
+        small.flat[:2] = -(1 << 23), (1 << 23) - 1
+        scale = np.where(rng.random(scale.shape) < 0.01, scale, small) if scales == "few large" else small
+    got = host(ctx.ring_gemm_q4(dev(a), dev(q4_pack(w)), dev(scale), group), ctx.bw)
+    if ctx.bw == 32:  # the same modulo 2^32 in float64 halves: 2^16 * 2^3 * K < 2^53
+        a64 = np.stack([a & 0xFFFF, a >> 16]).astype(np.float64)
+        want = np.zeros((M, N), np.uint64)
+        for g in range(scale.shape[0]):
+            k = slice(g * group, (g + 1) * group)
+            lo, hi = (a64[:, :, k] @ w[:, k].T.astype(np.float64)).astype(np.int64).astype(np.uint64)
+            want += (lo + (hi << np.uint64(16))) * scale[g].astype(np.int64).astype(np.uint64)
+    else:
+        want = q4_plain(a, w, scale, group)
+    assert np.array_equal(got, want.astype(ctx.T))
+
+
 def test_q4_work_bytes_at_the_ends_of_the_sizes(ctx):
     """What the rows' digits take, whole tiles of 32 or 16 rows and steps of 128 words;
     nothing for sizes that are refused."""
@@ -49,6 +89,15 @@ def test_q4_work_bytes_at_the_ends_of_the_sizes(ctx):
         assert ctx.lib.mpcx_ring_gemm_q4_work_bytes(ctx.h, M, K) == want(M, K)
     for M, K in ((0, 1), (1, 0), (-1, 5), (top, 1), (top - 254, 1), (1, top), (1, (1 << 24) + 1)):
         assert ctx.lib.mpcx_ring_gemm_q4_work_bytes(ctx.h, M, K) == 0
+
+
+def test_q4_sizes_past_the_bounds(ctx):
+    import torch
+    t = torch.zeros(64, dtype=torch.int64, device="cuda").data_ptr()
+    top, wide = (1 << 31) - 1, 1 << 40
+    for M, K, N in ((top, 1, 1), (top - 254, 1, 1), (1, 1, top), (1, 1, top - 254), (1, (1 << 24) + 1, 1), (1, top, 1)):
+        assert ctx.lib.mpcx_ring_gemm_q4(ctx.h, M, K, N, 32, t, wide, t, t, t + 256, wide, t) == EINVAL, (M, K, N)
+        assert b"bad argument" in ctx.lib.mpcx_last_error(ctx.h)
 
 
 # ---------------- launches ----------------
@@ -91,10 +140,57 @@ def test_launch_hints_of_any_size(ctx, max_q, max_keys):
         assert np.array_equal(got, B.mix(p - rp, B.y - B.b0 - B.b1) + host(ro, ctx.bw))
 
 
+# ---------------- the attention kernels' instances ----------------
+TWO_TILES = [  # rows enough for two tiles of them a workgroup in both rings
+    (4, 32, 50, 64, 8, 64, 16, "causal"), (4, 33, 70, 64, 8, 33, 16, "prefix"), (3, 70, 90, 32, 8, 128, 24, "window"),
+    (5, 20, 40, 96, 8, 100, 16, "ragged"), (16, 17, 33, 32, 16, 24, 7, "ragged")]
+
+
+@pytest.mark.parametrize("seqs,q,keys,heads,kv,dim,page,mask", TWO_TILES)
+@pytest.mark.parametrize("gap", [0, 3])
+def test_scores_of_two_tiles(ctx, seqs, q, keys, heads, kv, dim, page, mask, gap):
+    """Both parties together, the dealer's form and each party's message, with the bias
+    and without."""
+    B = Batch(ctx.bw, seqs, q, keys, heads, kv, dim, page, mask, seed=7, gap=gap)
+    rq, qhat = words(B.rng, (B.tokens, heads, dim), ctx.bw), words(B.rng, (B.tokens, heads, dim), ctx.bw)
+    slope = words(B.rng, (heads,), ctx.bw)
+    g, planes = B.gpu(), [dev(v) for v in (B.y, B.b0, B.b1)]
+    k0, k1, rs = ctx.attn_scores_keygen(g, dev(rq), planes[1], planes[2], seed=3, gate=9)
+    extra = dict(slope=dev(slope), pos=dev(B.pos)) if gap else {}
+    got = host(ctx.attn_scores_eval(g, k0, k1, dev(qhat), *planes, **extra), ctx.bw)
+    parts = [host(ctx.attn_scores_message(p, g, k, dev(qhat), planes[0], planes[1 + p], **extra), ctx.bw)
+             for p, k in ((0, k0), (1, k1))]
+    with np.errstate(over="ignore"):
+        want = B.scores(qhat - rq, B.y - B.b0 - B.b1) + host(rs, ctx.bw) + (B.bias(slope) if gap else 0)
+        m = B.inside()
+        assert np.array_equal(got[m], want[m])
+        assert np.array_equal((parts[0] + parts[1])[m], want[m])
+
+
+def test_sums_past_the_matrix_cores_sums(ctx):
+    """Every digit at -128 and every term of the gate the same product, over more keys a
+    wave than 31 bits of digit sums hold (Z_2^32 wraps, Z_2^64 folds in between)."""
+    import torch
+    seqs, keys, dim, page = 256, 100000, 4, 64  # a workgroup for each sequence: no splits
+    w = (-sum(128 << (8 * p) for p in range(ctx.bw // 8))) % (1 << ctx.bw)
+    word = torch.int32 if ctx.bw == 32 else torch.int64
+
+    def full(shape, v):
+        v %= 1 << ctx.bw
+        return torch.full(shape, v - (1 << ctx.bw) if v >> (ctx.bw - 1) else v, dtype=word, device="cuda")
+
+    n, pages, i32 = seqs * keys, -(-keys // page), np.int32
+    g = mpcx.AttnBatch(dev(np.tile(np.arange(pages, dtype=i32), (seqs, 1))), dev(np.arange(seqs + 1, dtype=i32)),
+                       dev(np.zeros(seqs, i32)), dev(np.full(seqs, keys, i32)), dev(np.arange(seqs) * keys), n, 1, 1, keys)
+    shape, tail = (pages, 1, page, dim), torch.zeros(-(-seqs * dim * ctx.bw // 2048) * 256, dtype=torch.uint8, device="cuda")
+    assert n * ctx.bw // 8 % 256 == 0
+    # (x - a0)(y - b0) = (-x) b1 = (-a1) y = w w
+    k0, k1 = (torch.cat((full((n,), v).view(torch.uint8), tail)) for v in (-2 * w, -w))
+    got = host(ctx.attn_mix_eval(g, k0, k1, full((n,), -w), full(shape, w), full(shape, 0), full(shape, w)), ctx.bw)
+    assert (got == 3 * keys * w * w % (1 << ctx.bw)).all()
+
+
 # ---------------- buffers ----------------
-EINVAL = 1
-
-
 def test_q4_output_or_workspace_over_another_buffer(ctx):
     import torch
     M, K, N, group, tb = 6, 64, 40, 32, ctx.bw // 8
