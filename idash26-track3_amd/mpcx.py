@@ -244,12 +244,6 @@ def from_dev(t, dtype, count=None):
     return out if count is None else out[:count]
 
 
-def _c_ints(what, *sizes):
-    """Refuses sizes past a C int, which ctypes would cut short."""
-    if max(sizes) > 0x7FFFFFFF:
-        raise MpcxError(f"{what}: a size of {max(sizes)}")
-
-
 def dptr(t):
     return C.c_void_p(t.data_ptr()) if t is not None else None
 
@@ -643,12 +637,11 @@ class Ctx:
         """mpcx_ring_gemm_q4: a (M, K) ring words (rows may be apart), q (N, rows of
         whole 32 weights) uint8, scale (groups, N) int32 -> (M, N)."""
         torch = _torch()
-        if group < 1:
-            raise MpcxError(f"ring_gemm_q4: groups of {group}")
         ap, lda = self._rows(a, "ring_gemm_q4: a")
         M, K = a.shape
         N = q.shape[0]
-        _c_ints("ring_gemm_q4", M, K, N, group)
+        if group < 1 or (M | K | N | group) >> 31:  # sizes past a C int would be cut short
+            raise MpcxError(f"ring_gemm_q4: sizes {M}, {K}, {N}, groups of {group}")
         if out is None:
             out = self._new((M, N))
         op, ldc = self._rows(out, "ring_gemm_q4: out")
@@ -666,11 +659,6 @@ class Ctx:
         self._leave(same)
         return out
 
-    @staticmethod
-    def _cache(pool):
-        n, heads, page, dim = pool.shape
-        return Cache(heads, dim, page, n)
-
     def cache_append(self, planes, slot, pos=None, rotation=None):
         """mpcx_cache_append: planes is a list of (rows, pool, rotate), rows (tokens,
         heads, dim) ring words (tokens may be apart), pool (pages, heads, page size,
@@ -678,26 +666,30 @@ class Ctx:
         torch = _torch()
         n = slot.shape[0]
         pool = planes[0][1].shape
-        _c_ints("cache_append", *pool[1:])
-        shape, near = (n, pool[1], pool[3]), (pool[3], 1)
+        pages, heads, page, dim = pool
+        if (heads | page | dim) >> 31:  # past a C int, as below
+            raise MpcxError(f"cache_append: pool of {tuple(pool)}")
+        shape, near = (n, heads, dim), (dim, 1)
         sp = self._ints(slot, "cache_append: slot", torch.int64, (n,))
         pp = self._ints(pos, "cache_append: pos", torch.int32, (n,)) if pos is not None else None
         arr = []
         for r, p, rotate in planes:
             to, st = self._words(p, "cache_append: pool", pool), r.stride()
             if r.shape != shape or r.dtype is not self._word or r.get_device() != self._device or \
-                    (st[1:] != near and not ((shape[1] == 1 or st[1] == shape[2]) and (shape[2] == 1 or st[2] == 1))):
+                    (st[1:] != near and not ((heads == 1 or st[1] == dim) and (dim == 1 or st[2] == 1))):
                 raise MpcxError(f"cache_append: rows: need int{self.bw} rows of shape {shape} on GPU {self._device}")
-            arr.append(_CachePlane(r.data_ptr(), st[0] if n > 1 else shape[1] * shape[2], to, rotate))
+            arr.append(_CachePlane(r.data_ptr(), st[0] if n > 1 else heads * dim, to, rotate))
         rot = None
         if rotation is not None:
             c = rotation.cos
-            _c_ints("cache_append", *c.shape, rotation.shift)
-            rot = C.byref(_Rotation(c.shape[1], int(rotation.pairs), c.shape[0], rotation.shift,
+            n_pos, half = c.shape
+            if (n_pos | half | rotation.shift) >> 31:
+                raise MpcxError(f"cache_append: tables of {(n_pos, half)}, shift {rotation.shift}")
+            rot = C.byref(_Rotation(half, int(rotation.pairs), n_pos, rotation.shift,
                                     self._words(c, "cache_append: cos"),
                                     self._words(rotation.sin, "cache_append: sin", c.shape)))
         same = self._enter()
-        self.check(self.lib.mpcx_cache_append(self.h, C.byref(Cache(pool[1], pool[3], pool[2], pool[0])), n, sp, pp, rot,
+        self.check(self.lib.mpcx_cache_append(self.h, C.byref(Cache(heads, dim, page, pages)), n, sp, pp, rot,
                                               len(arr), (_CachePlane * len(arr))(*arr)), "cache_append")
         self._leave(same)
 
@@ -736,13 +728,16 @@ class Ctx:
 
     def _attn(self, b, pool):
         torch = _torch()
-        n, seqs = b.lo.shape[0], b.pages.shape[0]
-        _c_ints("attn", n, *b.pages.shape, b.heads, b.max_q, b.max_keys, *pool.shape[1:])
-        i32 = torch.int32
-        return _Attn(self._cache(pool), b.heads, n, seqs, b.pages.shape[1], b.max_q, b.max_keys, b.n_scores,
-                     self._ints(b.pages, "attn: pages", i32, b.pages.shape),
-                     self._ints(b.qstart, "attn: qstart", i32, (seqs + 1,)), self._ints(b.lo, "attn: lo", i32, (n,)),
-                     self._ints(b.hi, "attn: hi", i32, (n,)), self._ints(b.off, "attn: off", torch.int64, (n,)))
+        pages, qstart, lo, hi, off, n_scores, heads, max_q, max_keys = b
+        n, table, (n_pages, kv, page, dim), i32 = lo.shape[0], pages.shape, pool.shape, torch.int32
+        seqs, width = table
+        if (n | seqs | width | heads | max_q | max_keys | kv | page | dim) >> 31:  # past a C int, or negative
+            raise MpcxError(f"attn: a batch of {n} tokens, {heads} heads, tables {tuple(table)}, max_q {max_q}, "
+                            f"max_keys {max_keys}, cache {tuple(pool.shape)}")
+        return _Attn(Cache(kv, dim, page, n_pages), heads, n, seqs, width, max_q, max_keys, n_scores,
+                     self._ints(pages, "attn: pages", i32, table), self._ints(qstart, "attn: qstart", i32, (seqs + 1,)),
+                     self._ints(lo, "attn: lo", i32, (n,)), self._ints(hi, "attn: hi", i32, (n,)),
+                     self._ints(off, "attn: off", torch.int64, (n,)))
 
     def _key(self, k, nb, what):
         if k.numel() * k.element_size() < nb or k.get_device() != self._device or not k.is_contiguous():
