@@ -312,16 +312,22 @@ __device__ __forceinline__ void group_planes(uint4 u, uint4 v, uint32_t (&o)[siz
 // [k0, k0 + kn) of the heads, as many as LDS holds of the queries; `more`: the sums so
 // far are in out.
 // One token a sequence is bound by the cache's bytes: 8 sequences of up to 4096 keys, 8
-// cache heads of 128 in Z_2^32: 76.8 us for 296 MB, 3.9 TB/s (equal lengths: 72 us; the
-// start, some 10 us from the first page number to the first product, and the longest
-// sequence's end are what is left).  Prompts are bound by a wave's own order: 6 us of start
-// and then 4 us a step, of which at two waves a SIMD half is issue (two thirds of that
-// vector instructions, most of them the digits', one third MFMAs), the rest what the waves
-// wait for one another, LDS and the rows (asked for before the products instead of after
-// them: no faster).  4 x 512 tokens, 8 heads of 64 in Z_2^32: 47.1 us.
-// Four waves, so that one workgroup's start runs beside another's products: with calls and
-// launches eight take 55.2 us for 4 x 256 tokens against 1024 keys, four 46.6; 62.7 for
-// 3 x 400 of 16 heads of 128, four 53.6; but 44.9 for the 4 x 512, four 49.8.
+// cache heads of 128 in Z_2^32: 77 us a call for 296 MB, 3.8 TB/s (the start, some 10 us
+// from the first page number to the first product, and the longest sequence's end are what
+// is left); in Z_2^64 226 us for 592 MB, 2.6 TB/s, one party's message 97: at 344 registers
+// a wave of the form of both parties runs alone on its SIMD.
+// Prompts are bound by the order of work in the waves of the longest rows: 4 x 512 tokens,
+// 8 heads of 64 in Z_2^32, 45.4 us a call.  All their workgroups run at once, two waves a
+// SIMD, so the launch ends with the waves that take eight steps of 16 keys, while the mean is
+// 3.3: over the launch vector instructions issue 15% of the time (2083 a wave, most of them
+// the digits') and MFMAs are busy 6% (198 a wave).  A step is some 630 vector instructions
+// and 60 MFMAs a wave, 2.9 us of issue for the two waves of a SIMD; the rest of its 4 to 5 us
+// they wait for one another, LDS and the rows (asked for before the products instead of
+// after them: no faster).
+// Four waves, so that one workgroup's start runs beside another's products: calls in
+// Z_2^32 by eight take 51.2 us for 4 x 256 tokens against 1024 keys, by four 41.9; 60.7 for
+// 3 x 400 of 16 heads of 128, by four 53.2; but 40.4 for the 4 x 512, by four 45.4.  In
+// Z_2^64 eight spill: 200 us for the 4 x 512, by four 108.
 // ---------------------------------------------------------------------------
 constexpr int kScoreWaves = 4;
 template <AttnForm F, typename T, bool VEC, int RT>
@@ -530,9 +536,10 @@ __global__ __launch_bounds__(64 * kScoreWaves, sizeof(T) == 4 ? 2 : 1) void k_at
 // the keys out; their sums meet in LDS and in integer additions to the output, whose order
 // does not matter.
 // One token a sequence is bound by the cache's bytes: 8 sequences of up to 4096 keys, 8
-// heads of 128 in Z_2^32: 68.2 us for 296 MB, 4.3 TB/s; one of 50000 keys, 4 heads: 63.1
-// us, 317 MB at 5.0 TB/s.  Prompts are bound by the digits' vector instructions, which
-// every tile of rows repeats: 3 of up to 301 tokens, 6 heads of 72 in Z_2^64: 40.2 us.
+// heads of 128 in Z_2^32: 71 us a call for 296 MB, 4.2 TB/s (Z_2^64: 143 for 592 MB); one
+// of 50000 keys, 4 heads: 66 us, 317 MB at 4.8 TB/s.  Prompts are bound by the digits'
+// vector instructions, which every tile of rows repeats: 3 of up to 301 tokens, 6 heads of
+// 72 in Z_2^64: 38.4 us.
 // (Values' planes staged in LDS for eight tiles of rows were slower, for their longer
 // start: 86.8 us against 72.8 for 597 tokens and 1061 keys, 16.4 against 7.3 for 26.)
 // Eight waves: four take 94.6 us for the 8 sequences, 58.6 for the prompts.

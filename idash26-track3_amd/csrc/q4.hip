@@ -11,7 +11,7 @@
 // Accumulator register r of lane (li, lg) is row 4 lg + r, column li: a lane holds
 // four planes of one word, folds them, and multiplies by the group's scale.
 // A chunk is S = 128, 64 or 32 k, the largest that divides the group; the sums of a
-// chunk are below 2^21, so the fold's shifts stay exact in 32 bits:
+// chunk are at most 2^21, so the fold's shifts stay exact in 32 bits:
 //   sum_p 2^(8p) a_p / 16 = (a_0 >> 4) + (a_1 << 4) + (a_2 << 12) + (a_3 << 20),
 // in Z_2^64 with 64-bit sums of the pairs (a_0, a_1), (a_2, a_3), and the lanes of
 // planes 4..7 (odd lg) shifted up by 32 at the end.
@@ -119,7 +119,7 @@ __device__ __forceinline__ void plane8(const T (&w)[8], int p, uint32_t *even, u
 // 4096 waves, each with a few loads of the weights in flight.  DIRECT: a lane forms its
 // digits from the words themselves (a word's planes are the rows li of its tile, so each
 // word is taken apart once for every plane and column tile); else from the workspace.
-// 1 x 4096 x 4096 in Z_2^32: 6.8 us, 9 MB of weights and scales at 1.3 TB/s, of which an
+// 1 x 4096 x 4096 in Z_2^32: 6.6 us, 9 MB of weights and scales at 1.4 TB/s, of which an
 // empty kernel is 3; 5 x 8192 x 2047 in Z_2^64, groups of 64: 12.2 us and the digits' 4.8.
 // ---------------------------------------------------------------------------
 template <typename T, int S, int MT, bool DIRECT>
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(1024) void k_q4_few(Q4Args<T> g, bool vec, int step
 // Digits once for all columns, in the order the lanes take them.  The workspace holds,
 // per MFMA tile of rows and step of 128 k, 2 KB of operands: 128 / S chunks of S / 64
 // operands (64 lanes of 16 bytes; S = 32: one of 8 bytes).  768 x 4096 words of Z_2^32:
-// 10.6 us, 25 MB in and out at 2.4 TB/s.
+// 10.7 us, 25 MB in and out at 2.4 TB/s.
 // ---------------------------------------------------------------------------
 template <typename T, int S>
 __global__ __launch_bounds__(256) void k_q4_digits(Q4Args<T> g, bool vec, int tiles, int steps, uint8_t *work) {
@@ -223,7 +223,7 @@ __global__ __launch_bounds__(256) void k_q4_digits(Q4Args<T> g, bool vec, int ti
 }
 
 // Sums over chunks of plane sums times scales.  Z_2^32: one 24-bit multiply-add a plane
-// (a chunk's plane sums are below 2^21, divided by 16 in plane 0 so that no bit of the
+// (a chunk's plane sums are at most 2^21, divided by 16 in plane 0 so that no bit of the
 // word is lost; the planes above need 4 fewer bits), the planes folded at the end; a
 // scale past 24 bits is its low 12 bits and, in a second pass, the others.  Z_2^64:
 // 64-bit sums of the plane pairs.
@@ -269,10 +269,10 @@ struct Q4Sum<uint64_t> {
 // the weights and scales, which only two waves share, to the lanes' registers (through
 // LDS, too, they took as long); all are asked for a step ahead (two ahead: as long).  Two
 // waves a SIMD (256 registers each), so that one's scales run beside the other's MFMAs.
-// 768 x 4096 x 4096 in Z_2^32: 79.9 us, 1.29 POP/s of digits against 1.8 of a large int8
-// product: vector instructions issue 44% of the time and MFMAs 26%, each waiting for the
-// other in a wave (all of a step's products in one block of code, the rare scales done over:
-// 84), and 768 workgroups at two a CU are one and a half rounds.
+// 768 x 4096 x 4096 in Z_2^32: 80.5 us, 1.28 POP/s of digits against 1.8 of a large int8
+// product (Z_2^64: 163, 1.27): vector instructions issue 44% of the time and MFMAs 26%, each
+// waiting for the other in a wave (all of a step's products in one block of code, the rare
+// scales done over: 84), and 768 workgroups at two a CU are one and a half rounds.
 template <typename T, int S, int MT, int NT>
 __global__ __launch_bounds__(256, 2) void k_q4_many(Q4Args<T> g, int steps, const uint8_t *work) {
   constexpr int R = kRows<T>, ND = S / 32, CH = 128 / S;
@@ -423,9 +423,11 @@ bool few_rows(int M) {
   return row_tiles<T>(M) <= kFewTiles;
 }
 // Its lanes form the digits themselves while that is little work, which the launch that
-// forms them in the workspace costs more than: 64 x 1024 x 1024 7.2 us, with it 9.8; 1 x
-// 4096 x 4096 8.4, with it 10.0; 16 x 4096 x 4096 14.6, with it 12.0; Z_2^64: 4 x 4096 x
-// 4096 15.5, with it 12.2.
+// forms them in the workspace costs more than.  Kernels, direct and with that launch:
+// Z_2^32 32 x 1024 x 1024 5.5 us and 6.9, 1 x 4096 x 4096 6.6 and 7.7, at the line; 16 x
+// 4096 x 4096 12.7 and 10.1, 1 x 8192 x 8192 20.1 and 17.0.  Z_2^64 1 x 2896 x 2880 7.3
+// and 7.8, 4 x 2048 x 2048 7.6 and 8.1, at the line; 1 x 4096 x 4096 8.9 and 8.6, 4 x 4096
+// x 4096 12.6 and 10.0.
 template <typename T>
 bool direct_rows(int M, int K, int N) {
   constexpr size_t most = size_t(sizeof(T) == 4 ? 1 << 20 : 1 << 19);  // words by column tile
