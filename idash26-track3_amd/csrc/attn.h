@@ -7,6 +7,9 @@
 
 namespace mpcx {
 
+// HIP's limit on the threads of a launch along one dimension
+constexpr size_t kMostThreads = UINT32_MAX;
+
 // ---------------- products with 4-bit weights ----------------
 // C[m, n] = sum_g scale[g, n] sum_{k in group g} q[n, k] A[m, k] mod 2^bw.
 // q: N rows of q4_row_bytes(K) bytes, weight k of a row in the low (k even) or

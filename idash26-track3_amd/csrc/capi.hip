@@ -16,6 +16,7 @@
 #include "launch_util.h"
 #include "model.h"
 #include "mpcx_core.h"
+#include "overlap.h"
 #include "peer.h"
 
 // ---------------------------------------------------------------------------

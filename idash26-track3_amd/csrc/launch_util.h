@@ -7,7 +7,6 @@
 #include <cstdint>
 
 #include "kernels.h"
-#include "overlap.h"
 
 namespace mpcx {
 
@@ -37,9 +36,6 @@ inline int variant_block(const Launch &L) {
   return (L.aes_variant >= 0 && L.aes_variant < n) ? v[L.aes_variant].block : 256;
 }
 
-// HIP's limit on the threads of a launch along one dimension
-constexpr size_t kMostThreads = UINT32_MAX;
-
 template <typename K>
 inline int grid_for(K kernel, int block, size_t n, int num_cu) {
   int occ = 0;
@@ -48,6 +44,13 @@ inline int grid_for(K kernel, int block, size_t n, int num_cu) {
   size_t cap = size_t(occ) * size_t(num_cu);
   size_t g = need < cap ? need : cap;
   return int(g < 1 ? 1 : g);
+}
+
+
+// True where n1 bytes at p and n2 bytes at q do not overlap.
+inline bool bytes_apart(const void *p, size_t n1, const void *q, size_t n2) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return a + n1 <= b || b + n2 <= a;
 }
 
 // A value in uniform memory that the kernel does not write (its arguments, a
