@@ -1114,6 +1114,8 @@ mpcx_status mpcx_cache_append(mpcx_ctx *c, const mpcx_cache *cache, size_t n_tok
   if (n_tok == 0) return MPCX_OK;
   if (!slot || (turned && (!pos || !rot->d_cos || !rot->d_sin)))
     return fail(c, MPCX_EINVAL, "cache_append: null pointer");
+  if (!aligned(slot, sizeof *slot) || !aligned(pos, sizeof *pos))
+    return fail(c, MPCX_EINVAL, "cache_append: misaligned pointer");
   for (int p = 0; p < n_planes; p++) {
     if (!planes[p].d_rows || !planes[p].d_pool) return fail(c, MPCX_EINVAL, "cache_append: null pointer");
     if (!aligned(planes[p].d_rows, tb) || !aligned(planes[p].d_pool, tb))
@@ -1184,6 +1186,10 @@ size_t attn_key_end(const mpcx_ctx *c, size_t first, size_t second) {
 }
 bool attn_has_tables(const mpcx_attn *a) {  // page rows of no page have no memory
   return (a->d_pages || a->max_pages == 0) && a->d_qstart && a->d_lo && a->d_hi && a->d_off;
+}
+bool tables_aligned(const mpcx_attn *a) {
+  return aligned(a->d_pages, 4) && aligned(a->d_qstart, 4) && aligned(a->d_lo, 4) && aligned(a->d_hi, 4) &&
+         aligned(a->d_off, 8);
 }
 // True where n bytes at p overlap none of the batch's tables.
 bool tables_apart(const mpcx_attn *a, const void *p, size_t n) {
@@ -1256,7 +1262,7 @@ mpcx_status attn_keygen(mpcx_ctx *c, bool scores, const mpcx_attn *a, const void
   if ((first && !rx) || !b0 || !b1 || !rz || !k0 || !k1 || (!attn_empty(a, scores) && !attn_has_tables(a)))
     return fail(c, MPCX_EINVAL, "attn_keygen: null pointer");
   if (!aligned(k0, 16) || !aligned(k1, 16) || !aligned(rx, tb) || !aligned(b0, tb) || !aligned(b1, tb) ||
-      !aligned(rz, tb))
+      !aligned(rz, tb) || !tables_aligned(a))
     return fail(c, MPCX_EINVAL, "attn_keygen: misaligned pointer");
   const size_t nz = second * tb, key = attn_key_end(c, first, second), plane = cache_plane_bytes(c, a->cache);
   auto apart = [&](const void *p, size_t n) {  // an output and the inputs
@@ -1309,7 +1315,8 @@ mpcx_status attn_eval(mpcx_ctx *c, bool scores, AttnForm form, const mpcx_attn *
     return fail(c, MPCX_EINVAL, "attn_eval: null pointer");
   for (const void *p : {x, y, b0, b1, slope, static_cast<const void *>(out)})
     if (!aligned(p, tb)) return fail(c, MPCX_EINVAL, "attn_eval: misaligned pointer");
-  if (!aligned(k0, 16) || !aligned(k1, 16)) return fail(c, MPCX_EINVAL, "attn_eval: misaligned pointer");
+  if (!aligned(k0, 16) || !aligned(k1, 16) || !aligned(pos, sizeof *pos) || !tables_aligned(a))
+    return fail(c, MPCX_EINVAL, "attn_eval: misaligned pointer");
   const size_t nb = second * tb, key = attn_key_end(c, first, second), plane = cache_plane_bytes(c, a->cache);
   if (!bytes_apart(out, nb, x, first * tb) || (p0 && !bytes_apart(out, nb, k0, key)) ||
       (p1 && !bytes_apart(out, nb, k1, key)) || !bytes_apart(out, nb, y, plane) ||

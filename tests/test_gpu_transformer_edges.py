@@ -340,6 +340,23 @@ def test_attn_keygen_output_over_another_buffer(ctx, scores):
     ctx.sync()
 
 
+@pytest.mark.parametrize("scores", [True, False])
+def test_misaligned_tables(ctx, scores):
+    g = Gate(ctx, scores)
+    calls = [(g.eval, "pages qstart lo hi off".split() + ["pos"] * scores), (g.keygen, "pages qstart lo hi off".split())]
+    for call, names in calls:
+        for n in names:
+            for by in (1, 2) + (4,) * (n == "off"):
+                assert call(**{n: g.at[n] + by}) == EINVAL, (n, by)
+                assert b"misaligned" in ctx.lib.mpcx_last_error(ctx.h)
+    planes = (mpcx._CachePlane * 1)(mpcx._CachePlane(g.at["x"], 16, g.at["y"], 0))
+    cache = mpcx.Cache(2, 8, 4, 3)
+    for slot, pos in ((4, 0), (1, 0), (0, 2)):
+        assert ctx.lib.mpcx_cache_append(ctx.h, C.byref(cache), 1, g.at["off"] + slot, g.at["pos"] + pos, None, 1,
+                                         planes) == EINVAL
+    ctx.sync()
+
+
 def test_split_mask_buffers(ctx):
     import torch
     n, tb = 300, ctx.bw // 8
