@@ -1,6 +1,6 @@
 // attn.h -- host-side launchers of the transformer operators: products with
-// public 4-bit weights (q4.hip), the paged cache and the attention products
-// that read it (attn.hip).
+// public 4-bit (q4.hip) and 8-bit weights (q8.hip), the paged cache and the
+// attention products that read it (attn.hip), the norm's gates (norm.hip).
 #pragma once
 #include "kernels.h"
 #include "q4_layout.h"
@@ -30,6 +30,61 @@ struct Q4Args {
 size_t q4_work_bytes(int bw, int M, int K);
 template <typename T>
 hipError_t launch_gemm_q4(const Launch &L, const Q4Args<T> &g);
+
+// ---------------- products with 8-bit weights ----------------
+// C[m, n] = tok[m] scale[n] sum_k q[n, k] A[m, k] mod 2^bw; scale, tok may be null (1).
+constexpr int kQ8MaxK = 1 << 24;
+template <typename T>
+struct Q8Args {
+  int M = 0, K = 0, N = 0;
+  const T *a = nullptr;
+  size_t lda = 0;
+  const int8_t *q = nullptr;  // rows of K weights, ldq (a multiple of 16) bytes apart
+  size_t ldq = 0;
+  const int32_t *scale = nullptr, *tok = nullptr;
+  T *c = nullptr;
+  size_t ldc = 0;
+};
+template <typename T>
+hipError_t launch_gemm_q8(const Launch &L, const Q8Args<T> &g);
+
+// ---------------- the norm's gates ----------------
+// What a launch computes: both parties' messages added up, one party's, or the
+// dealer's product term.
+enum class NormForm { BOTH, P0, P1, DEAL };
+// h = x + d (d may be null: h = x) and s[t] = sum_j h[t, j]^2, as
+//   P0    sum h (h - 2 a0) + c0
+//   P1    c1 - 2 sum h a1
+//   DEAL  sum h^2 + c0, and h to `copy`: with x, d masks and c0 the sums' mask
+template <typename T>
+struct NormSumsArgs {
+  size_t rows = 0, dim = 0;
+  const T *x = nullptr, *d = nullptr;
+  size_t ldx = 0, ldd = 0;
+  const T *a0 = nullptr, *a1 = nullptr, *c0 = nullptr, *c1 = nullptr;
+  T *h = nullptr;  // may be null, x or d
+  size_t ldh = 0;
+  T *copy = nullptr;
+  T *s = nullptr;
+};
+template <typename T>
+hipError_t launch_norm_sums(const Launch &L, NormForm form, const NormSumsArgs<T> &g);
+// y[t, j] = gain[j] h[t, j] v[t] (gain may be null: 1), as
+//   P0    gain (h - a0)(v - b0) + c0
+//   P1    c1 - gain (h b1 + a1 v)
+//   DEAL  c0 + gain ((a0 + a1) v - a0 b0): with v the factors' mask and c0 the output's
+template <typename T>
+struct NormScaleArgs {
+  size_t rows = 0, dim = 0;
+  const T *h = nullptr;
+  size_t ldh = 0;
+  const T *a0 = nullptr, *a1 = nullptr, *v = nullptr, *b0 = nullptr, *b1 = nullptr;
+  const T *c0 = nullptr, *c1 = nullptr, *gain = nullptr;
+  T *y = nullptr;  // may be h
+  size_t ldy = 0;
+};
+template <typename T>
+hipError_t launch_norm_scale(const Launch &L, NormForm form, const NormScaleArgs<T> &g);
 
 // ---------------- paged cache ----------------
 // A plane of the cache is n_pages x heads x page x dim ring words: a head's rows

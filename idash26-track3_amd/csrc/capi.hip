@@ -1049,6 +1049,42 @@ mpcx_status mpcx_ring_gemm_q4(mpcx_ctx *c, int M, int K, int N, int group, const
                      : gemm_q4_t<uint64_t>(c, M, K, N, group, a, lda, q, scale, out, ldc, work);
 }
 
+template <typename T>
+static mpcx_status gemm_q8_t(mpcx_ctx *c, int M, int K, int N, const void *a, size_t lda, const int8_t *q, size_t ldq,
+                             const int32_t *scale, const int32_t *tok, void *out, size_t ldc) {
+  Q8Args<T> g;
+  g.M = M;
+  g.K = K;
+  g.N = N;
+  g.a = static_cast<const T *>(a);
+  g.lda = lda;
+  g.q = q;
+  g.ldq = ldq;
+  g.scale = scale;
+  g.tok = tok;
+  g.c = static_cast<T *>(out);
+  g.ldc = ldc;
+  HIPC(c, launch_gemm_q8<T>(c->L, g), "ring_gemm_q8");
+  return MPCX_OK;
+}
+mpcx_status mpcx_ring_gemm_q8(mpcx_ctx *c, int M, int K, int N, const void *a, size_t lda, const int8_t *q, size_t ldq,
+                              const int32_t *scale, const int32_t *tok, void *out, size_t ldc) {
+  CHECK_CTX(c);
+  if (M < 1 || M > kQ4Most || K < 1 || K > kQ8MaxK || N < 1 || N > kQ4Most || lda < size_t(K) || ldq < size_t(K) ||
+      ldq % 16 != 0 || ldc < size_t(N))
+    return fail(c, MPCX_EINVAL, "ring_gemm_q8: bad argument");
+  if (!a || !q || !out) return fail(c, MPCX_EINVAL, "ring_gemm_q8: null pointer");
+  if (!aligned(q, 16) || !aligned(scale, 4) || !aligned(tok, 4) || !aligned(a, c->bw / 8) || !aligned(out, c->bw / 8))
+    return fail(c, MPCX_EINVAL, "ring_gemm_q8: misaligned pointer");
+  const ByteRows rc = word_rows(c, out, size_t(M), ldc, size_t(N));
+  const ByteRows rq = {q, size_t(N), std::min(ldq, size_t(1) << 60), size_t(K)};
+  if (!rows_apart(rc, word_rows(c, a, size_t(M), lda, size_t(K))) || !rows_apart(rc, rq) ||
+      (scale && !rows_apart(rc, scale, size_t(N) * 4)) || (tok && !rows_apart(rc, tok, size_t(M) * 4)))
+    return fail(c, MPCX_EINVAL, "ring_gemm_q8: the output overlaps an input");
+  return c->bw == 32 ? gemm_q8_t<uint32_t>(c, M, K, N, a, lda, q, ldq, scale, tok, out, ldc)
+                     : gemm_q8_t<uint64_t>(c, M, K, N, a, lda, q, ldq, scale, tok, out, ldc);
+}
+
 // The cache's sizes are positive, a token's words countable in 31 bits and all in 60.
 static bool valid_cache(const mpcx_cache &k) {
   if (k.n_heads < 1 || k.head_dim < 1 || k.page_size < 1 || k.n_pages < 1) return false;
@@ -1372,6 +1408,264 @@ mpcx_status mpcx_attn_mix_message(mpcx_ctx *c, int party, const mpcx_attn *a, co
   if (party == 0)
     return attn_eval(c, false, AttnForm::P0, a, key, nullptr, phat, vhat, vb, nullptr, nullptr, nullptr, msg);
   return attn_eval(c, false, AttnForm::P1, a, nullptr, key, phat, vhat, nullptr, vb, nullptr, nullptr, msg);
+}
+
+// ---------------- the norm's gates ----------------
+namespace {
+// rows * dim words, countable in 60 bits
+bool norm_sizes(size_t rows, int dim) { return dim >= 1 && rows <= (size_t(1) << 60) / size_t(dim); }
+// The same rows: an output may take an input's place.
+bool same_rows(const ByteRows &a, const ByteRows &b) { return a.p == b.p && (a.rows <= 1 || a.pitch == b.pitch); }
+bool same_or_apart(const ByteRows &a, const ByteRows &b) { return same_rows(a, b) || rows_apart(a, b); }
+
+struct SumsCall {  // the arguments of norm_sums' calls; null and 0 where a call has none
+  size_t rows;
+  int dim;
+  const void *k0, *k1, *x;
+  size_t ldx;
+  const void *d;
+  size_t ldd;
+  void *h;
+  size_t ldh;
+  void *s;
+};
+// The rows of a call: x's, the residual's and their sum's.  Null where they are valid, else
+// what is wrong.
+const char *sums_rows(const mpcx_ctx *c, const SumsCall &g, ByteRows *rx, ByteRows *rd, ByteRows *rh) {
+  const size_t n = size_t(g.dim), tb = size_t(c->bw) / 8;
+  if (g.ldx < n || (g.d && (g.ldd < n || g.ldh < n))) return "rows overlap";
+  if (!g.x || !g.s || (g.d && !g.h)) return "null pointer";
+  if (!g.d && g.h) return "a sum without a residual";
+  if (!aligned(g.x, tb) || !aligned(g.d, tb) || !aligned(g.h, tb) || !aligned(g.s, tb)) return "misaligned pointer";
+  *rx = word_rows(c, g.x, g.rows, g.ldx, n);
+  *rd = word_rows(c, g.d, g.d ? g.rows : 0, g.ldd, n);
+  *rh = word_rows(c, g.h, g.h ? g.rows : 0, g.ldh, n);
+  const size_t ns = g.rows * tb;
+  if (!same_or_apart(*rh, *rx) || !same_or_apart(*rh, *rd) || !rows_apart(*rx, g.s, ns) || !rows_apart(*rd, g.s, ns) ||
+      !rows_apart(*rh, g.s, ns))
+    return "an output overlaps another buffer";
+  return nullptr;
+}
+template <typename T>
+NormSumsArgs<T> sums_args(const SumsCall &g) {
+  NormSumsArgs<T> a;
+  a.rows = g.rows;
+  a.dim = size_t(g.dim);
+  a.x = static_cast<const T *>(g.x);
+  a.ldx = g.ldx;
+  a.d = static_cast<const T *>(g.d);
+  a.ldd = g.ldd;
+  a.h = static_cast<T *>(g.h);
+  a.ldh = g.ldh;
+  a.s = static_cast<T *>(g.s);
+  return a;
+}
+template <typename T>
+mpcx_status sums_keygen_t(mpcx_ctx *c, const SumsCall &g, uint64_t seed, uint32_t gate, uint8_t *k0, uint8_t *k1) {
+  const size_t n = g.rows * size_t(g.dim), at = attn_key_second(c, n);
+  T *A1 = reinterpret_cast<T *>(k1), *C1 = reinterpret_cast<T *>(k1 + at);
+  HIPC(c, launch_prf_ring<T>(c->L, seed, gate, F_ROUT, g.rows, static_cast<T *>(g.s)), "prf");
+  NormSumsArgs<T> a = sums_args<T>(g);
+  a.c0 = a.s;
+  a.s = C1;
+  a.copy = A1;
+  HIPC(c, launch_norm_sums<T>(c->L, NormForm::DEAL, a), "norm_sums_keygen");
+  // a mask and a term are split where party 1's share of them goes
+  HIPC(c, launch_split<T>(c->L, seed, gate, F_SPLIT + 0, n, A1, reinterpret_cast<T *>(k0), A1, nullptr), "split");
+  HIPC(c, launch_split<T>(c->L, seed, gate, F_SPLIT + 2, g.rows, C1, reinterpret_cast<T *>(k0 + at), C1, nullptr),
+       "split");
+  HIPC(c, hipStreamSynchronize(c->L.stream), "sync");
+  return MPCX_OK;
+}
+template <typename T>
+mpcx_status sums_eval_t(mpcx_ctx *c, NormForm form, const SumsCall &g) {
+  const size_t at = attn_key_second(c, g.rows * size_t(g.dim));
+  NormSumsArgs<T> a = sums_args<T>(g);
+  if (g.k0) {
+    a.a0 = static_cast<const T *>(g.k0);
+    a.c0 = reinterpret_cast<const T *>(static_cast<const uint8_t *>(g.k0) + at);
+  }
+  if (g.k1) {
+    a.a1 = static_cast<const T *>(g.k1);
+    a.c1 = reinterpret_cast<const T *>(static_cast<const uint8_t *>(g.k1) + at);
+  }
+  HIPC(c, launch_norm_sums<T>(c->L, form, a), "norm_sums");
+  if (form == NormForm::BOTH) c->counters.msg(g.rows, c->bw);
+  return MPCX_OK;
+}
+mpcx_status sums_eval(mpcx_ctx *c, NormForm form, const SumsCall &g) {
+  CHECK_CTX(c);
+  if (!norm_sizes(g.rows, g.dim)) return fail(c, MPCX_EINVAL, "norm_sums: bad argument");
+  if (g.rows == 0) return MPCX_OK;
+  ByteRows rx, rd, rh;
+  const char *bad = sums_rows(c, g, &rx, &rd, &rh);
+  if (bad) return fail(c, MPCX_EINVAL, std::string("norm_sums: ") + bad);
+  const bool p0 = form != NormForm::P1, p1 = form != NormForm::P0;
+  if ((p0 && !g.k0) || (p1 && !g.k1)) return fail(c, MPCX_EINVAL, "norm_sums: null pointer");
+  if (!aligned(g.k0, 16) || !aligned(g.k1, 16)) return fail(c, MPCX_EINVAL, "norm_sums: misaligned pointer");
+  const size_t ns = g.rows * (size_t(c->bw) / 8), key = attn_key_end(c, g.rows * size_t(g.dim), g.rows);
+  for (const void *k : {p0 ? g.k0 : nullptr, p1 ? g.k1 : nullptr})
+    if (k && (!rows_apart(rh, k, key) || !bytes_apart(g.s, ns, k, key)))
+      return fail(c, MPCX_EINVAL, "norm_sums: an output overlaps another buffer");
+  return c->bw == 32 ? sums_eval_t<uint32_t>(c, form, g) : sums_eval_t<uint64_t>(c, form, g);
+}
+}  // namespace
+
+size_t mpcx_norm_sums_key_bytes(mpcx_ctx *c, size_t rows, int dim) {
+  return c && norm_sizes(rows, dim) ? attn_key_end(c, rows * size_t(dim), rows) : 0;
+}
+mpcx_status mpcx_norm_sums_keygen(mpcx_ctx *c, size_t rows, int dim, const void *rx, size_t ldx, const void *rd,
+                                  size_t ldd, void *rh, size_t ldh, void *rs, uint64_t seed, uint32_t gate, void *k0,
+                                  void *k1) {
+  CHECK_CTX(c);
+  const SumsCall g = {rows, dim, nullptr, nullptr, rx, ldx, rd, ldd, rh, ldh, rs};
+  if (!norm_sizes(rows, dim)) return fail(c, MPCX_EINVAL, "norm_sums_keygen: bad argument");
+  if (rows == 0) return MPCX_OK;
+  ByteRows bx, bd, bh;
+  const char *bad = sums_rows(c, g, &bx, &bd, &bh);
+  if (bad) return fail(c, MPCX_EINVAL, std::string("norm_sums_keygen: ") + bad);
+  if (!k0 || !k1) return fail(c, MPCX_EINVAL, "norm_sums_keygen: null pointer");
+  if (!aligned(k0, 16) || !aligned(k1, 16)) return fail(c, MPCX_EINVAL, "norm_sums_keygen: misaligned pointer");
+  const size_t ns = rows * (size_t(c->bw) / 8), key = attn_key_end(c, rows * size_t(dim), rows);
+  for (const void *k : {k0, k1})
+    if (!rows_apart(bx, k, key) || !rows_apart(bd, k, key) || !rows_apart(bh, k, key) || !bytes_apart(rs, ns, k, key))
+      return fail(c, MPCX_EINVAL, "norm_sums_keygen: an output overlaps another buffer");
+  if (!bytes_apart(k0, key, k1, key))
+    return fail(c, MPCX_EINVAL, "norm_sums_keygen: an output overlaps another buffer");
+  uint8_t *b0 = static_cast<uint8_t *>(k0), *b1 = static_cast<uint8_t *>(k1);
+  return c->bw == 32 ? sums_keygen_t<uint32_t>(c, g, seed, gate, b0, b1) : sums_keygen_t<uint64_t>(c, g, seed, gate, b0, b1);
+}
+mpcx_status mpcx_norm_sums_eval(mpcx_ctx *c, size_t rows, int dim, const void *k0, const void *k1, const void *xhat,
+                                size_t ldx, const void *dhat, size_t ldd, void *hhat, size_t ldh, void *shat) {
+  return sums_eval(c, NormForm::BOTH, {rows, dim, k0, k1, xhat, ldx, dhat, ldd, hhat, ldh, shat});
+}
+mpcx_status mpcx_norm_sums_message(mpcx_ctx *c, int party, size_t rows, int dim, const void *key, const void *xhat,
+                                   size_t ldx, const void *dhat, size_t ldd, void *hhat, size_t ldh, void *msg) {
+  CHECK_CTX(c);
+  if (party != 0 && party != 1) return fail(c, MPCX_EINVAL, "norm_sums_message: bad party");
+  return sums_eval(c, party ? NormForm::P1 : NormForm::P0,
+                   {rows, dim, party ? nullptr : key, party ? key : nullptr, xhat, ldx, dhat, ldd, hhat, ldh, msg});
+}
+
+namespace {
+struct ScaleCall {  // the arguments of norm_scale's calls; null and 0 where a call has none
+  size_t rows;
+  int dim;
+  const void *k0, *k1, *h;
+  size_t ldh;
+  const void *a0, *a1, *v, *gain;
+  void *y;
+  size_t ldy;
+};
+template <typename T>
+NormScaleArgs<T> scale_args(const mpcx_ctx *c, const ScaleCall &g, const void *k0, const void *k1) {
+  const size_t at = attn_key_second(c, g.rows);
+  NormScaleArgs<T> a;
+  a.rows = g.rows;
+  a.dim = size_t(g.dim);
+  a.h = static_cast<const T *>(g.h);
+  a.ldh = g.ldh;
+  a.a0 = static_cast<const T *>(g.a0);
+  a.a1 = static_cast<const T *>(g.a1);
+  a.v = static_cast<const T *>(g.v);
+  a.gain = static_cast<const T *>(g.gain);
+  a.y = static_cast<T *>(g.y);
+  a.ldy = g.ldy;
+  if (k0) {
+    a.b0 = static_cast<const T *>(k0);
+    a.c0 = reinterpret_cast<const T *>(static_cast<const uint8_t *>(k0) + at);
+  }
+  if (k1) {
+    a.b1 = static_cast<const T *>(k1);
+    a.c1 = reinterpret_cast<const T *>(static_cast<const uint8_t *>(k1) + at);
+  }
+  return a;
+}
+template <typename T>
+mpcx_status scale_keygen_t(mpcx_ctx *c, const ScaleCall &g, uint64_t seed, uint32_t gate, uint8_t *k0, uint8_t *k1) {
+  const size_t n = g.rows * size_t(g.dim), at = attn_key_second(c, g.rows);
+  T *C1 = reinterpret_cast<T *>(k1 + at);
+  HIPC(c, launch_split<T>(c->L, seed, gate, F_SPLIT + 0, g.rows, static_cast<const T *>(g.v), reinterpret_cast<T *>(k0),
+                          reinterpret_cast<T *>(k1), nullptr),
+       "split");
+  HIPC(c, launch_prf_ring<T>(c->L, seed, gate, F_ROUT, n, static_cast<T *>(g.y)), "prf");
+  NormScaleArgs<T> a = scale_args<T>(c, g, k0, nullptr);
+  a.c0 = static_cast<const T *>(g.y);
+  a.y = C1;
+  a.ldy = size_t(g.dim);
+  HIPC(c, launch_norm_scale<T>(c->L, NormForm::DEAL, a), "norm_scale_keygen");
+  HIPC(c, launch_split<T>(c->L, seed, gate, F_SPLIT + 2, n, C1, reinterpret_cast<T *>(k0 + at), C1, nullptr), "split");
+  HIPC(c, hipStreamSynchronize(c->L.stream), "sync");
+  return MPCX_OK;
+}
+template <typename T>
+mpcx_status scale_eval_t(mpcx_ctx *c, NormForm form, const ScaleCall &g) {
+  HIPC(c, launch_norm_scale<T>(c->L, form, scale_args<T>(c, g, g.k0, g.k1)), "norm_scale");
+  if (form == NormForm::BOTH) c->counters.msg(g.rows * size_t(g.dim), c->bw);
+  return MPCX_OK;
+}
+mpcx_status scale_eval(mpcx_ctx *c, NormForm form, const ScaleCall &g) {
+  CHECK_CTX(c);
+  const size_t n = size_t(g.dim), tb = size_t(c->bw) / 8;
+  if (!norm_sizes(g.rows, g.dim)) return fail(c, MPCX_EINVAL, "norm_scale: bad argument");
+  if (g.rows == 0) return MPCX_OK;
+  if (g.ldh < n || g.ldy < n) return fail(c, MPCX_EINVAL, "norm_scale: rows overlap");
+  const bool p0 = form != NormForm::P1, p1 = form != NormForm::P0;
+  if ((p0 && (!g.k0 || !g.a0)) || (p1 && (!g.k1 || !g.a1)) || !g.h || !g.v || !g.y)
+    return fail(c, MPCX_EINVAL, "norm_scale: null pointer");
+  for (const void *p : {g.h, g.a0, g.a1, g.v, g.gain, static_cast<const void *>(g.y)})
+    if (!aligned(p, tb)) return fail(c, MPCX_EINVAL, "norm_scale: misaligned pointer");
+  if (!aligned(g.k0, 16) || !aligned(g.k1, 16)) return fail(c, MPCX_EINVAL, "norm_scale: misaligned pointer");
+  const size_t plane = g.rows * n * tb, key = attn_key_end(c, g.rows, g.rows * n);
+  const ByteRows ry = word_rows(c, g.y, g.rows, g.ldy, n);
+  if (!same_or_apart(ry, word_rows(c, g.h, g.rows, g.ldh, n)) || !rows_apart(ry, g.v, g.rows * tb) ||
+      (g.gain && !rows_apart(ry, g.gain, n * tb)) ||
+      (p0 && (!rows_apart(ry, g.k0, key) || !rows_apart(ry, g.a0, plane))) ||
+      (p1 && (!rows_apart(ry, g.k1, key) || !rows_apart(ry, g.a1, plane))))
+    return fail(c, MPCX_EINVAL, "norm_scale: the output overlaps another buffer");
+  return c->bw == 32 ? scale_eval_t<uint32_t>(c, form, g) : scale_eval_t<uint64_t>(c, form, g);
+}
+}  // namespace
+
+size_t mpcx_norm_scale_key_bytes(mpcx_ctx *c, size_t rows, int dim) {
+  return c && norm_sizes(rows, dim) ? attn_key_end(c, rows, rows * size_t(dim)) : 0;
+}
+mpcx_status mpcx_norm_scale_keygen(mpcx_ctx *c, size_t rows, int dim, const void *a0, const void *a1, const void *rv,
+                                   const void *gain, void *ry, uint64_t seed, uint32_t gate, void *k0, void *k1) {
+  CHECK_CTX(c);
+  const size_t n = size_t(dim), tb = size_t(c->bw) / 8;
+  if (!norm_sizes(rows, dim)) return fail(c, MPCX_EINVAL, "norm_scale_keygen: bad argument");
+  if (rows == 0) return MPCX_OK;
+  if (!a0 || !a1 || !rv || !ry || !k0 || !k1) return fail(c, MPCX_EINVAL, "norm_scale_keygen: null pointer");
+  if (!aligned(a0, tb) || !aligned(a1, tb) || !aligned(rv, tb) || !aligned(gain, tb) || !aligned(ry, tb) ||
+      !aligned(k0, 16) || !aligned(k1, 16))
+    return fail(c, MPCX_EINVAL, "norm_scale_keygen: misaligned pointer");
+  const size_t plane = rows * n * tb, key = attn_key_end(c, rows, rows * n);
+  auto apart = [&](const void *p, size_t nb) {  // an output and the inputs
+    return bytes_apart(p, nb, a0, plane) && bytes_apart(p, nb, a1, plane) && bytes_apart(p, nb, rv, rows * tb) &&
+           (!gain || bytes_apart(p, nb, gain, n * tb));
+  };
+  if (!apart(ry, plane) || !apart(k0, key) || !apart(k1, key) || !bytes_apart(ry, plane, k0, key) ||
+      !bytes_apart(ry, plane, k1, key) || !bytes_apart(k0, key, k1, key))
+    return fail(c, MPCX_EINVAL, "norm_scale_keygen: an output overlaps another buffer");
+  const ScaleCall g = {rows, dim, nullptr, nullptr, nullptr, 0, a0, a1, rv, gain, ry, n};
+  uint8_t *b0 = static_cast<uint8_t *>(k0), *b1 = static_cast<uint8_t *>(k1);
+  return c->bw == 32 ? scale_keygen_t<uint32_t>(c, g, seed, gate, b0, b1)
+                     : scale_keygen_t<uint64_t>(c, g, seed, gate, b0, b1);
+}
+mpcx_status mpcx_norm_scale_eval(mpcx_ctx *c, size_t rows, int dim, const void *k0, const void *k1, const void *a0,
+                                 const void *a1, const void *hhat, size_t ldh, const void *vhat, const void *gain,
+                                 void *yhat, size_t ldy) {
+  return scale_eval(c, NormForm::BOTH, {rows, dim, k0, k1, hhat, ldh, a0, a1, vhat, gain, yhat, ldy});
+}
+mpcx_status mpcx_norm_scale_message(mpcx_ctx *c, int party, size_t rows, int dim, const void *key, const void *a,
+                                    const void *hhat, size_t ldh, const void *vhat, const void *gain, void *msg,
+                                    size_t ldy) {
+  CHECK_CTX(c);
+  if (party != 0 && party != 1) return fail(c, MPCX_EINVAL, "norm_scale_message: bad party");
+  if (party == 0)
+    return scale_eval(c, NormForm::P0, {rows, dim, key, nullptr, hhat, ldh, a, nullptr, vhat, gain, msg, ldy});
+  return scale_eval(c, NormForm::P1, {rows, dim, nullptr, key, hhat, ldh, nullptr, a, vhat, gain, msg, ldy});
 }
 
 // ---------------- reveal ----------------

@@ -108,6 +108,22 @@ _SIGS = {
     "mpcx_ring_gemm_q4_work_bytes": (C.c_size_t, [C.c_void_p, C.c_int, C.c_int]),
     "mpcx_ring_gemm_q4": (C.c_int, [C.c_void_p] + [C.c_int] * 4 + [C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p,
                                                                   C.c_void_p, C.c_size_t, C.c_void_p]),
+    "mpcx_ring_gemm_q8": (C.c_int, [C.c_void_p] + [C.c_int] * 3 + [C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t,
+                                                                  C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]),
+    "mpcx_norm_sums_key_bytes": (C.c_size_t, [C.c_void_p, C.c_size_t, C.c_int]),
+    "mpcx_norm_sums_keygen": (C.c_int, [C.c_void_p, C.c_size_t, C.c_int] + [C.c_void_p, C.c_size_t] * 3 +
+                              [C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p, C.c_void_p]),
+    "mpcx_norm_sums_eval": (C.c_int, [C.c_void_p, C.c_size_t, C.c_int, C.c_void_p, C.c_void_p] +
+                            [C.c_void_p, C.c_size_t] * 3 + [C.c_void_p]),
+    "mpcx_norm_sums_message": (C.c_int, [C.c_void_p, C.c_int, C.c_size_t, C.c_int, C.c_void_p] +
+                               [C.c_void_p, C.c_size_t] * 3 + [C.c_void_p]),
+    "mpcx_norm_scale_key_bytes": (C.c_size_t, [C.c_void_p, C.c_size_t, C.c_int]),
+    "mpcx_norm_scale_keygen": (C.c_int, [C.c_void_p, C.c_size_t, C.c_int] + [C.c_void_p] * 5 +
+                               [C.c_uint64, C.c_uint32, C.c_void_p, C.c_void_p]),
+    "mpcx_norm_scale_eval": (C.c_int, [C.c_void_p, C.c_size_t, C.c_int] + [C.c_void_p] * 5 +
+                             [C.c_size_t, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]),
+    "mpcx_norm_scale_message": (C.c_int, [C.c_void_p, C.c_int, C.c_size_t, C.c_int] + [C.c_void_p] * 3 +
+                                [C.c_size_t, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]),
     "mpcx_cache_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
                                     C.c_void_p]),
     "mpcx_split_mask": (C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p,
@@ -594,8 +610,8 @@ class Ctx:
     # ---------------- transformer layers (GPU tensors in and out) ----------------
     # Ring words are int32 (bw = 32) or int64 tensors on the context's device.
     # Where the context works on torch's current stream (set_stream) ring_gemm_q4,
-    # cache_append, split_mask and the attention evaluations and messages only
-    # enqueue, so a graph can capture them; gate_eval and the keygens wait for the
+    # ring_gemm_q8, cache_append, split_mask and the evaluations and messages of the
+    # attention and of the norm only enqueue, so a graph can capture them; gate_eval and the keygens wait for the
     # stream there, too.  Inputs made on another stream are the caller's to order
     # (Stream.wait_stream).  On any other stream all of them wait for torch's current
     # stream first and for their own work at the end, as the methods above do.
@@ -629,7 +645,7 @@ class Ctx:
     def _rows(self, t, what):
         """A matrix of ring words whose rows may be apart: its address and row stride."""
         if t.dtype is not self._word or t.get_device() != self._device or t.dim() != 2 or \
-                (t.shape[1] > 1 and t.stride(1) != 1):
+                (t.shape[1] > 1 and t.stride(1) != 1 and t.shape[0] > 0):
             raise MpcxError(f"{what}: need int{self.bw} rows on GPU {self._device}")
         return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
@@ -656,6 +672,35 @@ class Ctx:
         same = self._enter()
         self.check(self.lib.mpcx_ring_gemm_q4(self.h, M, K, N, group, ap, lda, qp, sp, op, ldc,
                                               work.data_ptr() if nb else None), "ring_gemm_q4")
+        self._leave(same)
+        return out
+
+    def ring_gemm_q8(self, a, q, scale=None, tokens=None, out=None):
+        """mpcx_ring_gemm_q8: a (M, K) ring words (rows may be apart), q (N, K, or K
+        rounded up to 16) int8 with rows at whole 16 bytes, scale (N) and tokens (M)
+        int32 or None -> (M, N)."""
+        torch = _torch()
+        ap, lda = self._rows(a, "ring_gemm_q8: a")
+        (M, K), (N, wide) = a.shape, q.shape
+        padded = (K + 15) // 16 * 16
+        if (M | K | N) >> 31:  # past a C int
+            raise MpcxError(f"ring_gemm_q8: sizes {M}, {K}, {N}")
+        ldq = q.stride(0) if N > 1 else padded
+        if q.dtype is not torch.int8 or q.get_device() != self._device or (wide != K and wide != padded) or \
+                (wide > 1 and q.stride(1) != 1) or ldq % 16 or ldq < K:
+            raise MpcxError(f"ring_gemm_q8: q: need int8 rows of {K} weights at whole 16 bytes on GPU {self._device}")
+        if out is None:
+            out = self._new((M, N))
+        op, ldc = self._rows(out, "ring_gemm_q8: out")
+        if out.shape != (M, N):
+            raise MpcxError(f"ring_gemm_q8: out: shape {tuple(out.shape)}, need {(M, N)}")
+        sp = self._ints(scale, "ring_gemm_q8: scale", torch.int32, (N,)) if scale is not None else None
+        tp = self._ints(tokens, "ring_gemm_q8: tokens", torch.int32, (M,)) if tokens is not None else None
+        if M == 0:
+            return out
+        same = self._enter()
+        self.check(self.lib.mpcx_ring_gemm_q8(self.h, M, K, N, ap, lda, q.data_ptr(), ldq, sp, tp, op, ldc),
+                   "ring_gemm_q8")
         self._leave(same)
         return out
 
@@ -799,6 +844,108 @@ class Ctx:
         same = self._enter()
         self.check(getattr(self.lib, "mpcx_" + what)(self.h, *([] if party is None else [party]), C.byref(a), *args,
                                                      out.data_ptr()), what)
+        self._leave(same)
+        return out
+
+    def _norm_rows(self, what, t, shape=None):
+        p, ld = self._rows(t, what)
+        if t.shape[1] >> 31 or (shape is not None and t.shape != shape):
+            raise MpcxError(f"{what}: shape {tuple(t.shape)}" + (f", need {tuple(shape)}" if shape is not None else ""))
+        return p, ld
+
+    def _norm_sums(self, what, x, d, out):
+        """The rows of a call: x's, d's and the sum's addresses and strides; the sum."""
+        xp, ldx = self._norm_rows(what, x)
+        if d is None:
+            if out is not None:
+                raise MpcxError(f"{what}: a sum without a residual")
+            return x, (xp, ldx, None, 0, None, 0)
+        if out is None:
+            out = self._new(x.shape)
+        return out, (xp, ldx) + self._norm_rows(what, d, x.shape) + self._norm_rows(what, out, x.shape)
+
+    def norm_sums_keygen(self, rx, rd=None, seed=1, gate=1):
+        """Keys of norm_sums_eval from the masks of x and of the residual (rows, dim):
+        the parties' keys, the mask of h (rx itself without a residual) and the sums'."""
+        what = "norm_sums_keygen"
+        rh, args = self._norm_sums(what, rx, rd, None)
+        rows, dim = rx.shape
+        nb = self.lib.mpcx_norm_sums_key_bytes(self.h, rows, dim)
+        k0, k1, rs = empty_dev(nb, self._device), empty_dev(nb, self._device), self._new((rows,))
+        same = self._enter()
+        self.check(self.lib.mpcx_norm_sums_keygen(self.h, rows, dim, *args, rs.data_ptr(), seed, gate, dptr(k0),
+                                                  dptr(k1)), what)
+        self._leave(same)
+        return k0, k1, rh, rs
+
+    def norm_sums_eval(self, k0, k1, xhat, dhat=None, out=None):
+        """mpcx_norm_sums_eval: h = x + d (x itself without d; out: where it goes, x or
+        d among others) and the rows' sums of squares.  Rows may be apart."""
+        return self._norm_sums_eval("norm_sums_eval", None, (k0, k1), xhat, dhat, out)
+
+    def norm_sums_message(self, party, key, xhat, dhat=None, out=None):
+        """h and one party's message of the sums; both messages add up to them."""
+        return self._norm_sums_eval("norm_sums_message", party, (key,), xhat, dhat, out)
+
+    def _norm_sums_eval(self, what, party, keys, x, d, out):
+        h, args = self._norm_sums(what, x, d, out)
+        rows, dim = x.shape
+        nb = self.lib.mpcx_norm_sums_key_bytes(self.h, rows, dim)
+        keys = [self._key(k, nb, what) for k in keys]
+        s = self._new((rows,))
+        same = self._enter()
+        if party is None:
+            st = self.lib.mpcx_norm_sums_eval(self.h, rows, dim, *keys, *args, s.data_ptr())
+        else:
+            st = self.lib.mpcx_norm_sums_message(self.h, party, rows, dim, *keys, *args, s.data_ptr())
+        self.check(st, what)
+        self._leave(same)
+        return h, s
+
+    def norm_scale_keygen(self, a0, a1, rv, dim, gain=None, seed=1, gate=1):
+        """Keys of norm_scale_eval from the shares of h's mask (norm_sums' keys: they begin
+        with them), the factors' mask (rows) and the gain; and the mask of y (rows, dim)."""
+        what = "norm_scale_keygen"
+        if rv.dim() != 1 or dim < 1 or dim >> 31:
+            raise MpcxError(f"{what}: factors of shape {tuple(rv.shape)}, rows of {dim}")
+        rows = rv.shape[0]
+        plane = rows * dim * self.bw // 8
+        ptrs = [self._key(a0, plane, what), self._key(a1, plane, what), self._words(rv, what),
+                self._words(gain, what, (dim,)) if gain is not None else None]
+        nb = self.lib.mpcx_norm_scale_key_bytes(self.h, rows, dim)
+        k0, k1, ry = empty_dev(nb, self._device), empty_dev(nb, self._device), self._new((rows, dim))
+        same = self._enter()
+        self.check(self.lib.mpcx_norm_scale_keygen(self.h, rows, dim, *ptrs, ry.data_ptr(), seed, gate, dptr(k0),
+                                                   dptr(k1)), what)
+        self._leave(same)
+        return k0, k1, ry
+
+    def norm_scale_eval(self, k0, k1, a0, a1, hhat, vhat, gain=None, out=None):
+        """mpcx_norm_scale_eval: rows (rows, dim) times their factors (rows) and the gain
+        (dim); a0, a1: the shares of h's mask (norm_sums' keys); out: where the rows
+        go, h among others."""
+        return self._norm_scale_eval("norm_scale_eval", None, (k0, k1), (a0, a1), hhat, vhat, gain, out)
+
+    def norm_scale_message(self, party, key, a, hhat, vhat, gain=None, out=None):
+        """One party's message of the scaled rows; both messages add up to them."""
+        return self._norm_scale_eval("norm_scale_message", party, (key,), (a,), hhat, vhat, gain, out)
+
+    def _norm_scale_eval(self, what, party, keys, shares, h, v, gain, out):
+        hp, ldh = self._norm_rows(what, h)
+        rows, dim = h.shape
+        if out is None:
+            out = self._new((rows, dim))
+        yp, ldy = self._norm_rows(what, out, h.shape)
+        nb, plane = self.lib.mpcx_norm_scale_key_bytes(self.h, rows, dim), rows * dim * self.bw // 8
+        ptrs = [self._key(k, nb, what) for k in keys] + [self._key(a, plane, what) for a in shares]
+        vp = self._words(v, what, (rows,))
+        gp = self._words(gain, what, (dim,)) if gain is not None else None
+        same = self._enter()
+        if party is None:
+            st = self.lib.mpcx_norm_scale_eval(self.h, rows, dim, *ptrs, hp, ldh, vp, gp, yp, ldy)
+        else:
+            st = self.lib.mpcx_norm_scale_message(self.h, party, rows, dim, *ptrs, hp, ldh, vp, gp, yp, ldy)
+        self.check(st, what)
         self._leave(same)
         return out
 

@@ -23,7 +23,8 @@
  * ordered before that stream, when the call is made.  mpcx_prg_hash, mpcx_prf,
  * mpcx_dcf_*, mpcx_tr_keygen, mpcx_mul_keygen, mpcx_lut8_keygen,
  * mpcx_reveal_keygen, mpcx_ring_gemm, mpcx_ring_lincomb, mpcx_ring_gemm_q4,
- * mpcx_cache_append, mpcx_split_mask, mpcx_attn_*_eval, mpcx_attn_*_message,
+ * mpcx_ring_gemm_q8, mpcx_cache_append, mpcx_split_mask, mpcx_attn_*_eval,
+ * mpcx_attn_*_message, mpcx_norm_*_eval, mpcx_norm_*_message,
  * mpcx_maxpool_eval_noalloc and, with mpcx_set_party_sync(ctx, 0),
  * mpcx_party_* return with their work enqueued there: their buffers stay in
  * use until the stream has reached it.
@@ -322,16 +323,16 @@ mpcx_status mpcx_ring_lincomb(mpcx_ctx *ctx, size_t rows, size_t cols, uint64_t 
 
 /* ---------------- transformer layers ----------------
  * Secure transformer inference on the same masked-public values: projections
- * with public 4-bit weights, a paged cache of masked keys and values, and the
- * two attention products that read it.  GPU-MPC's users reach such layers through
+ * with public 4-bit or 8-bit weights, a paged cache of masked keys and values, the
+ * two attention products that read it, and the two gates of a root-mean-square norm.  GPU-MPC's users reach such layers through
  * the calls that the reference makes for its own (gpuMatmul, gpu_mpc/ddg_orca_base.h:
  * 170-271); the reference has no counterpart of these.  Every operator is exact
  * modulo 2^bw.  All calls of this section but the keygens return with their work
  * enqueued on the context's stream (see the top of this file); the keygens
  * synchronize it.  Between the two products a caller uses the truncation and
  * ReLU gates above on the n_scores words (ReLU attention).  A scale, a table or
- * a bias is public, so the dealer's masks go through ring_gemm_q4 and
- * cache_append as the masked values do. */
+ * a bias is public, so the dealer's masks go through ring_gemm_q4, ring_gemm_q8
+ * and cache_append as the masked values do. */
 
 /* C = A . W mod 2^bw with public 4-bit weights W (K x N) and group scales:
  *   C[m, n] = sum_g scale[g, n] * sum_{k / group = g} q[n, k] * A[m, k],
@@ -349,6 +350,18 @@ mpcx_status mpcx_ring_lincomb(mpcx_ctx *ctx, size_t rows, size_t cols, uint64_t 
 size_t mpcx_ring_gemm_q4_work_bytes(mpcx_ctx *ctx, int M, int K);
 mpcx_status mpcx_ring_gemm_q4(mpcx_ctx *ctx, int M, int K, int N, int group, const void *d_a, size_t lda,
                               const uint8_t *d_q, const int32_t *d_scale, void *d_c, size_t ldc, void *d_work);
+/* C = A . W mod 2^bw with public 8-bit weights and a scale for each output channel
+ * and each token:
+ *   C[m, n] = tok[m] * scale[n] * sum_k q[n, k] * A[m, k],
+ * no key and no exchange (like mpcx_ring_gemm_q4; a token scale of 0 clears the
+ * row of a padding token).  d_a: M rows of K ring words, lda >= K words apart.
+ * d_q: N rows of K weights (-128..127), 16-byte aligned, ldq >= K bytes apart, a
+ * multiple of 16; what lies between K and the next multiple of 16 may be read and
+ * does not matter.  d_scale: N int32 steps, d_tok: M int32 steps; NULL: 1.  K up
+ * to 2^24.  d_c: M rows of N words, ldc >= N words apart; it overlaps no input
+ * (refused; d_a and d_c may be columns of one larger matrix). */
+mpcx_status mpcx_ring_gemm_q8(mpcx_ctx *ctx, int M, int K, int N, const void *d_a, size_t lda, const int8_t *d_q,
+                              size_t ldq, const int32_t *d_scale, const int32_t *d_tok, void *d_c, size_t ldc);
 
 /* A paged cache: n_pages pages of page_size slots for each of n_heads key /
  * value heads of head_dim words.  One plane (masked keys, a party's share of
@@ -456,6 +469,48 @@ mpcx_status mpcx_attn_scores_message(mpcx_ctx *ctx, int party, const mpcx_attn *
                                      const int32_t *d_pos, void *d_msg);
 mpcx_status mpcx_attn_mix_message(mpcx_ctx *ctx, int party, const mpcx_attn *a, const void *d_key,
                                   const void *d_phat, const void *d_vhat, const void *d_vb, void *d_msg);
+
+/* The two gates of a root-mean-square norm over rows of dim words, with the
+ * residual's addition; between them a caller takes the reciprocal root of one word
+ * a row with the gates above (mpcx_tr_*, mpcx_lut8_*, mpcx_mul_*).
+ *
+ * Sums (Beaver): h = x + d and s[t] = sum_j h[t, j]^2.  Rows of x, d and h: ldx, ldd,
+ * ldh >= dim words apart; d_h may be d_x or d_d.  Without a residual d_d and d_h
+ * are NULL and h = x.  Keygen takes the masks of x and d, writes the masks of h (at
+ * d_rh, where there is a residual) and s and the parties' keys: the share of
+ * h's mask (rows * dim words), then, from the next multiple of 256 bytes on, the
+ * share of the sums' term (rows words). */
+size_t mpcx_norm_sums_key_bytes(mpcx_ctx *ctx, size_t rows, int dim);
+mpcx_status mpcx_norm_sums_keygen(mpcx_ctx *ctx, size_t rows, int dim, const void *d_rx, size_t ldx, const void *d_rd,
+                                  size_t ldd, void *d_rh, size_t ldh, void *d_rs, uint64_t seed, uint32_t gate,
+                                  void *d_key0, void *d_key1);
+mpcx_status mpcx_norm_sums_eval(mpcx_ctx *ctx, size_t rows, int dim, const void *d_key0, const void *d_key1,
+                                const void *d_xhat, size_t ldx, const void *d_dhat, size_t ldd, void *d_hhat,
+                                size_t ldh, void *d_shat);
+/* Scale (Beaver): y[t, j] = gain[j] * h[t, j] * v[t], one factor v a row; d_gain: dim
+ * public ring words, NULL: 1.  d_a0, d_a1: the parties' shares of h's mask (rows *
+ * dim words each), which norm_sums' keys begin with: the mask is shared once for both
+ * gates.  Keygen takes them and the factors' mask, writes y's mask (rows * dim words)
+ * and the keys: the share of the factors' mask (rows words), then, 256-byte
+ * aligned, of the product term (rows * dim words).  Rows of h and y: ldh, ldy >=
+ * dim words apart; d_yhat may be d_hhat.
+ * Any other overlap of an output of these calls with another buffer is refused. */
+size_t mpcx_norm_scale_key_bytes(mpcx_ctx *ctx, size_t rows, int dim);
+mpcx_status mpcx_norm_scale_keygen(mpcx_ctx *ctx, size_t rows, int dim, const void *d_a0, const void *d_a1,
+                                   const void *d_rv, const void *d_gain, void *d_ry, uint64_t seed, uint32_t gate,
+                                   void *d_key0, void *d_key1);
+mpcx_status mpcx_norm_scale_eval(mpcx_ctx *ctx, size_t rows, int dim, const void *d_key0, const void *d_key1,
+                                 const void *d_a0, const void *d_a1, const void *d_hhat, size_t ldh,
+                                 const void *d_vhat, const void *d_gain, void *d_yhat, size_t ldy);
+/* One party's message of the two gates (party 0 or 1, its own key and share): both
+ * parties' messages add up to the gate's output.  norm_sums' also writes h, which
+ * every party forms by itself. */
+mpcx_status mpcx_norm_sums_message(mpcx_ctx *ctx, int party, size_t rows, int dim, const void *d_key,
+                                   const void *d_xhat, size_t ldx, const void *d_dhat, size_t ldd, void *d_hhat,
+                                   size_t ldh, void *d_msg);
+mpcx_status mpcx_norm_scale_message(mpcx_ctx *ctx, int party, size_t rows, int dim, const void *d_key,
+                                    const void *d_a, const void *d_hhat, size_t ldh, const void *d_vhat,
+                                    const void *d_gain, void *d_msg, size_t ldm);
 
 /* ---------------- reveal ----------------
  * Additive shares v0, v1 -> masked public v + r (revealIfLeaf,
