@@ -176,20 +176,26 @@ __global__ __launch_bounds__(1024) void k_q8_few(Q8Args<T> g) {
 
 // ---------------------------------------------------------------------------
 // Many rows: a workgroup of 2 x 4 waves takes 32 MT words by 64 NT columns.  A step is 128
-// k.  The workgroup forms the words' digits once and puts them into LDS in the order of the
-// MFMA's lanes; the weights, which only the two waves of a column share, go straight to the
-// lanes' registers.  Words and weights are asked for a step ahead.
-// LDS: plane, tile of 16 words, half of the step: 64 lanes' 16 bytes.  A thread writes 4
-// bytes of each plane; lane group lg's 16 words are turned by 2 (4 kk + lg) places, so that
-// the 64 lanes of a write, two rows of 32 groups of 4 k, fall into different banks.
+// k, double-buffered in LDS and asked for a step ahead.  The workgroup forms the words'
+// digits once; the weights go straight into LDS (to the lanes' registers they would take
+// four times as long: the 16 rows of an operand are as many places in memory for each
+// group of 16 lanes, where here 8 lanes take a row's 128 bytes).
+// Places in LDS, both such that neither the writes' nor the reads' lanes meet in a bank
+// (a read of 16 bytes serves lanes 0-3, 12-15, 20-27 together, then 4-11, 16-19, 28-31):
+//   digits   plane, tile of 16 words, half of the step o: 64 lanes' 16 bytes, word li of
+//            lane group lg at li ^ 2 (4 o + lg);
+//   weights  8 columns: a column's 8 groups of 16 k, group o 4 + lg at that ^ q8_turn.
 // K may be split over workgroups, which then add to a cleared output: sums modulo 2^bw do
 // not depend on their order.
 // ---------------------------------------------------------------------------
+__device__ __forceinline__ int q8_turn(int col) {  // of column col of a tile of 16
+  return (col >> 1 & 1) << 2 | (0x78 >> (col >> 2 << 1) & 3);
+}
 template <typename T, int MT, int NT>
 __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, int rows, int cols, int splits) {
   constexpr int NP = int(sizeof(T)), TILES = 2 * MT, BM = 16 * TILES, QUADS = BM * 32 / 512;
-  constexpr int PLANE = TILES * 2 * 1024;  // bytes
-  __shared__ __align__(16) uint8_t lds[2][NP * PLANE];
+  constexpr int PLANE = TILES * 2 * 1024, WORDS = NP * PLANE, WEIGHTS = 64 * NT * 128;  // bytes
+  __shared__ __align__(16) uint8_t lds[2][WORDS + WEIGHTS];
   const int at = xcd_swizzle(int(blockIdx.x), int(gridDim.x));
   const int split = at % splits, m0 = at / splits % rows * BM, n0 = at / splits / rows * 64 * NT;
   const int tid = int(threadIdx.x), lane = tid & 63, li = lane & 15, lg = lane >> 4;
@@ -197,37 +203,48 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
   const int all = (g.K + 127) / 128, s0 = int(int64_t(all) * split / splits), s1 = int(int64_t(all) * (split + 1) / splits);
   const int end = q8_row(g.K) - 16;
   // this thread's groups of four words: rows tid / 32 + 16 i, k 4 (tid % 32)
-  const int kq = tid % 32, j = kq / 4;  // j: kk and lg of the group
+  const int kq = tid % 32, j = kq / 4;  // j: 4 o + lg of the group
   const T *a[QUADS];
   uint32_t to[QUADS];
 #pragma unroll
   for (int i = 0; i < QUADS; i++) {
     const int r = tid / 32 + 16 * i;
     a[i] = g.a + size_t(min(m0 + r, g.M - 1)) * g.lda;
-    to[i] = uint32_t(((r / 16 * 2 + j / 4) * 64 + j % 4 * 16 + ((r % 16 + 2 * j) & 15)) * 16 + kq % 4 * 4);
+    to[i] = uint32_t(((r / 16 * 2 + j / 4) * 64 + j % 4 * 16 + ((r % 16) ^ (2 * j))) * 16 + kq % 4 * 4);
   }
+  // this lane's group of 16 weights of 8 columns, of NT such: column lane / 8 of the wave's
+  // 8 columns i
   const int8_t *q[NT];
+  int kw[NT];
 #pragma unroll
-  for (int t = 0; t < NT; t++) q[t] = g.q + size_t(min(n0 + (wn * NT + t) * 16 + li, g.N - 1)) * g.ldq;
-  uint32_t from[2];
+  for (int i = 0; i < NT; i++) {
+    const int col = (wave * NT + i) * 8 + lane / 8;
+    q[i] = g.q + size_t(min(n0 + col, g.N - 1)) * g.ldq;
+    kw[i] = 16 * ((lane % 8) ^ q8_turn(col % 16));
+  }
+  uint32_t from[2], fromw[2];
 #pragma unroll
-  for (int o = 0; o < 2; o++)
-    from[o] = uint32_t((o * 64 + lg * 16 + ((li + 2 * (4 * o + lg)) & 15)) * 16 + wm * MT * 2048);
+  for (int o = 0; o < 2; o++) {
+    from[o] = uint32_t((o * 64 + lg * 16 + (li ^ (2 * (4 * o + lg)))) * 16 + wm * MT * 2048);
+    fromw[o] = uint32_t(WORDS + wn * NT * 2048 + li * 128 + ((4 * o + lg) ^ q8_turn(li)) * 16);
+  }
 
   v4i_t acc[MT][NP][NT] = {};
   T w[QUADS][4];
-  v4i_t b[2][NT];
-  auto load_words = [&](int s) __attribute__((always_inline)) {
+  auto load_words = [&](int s) __attribute__((always_inline)) {  // of a step within K
+#pragma unroll
+    for (int i = 0; i < QUADS; i++) __builtin_memcpy(w[i], a[i] + (128 * s + 4 * kq), sizeof w[i]);
+  };
+  auto load_last = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < QUADS; i++) load4<T>(a[i], 128 * s + 4 * kq, g.K, w[i]);
   };
-  auto load_weights = [&](int s, v4i_t (&x)[2][NT]) __attribute__((always_inline)) {
+  auto load_weights = [&](int s, uint8_t *buf) __attribute__((always_inline)) {
 #pragma unroll
-    for (int o = 0; o < 2; o++) {
-      const int k = min(128 * s + 64 * o + 16 * lg, end);
-#pragma unroll
-      for (int t = 0; t < NT; t++) x[o][t] = *reinterpret_cast<const v4i_t *>(q[t] + k);
-    }
+    for (int i = 0; i < NT; i++)  // past the end of a row they meet words' zeros
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void *)(q[i] + min(128 * s + kw[i], end)),
+          (__attribute__((address_space(3))) void *)(buf + WORDS + (wave * NT + i) * 1024), 16, 0, 0);
   };
   auto put = [&](uint8_t *buf) __attribute__((always_inline)) {
 #pragma unroll
@@ -238,60 +255,84 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
       for (int p = 0; p < NP; p++) *reinterpret_cast<uint32_t *>(buf + p * PLANE + to[i]) = d[p];
     }
   };
-  // this wave's LDS accesses are done, and every wave's
+  // this wave's LDS accesses are done, its loads into LDS (which the compiler does not wait
+  // for) among them, and every wave's
   auto barrier = [&]() __attribute__((always_inline)) {
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   };
-  load_words(s0);
-  load_weights(s0, b);
-  put(lds[0]);
-  barrier();
-  for (int s = s0; s < s1; s++) {
-    const uint8_t *buf = lds[(s - s0) & 1];
-    v4i_t next[2][NT];
-    const bool more = s + 1 < s1;
-    if (more) {
-      load_words(s + 1);
-      load_weights(s + 1, next);
-    }
+  auto compute = [&](const uint8_t *buf) __attribute__((always_inline)) {
 #pragma unroll
-    for (int o = 0; o < 2; o++)
+    for (int o = 0; o < 2; o++) {
+      v4i_t b[NT];
+#pragma unroll
+      for (int t = 0; t < NT; t++) b[t] = *reinterpret_cast<const v4i_t *>(buf + fromw[o] + t * 2048);
 #pragma unroll
       for (int p = 0; p < NP; p++)
 #pragma unroll
         for (int i = 0; i < MT; i++) {
           const v4i_t d = *reinterpret_cast<const v4i_t *>(buf + p * PLANE + i * 2048 + from[o]);
 #pragma unroll
-          for (int t = 0; t < NT; t++) acc[i][p][t] = mfma64(d, b[o][t], acc[i][p][t]);
+          for (int t = 0; t < NT; t++) acc[i][p][t] = mfma64(d, b[t], acc[i][p][t]);
         }
-    if (more) {
-      put(lds[(s - s0 + 1) & 1]);
-#pragma unroll
-      for (int o = 0; o < 2; o++)
-#pragma unroll
-        for (int t = 0; t < NT; t++) b[o][t] = next[o][t];
     }
+  };
+  // Steps within K have no branch between a load and its use (at a join the compiler waits
+  // for all of them); a last step past K is loaded word by word.
+  const int whole = min(s1, g.K / 128);
+  load_weights(s0, lds[0]);
+  if (s0 < whole) load_words(s0);
+  else load_last(s0);
+  put(lds[0]);
+  barrier();
+  int s = s0;
+  for (; s + 1 < whole; s++) {
+    uint8_t *buf = lds[(s - s0) & 1], *next = lds[(s + 1 - s0) & 1];
+    load_words(s + 1);
+    load_weights(s + 1, next);
+    __builtin_amdgcn_sched_barrier(0);  // asked for here, not where they are used
+    compute(buf);
+    __builtin_amdgcn_sched_barrier(0);
+    put(next);
     barrier();
   }
+  if (s + 1 < s1) {
+    uint8_t *buf = lds[(s - s0) & 1], *next = lds[(s + 1 - s0) & 1];
+    load_weights(s + 1, next);
+    load_last(s + 1);
+    compute(buf);
+    put(next);
+    barrier();
+    s++;
+  }
+  compute(lds[(s - s0) & 1]);
+
+  int32_t sn[NT], sm[MT][4];
+#pragma unroll
+  for (int t = 0; t < NT; t++) sn[t] = g.scale ? g.scale[min(n0 + (wn * NT + t) * 16 + li, g.N - 1)] : 1;
 #pragma unroll
   for (int i = 0; i < MT; i++)
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
-      const int n = n0 + (wn * NT + t) * 16 + li;
+    for (int r = 0; r < 4; r++) sm[i][r] = g.tok ? g.tok[min(m0 + (wm * MT + i) * 16 + 4 * lg + r, g.M - 1)] : 1;
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int m = m0 + (wm * MT + i) * 16 + 4 * lg + r;
-        if (m >= g.M || n >= g.N) continue;
+  for (int i = 0; i < MT; i++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const int m = m0 + (wm * MT + i) * 16 + 4 * lg + r;
+      if (m >= g.M) continue;
+      T *c = g.c + size_t(m) * g.ldc;
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        const int n = n0 + (wn * NT + t) * 16 + li;
         T v = 0;
 #pragma unroll
         for (int p = 0; p < NP; p++) v += plane_word<T>(acc[i][p][t][r], p);
-        v = scaled<T>(g, v, m, n);
-        T *c = g.c + size_t(m) * g.ldc + n;
+        v *= T(int64_t(sn[t])) * T(int64_t(sm[i][r]));
+        if (n >= g.N) continue;
         if (splits == 1) {
-          *c = v;
+          c[n] = v;
         } else {
           using W = std::conditional_t<sizeof(T) == 4, unsigned, unsigned long long>;
-          atomicAdd(reinterpret_cast<W *>(c), W(v));
+          atomicAdd(reinterpret_cast<W *>(c + n), W(v));
         }
       }
     }
