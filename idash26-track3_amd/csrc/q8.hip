@@ -195,116 +195,193 @@ template <typename T, int MT, int NT>
 __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, int rows, int cols, int splits) {
   constexpr int NP = int(sizeof(T)), TILES = 2 * MT, BM = 16 * TILES, QUADS = BM * 32 / 512;
   constexpr int PLANE = TILES * 2 * 1024, WORDS = NP * PLANE, WEIGHTS = 64 * NT * 128;  // bytes
-  __shared__ __align__(16) uint8_t lds[2][WORDS + WEIGHTS];
+  __shared__ __align__(16) uint8_t lds[2 * WORDS + 2 * WEIGHTS];
   const int at = xcd_swizzle(int(blockIdx.x), int(gridDim.x));
   const int split = at % splits, m0 = at / splits % rows * BM, n0 = at / splits / rows * 64 * NT;
   const int tid = int(threadIdx.x), lane = tid & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 2, wn = wave & 3;
   const int all = (g.K + 127) / 128, s0 = int(int64_t(all) * split / splits), s1 = int(int64_t(all) * (split + 1) / splits);
   const int end = q8_row(g.K) - 16;
-  // this thread's groups of four words: rows tid / 32 + 16 i, k 4 (tid % 32)
+  // This thread's groups of four words: rows tid / 32 + 16 i, k 4 (tid % 32).  A row's place is
+  // 32 bits from one that the workgroup shares (launch_gemm_q8 bounds the strides).
   const int kq = tid % 32, j = kq / 4;  // j: 4 o + lg of the group
   const T *a[QUADS];
-  uint32_t to[QUADS];
+  uint32_t ao[QUADS];
 #pragma unroll
   for (int i = 0; i < QUADS; i++) {
-    const int r = tid / 32 + 16 * i;
-    a[i] = g.a + size_t(min(m0 + r, g.M - 1)) * g.lda;
-    to[i] = uint32_t(((r / 16 * 2 + j / 4) * 64 + j % 4 * 16 + ((r % 16) ^ (2 * j))) * 16 + kq % 4 * 4);
+    const int r = min(m0 + 16 * i, g.M - 1);
+    a[i] = g.a + size_t(r) * g.lda;
+    ao[i] = uint32_t(min(tid / 32, g.M - 1 - r)) * uint32_t(g.lda) + uint32_t(4 * kq);
   }
+  const uint32_t to = uint32_t((j * 16 + ((tid / 32) ^ (2 * j))) * 16 + kq % 4 * 4);
   // this lane's group of 16 weights of 8 columns, of NT such: column lane / 8 of the wave's
   // 8 columns i
   const int8_t *q[NT];
-  int kw[NT];
+  uint32_t qo[NT];
+  const int kw[2] = {16 * ((lane % 8) ^ q8_turn(lane / 8)), 16 * ((lane % 8) ^ q8_turn(8 + lane / 8))};
+  auto half = [&](int i) { return (wave * NT + i) & 1; };  // of the tile of 16 columns
 #pragma unroll
   for (int i = 0; i < NT; i++) {
-    const int col = (wave * NT + i) * 8 + lane / 8;
-    q[i] = g.q + size_t(min(n0 + col, g.N - 1)) * g.ldq;
-    kw[i] = 16 * ((lane % 8) ^ q8_turn(col % 16));
+    const int n = min(n0 + (wave * NT + i) * 8, g.N - 1);
+    q[i] = g.q + size_t(n) * g.ldq;
+    qo[i] = uint32_t(min(lane / 8, g.N - 1 - n)) * uint32_t(g.ldq);
   }
   uint32_t from[2], fromw[2];
 #pragma unroll
   for (int o = 0; o < 2; o++) {
     from[o] = uint32_t((o * 64 + lg * 16 + (li ^ (2 * (4 * o + lg)))) * 16 + wm * MT * 2048);
-    fromw[o] = uint32_t(WORDS + wn * NT * 2048 + li * 128 + ((4 * o + lg) ^ q8_turn(li)) * 16);
+    fromw[o] = uint32_t(2 * WORDS + wn * NT * 2048 + li * 128 + ((4 * o + lg) ^ q8_turn(li)) * 16);
   }
 
   v4i_t acc[MT][NP][NT] = {};
-  T w[QUADS][4];
-  auto load_words = [&](int s) __attribute__((always_inline)) {  // of a step within K
-#pragma unroll
-    for (int i = 0; i < QUADS; i++) __builtin_memcpy(w[i], a[i] + (128 * s + 4 * kq), sizeof w[i]);
+  struct Words {
+    T w[QUADS][4];
   };
-  auto load_last = [&](int s) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < QUADS; i++) load4<T>(a[i], 128 * s + 4 * kq, g.K, w[i]);
+  auto load_words = [&](int s, Words &x, int i) __attribute__((always_inline)) {  // of a step within K
+    __builtin_memcpy(x.w[i], a[i] + 128 * s + ao[i], sizeof x.w[i]);
   };
-  auto load_weights = [&](int s, uint8_t *buf) __attribute__((always_inline)) {
+  auto load_last = [&](int s, Words &x) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < NT; i++)  // past the end of a row they meet words' zeros
+    for (int i = 0; i < QUADS; i++) load4<T>(a[i] + (ao[i] - 4 * kq), 128 * s + 4 * kq, g.K, x.w[i]);
+  };
+  auto load_weights = [&](int s, int buf, auto within) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+      const uint32_t k = uint32_t(kw[half(i)]);
+      // past the end of a row they meet words' zeros
+      const int8_t *p = decltype(within)::value ? q[i] + 128 * s + (qo[i] + k) : q[i] + (qo[i] + min(128 * s + k, uint32_t(end)));
       __builtin_amdgcn_global_load_lds(
-          (const __attribute__((address_space(1))) void *)(q[i] + min(128 * s + kw[i], end)),
-          (__attribute__((address_space(3))) void *)(buf + WORDS + (wave * NT + i) * 1024), 16, 0, 0);
-  };
-  auto put = [&](uint8_t *buf) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < QUADS; i++) {
-      uint32_t d[NP];
-      planes4<T>(w[i], d);
-#pragma unroll
-      for (int p = 0; p < NP; p++) *reinterpret_cast<uint32_t *>(buf + p * PLANE + to[i]) = d[p];
+          (const __attribute__((address_space(1))) void *)p,
+          (__attribute__((address_space(3))) void *)(lds + 2 * WORDS + buf * WEIGHTS + (wave * NT + i) * 1024), 16, 0, 0);
     }
   };
-  // this wave's LDS accesses are done, its loads into LDS (which the compiler does not wait
-  // for) among them, and every wave's
+  auto put = [&](int buf, const Words &x, int i) __attribute__((always_inline)) {
+    uint32_t d[NP];
+    planes4<T>(x.w[i], d);
+#pragma unroll
+    for (int p = 0; p < NP; p++) *reinterpret_cast<uint32_t *>(lds + to + (buf * WORDS + p * PLANE + i * 2048)) = d[p];
+  };
+  // This wave's LDS accesses are done, its loads into LDS (which the compiler does not wait
+  // for) among them, and every wave's.
   auto barrier = [&]() __attribute__((always_inline)) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   };
-  auto compute = [&](const uint8_t *buf) __attribute__((always_inline)) {
+  // The products of a step, an operand of words read ahead; between them, a few
+  // instructions for each operand, the next step's words become digits (more).  The order
+  // is held: left free, the compiler reads so far ahead that registers spill.
+  constexpr int F = 2 * NP * MT;           // operands of words
+  constexpr int STAGES = F / QUADS;        // operands by the time of a group of four words
+  static_assert(STAGES == NP, "four planes take four stages");
+  struct Turning {
+    uint32_t y[4], z[4], l[2], h[2];
+  };
+  auto turn = [&](int buf, const Words &x, Turning &v, int i, int stage) __attribute__((always_inline)) {
+    uint8_t *p = lds + to + (buf * WORDS + i * 2048 + (stage & 4) * PLANE);
+    if (stage == 0) {
 #pragma unroll
-    for (int o = 0; o < 2; o++) {
-      v4i_t b[NT];
-#pragma unroll
-      for (int t = 0; t < NT; t++) b[t] = *reinterpret_cast<const v4i_t *>(buf + fromw[o] + t * 2048);
-#pragma unroll
-      for (int p = 0; p < NP; p++)
-#pragma unroll
-        for (int i = 0; i < MT; i++) {
-          const v4i_t d = *reinterpret_cast<const v4i_t *>(buf + p * PLANE + i * 2048 + from[o]);
-#pragma unroll
-          for (int t = 0; t < NT; t++) acc[i][p][t] = mfma64(d, b[t], acc[i][p][t]);
+      for (int k = 0; k < 4; k++) {
+        if constexpr (NP == 4) {
+          v.y[k] = x.w[i][k] + 0x80808080u;
+        } else {
+          const uint64_t u = x.w[i][k] + 0x8080808080808080ull;
+          v.y[k] = uint32_t(u), v.z[k] = uint32_t(u >> 32);
         }
+      }
+    } else if (stage % 4 == 1 || stage == 4) {
+      const uint32_t(&y)[4] = stage & 4 ? v.z : v.y;
+      if (stage == 4) return;
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        v.l[k] = __builtin_amdgcn_perm(y[2 * k + 1], y[2 * k], 0x05010400u);
+        v.h[k] = __builtin_amdgcn_perm(y[2 * k + 1], y[2 * k], 0x07030602u);
+      }
+    } else {
+      const uint32_t(&u)[2] = stage & 1 ? v.h : v.l;
+      p += (stage & 1) * 2 * PLANE;
+      *reinterpret_cast<uint32_t *>(p) = __builtin_amdgcn_perm(u[1], u[0], 0x05040100u) ^ 0x80808080u;
+      *reinterpret_cast<uint32_t *>(p + PLANE) = __builtin_amdgcn_perm(u[1], u[0], 0x07060302u) ^ 0x80808080u;
     }
   };
-  // Steps within K have no branch between a load and its use (at a join the compiler waits
-  // for all of them); a last step past K is loaded word by word.
+  auto compute = [&](int buf, const Words &x, auto more) __attribute__((always_inline)) {
+    v4i_t b[NT];
+    Turning v;
+    auto operand = [&](int f) __attribute__((always_inline)) {
+      return *reinterpret_cast<const v4i_t *>(lds + from[f / (NP * MT)] +
+                                              (buf * WORDS + f / MT % NP * PLANE + f % MT * 2048));
+    };
+    v4i_t d = operand(0);
+#pragma unroll
+    for (int f = 0; f < F; f++) {
+      const int o = f / (NP * MT), p = f / MT % NP, i = f % MT;
+      if (f % (NP * MT) == 0) {
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+          b[t] = *reinterpret_cast<const v4i_t *>(lds + fromw[o] + (buf * WEIGHTS + t * 2048));
+      }
+      v4i_t ahead = d;
+      if (f + 1 < F) ahead = operand(f + 1);
+      if constexpr (decltype(more)::value) turn(buf ^ 1, x, v, f / STAGES, f % STAGES);
+#pragma unroll
+      for (int t = 0; t < NT; t++) acc[i][p][t] = mfma64(d, b[t], acc[i][p][t]);
+      d = ahead;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
+  // Words are asked for two steps ahead and weights one.  Steps within K have no branch
+  // between a load and its use (at a join the compiler waits for all of them); a last step
+  // past K is loaded word by word.
   const int whole = min(s1, g.K / 128);
-  load_weights(s0, lds[0]);
-  if (s0 < whole) load_words(s0);
-  else load_last(s0);
-  put(lds[0]);
+  Words x, y;
+  auto any_words = [&](int s, Words &v) __attribute__((always_inline)) {
+    if (s < whole) {
+#pragma unroll
+      for (int i = 0; i < QUADS; i++) load_words(s, v, i);
+    } else if (s < s1) {
+      load_last(s, v);
+    }
+  };
+  auto put_all = [&](int buf, const Words &v) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < QUADS; i++) put(buf, v, i);
+  };
+  load_weights(s0, 0, no);
+  {
+    Words first;
+    any_words(s0, first);
+    any_words(s0 + 1, x);
+    put_all(0, first);
+  }
   barrier();
   int s = s0;
-  for (; s + 1 < whole; s++) {
-    uint8_t *buf = lds[(s - s0) & 1], *next = lds[(s + 1 - s0) & 1];
-    load_words(s + 1);
-    load_weights(s + 1, next);
+  auto step = [&](auto buf, Words &cur, Words &ahead) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < QUADS; i++)  // here, so that their use does not wait for the loads that leave next
+#pragma unroll
+      for (int k = 0; k < 4; k++) asm volatile("" : "+v"(cur.w[i][k]));
+#pragma unroll
+    for (int i = 0; i < QUADS; i++) load_words(s + 2, ahead, i);
+    load_weights(s + 1, buf ^ 1, yes);
     __builtin_amdgcn_sched_barrier(0);  // asked for here, not where they are used
-    compute(buf);
-    __builtin_amdgcn_sched_barrier(0);
-    put(next);
-    barrier();
-  }
-  if (s + 1 < s1) {
-    uint8_t *buf = lds[(s - s0) & 1], *next = lds[(s + 1 - s0) & 1];
-    load_weights(s + 1, next);
-    load_last(s + 1);
-    compute(buf);
-    put(next);
+    compute(buf, cur, yes);
     barrier();
     s++;
+  };
+  while (s + 3 < whole) {
+    step(std::integral_constant<int, 0>{}, x, y);
+    step(std::integral_constant<int, 1>{}, y, x);
   }
-  compute(lds[(s - s0) & 1]);
+  // the last three or fewer
+  for (int buf = 0; s < s1; s++, buf ^= 1) {
+    if (s + 1 < s1) load_weights(s + 1, buf ^ 1, no);
+    compute(buf, x, no);
+    if (s + 1 < s1) {
+      put_all(buf ^ 1, x);
+      any_words(s + 2, x);
+      barrier();
+    }
+  }
 
   int32_t sn[NT], sm[MT][4];
 #pragma unroll
@@ -393,6 +470,19 @@ hipError_t launch_part(const Launch &L, const Q8Args<T> &g) {
 template <typename T>
 hipError_t launch_gemm_q8(const Launch &L, const Q8Args<T> &g) {
   if (g.K > kQ8MaxK) return hipErrorInvalidValue;
+  // rows that lie gigabytes apart: by the kernel of few rows, whose places are 64 bits wide
+  if (g.M > 16 && (g.lda >= size_t(1) << 25 || g.ldq >= size_t(1) << 28)) {
+    for (int64_t m = 0; m < g.M; m += 16) {
+      Q8Args<T> p = g;
+      p.M = int(std::min<int64_t>(g.M - m, 16));
+      p.a += size_t(m) * g.lda;
+      if (p.tok) p.tok += m;
+      p.c += size_t(m) * g.ldc;
+      const hipError_t e = launch_gemm_q8<T>(L, p);
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  }
   // HIP cuts a launch of 2^32 threads along a dimension short: in parts of at most 2^16
   // rows by 2^14 columns, 2^11 by 2^8 tiles of 512 threads, and K in up to 2^8 parts, the
   // grid stays below that
