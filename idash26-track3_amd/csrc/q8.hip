@@ -21,6 +21,7 @@ namespace mpcx {
 namespace {
 
 constexpr int kExact = 1 << 16;  // terms of a 32-bit plane sum
+constexpr int kRsrcWord3 = 0x00020000;  // buffer resource: 32-bit offsets
 
 __device__ __forceinline__ v4i_t mfma64(v4i_t a, v4i_t b, v4i_t c) {
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
@@ -195,7 +196,8 @@ template <typename T, int MT, int NT>
 __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, int rows, int cols, int splits) {
   constexpr int NP = int(sizeof(T)), TILES = 2 * MT, BM = 16 * TILES, QUADS = BM * 32 / 512;
   constexpr int PLANE = TILES * 2 * 1024, WORDS = NP * PLANE, WEIGHTS = 64 * NT * 128;  // bytes
-  __shared__ __align__(16) uint8_t lds[2 * WORDS + 2 * WEIGHTS];
+  constexpr int WB = 3;  // steps of weights in LDS: in use, there, on their way
+  __shared__ __align__(16) uint8_t lds[2 * WORDS + WB * WEIGHTS];
   const int at = xcd_swizzle(int(blockIdx.x), int(gridDim.x));
   const int split = at % splits, m0 = at / splits % rows * BM, n0 = at / splits / rows * 64 * NT;
   const int tid = int(threadIdx.x), lane = tid & 63, li = lane & 15, lg = lane >> 4;
@@ -216,15 +218,16 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
   const uint32_t to = uint32_t((j * 16 + ((tid / 32) ^ (2 * j))) * 16 + kq % 4 * 4);
   // this lane's group of 16 weights of 8 columns, of NT such: column lane / 8 of the wave's
   // 8 columns i
-  const int8_t *q[NT];
-  uint32_t qo[NT];
-  const int kw[2] = {16 * ((lane % 8) ^ q8_turn(lane / 8)), 16 * ((lane % 8) ^ q8_turn(8 + lane / 8))};
-  auto half = [&](int i) { return (wave * NT + i) & 1; };  // of the tile of 16 columns
+  const int8_t *q = g.q + size_t(n0) * g.ldq;
+  const int nq = min(g.N - n0, 64 * NT);
+  const __amdgpu_buffer_rsrc_t qr = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<int8_t *>(q), short(0), int(uint32_t(nq - 1) * uint32_t(g.ldq) + uint32_t(end + 16)), kRsrcWord3);
+  uint32_t qo[NT], qk[NT];
 #pragma unroll
   for (int i = 0; i < NT; i++) {
-    const int n = min(n0 + (wave * NT + i) * 8, g.N - 1);
-    q[i] = g.q + size_t(n) * g.ldq;
-    qo[i] = uint32_t(min(lane / 8, g.N - 1 - n)) * uint32_t(g.ldq);
+    const int col = (wave * NT + i) * 8 + lane / 8;
+    qk[i] = uint32_t(16 * ((lane % 8) ^ q8_turn(col % 16)));
+    qo[i] = uint32_t(min(col, nq - 1)) * uint32_t(g.ldq);
   }
   uint32_t from[2], fromw[2];
 #pragma unroll
@@ -247,12 +250,11 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
   auto load_weights = [&](int s, int buf, auto within) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NT; i++) {
-      const uint32_t k = uint32_t(kw[half(i)]);
-      // past the end of a row they meet words' zeros
-      const int8_t *p = decltype(within)::value ? q[i] + 128 * s + (qo[i] + k) : q[i] + (qo[i] + min(128 * s + k, uint32_t(end)));
-      __builtin_amdgcn_global_load_lds(
-          (const __attribute__((address_space(1))) void *)p,
-          (__attribute__((address_space(3))) void *)(lds + 2 * WORDS + buf * WEIGHTS + (wave * NT + i) * 1024), 16, 0, 0);
+      auto *to = (__attribute__((address_space(3))) void *)(lds + 2 * WORDS + buf * WEIGHTS + (wave * NT + i) * 1024);
+      if constexpr (decltype(within)::value)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(qr, to, 16, int(qo[i] + qk[i]), 128 * s, 0, 0);
+      else  // past the end of a row they meet words' zeros
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(qr, to, 16, int(qo[i] + min(128 * s + qk[i], uint32_t(end))), 0, 0, 0);
     }
   };
   auto put = [&](int buf, const Words &x, int i) __attribute__((always_inline)) {
@@ -262,10 +264,11 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
     for (int p = 0; p < NP; p++) *reinterpret_cast<uint32_t *>(lds + to + (buf * WORDS + p * PLANE + i * 2048)) = d[p];
   };
   // This wave's LDS accesses are done, its loads into LDS (which the compiler does not wait
-  // for) among them, and every wave's.
-  auto barrier = [&]() __attribute__((always_inline)) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  // for) but for the last `later` loads among them, and every wave's.
+  auto barrier = [&](auto later) __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(later)::value) : "memory");
   };
+  constexpr std::integral_constant<int, 0> none{};
   // The products of a step, an operand of words read ahead; between them, a few
   // instructions for each operand, the next step's words become digits (more).  The order
   // is held: left free, the compiler reads so far ahead that registers spill.
@@ -302,7 +305,7 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
       *reinterpret_cast<uint32_t *>(p + PLANE) = __builtin_amdgcn_perm(u[1], u[0], 0x07060302u) ^ 0x80808080u;
     }
   };
-  auto compute = [&](int buf, const Words &x, auto more) __attribute__((always_inline)) {
+  auto compute = [&](int buf, int wbuf, const Words &x, auto more) __attribute__((always_inline)) {
     v4i_t b[NT];
     Turning v;
     auto operand = [&](int f) __attribute__((always_inline)) {
@@ -316,7 +319,7 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
       if (f % (NP * MT) == 0) {
 #pragma unroll
         for (int t = 0; t < NT; t++)
-          b[t] = *reinterpret_cast<const v4i_t *>(lds + fromw[o] + (buf * WEIGHTS + t * 2048));
+          b[t] = *reinterpret_cast<const v4i_t *>(lds + (fromw[o] + uint32_t(wbuf * WEIGHTS)) + t * 2048);
       }
       v4i_t ahead = d;
       if (f + 1 < F) ahead = operand(f + 1);
@@ -329,9 +332,9 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
   };
   constexpr std::true_type yes{};
   constexpr std::false_type no{};
-  // Words are asked for two steps ahead and weights one.  Steps within K have no branch
-  // between a load and its use (at a join the compiler waits for all of them); a last step
-  // past K is loaded word by word.
+  // Words and weights are asked for two steps ahead: words have a step to come and are then
+  // turned, weights have two.  Steps within K have no branch between a load and its use (at a
+  // join the compiler waits for all of them); a last step past K is loaded word by word.
   const int whole = min(s1, g.K / 128);
   Words x, y;
   auto any_words = [&](int s, Words &v) __attribute__((always_inline)) {
@@ -347,14 +350,20 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
     for (int i = 0; i < QUADS; i++) put(buf, v, i);
   };
   load_weights(s0, 0, no);
+  if (s0 + 1 < s1) load_weights(s0 + 1, 1, no);
   {
     Words first;
     any_words(s0, first);
     any_words(s0 + 1, x);
     put_all(0, first);
   }
-  barrier();
-  int s = s0;
+  barrier(none);
+  int s = s0, wb = 0, wnext = 2;  // buffers of this step's weights and of those asked for next
+  auto turn_buffers = [&]() {
+    s++;
+    wb = wb == WB - 1 ? 0 : wb + 1;
+    wnext = wnext == WB - 1 ? 0 : wnext + 1;
+  };
   auto step = [&](auto buf, Words &cur, Words &ahead) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < QUADS; i++)  // here, so that their use does not wait for the loads that leave next
@@ -362,24 +371,25 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
       for (int k = 0; k < 4; k++) asm volatile("" : "+v"(cur.w[i][k]));
 #pragma unroll
     for (int i = 0; i < QUADS; i++) load_words(s + 2, ahead, i);
-    load_weights(s + 1, buf ^ 1, yes);
+    load_weights(s + 2, wnext, yes);
     __builtin_amdgcn_sched_barrier(0);  // asked for here, not where they are used
-    compute(buf, cur, yes);
-    barrier();
-    s++;
+    compute(buf, wb, cur, yes);
+    // the next step's weights are older than these loads, at least one for each 16 bytes
+    barrier(std::integral_constant<int, QUADS * int(sizeof(T)) / 4 + NT>{});
+    turn_buffers();
   };
   while (s + 3 < whole) {
     step(std::integral_constant<int, 0>{}, x, y);
     step(std::integral_constant<int, 1>{}, y, x);
   }
   // the last three or fewer
-  for (int buf = 0; s < s1; s++, buf ^= 1) {
-    if (s + 1 < s1) load_weights(s + 1, buf ^ 1, no);
-    compute(buf, x, no);
+  for (int buf = 0; s < s1; turn_buffers(), buf ^= 1) {
+    if (s + 2 < s1) load_weights(s + 2, wnext, no);
+    compute(buf, wb, x, no);
     if (s + 1 < s1) {
       put_all(buf ^ 1, x);
       any_words(s + 2, x);
-      barrier();
+      barrier(none);
     }
   }
 
@@ -471,7 +481,7 @@ template <typename T>
 hipError_t launch_gemm_q8(const Launch &L, const Q8Args<T> &g) {
   if (g.K > kQ8MaxK) return hipErrorInvalidValue;
   // rows that lie gigabytes apart: by the kernel of few rows, whose places are 64 bits wide
-  if (g.M > 16 && (g.lda >= size_t(1) << 25 || g.ldq >= size_t(1) << 28)) {
+  if (g.M > 16 && (g.lda >= size_t(1) << 25 || g.ldq >= size_t(1) << 23)) {
     for (int64_t m = 0; m < g.M; m += 16) {
       Q8Args<T> p = g;
       p.M = int(std::min<int64_t>(g.M - m, 16));
