@@ -11,6 +11,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "attn.h"
@@ -199,7 +200,10 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
   constexpr int WB = 3;  // steps of weights in LDS: in use, there, on their way
   __shared__ __align__(16) uint8_t lds[2 * WORDS + WB * WEIGHTS];
   const int at = xcd_swizzle(int(blockIdx.x), int(gridDim.x));
-  const int split = at % splits, m0 = at / splits % rows * BM, n0 = at / splits / rows * 64 * NT;
+  // tiles in bands of 8 rows, column by column: an XCD's consecutive tiles share rows and
+  // columns (1000 x 4096 x 4096 1.6 us less than down all rows)
+  const int split = at % splits, tile = at / splits, band = tile / (8 * cols), in = tile % (8 * cols);
+  const int high = min(8, rows - 8 * band), m0 = (8 * band + in % high) * BM, n0 = in / high * 64 * NT;
   const int tid = int(threadIdx.x), lane = tid & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 2, wn = wave & 3;
   const int all = (g.K + 127) / 128, s0 = int(int64_t(all) * split / splits), s1 = int(int64_t(all) * (split + 1) / splits);
@@ -443,36 +447,49 @@ hipError_t launch_part(const Launch &L, const Q8Args<T> &g) {
     return hipGetLastError();
   }
   const int steps = (g.K + 127) / 128, exact = (steps + kExact / 128 - 1) / (kExact / 128);
-  auto many = [&](auto mt, auto nt) {
-    constexpr int MT = decltype(mt)::value, NT = decltype(nt)::value;
-    const int rows = (g.M + 32 * MT - 1) / (32 * MT), cols = (g.N + 64 * NT - 1) / (64 * NT);
-    const size_t tiles = size_t(rows) * size_t(cols);
-    // K is split where the tiles leave CUs without work, into no fewer than four steps
-    const int fill = int(std::min<size_t>(size_t(std::max(steps / 4, 1)), std::max<size_t>(size_t(L.num_cu) / tiles, 1)));
-    const int splits = std::max(exact, fill);
-    if (tiles * size_t(splits) > kMostThreads / 512) return hipErrorInvalidValue;  // more memory than there is
-    if (splits > 1) {
-      const size_t want = (size_t(g.M) * size_t(g.N) + 255) / 256;
-      hipLaunchKernelGGL((k_q8_clear<T>), dim3(unsigned(std::min(want, size_t(L.num_cu) * 8))), dim3(256), 0, L.stream, g);
-      const hipError_t e = hipGetLastError();
-      if (e != hipSuccess) return e;
+  const bool low = NP == 4 && g.M <= 32;  // tiles of 32 words; Z_2^64's always are
+  const int rows = NP == 4 && !low ? (g.M + 63) / 64 : (g.M + 31) / 32;
+  // The width of the tiles and the parts of K for which a launch takes least: its rounds of
+  // one workgroup a CU, each with its start and its steps, and, where K is split, the
+  // output's clearing and the sums' way through memory.  Measured (us, one MI355X): a step
+  // 0.45 + 0.32 nt, a round 8, splitting 3 and 0.6 a MB.  Widths 1, 2, 3, 4 for 4096 x 4096 in
+  // Z_2^32: 640 rows 90, 76, 50, 56; 512 65, 43, 46, 56; 384 60, 39, 45, 56; 64 rows by 4
+  // parts of K 16, 19, 21, 28, by one 31, 37, 44, 53.
+  int nt = 1, splits = exact;
+  float best = 0;
+  for (int w = 1; w <= 4; w++)
+    for (int p = exact; p == exact || (p <= steps / 4 && p <= 64); p *= 2) {
+      const float tiles = float(rows) * float((g.N + 64 * w - 1) / (64 * w)) * float(p);
+      float t = std::ceil(tiles / float(L.num_cu)) * (8.f + float((steps + p - 1) / p) * (0.45f + 0.32f * float(w)));
+      if (p > 1) t += 3.f + 0.6e-6f * float(g.M) * float(g.N) * float(p * NP);
+      if (best == 0 || t < best) best = t, nt = w, splits = p;
     }
-    hipLaunchKernelGGL((k_q8_many<T, MT, NT>), dim3(unsigned(tiles * size_t(splits))), dim3(512), 0, L.stream, g, rows, cols,
-                       splits);
+  const int cols = (g.N + 64 * nt - 1) / (64 * nt);
+  const size_t wgs = size_t(rows) * size_t(cols) * size_t(splits);
+  if (wgs > kMostThreads / 512) return hipErrorInvalidValue;  // more memory than there is
+  if (splits > 1) {
+    const size_t want = (size_t(g.M) * size_t(g.N) + 255) / 256;
+    hipLaunchKernelGGL((k_q8_clear<T>), dim3(unsigned(std::min(want, size_t(L.num_cu) * 8))), dim3(256), 0, L.stream, g);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  auto many = [&](auto w) {
+    constexpr int NT = decltype(w)::value;
+    const dim3 grid{unsigned(wgs)};
+    if constexpr (NP == 4)
+      if (!low) {
+        hipLaunchKernelGGL((k_q8_many<T, 2, NT>), grid, dim3(512), 0, L.stream, g, rows, cols, splits);
+        return hipGetLastError();
+      }
+    hipLaunchKernelGGL((k_q8_many<T, 1, NT>), grid, dim3(512), 0, L.stream, g, rows, cols, splits);
     return hipGetLastError();
   };
-  auto wide = [&](auto mt) {
-    constexpr int MT = decltype(mt)::value;
-    const size_t rows = size_t(g.M + 32 * MT - 1) / (32 * MT), cu = size_t(L.num_cu);
-    auto tiles = [&](int nt) { return rows * (size_t(g.N) + 64 * nt - 1) / (64 * nt); };
-    if (tiles(4) >= cu) return many(mt, std::integral_constant<int, 4>{});
-    if (tiles(3) >= cu) return many(mt, std::integral_constant<int, 3>{});
-    if (tiles(2) >= cu) return many(mt, std::integral_constant<int, 2>{});
-    return many(mt, std::integral_constant<int, 1>{});
-  };
-  if constexpr (NP == 4)
-    if (g.M > 32) return wide(std::integral_constant<int, 2>{});
-  return wide(std::integral_constant<int, 1>{});
+  switch (nt) {
+    case 1: return many(std::integral_constant<int, 1>{});
+    case 2: return many(std::integral_constant<int, 2>{});
+    case 3: return many(std::integral_constant<int, 3>{});
+    default: return many(std::integral_constant<int, 4>{});
+  }
 }
 
 }  // namespace
