@@ -93,7 +93,7 @@ __device__ __forceinline__ T plane_word(int32_t sum, int p) {
 }
 
 // bytes of a row of weights that may be read: whole 16
-__device__ __forceinline__ int q8_row(int K) { return (K + 15) & ~15; }
+__host__ __device__ __forceinline__ int q8_row(int K) { return (K + 15) & ~15; }
 
 template <typename T>
 __device__ __forceinline__ T scaled(const Q8Args<T> &g, T v, int m, int n) {
@@ -102,55 +102,92 @@ __device__ __forceinline__ T scaled(const Q8Args<T> &g, T v, int m, int n) {
   return v;
 }
 
+// Which of a column's 8 groups of 16 weights of a 128-k step lies where in LDS, for the
+// reads' banks: column col of a tile of 16.
+__device__ __forceinline__ int q8_turn(int col) {
+  return (col >> 1 & 1) << 2 | (0x78 >> (col >> 2 << 1) & 3);
+}
+
 // ---------------------------------------------------------------------------
-// Few rows: a workgroup takes 16 columns, its (up to 16) waves the 128-k steps of K in turn
-// and add up their sums through LDS; each lane forms its digits from the words.  PACKED
-// (rows <= 16 / planes): the MFMA's 16 rows are all planes of those words.  Else its rows
-// are the words and each plane has an MFMA of its own, whose operands a lane forms together.
+// Few rows, R at most: a workgroup takes 16 columns, its waves the 128-k steps of K in
+// turn, each by itself: D steps ahead it asks for the weights and words of a step, straight
+// into its own part of LDS (in lines of memory; to the lanes' registers, 16 rows of them, they
+// would take four times the cache's accesses), reads its operands back and forms the
+// digits in its lanes.  The waves' sums are added up through LDS.
+// Packed (R <= 16 / planes): the MFMA's 16 rows are all planes of the words.  Else they are
+// the words, and each plane has an MFMA of its own, whose operands a lane forms together.
+// Places: a read of 16 bytes serves lanes 0-3, 12-15, 20-27 together, then 4-11, 16-19,
+// 28-31; a row's groups of 16 bytes are turned so that those fall into different banks.
 // ---------------------------------------------------------------------------
-template <typename T, bool PACKED>
-__global__ __launch_bounds__(1024) void k_q8_few(Q8Args<T> g) {
-  constexpr int NP = int(sizeof(T)), NA = PACKED ? 1 : NP;
-  __shared__ T red[16][PACKED ? 1 : 4][64];
+template <typename T, int R>
+struct Few {
+  static constexpr int NP = int(sizeof(T));
+  static constexpr bool PACKED = R <= 16 / NP;
+  static constexpr int ROW = 128 * NP;  // bytes of a row's step
+  static __device__ __forceinline__ int turn(int r) {
+    if constexpr (PACKED) return (NP == 4 ? 0x78 >> (2 * r) & 3 : r) << 2;
+    else if constexpr (NP == 4) return (R == 8 ? r >> 2 << 1 : 0x78 >> (r >> 2 << 1) & 3) << 2 | (r & 3);
+    else return (r >> (R == 8 ? 2 : 3)) << 2 | (r & 3);
+  }
+};
+template <typename T, int R, int WAVES, int D>
+__global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
+  using F = Few<T, R>;
+  constexpr int NP = F::NP, ROW = F::ROW, NA = F::PACKED ? 1 : NP, NR = F::PACKED ? 1 : 4;
+  constexpr int NW = 2, NB = R * ROW / 1024, STEP = (NW + NB) * 1024;  // loads of 1 KB, bytes
+  __shared__ __align__(16) uint8_t lds[WAVES * D * STEP];
+  static_assert(sizeof lds >= WAVES * NR * 64 * sizeof(T), "the sums' place");
   const int tid = int(threadIdx.x), lane = tid & 63, waves = int(blockDim.x) >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int li = lane & 15, lg = lane >> 4;
-  const int n = int(blockIdx.x) * 16 + li;
-  const int8_t *q = g.q + size_t(min(n, g.N - 1)) * g.ldq;
-  const int m = PACKED ? li / NP : li;
-  const T *a = g.a + size_t(min(m, g.M - 1)) * g.lda;
-  const int steps = (g.K + 127) / 128, end = q8_row(g.K) - 16;
-  T out[PACKED ? 1 : 4] = {};
-  for (int s0 = wave; s0 < steps; s0 += kExact / 128 * waves) {
-    v4i_t acc[NA] = {};
-    const int s1 = min(steps, s0 + kExact / 128 * waves);
-#pragma unroll 2
-    for (int s = s0; s < s1; s += waves) {
-      v4i_t b[2];
+  const int li = lane & 15, lg = lane >> 4, n0 = int(blockIdx.x) * 16;
+  uint8_t *own = lds + wave * D * STEP;
+  const int steps = (g.K + 127) / 128, whole = g.K / 128, end = q8_row(g.K) - 16, mine = (steps - wave + waves - 1) / waves;
+
+  // what this lane asks for: 16 bytes of column 8 i + lane / 8, of row lane / 32 + 2 i (one
+  // row a load in Z_2^64)
+  const int nq = min(g.N - n0, 16);
+  const __amdgpu_buffer_rsrc_t qr = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<int8_t *>(g.q + size_t(n0) * g.ldq), short(0), int(uint32_t(nq - 1) * uint32_t(g.ldq) + uint32_t(end + 16)),
+      kRsrcWord3);
+  const __amdgpu_buffer_rsrc_t ar = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<T *>(g.a), short(0), int((uint32_t(g.M - 1) * uint32_t(g.lda) + uint32_t(g.K)) * uint32_t(NP)), kRsrcWord3);
+  uint32_t qo[NW], qk[NW], ao[NB], ak[NB];
 #pragma unroll
-      for (int o = 0; o < 2; o++)  // past the end of a row they meet words' zeros
-        b[o] = *reinterpret_cast<const v4i_t *>(q + min(128 * s + 64 * o + 16 * lg, end));
+  for (int i = 0; i < NW; i++) {
+    const int col = 8 * i + lane / 8;
+    qo[i] = uint32_t(min(col, nq - 1)) * uint32_t(g.ldq);
+    qk[i] = uint32_t(16 * ((lane % 8) ^ q8_turn(col)));
+  }
 #pragma unroll
-      for (int o = 0; o < 2; o++) {
-        v4i_t d[NA];
+  for (int i = 0; i < NB; i++) {
+    const int at = 64 * i + lane, r = at * 16 / ROW, group = at % (ROW / 16);
+    ao[i] = uint32_t(min(r, g.M - 1)) * uint32_t(g.lda) * uint32_t(NP);
+    ak[i] = uint32_t(16 * (group ^ F::turn(r)));
+  }
+  const uint32_t last = uint32_t(max(g.K - 16 / NP, 0)) * uint32_t(NP);  // a row's last 16 bytes
+  auto ask = [&](int i) __attribute__((always_inline)) {
+    const int s = wave + i * waves;
+    uint8_t *to = own + i % D * STEP;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          T w[4];
-          load4<T>(a, 128 * s + 64 * o + 16 * lg + 4 * i, g.K, w);
-          if constexpr (PACKED) {
-            d[0][i] = int(plane4<T>(w, li % NP));
-          } else {
-            uint32_t p[NP];
-            planes4<T>(w, p);
+    for (int j = 0; j < NW; j++)  // past the end of a row they meet words' zeros
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(qr, (__attribute__((address_space(3))) void *)(to + 1024 * j), 16,
+                                               int(qo[j] + min(128 * s + qk[j], uint32_t(end))), 0, 0, 0);
 #pragma unroll
-            for (int j = 0; j < NP; j++) d[j][i] = int(p[j]);
-          }
-        }
+    for (int j = 0; j < NB; j++)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ar, (__attribute__((address_space(3))) void *)(to + 1024 * (NW + j)), 16,
+                                               int(ao[j] + min(uint32_t(ROW * s) + ak[j], last)), 0, 0, 0);
+  };
+  // where this lane's operands lie: weights of column li, words of row `row`
+  const int row = F::PACKED ? li / NP : li % R;
+  uint32_t fromw[2];
 #pragma unroll
-        for (int j = 0; j < NA; j++) acc[j] = mfma64(d[j], b[o], acc[j]);
-      }
-    }
-    if constexpr (PACKED) {  // four planes of one word; Z_2^64: the upper four where lg is odd
+  for (int o = 0; o < 2; o++) fromw[o] = uint32_t(li * 128 + ((4 * o + lg) ^ q8_turn(li)) * 16);
+  const T *arow = g.a + size_t(min(row, g.M - 1)) * g.lda;
+
+  T out[NR] = {};
+  v4i_t acc[NA] = {};
+  auto fold = [&]() __attribute__((always_inline)) {
+    if constexpr (F::PACKED) {  // four planes of one word; Z_2^64: the upper four where lg is odd
 #pragma unroll
       for (int r = 0; r < 4; r++) out[0] += plane_word<T>(acc[0][r], r);
     } else {
@@ -159,20 +196,79 @@ __global__ __launch_bounds__(1024) void k_q8_few(Q8Args<T> g) {
 #pragma unroll
         for (int j = 0; j < NP; j++) out[r] += plane_word<T>(acc[j][r], j);
     }
-  }
 #pragma unroll
-  for (int r = 0; r < (PACKED ? 1 : 4); r++) red[wave][r][lane] = out[r];
+    for (int j = 0; j < NA; j++) acc[j] = v4i_t{};
+  };
+  auto wait = [&](auto groups) __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(decltype(groups)::value * (NW + NB)) : "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < D; i++)
+    if (i < mine) ask(i);
+  for (int i = 0; i < mine; i++) {
+    // this step's loads have landed; those of the D - 1 that follow, where there are such, may not
+    if (i + D <= mine) wait(std::integral_constant<int, D - 1>{});
+    else if (D == 3 && i + 2 == mine) wait(std::integral_constant<int, 1>{});
+    else wait(std::integral_constant<int, 0>{});
+    const int s = wave + i * waves;
+    const uint8_t *buf = own + i % D * STEP;
+#pragma unroll
+    for (int o = 0; o < 2; o++) {
+      const v4i_t b = *reinterpret_cast<const v4i_t *>(buf + fromw[o]);
+      T w[16];
+      if (s < whole) {
+#pragma unroll
+        for (int j = 0; j < NP; j++) {
+          const uint4 x = *reinterpret_cast<const uint4 *>(
+              buf + NW * 1024 + row * ROW + (((4 * o + lg) * NP + j) ^ F::turn(row)) * 16);
+          __builtin_memcpy(&w[j * 16 / NP], &x, 16);
+        }
+      } else {  // past K, word by word
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          T v[4];
+          load4<T>(arow, 128 * s + 64 * o + 16 * lg + 4 * j, g.K, v);
+          __builtin_memcpy(&w[4 * j], v, sizeof v);
+        }
+      }
+      v4i_t d[NA];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const T v[4] = {w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]};
+        if constexpr (F::PACKED) {
+          d[0][j] = int(plane4<T>(v, li % NP));
+        } else {
+          uint32_t p[NP];
+          planes4<T>(v, p);
+#pragma unroll
+          for (int k = 0; k < NP; k++) d[k][j] = int(p[k]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < NA; k++) acc[k] = mfma64(d[k], b, acc[k]);
+    }
+    if (i + D < mine) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this step's operands have been read
+      ask(i + D);
+    }
+    if (i % (kExact / 128) == kExact / 128 - 1) fold();
+  }
+  fold();
   __syncthreads();
-  constexpr int R = PACKED ? 16 / NP : 16;  // words of the tile
+  T *red = reinterpret_cast<T *>(lds);  // wave, register, lane
+#pragma unroll
+  for (int r = 0; r < NR; r++) red[(wave * NR + r) * 64 + lane] = out[r];
+  __syncthreads();
   for (int e = tid; e < R * 16; e += int(blockDim.x)) {
-    const int r = e / 16, col = e % 16, on = int(blockIdx.x) * 16 + col;
+    const int r = e / 16, c = e % 16, n = n0 + c;
     T v = 0;
     for (int w = 0; w < waves; w++) {
-      if constexpr (!PACKED) v += red[w][r % 4][16 * (r / 4) + col];
-      else if constexpr (NP == 4) v += red[w][0][16 * r + col];
-      else v += red[w][0][32 * r + col] + (red[w][0][32 * r + 16 + col] << 32);
+      const T *x = red + w * NR * 64;
+      if constexpr (!F::PACKED) v += x[r % 4 * 64 + 16 * (r / 4) + c];
+      else if constexpr (NP == 4) v += x[16 * r + c];
+      else v += x[32 * r + c] + (x[32 * r + 16 + c] << 32);
     }
-    if (r < g.M && on < g.N) g.c[size_t(r) * g.ldc + on] = scaled<T>(g, v, r, on);
+    if (r < g.M && n < g.N) g.c[size_t(r) * g.ldc + n] = scaled<T>(g, v, r, n);
   }
 }
 
@@ -190,9 +286,6 @@ __global__ __launch_bounds__(1024) void k_q8_few(Q8Args<T> g) {
 // K may be split over workgroups, which then add to a cleared output: sums modulo 2^bw do
 // not depend on their order.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ int q8_turn(int col) {  // of column col of a tile of 16
-  return (col >> 1 & 1) << 2 | (0x78 >> (col >> 2 << 1) & 3);
-}
 template <typename T, int MT, int NT>
 __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, int rows, int cols, int splits) {
   constexpr int NP = int(sizeof(T)), TILES = 2 * MT, BM = 16 * TILES, QUADS = BM * 32 / 512;
@@ -436,16 +529,48 @@ __global__ __launch_bounds__(256) void k_q8_clear(Q8Args<T> g) {
     g.c[i / g.N * g.ldc + i % g.N] = 0;
 }
 
+// Rounds of one workgroup a CU times the steps of a wave: what a launch of k_q8_few that
+// forms its digits plane by plane takes, some 1.2 us each in Z_2^32 and 1.7 in Z_2^64.
+template <typename T>
+size_t few_steps(const Launch &L, const Q8Args<T> &g) {
+  const size_t waves = sizeof(T) == 4 || g.M <= 8 ? 8 : 4;
+  return ((size_t(g.N) + 15) / 16 + size_t(L.num_cu) - 1) / size_t(L.num_cu) * ((size_t(g.K) + 127) / 128 + waves - 1) / waves;
+}
+template <typename T>
+hipError_t launch_few(const Launch &L, const Q8Args<T> &g) {
+  constexpr int NP = int(sizeof(T)), PACKED = 16 / NP;
+  const int steps = (g.K + 127) / 128;
+  auto few = [&](auto rows, auto most, auto depth) {
+    constexpr int WAVES = decltype(most)::value;
+    hipLaunchKernelGGL((k_q8_few<T, decltype(rows)::value, WAVES, decltype(depth)::value>), dim3(unsigned((g.N + 15) / 16)),
+                       dim3(64u * unsigned(std::min(steps, WAVES))), 0, L.stream, g);
+    return hipGetLastError();
+  };
+  std::integral_constant<int, 2> two;
+  std::integral_constant<int, 3> three;
+  std::integral_constant<int, 4> four;
+  std::integral_constant<int, 8> eight;
+  std::integral_constant<int, 16> sixteen;
+  if (g.M <= PACKED) {
+    // eight waves where they have a step each: two workgroups fit a CU
+    std::integral_constant<int, PACKED> packed;
+    return steps <= 8 ? few(packed, eight, two) : few(packed, sixteen, two);
+  }
+  if (g.M <= 8) {
+    if constexpr (NP == 4) return few(eight, eight, three);
+    else return few(eight, eight, two);
+  }
+  if constexpr (NP == 4) return few(sixteen, eight, two);
+  else return few(sixteen, four, two);
+}
+
 template <typename T>
 hipError_t launch_part(const Launch &L, const Q8Args<T> &g) {
   constexpr int NP = int(sizeof(T));
-  if (g.M <= 16) {
-    const int steps = (g.K + 127) / 128, waves = std::min(steps, 16);
-    const dim3 grid(unsigned((g.N + 15) / 16)), block(64u * unsigned(waves));
-    if (g.M <= 16 / NP) hipLaunchKernelGGL((k_q8_few<T, true>), grid, block, 0, L.stream, g);
-    else hipLaunchKernelGGL((k_q8_few<T, false>), grid, block, 0, L.stream, g);
-    return hipGetLastError();
-  }
+  // 4096 x 4096, few and many (us): Z_2^32 1 row 4.9 and 8.1, 8 rows 7.6 and 10.4, 16 rows 9.2
+  // and 10.9; Z_2^64 1 row 5.6 and 10.1, 8 rows 10.9 and 11.5, 16 rows 16.3 and 13.1.  8192 x
+  // 8192: 1 row 15.4 and 16.7, 8 rows 22.0 and 20.9; Z_2^64 8 rows 31.2 and 22.1.
+  if (g.M <= 16 / NP || (g.M <= 16 && few_steps(L, g) <= (NP == 4 ? 8 : 4))) return launch_few<T>(L, g);
   const int steps = (g.K + 127) / 128, exact = (steps + kExact / 128 - 1) / (kExact / 128);
   const bool low = NP == 4 && g.M <= 32;  // tiles of 32 words; Z_2^64's always are
   const int rows = NP == 4 && !low ? (g.M + 63) / 64 : (g.M + 31) / 32;
@@ -492,22 +617,38 @@ hipError_t launch_part(const Launch &L, const Q8Args<T> &g) {
   }
 }
 
+// rows m.. and columns n.. of a product
+template <typename T>
+Q8Args<T> part(const Q8Args<T> &g, int64_t m, int rows, int64_t n, int cols) {
+  Q8Args<T> p = g;
+  p.M = int(std::min<int64_t>(g.M - m, rows));
+  p.N = int(std::min<int64_t>(g.N - n, cols));
+  p.a += size_t(m) * g.lda;
+  p.q += size_t(n) * g.ldq;
+  if (p.scale) p.scale += n;
+  if (p.tok) p.tok += m;
+  p.c += size_t(m) * g.ldc + size_t(n);
+  return p;
+}
+
 }  // namespace
 
 template <typename T>
 hipError_t launch_gemm_q8(const Launch &L, const Q8Args<T> &g) {
   if (g.K > kQ8MaxK) return hipErrorInvalidValue;
-  // rows that lie gigabytes apart: by the kernel of few rows, whose places are 64 bits wide
-  if (g.M > 16 && (g.lda >= size_t(1) << 25 || g.ldq >= size_t(1) << 23)) {
-    for (int64_t m = 0; m < g.M; m += 16) {
-      Q8Args<T> p = g;
-      p.M = int(std::min<int64_t>(g.M - m, 16));
-      p.a += size_t(m) * g.lda;
-      if (p.tok) p.tok += m;
-      p.c += size_t(m) * g.ldc;
-      const hipError_t e = launch_gemm_q8<T>(L, p);
-      if (e != hipSuccess) return e;
-    }
+  // Rows' places are 32 bits from what a workgroup shares: rows that lie further apart are
+  // taken one by one, weights in columns of their own.
+  const bool far_a = g.lda >= size_t(1) << 24, far_q = g.ldq >= size_t(1) << 23;
+  if ((far_a && g.M > 1) || (far_q && g.N > 1)) {
+    const int rows = far_a ? 1 : g.M, cols = far_q ? 1 : g.N;
+    for (int64_t m = 0; m < g.M; m += rows)
+      for (int64_t n = 0; n < g.N; n += cols) {
+        Q8Args<T> p = part(g, m, rows, n, cols);
+        p.lda = p.M == 1 ? size_t(p.K) : p.lda;
+        p.ldq = p.N == 1 ? size_t(q8_row(p.K)) : p.ldq;
+        const hipError_t e = launch_gemm_q8<T>(L, p);
+        if (e != hipSuccess) return e;
+      }
     return hipSuccess;
   }
   // HIP cuts a launch of 2^32 threads along a dimension short: in parts of at most 2^16
@@ -516,15 +657,7 @@ hipError_t launch_gemm_q8(const Launch &L, const Q8Args<T> &g) {
   constexpr int rows = 1 << 16, cols = 1 << 14;
   for (int64_t m = 0; m < g.M; m += rows)
     for (int64_t n = 0; n < g.N; n += cols) {
-      Q8Args<T> p = g;
-      p.M = int(std::min<int64_t>(g.M - m, rows));
-      p.N = int(std::min<int64_t>(g.N - n, cols));
-      p.a += size_t(m) * g.lda;
-      p.q += size_t(n) * g.ldq;
-      if (p.scale) p.scale += n;
-      if (p.tok) p.tok += m;
-      p.c += size_t(m) * g.ldc + size_t(n);
-      const hipError_t e = launch_part<T>(L, p);
+      const hipError_t e = launch_part<T>(L, part(g, m, rows, n, cols));
       if (e != hipSuccess) return e;
     }
   return hipSuccess;
