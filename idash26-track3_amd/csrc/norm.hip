@@ -11,6 +11,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attn.h"
 #include "launch_util.h"
@@ -18,26 +19,74 @@
 namespace mpcx {
 namespace {
 
-// A wave a row.
-template <NormForm F, typename T>
-__global__ __launch_bounds__(256) void k_norm_sums(NormSumsArgs<T> g) {
-  const size_t waves = size_t(gridDim.x) * 4;
-  const int lane = int(threadIdx.x) & 63;
-  for (size_t t = size_t(blockIdx.x) * 4 + (threadIdx.x >> 6); t < g.rows; t += waves) {
+// 16 bytes of words; rows start at any word, so the loads are not assumed aligned to more.
+template <typename T>
+struct Words {
+  static constexpr int N = 16 / int(sizeof(T));
+  T w[N];
+  __device__ __forceinline__ void load(const T *p) { __builtin_memcpy(w, p, 16); }
+  __device__ __forceinline__ void store(T *p) const { __builtin_memcpy(p, w, 16); }
+};
+
+// ---------------------------------------------------------------------------
+// W waves a row (W a power of two; a workgroup is 4 waves or W).  The bytes are all there is
+// to it: four words in (two without a residual) and one out for one multiplication.
+// ---------------------------------------------------------------------------
+template <NormForm F, typename T, int W, bool RES>
+__global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_norm_sums(NormSumsArgs<T> g) {
+  constexpr int GROUP = W > 4 ? W : 4, ROWS = GROUP / W, N = Words<T>::N;
+  __shared__ T part[GROUP];
+  const int wave = int(threadIdx.x) >> 6, at = int(threadIdx.x) % (64 * W);
+  for (size_t t0 = size_t(blockIdx.x) * ROWS; t0 < g.rows; t0 += size_t(gridDim.x) * ROWS) {
+    const size_t t = t0 + wave / W;
     T sum = 0;
-    for (size_t j = lane; j < g.dim; j += 64) {
-      T h = g.x[t * g.ldx + j];
-      if (g.d) h += g.d[t * g.ldd + j];
-      const size_t i = t * g.dim + j;
-      if constexpr (F == NormForm::BOTH) sum += h * (h - T(2) * (g.a0[i] + g.a1[i]));
-      if constexpr (F == NormForm::P0) sum += h * (h - T(2) * g.a0[i]);
-      if constexpr (F == NormForm::P1) sum -= T(2) * h * g.a1[i];
-      if constexpr (F == NormForm::DEAL) sum += h * h, g.copy[i] = h;
-      if (g.h) g.h[t * g.ldh + j] = h;
+    if (t < g.rows) {
+      const T *x = g.x + t * g.ldx, *d = RES ? g.d + t * g.ldd : nullptr;
+      const T *a0 = g.a0 + t * g.dim, *a1 = g.a1 + t * g.dim;
+      T *h = RES ? g.h + t * g.ldh : nullptr, *copy = F == NormForm::DEAL ? g.copy + t * g.dim : nullptr;
+      auto word = [&](T v, T b0, T b1) __attribute__((always_inline)) {
+        if constexpr (F == NormForm::BOTH) return v * (v - T(2) * (b0 + b1));
+        if constexpr (F == NormForm::P0) return v * (v - T(2) * b0);
+        if constexpr (F == NormForm::P1) return T(0) - T(2) * v * b1;
+        return v * v;
+      };
+      constexpr bool A0 = F == NormForm::BOTH || F == NormForm::P0, A1 = F == NormForm::BOTH || F == NormForm::P1;
+      size_t j = size_t(at) * N;
+#pragma unroll 2
+      for (; j + N <= g.dim; j += 64 * W * N) {
+        Words<T> v, r, b0, b1;
+        v.load(x + j);
+        if constexpr (RES) r.load(d + j);
+        if constexpr (A0) b0.load(a0 + j);
+        if constexpr (A1) b1.load(a1 + j);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+          if constexpr (RES) v.w[i] += r.w[i];
+          sum += word(v.w[i], A0 ? b0.w[i] : T(0), A1 ? b1.w[i] : T(0));
+        }
+        if constexpr (RES) v.store(h + j);
+        if constexpr (F == NormForm::DEAL) v.store(copy + j);
+      }
+      for (; j < g.dim; j++) {  // one lane's, fewer than N
+        T v = x[j];
+        if constexpr (RES) v += d[j];
+        sum += word(v, A0 ? a0[j] : T(0), A1 ? a1[j] : T(0));
+        if constexpr (RES) h[j] = v;
+        if constexpr (F == NormForm::DEAL) copy[j] = v;
+      }
     }
 #pragma unroll
     for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if (lane == 0) {
+    if constexpr (W > 1) {
+      if (threadIdx.x % 64 == 0) part[wave] = sum;
+      __syncthreads();
+      sum = 0;
+      if (at == 0)
+#pragma unroll
+        for (int w = 0; w < W; w++) sum += part[wave + w];
+      __syncthreads();
+    }
+    if (at == 0 && t < g.rows) {
       if constexpr (F != NormForm::P1) sum += g.c0[t];
       if constexpr (F == NormForm::BOTH || F == NormForm::P1) sum += g.c1[t];
       g.s[t] = sum;
@@ -68,16 +117,35 @@ __global__ __launch_bounds__(256) void k_norm_scale(NormScaleArgs<T> g) {
 
 }  // namespace
 
+namespace {
+template <NormForm F, typename T, bool RES>
+hipError_t sums_form(const Launch &L, const NormSumsArgs<T> &g) {
+  auto waves = [&](auto w) {
+    constexpr int W = decltype(w)::value, ROWS = W > 4 ? 1 : 4 / W;
+    const size_t want = (g.rows + ROWS - 1) / ROWS, cap = size_t(L.num_cu) * 16;
+    hipLaunchKernelGGL((k_norm_sums<F, T, W, RES>), dim3(unsigned(std::min(want, cap))), dim3(64 * std::max(W, 4)), 0,
+                       L.stream, g);
+    return hipGetLastError();
+  };
+  const size_t turns = (g.dim * sizeof(T) + 1023) / 1024;  // of a wave, to pass a row
+  if (turns > 8 && g.rows < size_t(L.num_cu) * 2) return waves(std::integral_constant<int, 16>{});
+  if (turns > 2) return waves(std::integral_constant<int, 4>{});
+  return waves(std::integral_constant<int, 1>{});
+}
+}  // namespace
+
 template <typename T>
 hipError_t launch_norm_sums(const Launch &L, NormForm form, const NormSumsArgs<T> &g) {
-  const dim3 grid(unsigned(std::min<size_t>((g.rows + 3) / 4, size_t(L.num_cu) * 8)));
-  switch (form) {
-    case NormForm::BOTH: hipLaunchKernelGGL((k_norm_sums<NormForm::BOTH, T>), grid, dim3(256), 0, L.stream, g); break;
-    case NormForm::P0: hipLaunchKernelGGL((k_norm_sums<NormForm::P0, T>), grid, dim3(256), 0, L.stream, g); break;
-    case NormForm::P1: hipLaunchKernelGGL((k_norm_sums<NormForm::P1, T>), grid, dim3(256), 0, L.stream, g); break;
-    case NormForm::DEAL: hipLaunchKernelGGL((k_norm_sums<NormForm::DEAL, T>), grid, dim3(256), 0, L.stream, g); break;
-  }
-  return hipGetLastError();
+  auto with = [&](auto res) {
+    constexpr bool RES = decltype(res)::value;
+    switch (form) {
+      case NormForm::BOTH: return sums_form<NormForm::BOTH, T, RES>(L, g);
+      case NormForm::P0: return sums_form<NormForm::P0, T, RES>(L, g);
+      case NormForm::P1: return sums_form<NormForm::P1, T, RES>(L, g);
+      default: return sums_form<NormForm::DEAL, T, RES>(L, g);
+    }
+  };
+  return g.d ? with(std::true_type{}) : with(std::false_type{});
 }
 template <typename T>
 hipError_t launch_norm_scale(const Launch &L, NormForm form, const NormScaleArgs<T> &g) {

@@ -552,9 +552,10 @@ hipError_t launch_few(const Launch &L, const Q8Args<T> &g) {
   std::integral_constant<int, 8> eight;
   std::integral_constant<int, 16> sixteen;
   if (g.M <= PACKED) {
-    // eight waves where they have a step each: two workgroups fit a CU
+    // Eight waves, so that two workgroups fit a CU, where they have a step each or there are
+    // columns for it: 4096 x 32000 31.7 us and by sixteen 36.2, 8192 x 8192 14.3 and 15.5.
     std::integral_constant<int, PACKED> packed;
-    return steps <= 8 ? few(packed, eight, two) : few(packed, sixteen, two);
+    return steps <= 8 || g.N > 16 * L.num_cu ? few(packed, eight, two) : few(packed, sixteen, two);
   }
   if (g.M <= 8) {
     if constexpr (NP == 4) return few(eight, eight, three);
@@ -569,7 +570,7 @@ hipError_t launch_part(const Launch &L, const Q8Args<T> &g) {
   constexpr int NP = int(sizeof(T));
   // 4096 x 4096, few and many (us): Z_2^32 1 row 4.9 and 8.1, 8 rows 7.6 and 10.4, 16 rows 9.2
   // and 10.9; Z_2^64 1 row 5.6 and 10.1, 8 rows 10.9 and 11.5, 16 rows 16.3 and 13.1.  8192 x
-  // 8192: 1 row 15.4 and 16.7, 8 rows 22.0 and 20.9; Z_2^64 8 rows 31.2 and 22.1.
+  // 8192: 1 row 14.3 and 16.7, 8 rows 22.0 and 20.9; Z_2^64 8 rows 31.2 and 22.1.
   if (g.M <= 16 / NP || (g.M <= 16 && few_steps(L, g) <= (NP == 4 ? 8 : 4))) return launch_few<T>(L, g);
   const int steps = (g.K + 127) / 128, exact = (steps + kExact / 128 - 1) / (kExact / 128);
   const bool low = NP == 4 && g.M <= 32;  // tiles of 32 words; Z_2^64's always are
