@@ -94,24 +94,47 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_norm_sums(NormSumsArgs
   }
 }
 
-template <NormForm F, typename T>
-__global__ __launch_bounds__(256) void k_norm_scale(NormScaleArgs<T> g) {
-  const size_t n = g.rows * g.dim;
-  for (size_t i = size_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += size_t(gridDim.x) * 256) {
-    const size_t t = i / g.dim, j = i % g.dim;
-    const T v = g.v[t];
-    T z = 0;
-    if constexpr (F != NormForm::DEAL) {
-      const T h = g.h[t * g.ldh + j];
-      if constexpr (F != NormForm::P1) z += (h - g.a0[i]) * (v - g.b0[t]);
-      if constexpr (F != NormForm::P0) z -= h * g.b1[t] + g.a1[i] * v;
+// ---------------------------------------------------------------------------
+// A workgroup takes 256 groups of 16 bytes of a row at a time.  Bound by its bytes, too:
+// five words in and one out.
+// ---------------------------------------------------------------------------
+template <NormForm F, typename T, bool GAIN>
+__global__ __launch_bounds__(256) void k_norm_scale(NormScaleArgs<T> g, uint32_t chunks) {
+  constexpr int N = Words<T>::N;
+  constexpr bool P0 = F != NormForm::P1, P1 = F == NormForm::BOTH || F == NormForm::P1, DEAL = F == NormForm::DEAL;
+  const size_t units = g.rows * chunks;
+  for (size_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const size_t t = u / chunks, j = (u % chunks * 256 + threadIdx.x) * N, i = t * g.dim + j;
+    if (j >= g.dim) continue;
+    const T v = g.v[t], b0 = P0 ? g.b0[t] : T(0), b1 = P1 ? g.b1[t] : T(0);
+    const T *h = DEAL ? nullptr : g.h + t * g.ldh;
+    T *y = g.y + t * g.ldy;
+    auto word = [&](T x, T a0, T a1, T c0, T c1, T gain) __attribute__((always_inline)) {
+      T z = 0;
+      if constexpr (DEAL) {
+        z = (a0 + a1) * v - a0 * b0;
+      } else {
+        if constexpr (P0) z += (x - a0) * (v - b0);
+        if constexpr (P1) z -= x * b1 + a1 * v;
+      }
+      if constexpr (GAIN) z *= gain;
+      return z + c0 + c1;
+    };
+    if (j + N <= g.dim) {
+      Words<T> x = {}, a0 = {}, a1 = {}, c0 = {}, c1 = {}, gain = {};
+      if constexpr (!DEAL) x.load(h + j);
+      if constexpr (P0) a0.load(g.a0 + i), c0.load(g.c0 + i);
+      if constexpr (P1 || DEAL) a1.load(g.a1 + i);
+      if constexpr (P1) c1.load(g.c1 + i);
+      if constexpr (GAIN) gain.load(g.gain + j);
+#pragma unroll
+      for (int k = 0; k < N; k++) x.w[k] = word(x.w[k], a0.w[k], a1.w[k], c0.w[k], c1.w[k], gain.w[k]);
+      x.store(y + j);
     } else {
-      z = (g.a0[i] + g.a1[i]) * v - g.a0[i] * g.b0[t];
+      for (size_t k = 0; j + k < g.dim; k++)
+        y[j + k] = word(DEAL ? T(0) : h[j + k], P0 ? g.a0[i + k] : T(0), P1 || DEAL ? g.a1[i + k] : T(0),
+                        P0 ? g.c0[i + k] : T(0), P1 ? g.c1[i + k] : T(0), GAIN ? g.gain[j + k] : T(0));
     }
-    if (g.gain) z *= g.gain[j];
-    if constexpr (F != NormForm::P1) z += g.c0[i];
-    if constexpr (F == NormForm::BOTH || F == NormForm::P1) z += g.c1[i];
-    g.y[t * g.ldy + j] = z;
   }
 }
 
@@ -149,14 +172,22 @@ hipError_t launch_norm_sums(const Launch &L, NormForm form, const NormSumsArgs<T
 }
 template <typename T>
 hipError_t launch_norm_scale(const Launch &L, NormForm form, const NormScaleArgs<T> &g) {
-  const dim3 grid(unsigned(std::min<size_t>((g.rows * g.dim + 255) / 256, size_t(L.num_cu) * 8)));
-  switch (form) {
-    case NormForm::BOTH: hipLaunchKernelGGL((k_norm_scale<NormForm::BOTH, T>), grid, dim3(256), 0, L.stream, g); break;
-    case NormForm::P0: hipLaunchKernelGGL((k_norm_scale<NormForm::P0, T>), grid, dim3(256), 0, L.stream, g); break;
-    case NormForm::P1: hipLaunchKernelGGL((k_norm_scale<NormForm::P1, T>), grid, dim3(256), 0, L.stream, g); break;
-    case NormForm::DEAL: hipLaunchKernelGGL((k_norm_scale<NormForm::DEAL, T>), grid, dim3(256), 0, L.stream, g); break;
-  }
-  return hipGetLastError();
+  const uint32_t chunks = uint32_t((g.dim * sizeof(T) + 4095) / 4096);
+  const dim3 grid(unsigned(std::min<size_t>(g.rows * chunks, size_t(L.num_cu) * 64)));
+  auto with = [&](auto gain) {
+    constexpr bool GAIN = decltype(gain)::value;
+    auto launch = [&](auto f) {
+      hipLaunchKernelGGL((k_norm_scale<decltype(f)::value, T, GAIN>), grid, dim3(256), 0, L.stream, g, chunks);
+      return hipGetLastError();
+    };
+    switch (form) {
+      case NormForm::BOTH: return launch(std::integral_constant<NormForm, NormForm::BOTH>{});
+      case NormForm::P0: return launch(std::integral_constant<NormForm, NormForm::P0>{});
+      case NormForm::P1: return launch(std::integral_constant<NormForm, NormForm::P1>{});
+      default: return launch(std::integral_constant<NormForm, NormForm::DEAL>{});
+    }
+  };
+  return g.gain ? with(std::true_type{}) : with(std::false_type{});
 }
 template hipError_t launch_norm_sums<uint32_t>(const Launch &, NormForm, const NormSumsArgs<uint32_t> &);
 template hipError_t launch_norm_sums<uint64_t>(const Launch &, NormForm, const NormSumsArgs<uint64_t> &);
