@@ -847,29 +847,36 @@ class Ctx:
         self._leave(same)
         return out
 
-    def _norm_rows(self, what, t, shape=None):
-        p, ld = self._rows(t, what)
-        if t.shape[1] >> 31 or (shape is not None and t.shape != shape):
-            raise MpcxError(f"{what}: shape {tuple(t.shape)}" + (f", need {tuple(shape)}" if shape is not None else ""))
-        return p, ld
+    def _norm_shape(self, what, t):
+        if t.dim() != 2 or t.shape[1] >> 31:  # a row past a C int
+            raise MpcxError(f"{what}: need rows of words, not {tuple(t.shape)}")
+        return t.shape
+
+    def _norm_rows(self, what, t, shape):
+        """The address and row stride of ring words of this shape; rows may be apart."""
+        st = t.stride()
+        if t.dtype is not self._word or t.shape != shape or t.get_device() != self._device or \
+                (st[1] != 1 and shape[1] > 1 and shape[0] > 0):
+            raise MpcxError(f"{what}: need int{self.bw} rows of shape {tuple(shape)} on GPU {self._device}")
+        return t.data_ptr(), st[0] if shape[0] > 1 else shape[1]
 
     def _norm_sums(self, what, x, d, out):
-        """The rows of a call: x's, d's and the sum's addresses and strides; the sum."""
-        xp, ldx = self._norm_rows(what, x)
+        """The shape of a call, the sum, and x's, d's and the sum's addresses and strides."""
+        shape = self._norm_shape(what, x)
         if d is None:
             if out is not None:
                 raise MpcxError(f"{what}: a sum without a residual")
-            return x, (xp, ldx, None, 0, None, 0)
+            return shape, x, (*self._norm_rows(what, x, shape), None, 0, None, 0)
         if out is None:
-            out = self._new(x.shape)
-        return out, (xp, ldx) + self._norm_rows(what, d, x.shape) + self._norm_rows(what, out, x.shape)
+            out = self._new(shape)
+        return shape, out, (*self._norm_rows(what, x, shape), *self._norm_rows(what, d, shape),
+                            *self._norm_rows(what, out, shape))
 
     def norm_sums_keygen(self, rx, rd=None, seed=1, gate=1):
         """Keys of norm_sums_eval from the masks of x and of the residual (rows, dim):
         the parties' keys, the mask of h (rx itself without a residual) and the sums'."""
         what = "norm_sums_keygen"
-        rh, args = self._norm_sums(what, rx, rd, None)
-        rows, dim = rx.shape
+        (rows, dim), rh, args = self._norm_sums(what, rx, rd, None)
         nb = self.lib.mpcx_norm_sums_key_bytes(self.h, rows, dim)
         k0, k1, rs = empty_dev(nb, self._device), empty_dev(nb, self._device), self._new((rows,))
         same = self._enter()
@@ -888,8 +895,7 @@ class Ctx:
         return self._norm_sums_eval("norm_sums_message", party, (key,), xhat, dhat, out)
 
     def _norm_sums_eval(self, what, party, keys, x, d, out):
-        h, args = self._norm_sums(what, x, d, out)
-        rows, dim = x.shape
+        (rows, dim), h, args = self._norm_sums(what, x, d, out)
         nb = self.lib.mpcx_norm_sums_key_bytes(self.h, rows, dim)
         keys = [self._key(k, nb, what) for k in keys]
         s = self._new((rows,))
@@ -931,11 +937,11 @@ class Ctx:
         return self._norm_scale_eval("norm_scale_message", party, (key,), (a,), hhat, vhat, gain, out)
 
     def _norm_scale_eval(self, what, party, keys, shares, h, v, gain, out):
-        hp, ldh = self._norm_rows(what, h)
-        rows, dim = h.shape
+        rows, dim = shape = self._norm_shape(what, h)
         if out is None:
-            out = self._new((rows, dim))
-        yp, ldy = self._norm_rows(what, out, h.shape)
+            out = self._new(shape)
+        hp, ldh = self._norm_rows(what, h, shape)
+        yp, ldy = self._norm_rows(what, out, shape)
         nb, plane = self.lib.mpcx_norm_scale_key_bytes(self.h, rows, dim), rows * dim * self.bw // 8
         ptrs = [self._key(k, nb, what) for k in keys] + [self._key(a, plane, what) for a in shares]
         vp = self._words(v, what, (rows,))
