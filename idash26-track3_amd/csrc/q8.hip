@@ -652,10 +652,10 @@ hipError_t launch_gemm_q8(const Launch &L, const Q8Args<T> &g) {
       }
     return hipSuccess;
   }
-  // HIP cuts a launch of 2^32 threads along a dimension short: in parts of at most 2^16
-  // rows by 2^14 columns, 2^11 by 2^8 tiles of 512 threads, and K in up to 2^8 parts, the
-  // grid stays below that
-  constexpr int rows = 1 << 16, cols = 1 << 14;
+  // HIP cuts a launch of 2^32 threads along a dimension short: in parts of at most 2^14
+  // rows by 2^18 columns, 2^9 by 2^12 tiles of 512 threads, of fewer columns where K is
+  // split in 2^16s, the grid stays below that.
+  const int rows = 1 << 14, cols = std::max(64, (1 << 18) / ((g.K + kExact - 1) / kExact));
   for (int64_t m = 0; m < g.M; m += rows)
     for (int64_t n = 0; n < g.N; n += cols) {
       const hipError_t e = launch_part<T>(L, part(g, m, rows, n, cols));

@@ -100,6 +100,67 @@ def test_q8_rows_apart(ctx, M):
     assert (got[:, :3] == 17).all() and (got[:, 3 + N:] == 17).all()
 
 
+def q8_wide(a, w):
+    """q8_plain without scales, by float64 products of 16-bit limbs: below 2^53, so exact."""
+    wide = w.T.astype(np.float64)
+    with np.errstate(over="ignore"):
+        return sum((np.matmul((a >> a.dtype.type(16 * i) & a.dtype.type(0xFFFF)).astype(np.float64), wide).astype(np.int64)
+                    .astype(np.uint64) << np.uint64(16 * i) for i in range(a.itemsize // 2)), np.uint64(0)).astype(a.dtype)
+
+
+# rows and columns for which a tile is 32 or 64 rows by 1, 2, 3, 4 times 64 columns; K one
+# step, a few, a whole number of them, and past the last
+@pytest.mark.parametrize("M,N", [(256, 4096), (384, 4096), (640, 4096), (1000, 4096), (20, 20000), (20, 40000),
+                                 (20, 60000), (70, 20001)])
+@pytest.mark.parametrize("K", [16, 127, 128, 130, 384, 500, 640, 769])
+def test_q8_tiles(ctx, M, K, N):
+    rng = np.random.default_rng(M + K)
+    a, w = words(rng, (M, K), ctx.bw), rng.integers(-128, 128, (N, K)).astype(np.int8)
+    assert np.array_equal(host(ctx.ring_gemm_q8(dev(a), q8_rows(w)), ctx.bw), q8_wide(a, w))
+
+
+# K in parts: their sums added up in memory
+@pytest.mark.parametrize("M,K,N", [(20, 8191, 300), (33, 4096, 100), (100, 4097, 500), (17, 20000, 20), (64, 1100, 64)])
+def test_q8_parts_of_k(ctx, M, K, N):
+    torch = _torch()
+    rng = np.random.default_rng(K)
+    a, w, scale = words(rng, (M, K), ctx.bw), rng.integers(-128, 128, (N, K)).astype(np.int8), steps(rng, N)
+    to = torch.full((M, N + 5), 41, dtype=torch.int32 if ctx.bw == 32 else torch.int64, device="cuda")
+    for _ in range(2):  # the output is not added to
+        ctx.ring_gemm_q8(dev(a), q8_rows(w), dev(scale), out=to[:, 2:2 + N])
+        got = host(to, ctx.bw)
+        with np.errstate(over="ignore"):
+            assert np.array_equal(got[:, 2:2 + N], q8_wide(a, w) * scale.astype(np.int64).astype(ctx.T))
+        assert (got[:, :2] == 41).all() and (got[:, 2 + N:] == 41).all()
+
+
+def test_q8_long_sums_of_a_token(ctx):
+    """One token, a K past what a wave sums in 32 bits."""
+    K, N = (1 << 21) + 5, 3
+    w = np.full((N, K), -128, np.int8)
+    w[1, 7::2] = 127
+    a = np.full((1, K), 0x8080808080808080, np.uint64).astype(ctx.T)
+    got = host(ctx.ring_gemm_q8(dev(a), q8_rows(w)), ctx.bw)
+    with np.errstate(over="ignore"):
+        assert np.array_equal(got[0], w.sum(1, dtype=np.int64).astype(np.uint64).astype(ctx.T) * a[0, 0])
+
+
+@pytest.mark.parametrize("M", [1, 2, 5, 20])
+def test_q8_rows_far_apart(ctx, M):
+    """Rows and weights further apart than a workgroup's 32-bit places reach."""
+    torch = _torch()
+    rng = np.random.default_rng(M)
+    K, N, ld, ldq = 40, 3, 1 << 24, 1 << 23
+    a, w = words(rng, (M, K), ctx.bw), rng.integers(-128, 128, (N, K)).astype(np.int8)
+    big = torch.empty(((M - 1) * ld + K,), dtype=torch.int32 if ctx.bw == 32 else torch.int64, device="cuda")
+    wide = torch.empty(((N - 1) * ldq + 48,), dtype=torch.int8, device="cuda")
+    x, q = big.as_strided((M, K), (ld, 1)), wide.as_strided((N, K), (ldq, 1))
+    x.copy_(dev(a))
+    q.copy_(q8_rows(w)[:, :K])
+    torch.cuda.synchronize()
+    assert np.array_equal(host(ctx.ring_gemm_q8(x, q), ctx.bw), q8_plain(a, w))
+
+
 def test_q8_padding_tokens(ctx):
     """A token scale of zero clears its row, the others stay."""
     rng = np.random.default_rng(8)
