@@ -28,17 +28,27 @@ __device__ __forceinline__ v4i_t mfma64(v4i_t a, v4i_t b, v4i_t c) {
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
 }
 
-// Four words of a row from k on, zero from K on; rows start at any word, so the loads of
-// 16 bytes are not assumed aligned to more than a word.
+// Four words of a row from k on, zero from K on: the row's last four, moved down.  Without a
+// branch a lane: at a join the compiler waits for the loads before it, group after group.
 template <typename T>
-__device__ __forceinline__ void load4(const T *row, int k, int K, T (&w)[4]) {
-  if (k + 4 <= K) {
-    __builtin_memcpy(w, row + k, sizeof w);
-  } else {
+struct Four {
+  T w[4];
+  __device__ __forceinline__ void load(const T *row, int k, int K) {
+    if (K >= 4) {
+      __builtin_memcpy(w, row + min(k, K - 4), sizeof w);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; i++) w[i] = k + i < K ? row[k + i] : T(0);
+      for (int i = 0; i < 4; i++) w[i] = row[min(i, K - 1)];
+    }
   }
-}
+  __device__ __forceinline__ void cut(int k, int K) {
+    const int down = K >= 4 ? max(k - (K - 4), 0) : 0, have = K - k;
+    if (down & 1) w[0] = w[1], w[1] = w[2], w[2] = w[3];
+    if (down & 2) w[0] = w[2], w[1] = w[3];
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = i < have ? w[i] : T(0);
+  }
+};
 // Bytes 0..3 of four 32-bit words, each byte's four side by side: with the words offset by
 // 0x80 a byte, the digits.
 __device__ __forceinline__ void bytes4(const uint32_t (&y)[4], uint32_t *d) {
@@ -223,12 +233,14 @@ __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
               buf + NW * 1024 + row * ROW + (((4 * o + lg) * NP + j) ^ F::turn(row)) * 16);
           __builtin_memcpy(&w[j * 16 / NP], &x, 16);
         }
-      } else {  // past K, word by word
+      } else {  // past K: what is there, once more
+        Four<T> v[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j].load(arow, 128 * s + 64 * o + 16 * lg + 4 * j, g.K);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          T v[4];
-          load4<T>(arow, 128 * s + 64 * o + 16 * lg + 4 * j, g.K, v);
-          __builtin_memcpy(&w[4 * j], v, sizeof v);
+          v[j].cut(128 * s + 64 * o + 16 * lg + 4 * j, g.K);
+          __builtin_memcpy(&w[4 * j], v[j].w, sizeof v[j].w);
         }
       }
       v4i_t d[NA];
@@ -335,14 +347,20 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
 
   v4i_t acc[MT][NP][NT] = {};
   struct Words {
-    T w[QUADS][4];
+    Four<T> w[QUADS];
   };
+  const int whole = min(s1, g.K / 128);  // steps up to here are within K
   auto load_words = [&](int s, Words &x, int i) __attribute__((always_inline)) {  // of a step within K
-    __builtin_memcpy(x.w[i], a[i] + 128 * s + ao[i], sizeof x.w[i]);
+    __builtin_memcpy(x.w[i].w, a[i] + 128 * s + ao[i], sizeof x.w[i].w);
   };
-  auto load_last = [&](int s, Words &x) __attribute__((always_inline)) {
+  auto load_last = [&](int s, Words &x) __attribute__((always_inline)) {  // to be cut
 #pragma unroll
-    for (int i = 0; i < QUADS; i++) load4<T>(a[i] + (ao[i] - 4 * kq), 128 * s + 4 * kq, g.K, x.w[i]);
+    for (int i = 0; i < QUADS; i++) x.w[i].load(a[i] + (ao[i] - 4 * kq), 128 * s + 4 * kq, g.K);
+  };
+  auto cut = [&](int s, Words &x) __attribute__((always_inline)) {
+    if (s < whole) return;
+#pragma unroll
+    for (int i = 0; i < QUADS; i++) x.w[i].cut(128 * s + 4 * kq, g.K);
   };
   auto load_weights = [&](int s, int buf, auto within) __attribute__((always_inline)) {
 #pragma unroll
@@ -356,7 +374,7 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
   };
   auto put = [&](int buf, const Words &x, int i) __attribute__((always_inline)) {
     uint32_t d[NP];
-    planes4<T>(x.w[i], d);
+    planes4<T>(x.w[i].w, d);
 #pragma unroll
     for (int p = 0; p < NP; p++) *reinterpret_cast<uint32_t *>(lds + to + (buf * WORDS + p * PLANE + i * 2048)) = d[p];
   };
@@ -381,9 +399,9 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
 #pragma unroll
       for (int k = 0; k < 4; k++) {
         if constexpr (NP == 4) {
-          v.y[k] = x.w[i][k] + 0x80808080u;
+          v.y[k] = x.w[i].w[k] + 0x80808080u;
         } else {
-          const uint64_t u = x.w[i][k] + 0x8080808080808080ull;
+          const uint64_t u = x.w[i].w[k] + 0x8080808080808080ull;
           v.y[k] = uint32_t(u), v.z[k] = uint32_t(u >> 32);
         }
       }
@@ -431,8 +449,7 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
   constexpr std::false_type no{};
   // Words and weights are asked for two steps ahead: words have a step to come and are then
   // turned, weights have two.  Steps within K have no branch between a load and its use (at a
-  // join the compiler waits for all of them); a last step past K is loaded word by word.
-  const int whole = min(s1, g.K / 128);
+  // join the compiler waits for all of them); a last step past K has its words cut.
   Words x, y;
   auto any_words = [&](int s, Words &v) __attribute__((always_inline)) {
     if (s < whole) {
@@ -452,6 +469,7 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
     Words first;
     any_words(s0, first);
     any_words(s0 + 1, x);
+    cut(s0, first);
     put_all(0, first);
   }
   barrier(none);
@@ -465,7 +483,7 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
 #pragma unroll
     for (int i = 0; i < QUADS; i++)  // here, so that their use does not wait for the loads that leave next
 #pragma unroll
-      for (int k = 0; k < 4; k++) asm volatile("" : "+v"(cur.w[i][k]));
+      for (int k = 0; k < 4; k++) asm volatile("" : "+v"(cur.w[i].w[k]));
 #pragma unroll
     for (int i = 0; i < QUADS; i++) load_words(s + 2, ahead, i);
     load_weights(s + 2, wnext, yes);
@@ -484,6 +502,7 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
     if (s + 2 < s1) load_weights(s + 2, wnext, no);
     compute(buf, wb, x, no);
     if (s + 1 < s1) {
+      cut(s + 1, x);
       put_all(buf ^ 1, x);
       any_words(s + 2, x);
       barrier(none);
