@@ -405,15 +405,14 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
           v.y[k] = uint32_t(u), v.z[k] = uint32_t(u >> 32);
         }
       }
-    } else if (stage % 4 == 1 || stage == 4) {
+    } else if (stage % 4 == 1) {
       const uint32_t(&y)[4] = stage & 4 ? v.z : v.y;
-      if (stage == 4) return;
 #pragma unroll
       for (int k = 0; k < 2; k++) {
         v.l[k] = __builtin_amdgcn_perm(y[2 * k + 1], y[2 * k], 0x05010400u);
         v.h[k] = __builtin_amdgcn_perm(y[2 * k + 1], y[2 * k], 0x07030602u);
       }
-    } else {
+    } else if (stage != 4) {
       const uint32_t(&u)[2] = stage & 1 ? v.h : v.l;
       p += (stage & 1) * 2 * PLANE;
       *reinterpret_cast<uint32_t *>(p) = __builtin_amdgcn_perm(u[1], u[0], 0x05040100u) ^ 0x80808080u;
@@ -465,6 +464,13 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
   };
   load_weights(s0, 0, no);
   if (s0 + 1 < s1) load_weights(s0 + 1, 1, no);
+  int32_t sn[NT], sm[MT][4];
+#pragma unroll
+  for (int t = 0; t < NT; t++) sn[t] = g.scale ? g.scale[min(n0 + (wn * NT + t) * 16 + li, g.N - 1)] : 1;
+#pragma unroll
+  for (int i = 0; i < MT; i++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) sm[i][r] = g.tok ? g.tok[min(m0 + (wm * MT + i) * 16 + 4 * lg + r, g.M - 1)] : 1;
   {
     Words first;
     any_words(s0, first);
@@ -472,6 +478,12 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
     cut(s0, first);
     put_all(0, first);
   }
+#pragma unroll
+  for (int t = 0; t < NT; t++) asm volatile("" : "+v"(sn[t]));  // here, not where they are used
+#pragma unroll
+  for (int i = 0; i < MT; i++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) asm volatile("" : "+v"(sm[i][r]));
   barrier(none);
   int s = s0, wb = 0, wnext = 2;  // buffers of this step's weights and of those asked for next
   auto turn_buffers = [&]() {
@@ -509,13 +521,6 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
     }
   }
 
-  int32_t sn[NT], sm[MT][4];
-#pragma unroll
-  for (int t = 0; t < NT; t++) sn[t] = g.scale ? g.scale[min(n0 + (wn * NT + t) * 16 + li, g.N - 1)] : 1;
-#pragma unroll
-  for (int i = 0; i < MT; i++)
-#pragma unroll
-    for (int r = 0; r < 4; r++) sm[i][r] = g.tok ? g.tok[min(m0 + (wm * MT + i) * 16 + 4 * lg + r, g.M - 1)] : 1;
 #pragma unroll
   for (int i = 0; i < MT; i++)
 #pragma unroll
