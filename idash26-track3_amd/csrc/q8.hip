@@ -128,6 +128,9 @@ __device__ __forceinline__ int q8_turn(int col) {
 // the words, and each plane has an MFMA of its own, whose operands a lane forms together.
 // Places: a read of 16 bytes serves lanes 0-3, 12-15, 20-27 together, then 4-11, 16-19,
 // 28-31; a row's groups of 16 bytes are turned so that those fall into different banks.
+// Bound by the weights' bytes and, below some 20 MB, by a launch's start and the waves'
+// first loads: 1 x 4096 x 4096 in Z_2^32 5.4 us (3.1 TB/s), 1 x 4096 x 32000 27.8 (4.7); plane
+// by plane by the digits: 16 x 4096 x 4096 9.4, 6 x 8191 x 2048 in Z_2^64 16 (k_q8_many: 13).
 // ---------------------------------------------------------------------------
 template <typename T, int R>
 struct Few {
@@ -285,11 +288,14 @@ __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
 }
 
 // ---------------------------------------------------------------------------
-// Many rows: a workgroup of 2 x 4 waves takes 32 MT words by 64 NT columns.  A step is 128
-// k, double-buffered in LDS and asked for a step ahead.  The workgroup forms the words'
-// digits once; the weights go straight into LDS (to the lanes' registers they would take
-// four times as long: the 16 rows of an operand are as many places in memory for each
-// group of 16 lanes, where here 8 lanes take a row's 128 bytes).
+// Many rows: a workgroup of 2 x 4 waves takes 32 MT words by 64 NT columns, 128 k a step.
+// It forms the words' digits once, for the next step between the matrix instructions of
+// this one; the weights go straight into LDS (to the lanes' registers they would take four
+// times the cache's accesses: an operand's 16 rows are as many places for 16 lanes, where here
+// 8 lanes take a row's 128 bytes: 94 us, and 73).  1000 x 4096 x 4096 in Z_2^32: 65 to 72 us,
+// 1.9 to 2.1 POP/s of digits (a large int8 library product 2.1), by the card's clock: 62 with words and
+// weights of zeros.  The matrix cores are busy half of the waves' time; 32 steps take 1.8 us
+// each, the start and the output's way to memory 8.
 // Places in LDS, both such that neither the writes' nor the reads' lanes meet in a bank
 // (a read of 16 bytes serves lanes 0-3, 12-15, 20-27 together, then 4-11, 16-19, 28-31):
 //   digits   plane, tile of 16 words, half of the step o: 64 lanes' 16 bytes, word li of
@@ -602,16 +608,17 @@ hipError_t launch_part(const Launch &L, const Q8Args<T> &g) {
   // The width of the tiles and the parts of K for which a launch takes least: its rounds of
   // one workgroup a CU, each with its start and its steps, and, where K is split, the
   // output's clearing and the sums' way through memory.  Measured (us, one MI355X): a step
-  // 0.45 + 0.32 nt, a round 8, splitting 3 and 0.6 a MB.  Widths 1, 2, 3, 4 for 4096 x 4096 in
-  // Z_2^32: 640 rows 90, 76, 50, 56; 512 65, 43, 46, 56; 384 60, 39, 45, 56; 64 rows by 4
-  // parts of K 16, 19, 21, 28, by one 31, 37, 44, 53.
+  // 0.6 + 0.3 nt with all CUs at work, a round 6, splitting 3, 0.1 a part and 0.6 a MB.  4096 x
+  // 4096 in Z_2^32, widths 1, 2, 3, 4: 640 rows 90, 76, 50, 56; 512 65, 43, 46, 56; 384 60, 39,
+  // 45, 56; by two parts of K 256 rows 41, 29, 33, 42, by one 36, 37, 45, 54; by four 64 rows
+  // 15, 17, 21, 28, by one 30, 36, 44, 53.
   int nt = 1, splits = exact;
   float best = 0;
   for (int w = 1; w <= 4; w++)
     for (int p = exact; p == exact || (p <= steps / 4 && p <= 64); p *= 2) {
       const float tiles = float(rows) * float((g.N + 64 * w - 1) / (64 * w)) * float(p);
-      float t = std::ceil(tiles / float(L.num_cu)) * (8.f + float((steps + p - 1) / p) * (0.45f + 0.32f * float(w)));
-      if (p > 1) t += 3.f + 0.6e-6f * float(g.M) * float(g.N) * float(p * NP);
+      float t = std::ceil(tiles / float(L.num_cu)) * (6.f + float((steps + p - 1) / p) * (0.6f + 0.3f * float(w)));
+      if (p > 1) t += 3.f + 0.1f * float(p) + 0.6e-6f * float(g.M) * float(g.N) * float(p * NP);
       if (best == 0 || t < best) best = t, nt = w, splits = p;
     }
   const int cols = (g.N + 64 * nt - 1) / (64 * nt);
