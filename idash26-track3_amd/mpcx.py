@@ -285,6 +285,7 @@ class Ctx:
         self.T = np.uint32 if bw == 32 else np.uint64
         self._word = torch.int32 if bw == 32 else torch.int64
         self._device, self._stream, self._stream_id = device, None, 0
+        self._current = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         h = C.c_void_p()
         st = self.lib.mpcx_create(bw, scale, device, C.byref(h))
         if st != 0:
@@ -615,7 +616,11 @@ class Ctx:
     # stream there, too.  Inputs made on another stream are the caller's to order
     # (Stream.wait_stream).  On any other stream all of them wait for torch's current
     # stream first and for their own work at the end, as the methods above do.
+    _current = None  # torch's current stream of a GPU as a handle, where torch has it (1 us less a call)
+
     def _enter(self):
+        if self._current is not None and self._stream_id != 0 and self._current(self._device) == self._stream_id:
+            return True
         cur = _torch_module.cuda.current_stream(self._device)
         if self._stream_id == cur.cuda_stream != 0:
             return True
