@@ -873,7 +873,7 @@ class Ctx:
                 raise MpcxError(f"{what}: a sum without a residual")
             return shape, x, (*self._norm_rows(what, x, shape), None, 0, None, 0)
         if out is None:
-            out = self._new(shape)
+            out = _torch_module.empty_like(x)
         return shape, out, (*self._norm_rows(what, x, shape), *self._norm_rows(what, d, shape),
                             *self._norm_rows(what, out, shape))
 
@@ -903,7 +903,7 @@ class Ctx:
         (rows, dim), h, args = self._norm_sums(what, x, d, out)
         nb = self.lib.mpcx_norm_sums_key_bytes(self.h, rows, dim)
         keys = [self._key(k, nb, what) for k in keys]
-        s = self._new((rows,))
+        s = x.new_empty(rows)
         same = self._enter()
         if party is None:
             st = self.lib.mpcx_norm_sums_eval(self.h, rows, dim, *keys, *args, s.data_ptr())
@@ -944,7 +944,7 @@ class Ctx:
     def _norm_scale_eval(self, what, party, keys, shares, h, v, gain, out):
         rows, dim = shape = self._norm_shape(what, h)
         if out is None:
-            out = self._new(shape)
+            out = _torch_module.empty_like(h)
         hp, ldh = self._norm_rows(what, h, shape)
         yp, ldy = self._norm_rows(what, out, shape)
         nb, plane = self.lib.mpcx_norm_scale_key_bytes(self.h, rows, dim), rows * dim * self.bw // 8

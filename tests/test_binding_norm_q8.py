@@ -13,8 +13,10 @@ KEY = Tensor((1000,), BYTE)
 
 
 @pytest.fixture
-def c(ctx):  # noqa: F811
+def c(ctx, monkeypatch):  # noqa: F811
     mpcx._torch_module.int8 = INT8
+    mpcx._torch_module.empty_like = lambda t: Tensor(t.shape, t.dtype, t.device_index)
+    monkeypatch.setattr(Tensor, "new_empty", lambda t, n: Tensor((n,), t.dtype, t.device_index), raising=False)
     return ctx
 
 
