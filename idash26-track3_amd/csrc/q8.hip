@@ -130,7 +130,7 @@ __device__ __forceinline__ int q8_turn(int col) {
 // 28-31; a row's groups of 16 bytes are turned so that those fall into different banks.
 // Bound by the weights' bytes and, below some 20 MB, by a launch's start and the waves'
 // first loads: 1 x 4096 x 4096 in Z_2^32 5.4 us (3.1 TB/s), 1 x 4096 x 32000 27.8 (4.7); plane
-// by plane by the digits: 16 x 4096 x 4096 9.4, 6 x 8191 x 2048 in Z_2^64 16 (k_q8_many: 13).
+// by plane by the digits: 16 x 4096 x 4096 9.2 us.
 // ---------------------------------------------------------------------------
 template <typename T, int R>
 struct Few {
@@ -288,7 +288,9 @@ __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
 }
 
 // ---------------------------------------------------------------------------
-// Many rows: a workgroup of 2 x 4 waves takes 32 MT words by 64 NT columns, 128 k a step.
+// Many rows: a workgroup of 2 x 4 waves takes a tile of TILES times 16 words by 64 NT columns,
+// 128 k a step: 64 or 32 words of Z_2^32, 32 or 16 of Z_2^64, whose planes the two rows of waves
+// share where there are but 16.
 // It forms the words' digits once, for the next step between the matrix instructions of
 // this one; the weights go straight into LDS (to the lanes' registers they would take four
 // times the cache's accesses: an operand's 16 rows are as many places for 16 lanes, where here
@@ -304,9 +306,11 @@ __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
 // K may be split over workgroups, which then add to a cleared output: sums modulo 2^bw do
 // not depend on their order.
 // ---------------------------------------------------------------------------
-template <typename T, int MT, int NT>
+template <typename T, int TILES, int NT>
 __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, int rows, int cols, int splits) {
-  constexpr int NP = int(sizeof(T)), TILES = 2 * MT, BM = 16 * TILES, QUADS = BM * 32 / 512;
+  constexpr int NP = int(sizeof(T)), BM = 16 * TILES, QUADS = BM * 32 / 512;
+  constexpr bool SHARED = TILES == 1;                              // a wave has half of the planes
+  constexpr int MT = SHARED ? 1 : TILES / 2, PW = SHARED ? NP / 2 : NP;  // a wave's tiles and planes
   constexpr int PLANE = TILES * 2 * 1024, WORDS = NP * PLANE, WEIGHTS = 64 * NT * 128;  // bytes
   constexpr int WB = 3;  // steps of weights in LDS: in use, there, on their way
   __shared__ __align__(16) uint8_t lds[2 * WORDS + WB * WEIGHTS];
@@ -317,6 +321,7 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
   const int high = min(8, rows - 8 * band), m0 = (8 * band + in % high) * BM, n0 = in / high * 64 * NT;
   const int tid = int(threadIdx.x), lane = tid & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 2, wn = wave & 3;
+  const int wrow = SHARED ? 0 : wm * MT;  // the wave's first tile
   const int all = (g.K + 127) / 128, s0 = int(int64_t(all) * split / splits), s1 = int(int64_t(all) * (split + 1) / splits);
   const int end = q8_row(g.K) - 16;
   // This thread's groups of four words: rows tid / 32 + 16 i, k 4 (tid % 32).  A row's place is
@@ -347,11 +352,11 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
   uint32_t from[2], fromw[2];
 #pragma unroll
   for (int o = 0; o < 2; o++) {
-    from[o] = uint32_t((o * 64 + lg * 16 + (li ^ (2 * (4 * o + lg)))) * 16 + wm * MT * 2048);
+    from[o] = uint32_t((o * 64 + lg * 16 + (li ^ (2 * (4 * o + lg)))) * 16 + wm * (SHARED ? PW * PLANE : MT * 2048));
     fromw[o] = uint32_t(2 * WORDS + wn * NT * 2048 + li * 128 + ((4 * o + lg) ^ q8_turn(li)) * 16);
   }
 
-  v4i_t acc[MT][NP][NT] = {};
+  v4i_t acc[MT][PW][NT] = {};
   struct Words {
     Four<T> w[QUADS];
   };
@@ -393,7 +398,7 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
   // The products of a step, an operand of words read ahead; between them, a few
   // instructions for each operand, the next step's words become digits (more).  The order
   // is held: left free, the compiler reads so far ahead that registers spill.
-  constexpr int F = 2 * NP * MT;           // operands of words
+  constexpr int F = 2 * PW * MT;           // operands of words
   constexpr int STAGES = F / QUADS;        // operands by the time of a group of four words
   static_assert(STAGES == NP, "four planes take four stages");
   struct Turning {
@@ -429,14 +434,14 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
     v4i_t b[NT];
     Turning v;
     auto operand = [&](int f) __attribute__((always_inline)) {
-      return *reinterpret_cast<const v4i_t *>(lds + from[f / (NP * MT)] +
-                                              (buf * WORDS + f / MT % NP * PLANE + f % MT * 2048));
+      return *reinterpret_cast<const v4i_t *>(lds + from[f / (PW * MT)] +
+                                              (buf * WORDS + f / MT % PW * PLANE + f % MT * 2048));
     };
     v4i_t d = operand(0);
 #pragma unroll
     for (int f = 0; f < F; f++) {
-      const int o = f / (NP * MT), p = f / MT % NP, i = f % MT;
-      if (f % (NP * MT) == 0) {
+      const int o = f / (PW * MT), p = f / MT % PW, i = f % MT;
+      if (f % (PW * MT) == 0) {
 #pragma unroll
         for (int t = 0; t < NT; t++)
           b[t] = *reinterpret_cast<const v4i_t *>(lds + (fromw[o] + uint32_t(wbuf * WEIGHTS)) + t * 2048);
@@ -476,7 +481,7 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
 #pragma unroll
   for (int i = 0; i < MT; i++)
 #pragma unroll
-    for (int r = 0; r < 4; r++) sm[i][r] = g.tok ? g.tok[min(m0 + (wm * MT + i) * 16 + 4 * lg + r, g.M - 1)] : 1;
+    for (int r = 0; r < 4; r++) sm[i][r] = g.tok ? g.tok[min(m0 + (wrow + i) * 16 + 4 * lg + r, g.M - 1)] : 1;
   {
     Words first;
     any_words(s0, first);
@@ -527,11 +532,28 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
     }
   }
 
+  uint32_t *upper = reinterpret_cast<uint32_t *>(lds);  // shared planes: a word's upper half
+  if constexpr (SHARED) {
+    barrier(none);  // the last step's operands have been read
+    if (wm == 1) {
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          uint32_t v = 0;
+#pragma unroll
+          for (int p = 0; p < PW; p++) v += uint32_t(acc[0][p][t][r]) << (8 * p);
+          upper[((wn * NT + t) * 4 + r) * 64 + lane] = v;
+        }
+    }
+    barrier(none);
+    if (wm == 1) return;
+  }
 #pragma unroll
   for (int i = 0; i < MT; i++)
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-      const int m = m0 + (wm * MT + i) * 16 + 4 * lg + r;
+      const int m = m0 + (wrow + i) * 16 + 4 * lg + r;
       if (m >= g.M) continue;
       T *c = g.c + size_t(m) * g.ldc;
 #pragma unroll
@@ -539,7 +561,8 @@ __global__ __launch_bounds__(512, NT >= 2 ? 2 : 4) void k_q8_many(Q8Args<T> g, i
         const int n = n0 + (wn * NT + t) * 16 + li;
         T v = 0;
 #pragma unroll
-        for (int p = 0; p < NP; p++) v += plane_word<T>(acc[i][p][t][r], p);
+        for (int p = 0; p < PW; p++) v += plane_word<T>(acc[i][p][t][r], p);
+        if constexpr (SHARED) v += T(upper[((wn * NT + t) * 4 + r) * 64 + lane]) << 32;
         v *= T(int64_t(sn[t])) * T(int64_t(sm[i][r]));
         if (n >= g.N) continue;
         if (splits == 1) {
@@ -596,31 +619,38 @@ hipError_t launch_few(const Launch &L, const Q8Args<T> &g) {
 }
 
 template <typename T>
+constexpr int kLarge = 16 / int(sizeof(T));  // tiles of 16 words of a large tile of k_q8_many
+template <typename T>
 hipError_t launch_part(const Launch &L, const Q8Args<T> &g) {
   constexpr int NP = int(sizeof(T));
-  // 4096 x 4096, few and many (us): Z_2^32 1 row 4.9 and 8.1, 8 rows 7.6 and 10.4, 16 rows 9.2
-  // and 10.9; Z_2^64 1 row 5.6 and 10.1, 8 rows 10.9 and 11.5, 16 rows 16.3 and 13.1.  8192 x
-  // 8192: 1 row 14.3 and 16.7, 8 rows 22.0 and 20.9; Z_2^64 8 rows 31.2 and 22.1.
-  if (g.M <= 16 / NP || (g.M <= 16 && few_steps(L, g) <= (NP == 4 ? 8 : 4))) return launch_few<T>(L, g);
+  // Few and many (us), 4096 x 4096: Z_2^32 1 row 5.1 and 8.0, 8 rows 7.6 and 9.4, 16 rows 9.0 and
+  // 10.0; Z_2^64 1 row 5.9 and 8.2, 8 rows 11.0 and 10.1, 16 rows 16 and 11.  8192 x 2048: 8 rows
+  // 10.9 and 9.8; Z_2^64 2 rows 8.0 and 9.1.  2048 x 2048, 8 rows: 4.5 and 7.0; Z_2^64 6.1 and 7.0.
+  if (g.M <= 16 / NP || (g.M <= 16 && few_steps(L, g) <= (NP == 4 ? 4 : 2))) return launch_few<T>(L, g);
   const int steps = (g.K + 127) / 128, exact = (steps + kExact / 128 - 1) / (kExact / 128);
-  const bool low = NP == 4 && g.M <= 32;  // tiles of 32 words; Z_2^64's always are
-  const int rows = NP == 4 && !low ? (g.M + 63) / 64 : (g.M + 31) / 32;
-  // The width of the tiles and the parts of K for which a launch takes least: its rounds of
-  // one workgroup a CU, each with its start and its steps, and, where K is split, the
-  // output's clearing and the sums' way through memory.  Measured (us, one MI355X): a step
-  // 0.6 + 0.3 nt with all CUs at work, a round 6, splitting 3, 0.1 a part and 0.6 a MB.  4096 x
-  // 4096 in Z_2^32, widths 1, 2, 3, 4: 640 rows 90, 76, 50, 56; 512 65, 43, 46, 56; 384 60, 39,
-  // 45, 56; by two parts of K 256 rows 41, 29, 33, 42, by one 36, 37, 45, 54; by four 64 rows
-  // 15, 17, 21, 28, by one 30, 36, 44, 53.
+  // The tile and the parts of K for which a launch takes least: its rounds of one workgroup a
+  // CU, each with its start and its steps (two workgroups of the smallest tiles fit a CU, and
+  // start together), and, where K is split, the output's clearing and the sums' way through
+  // memory.  Measured (us, one MI355X, all CUs at work): a large tile's step 0.6 + 0.3 nt, its
+  // start 6; a small one's 0.27 + 0.19 nt and 4; splitting 2.5, 0.1 a part and 0.25 a MB.  4096 x 4096 in
+  // Z_2^32 by large and by small tiles of width 1, 2, 3, 4: 1000 rows 124, 81, 93, 63 and 115, 81,
+  // 89, 72; 640 89, 75, 48, 54 and 73, 59, 60, 67; 512 64, 41, 45, 53 and 59, 42, 58, 37; 256 32, 37, 44,
+  // 52 and 31, 24, 29, 33; 64 rows by four parts of K 16, 17, 19, 21 and 14, 13, 14, 15.
   int nt = 1, splits = exact;
+  bool large = false;
   float best = 0;
-  for (int w = 1; w <= 4; w++)
-    for (int p = exact; p == exact || (p <= steps / 4 && p <= 64); p *= 2) {
-      const float tiles = float(rows) * float((g.N + 64 * w - 1) / (64 * w)) * float(p);
-      float t = std::ceil(tiles / float(L.num_cu)) * (6.f + float((steps + p - 1) / p) * (0.6f + 0.3f * float(w)));
-      if (p > 1) t += 3.f + 0.1f * float(p) + 0.6e-6f * float(g.M) * float(g.N) * float(p * NP);
-      if (best == 0 || t < best) best = t, nt = w, splits = p;
-    }
+  for (int big = 0; big < 2; big++)
+    for (int w = big ? 3 : 1; w <= 4; w++)  // narrower large tiles take longer than wider small ones
+      for (int p = exact; p == exact || (p <= steps / 4 && p <= 64); p *= 2) {
+        const int words = big ? kLarge<T> * 16 : kLarge<T> * 8;
+        const float tiles = float((g.M + words - 1) / words) * float((g.N + 64 * w - 1) / (64 * w)) * float(p);
+        const float rounds = std::ceil(tiles / float(L.num_cu)), starts = !big && w <= 2 ? 1.f : rounds;
+        const float step = big ? 0.6f + 0.3f * float(w) : 0.27f + 0.19f * float(w);
+        float t = starts * (big ? 6.f : 4.f) + rounds * float((steps + p - 1) / p) * step;
+        if (p > 1) t += 2.5f + 0.1f * float(p) + 0.25e-6f * float(g.M) * float(g.N) * float(p * NP);
+        if (best == 0 || t < best) best = t, nt = w, splits = p, large = big != 0;
+      }
+  const int words = large ? kLarge<T> * 16 : kLarge<T> * 8, rows = (g.M + words - 1) / words;
   const int cols = (g.N + 64 * nt - 1) / (64 * nt);
   const size_t wgs = size_t(rows) * size_t(cols) * size_t(splits);
   if (wgs > kMostThreads / 512) return hipErrorInvalidValue;  // more memory than there is
@@ -630,22 +660,18 @@ hipError_t launch_part(const Launch &L, const Q8Args<T> &g) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  auto many = [&](auto w) {
-    constexpr int NT = decltype(w)::value;
-    const dim3 grid{unsigned(wgs)};
-    if constexpr (NP == 4)
-      if (!low) {
-        hipLaunchKernelGGL((k_q8_many<T, 2, NT>), grid, dim3(512), 0, L.stream, g, rows, cols, splits);
-        return hipGetLastError();
-      }
-    hipLaunchKernelGGL((k_q8_many<T, 1, NT>), grid, dim3(512), 0, L.stream, g, rows, cols, splits);
+  auto many = [&](auto tiles, auto w) {
+    hipLaunchKernelGGL((k_q8_many<T, decltype(tiles)::value, decltype(w)::value>), dim3(unsigned(wgs)), dim3(512), 0, L.stream, g,
+                       rows, cols, splits);
     return hipGetLastError();
   };
+  constexpr std::integral_constant<int, kLarge<T>> most{};
+  constexpr std::integral_constant<int, kLarge<T> / 2> half{};
   switch (nt) {
-    case 1: return many(std::integral_constant<int, 1>{});
-    case 2: return many(std::integral_constant<int, 2>{});
-    case 3: return many(std::integral_constant<int, 3>{});
-    default: return many(std::integral_constant<int, 4>{});
+    case 1: return many(half, std::integral_constant<int, 1>{});
+    case 2: return many(half, std::integral_constant<int, 2>{});
+    case 3: return large ? many(most, std::integral_constant<int, 3>{}) : many(half, std::integral_constant<int, 3>{});
+    default: return large ? many(most, std::integral_constant<int, 4>{}) : many(half, std::integral_constant<int, 4>{});
   }
 }
 
@@ -683,10 +709,10 @@ hipError_t launch_gemm_q8(const Launch &L, const Q8Args<T> &g) {
       }
     return hipSuccess;
   }
-  // HIP cuts a launch of 2^32 threads along a dimension short: in parts of at most 2^14
+  // HIP cuts a launch of 2^32 threads along a dimension short: in parts of at most 2^13
   // rows by 2^18 columns, 2^9 by 2^12 tiles of 512 threads, of fewer columns where K is
   // split in 2^16s, the grid stays below that.
-  const int rows = 1 << 14, cols = std::max(64, (1 << 18) / ((g.K + kExact - 1) / kExact));
+  const int rows = 1 << 13, cols = std::max(64, (1 << 18) / ((g.K + kExact - 1) / kExact));
   for (int64_t m = 0; m < g.M; m += rows)
     for (int64_t n = 0; n < g.N; n += cols) {
       const hipError_t e = launch_part<T>(L, part(g, m, rows, n, cols));

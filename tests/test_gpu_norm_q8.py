@@ -108,13 +108,35 @@ def q8_wide(a, w):
                     .astype(np.uint64) << np.uint64(16 * i) for i in range(a.itemsize // 2)), np.uint64(0)).astype(a.dtype)
 
 
-# rows and columns for which a tile is 32 or 64 rows by 1, 2, 3, 4 times 64 columns; K one
-# step, a few, a whole number of them, and past the last
-@pytest.mark.parametrize("M,N", [(256, 4096), (384, 4096), (640, 4096), (1000, 4096), (20, 20000), (20, 40000),
-                                 (20, 60000), (70, 20001)])
+# rows and columns for which a small tile is 1, 2, 3, 4 times 64 columns wide and, with some
+# steps of K, a large one 3 or 4 times; K one step, a few, a whole number, and past the last
+@pytest.mark.parametrize("M,N", [(256, 4096), (384, 4096), (640, 4096), (1000, 4096), (320, 4096), (500, 4096), (20, 20000),
+                                 (20, 40000), (20, 60000), (70, 20001), (17, 33000), (33, 33001)])
 @pytest.mark.parametrize("K", [16, 127, 128, 130, 384, 500, 640, 769])
 def test_q8_tiles(ctx, M, K, N):
     rng = np.random.default_rng(M + K)
+    a, w = words(rng, (M, K), ctx.bw), rng.integers(-128, 128, (N, K)).astype(np.int8)
+    assert np.array_equal(host(ctx.ring_gemm_q8(dev(a), q8_rows(w)), ctx.bw), q8_wide(a, w))
+
+
+# more steps, by small and large tiles of each width, some with K in parts, most in one ring only
+@pytest.mark.parametrize("M,K,N", [(1000, 1100, 4096), (640, 2049, 4096), (500, 2049, 4096), (320, 2049, 4096), (70, 4097, 2003),
+                                   (34, 4046, 4406), (130, 8191, 1003), (33, 4082, 3369), (196, 8986, 2317), (1028, 7444, 587),
+                                   (273, 4046, 208), (49, 8659, 4120), (715, 7163, 420), (568, 1969, 72)])
+def test_q8_tiles_of_long_rows(ctx, M, K, N):
+    rng = np.random.default_rng(N)
+    a, w = words(rng, (M, K), ctx.bw), rng.integers(-128, 128, (N, K)).astype(np.int8)
+    scale, tokens = steps(rng, N), steps(rng, M)
+    with np.errstate(over="ignore"):
+        want = q8_wide(a, w) * scale.astype(np.int64).astype(ctx.T) * tokens.astype(np.int64).astype(ctx.T)[:, None]
+    assert np.array_equal(host(ctx.ring_gemm_q8(dev(a), q8_rows(w), dev(scale), dev(tokens)), ctx.bw), want)
+
+
+# a few rows by many columns or a long K, by either kernel
+@pytest.mark.parametrize("M", [2, 3, 5, 8, 9, 16])
+@pytest.mark.parametrize("K,N", [(2048, 500), (4099, 4096), (8191, 2048), (130, 30001), (20001, 100)])
+def test_q8_few_or_many(ctx, M, K, N):
+    rng = np.random.default_rng(M * N)
     a, w = words(rng, (M, K), ctx.bw), rng.integers(-128, 128, (N, K)).astype(np.int8)
     assert np.array_equal(host(ctx.ring_gemm_q8(dev(a), q8_rows(w)), ctx.bw), q8_wide(a, w))
 
