@@ -78,24 +78,6 @@ __device__ __forceinline__ void planes4(const T (&w)[4], uint32_t (&d)[sizeof(T)
     bytes4(z, d + 4);
   }
 }
-// Plane p (a lane's own) of four words.
-template <typename T>
-__device__ __forceinline__ uint32_t plane4(const T (&w)[4], int p) {
-  uint32_t y[4];
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    if constexpr (sizeof(T) == 4) {
-      y[i] = w[i] + 0x80808080u;
-    } else {
-      const uint64_t v = w[i] + 0x8080808080808080ull;
-      y[i] = p & 4 ? uint32_t(v >> 32) : uint32_t(v);
-    }
-  }
-  const uint32_t b = uint32_t(p & 3), sel = b | (b + 4) << 8;
-  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(y[3], y[2], sel), __builtin_amdgcn_perm(y[1], y[0], sel),
-                               0x05040100u) ^
-         0x80808080u;
-}
 // 2^(8p) times a plane's sum
 template <typename T>
 __device__ __forceinline__ T plane_word(int32_t sum, int p) {
@@ -120,51 +102,47 @@ __device__ __forceinline__ int q8_turn(int col) {
 
 // ---------------------------------------------------------------------------
 // Few rows, R at most: a workgroup takes 16 columns, its waves the 128-k steps of K in
-// turn, each by itself: D steps ahead it asks for the weights and words of a step, straight
-// into its own part of LDS (in lines of memory; to the lanes' registers, 16 rows of them, they
-// would take four times the cache's accesses), reads its operands back and forms the
-// digits in its lanes.  The waves' sums are added up through LDS.
-// Packed (R <= 16 / planes): the MFMA's 16 rows are all planes of the words.  Else they are
-// the words, and each plane has an MFMA of its own, whose operands a lane forms together.
+// turn, each by itself: it asks for a step's weights, straight into its own part of LDS (in
+// lines of memory; to the lanes' registers, 16 rows of them, they would take four times the
+// cache's accesses), and words, one or, of few rows, two steps ahead (two of 8 rows in Z_2^64
+// leave room for half as many waves: 4096 x 11008 21.9 us, and 16.9; of one row in Z_2^32 9.6, and 10.3
+// by one).  It forms the words' digits, four words a lane at a time, and turns them by its
+// part of LDS into operands (formed in the lanes that need them, each word by as many
+// lanes as there are planes or parts: 4096 x 11008, one row 12.7 us, and 9.6; 8 rows 18.2, and 11.3).
+// The waves' sums are added up through LDS.
+// The MFMA's 16 rows are the words' by the planes' parts: of 8 words in Z_2^32, say, planes
+// 0 and 1, then 2 and 3, so that a step has 2 R planes / 16 MFMAs.
 // Places: a read of 16 bytes serves lanes 0-3, 12-15, 20-27 together, then 4-11, 16-19,
-// 28-31; a row's groups of 16 bytes are turned so that those fall into different banks.
+// 28-31; groups of 16 bytes are turned so that those fall into different banks.
 // Bound by the weights' bytes and, below some 20 MB, by a launch's start and the waves'
-// first loads: 1 x 4096 x 4096 in Z_2^32 5.4 us (3.1 TB/s), 1 x 4096 x 32000 27.8 (4.7); plane
-// by plane by the digits: 16 x 4096 x 4096 9.2 us.
+// first loads: in Z_2^32 1 x 4096 x 4096 4.1 us, 1 x 4096 x 11008 9.9 (4.6 TB/s), 1 x 8192 x 8192 13.4; with
+// more rows by the digits, which each workgroup forms: 4096 x 4096, 8 rows 5.9, 16 rows 8.0.
 // ---------------------------------------------------------------------------
-template <typename T, int R>
-struct Few {
-  static constexpr int NP = int(sizeof(T));
-  static constexpr bool PACKED = R <= 16 / NP;
-  static constexpr int ROW = 128 * NP;  // bytes of a row's step
-  static __device__ __forceinline__ int turn(int r) {
-    if constexpr (PACKED) return (NP == 4 ? 0x78 >> (2 * r) & 3 : r) << 2;
-    else if constexpr (NP == 4) return (R == 8 ? r >> 2 << 1 : 0x78 >> (r >> 2 << 1) & 3) << 2 | (r & 3);
-    else return (r >> (R == 8 ? 2 : 3)) << 2 | (r & 3);
-  }
-};
-template <typename T, int R, int WAVES, int D>
+template <typename T, int R, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
-  using F = Few<T, R>;
-  constexpr int NP = F::NP, ROW = F::ROW, NA = F::PACKED ? 1 : NP, NR = F::PACKED ? 1 : 4;
-  constexpr int NW = 2, NB = R * ROW / 1024, STEP = (NW + NB) * 1024;  // loads of 1 KB, bytes
-  __shared__ __align__(16) uint8_t lds[WAVES * D * STEP];
+  constexpr int NP = int(sizeof(T)), PARTS = 16 / R < NP ? 16 / R : NP, PW = NP / PARTS;  // planes of a part
+  constexpr int NR = PARTS < 4 ? 4 / PARTS : 1;                // a lane's words of the output
+  constexpr int QUADS = R / 2;                                 // a lane's groups of four words of a step
+  constexpr int NW = 2, NB = QUADS * NP / 4;                   // loads of a step's weights and words
+  constexpr int D = R <= 4 ? 2 : 1;                            // steps asked for ahead
+  constexpr int DIGITS = R * NP * 128, OWN = D * NW * 1024 + DIGITS;  // bytes: of a step's digits, of a wave
+  __shared__ __align__(16) uint8_t lds[WAVES * OWN];
   static_assert(sizeof lds >= WAVES * NR * 64 * sizeof(T), "the sums' place");
   const int tid = int(threadIdx.x), lane = tid & 63, waves = int(blockDim.x) >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int li = lane & 15, lg = lane >> 4, n0 = int(blockIdx.x) * 16;
-  uint8_t *own = lds + wave * D * STEP;
+  uint8_t *own = lds + wave * OWN, *digits = own + D * NW * 1024;
   const int steps = (g.K + 127) / 128, whole = g.K / 128, end = q8_row(g.K) - 16, mine = (steps - wave + waves - 1) / waves;
 
-  // what this lane asks for: 16 bytes of column 8 i + lane / 8, of row lane / 32 + 2 i (one
-  // row a load in Z_2^64)
-  const int nq = min(g.N - n0, 16);
+  // what this lane asks for: 16 weights of columns lane / 8 and 8 + lane / 8, four words of
+  // rows lane / 32 + 2 i
+  const int nq = min(g.N - n0, 16), kq = lane % 32;
   const __amdgpu_buffer_rsrc_t qr = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<int8_t *>(g.q + size_t(n0) * g.ldq), short(0), int(uint32_t(nq - 1) * uint32_t(g.ldq) + uint32_t(end + 16)),
       kRsrcWord3);
   const __amdgpu_buffer_rsrc_t ar = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<T *>(g.a), short(0), int((uint32_t(g.M - 1) * uint32_t(g.lda) + uint32_t(g.K)) * uint32_t(NP)), kRsrcWord3);
-  uint32_t qo[NW], qk[NW], ao[NB], ak[NB];
+  uint32_t qo[NW], qk[NW], ao[QUADS], to[QUADS];
 #pragma unroll
   for (int i = 0; i < NW; i++) {
     const int col = 8 * i + lane / 8;
@@ -172,101 +150,114 @@ __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
     qk[i] = uint32_t(16 * ((lane % 8) ^ q8_turn(col)));
   }
 #pragma unroll
-  for (int i = 0; i < NB; i++) {
-    const int at = 64 * i + lane, r = at * 16 / ROW, group = at % (ROW / 16);
-    ao[i] = uint32_t(min(r, g.M - 1)) * uint32_t(g.lda) * uint32_t(NP);
-    ak[i] = uint32_t(16 * (group ^ F::turn(r)));
+  for (int i = 0; i < QUADS; i++) ao[i] = uint32_t(min(lane / 32 + 2 * i, g.M - 1)) * uint32_t(g.lda) * uint32_t(NP);
+  // Digits: plane, row, 128 bytes; group j of 16 bytes at j ^ (the plane's part + PARTS (row / 2)).
+#pragma unroll
+  for (int i = 0; i < QUADS; i++) to[i] = uint32_t((lane / 32 + 2 * i) * 128 + kq % 4 * 4 + ((kq / 4) ^ (PARTS * i)) * 16);
+  const int row = R * PARTS < 16 ? li / PARTS % R : li / PARTS, part = li % PARTS;
+  uint32_t fromw[2], from[2];
+#pragma unroll
+  for (int o = 0; o < 2; o++) {
+    fromw[o] = uint32_t(li * 128 + ((4 * o + lg) ^ q8_turn(li)) * 16);
+    from[o] = uint32_t((part * PW * R + row) * 128 + ((4 * o + lg) ^ (part + PARTS * (row / 2))) * 16);
   }
-  const uint32_t last = uint32_t(max(g.K - 16 / NP, 0)) * uint32_t(NP);  // a row's last 16 bytes
-  auto ask = [&](int i) __attribute__((always_inline)) {
+
+  struct Words {
+    Four<T> w[QUADS];
+  };
+  auto ask = [&](int i, Words &x) __attribute__((always_inline)) {
     const int s = wave + i * waves;
-    uint8_t *to = own + i % D * STEP;
 #pragma unroll
     for (int j = 0; j < NW; j++)  // past the end of a row they meet words' zeros
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(qr, (__attribute__((address_space(3))) void *)(to + 1024 * j), 16,
-                                               int(qo[j] + min(128 * s + qk[j], uint32_t(end))), 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          qr, (__attribute__((address_space(3))) void *)(own + (i % D * NW + j) * 1024), 16,
+          int(qo[j] + min(128 * s + qk[j], uint32_t(end))), 0, 0, 0);
+    const uint32_t k = uint32_t(min(128 * s + 4 * kq, g.K - 4) * NP);  // past K: the last four, to be cut
 #pragma unroll
-    for (int j = 0; j < NB; j++)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ar, (__attribute__((address_space(3))) void *)(to + 1024 * (NW + j)), 16,
-                                               int(ao[j] + min(uint32_t(ROW * s) + ak[j], last)), 0, 0, 0);
+    for (int j = 0; j < QUADS; j++)
+#pragma unroll
+      for (int h = 0; h < NP / 4; h++) {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b128(ar, int(ao[j] + k + 16 * h), 0, 0);
+        __builtin_memcpy(reinterpret_cast<uint8_t *>(x.w[j].w) + 16 * h, &v, 16);
+      }
+    __builtin_amdgcn_sched_barrier(0);  // here, not where they are used
   };
-  // where this lane's operands lie: weights of column li, words of row `row`
-  const int row = F::PACKED ? li / NP : li % R;
-  uint32_t fromw[2];
-#pragma unroll
-  for (int o = 0; o < 2; o++) fromw[o] = uint32_t(li * 128 + ((4 * o + lg) ^ q8_turn(li)) * 16);
-  const T *arow = g.a + size_t(min(row, g.M - 1)) * g.lda;
 
   T out[NR] = {};
-  v4i_t acc[NA] = {};
+  v4i_t acc[PW] = {};
   auto fold = [&]() __attribute__((always_inline)) {
-    if constexpr (F::PACKED) {  // four planes of one word; Z_2^64: the upper four where lg is odd
+    // a register's row of 4: part j % PARTS of a word; of eight parts, the upper four where lg is odd
 #pragma unroll
-      for (int r = 0; r < 4; r++) out[0] += plane_word<T>(acc[0][r], r);
-    } else {
+    for (int k = 0; k < PW; k++) {
 #pragma unroll
-      for (int r = 0; r < 4; r++)
-#pragma unroll
-        for (int j = 0; j < NP; j++) out[r] += plane_word<T>(acc[j][r], j);
+      for (int j = 0; j < 4; j++) out[j / (4 / NR)] += plane_word<T>(acc[k][j], j % (4 / NR) * PW + k);
+      acc[k] = v4i_t{};
     }
-#pragma unroll
-    for (int j = 0; j < NA; j++) acc[j] = v4i_t{};
   };
-  auto wait = [&](auto groups) __attribute__((always_inline)) {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(decltype(groups)::value * (NW + NB)) : "memory");
-  };
+  // Step i of this wave, in x; `later` of its steps have been asked for since; more: x asks for step i + D.
+  auto step = [&](int i, Words &x, auto later, auto more) __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(decltype(later)::value * (NW + NB)) : "memory");
 #pragma unroll
-  for (int i = 0; i < D; i++)
-    if (i < mine) ask(i);
-  for (int i = 0; i < mine; i++) {
-    // this step's loads have landed; those of the D - 1 that follow, where there are such, may not
-    if (i + D <= mine) wait(std::integral_constant<int, D - 1>{});
-    else if (D == 3 && i + 2 == mine) wait(std::integral_constant<int, 1>{});
-    else wait(std::integral_constant<int, 0>{});
+    for (int j = 0; j < QUADS; j++)  // not read before
+#pragma unroll
+      for (int k = 0; k < 4; k++) asm volatile("" : "+v"(x.w[j].w[k]));
     const int s = wave + i * waves;
-    const uint8_t *buf = own + i % D * STEP;
+    v4i_t b[2];
 #pragma unroll
-    for (int o = 0; o < 2; o++) {
-      const v4i_t b = *reinterpret_cast<const v4i_t *>(buf + fromw[o]);
-      T w[16];
-      if (s < whole) {
+    for (int o = 0; o < 2; o++) b[o] = *reinterpret_cast<const v4i_t *>(own + (fromw[o] + uint32_t(i % D * NW * 1024)));
+    if (s >= whole) {
 #pragma unroll
-        for (int j = 0; j < NP; j++) {
-          const uint4 x = *reinterpret_cast<const uint4 *>(
-              buf + NW * 1024 + row * ROW + (((4 * o + lg) * NP + j) ^ F::turn(row)) * 16);
-          __builtin_memcpy(&w[j * 16 / NP], &x, 16);
-        }
-      } else {  // past K: what is there, once more
-        Four<T> v[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[j].load(arow, 128 * s + 64 * o + 16 * lg + 4 * j, g.K);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          v[j].cut(128 * s + 64 * o + 16 * lg + 4 * j, g.K);
-          __builtin_memcpy(&w[4 * j], v[j].w, sizeof v[j].w);
-        }
-      }
-      v4i_t d[NA];
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const T v[4] = {w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]};
-        if constexpr (F::PACKED) {
-          d[0][j] = int(plane4<T>(v, li % NP));
-        } else {
-          uint32_t p[NP];
-          planes4<T>(v, p);
-#pragma unroll
-          for (int k = 0; k < NP; k++) d[k][j] = int(p[k]);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < NA; k++) acc[k] = mfma64(d[k], b, acc[k]);
+      for (int j = 0; j < QUADS; j++) x.w[j].cut(128 * s + 4 * kq, g.K);
     }
-    if (i + D < mine) {
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this step's operands have been read
-      ask(i + D);
+#pragma unroll
+    for (int j = 0; j < QUADS; j++) {
+      uint32_t d[NP];
+      planes4<T>(x.w[j].w, d);
+#pragma unroll
+      for (int p = 0; p < NP; p++)  // the part turns the groups: lanes' places differ by it in bits 4 to 6
+        *reinterpret_cast<uint32_t *>(digits + ((to[j] ^ uint32_t(p / PW * 16)) + uint32_t(p * R * 128))) = d[p];
+      __builtin_amdgcn_sched_barrier(0);  // left free, the compiler takes more registers than there are
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the weights have been read, the digits are there
+    if constexpr (decltype(more)::value) ask(i + D, x);
+#pragma unroll
+    for (int o = 0; o < 2; o++)
+#pragma unroll
+      for (int k = 0; k < PW; k++)
+        acc[k] = mfma64(*reinterpret_cast<const v4i_t *>(digits + (from[o] + uint32_t(k * R * 128))), b[o], acc[k]);
+    __builtin_amdgcn_sched_barrier(0);  // before the next step's words are waited for
     if (i % (kExact / 128) == kExact / 128 - 1) fold();
+  };
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
+  constexpr std::integral_constant<int, 0> none{};
+  constexpr std::integral_constant<int, 1> one{};
+  if constexpr (D == 1) {
+    Words x;
+    ask(0, x);
+    for (int i = 0; i + 1 < mine; i++) step(i, x, none, yes);
+    step(mine - 1, x, none, no);
+  } else {  // no branch of fewer loads before a load's use: behind it the compiler would wait for all
+    Words x, y;
+    if (mine > 1) {
+      ask(0, x);
+      ask(1, y);
+      int i = 0;
+      for (; i + 3 < mine; i += 2) {
+        step(i, x, one, yes);
+        step(i + 1, y, one, yes);
+      }
+      if (i + 2 < mine) {
+        step(i, x, one, yes);
+        step(i + 1, y, one, no);
+        y = x;
+      } else {
+        step(i, x, one, no);
+      }
+    } else {
+      ask(0, y);
+    }
+    step(mine - 1, y, none, no);
   }
   fold();
   __syncthreads();
@@ -278,10 +269,9 @@ __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
     const int r = e / 16, c = e % 16, n = n0 + c;
     T v = 0;
     for (int w = 0; w < waves; w++) {
-      const T *x = red + w * NR * 64;
-      if constexpr (!F::PACKED) v += x[r % 4 * 64 + 16 * (r / 4) + c];
-      else if constexpr (NP == 4) v += x[16 * r + c];
-      else v += x[32 * r + c] + (x[32 * r + 16 + c] << 32);
+      const T *z = red + w * NR * 64;
+      if constexpr (PARTS <= 4) v += z[r % NR * 64 + 16 * (r / NR) + c];
+      else v += z[32 * r + c] + (z[32 * r + 16 + c] << 32);
     }
     if (r < g.M && n < g.N) g.c[size_t(r) * g.ldc + n] = scaled<T>(g, v, r, n);
   }
@@ -582,40 +572,30 @@ __global__ __launch_bounds__(256) void k_q8_clear(Q8Args<T> g) {
     g.c[i / g.N * g.ldc + i % g.N] = 0;
 }
 
-// Rounds of one workgroup a CU times the steps of a wave: what a launch of k_q8_few that
-// forms its digits plane by plane takes, some 1.2 us each in Z_2^32 and 1.7 in Z_2^64.
+// Rounds of one workgroup a CU times the steps of a wave: of a launch of k_q8_few.
 template <typename T>
 size_t few_steps(const Launch &L, const Q8Args<T> &g) {
-  const size_t waves = sizeof(T) == 4 || g.M <= 8 ? 8 : 4;
-  return ((size_t(g.N) + 15) / 16 + size_t(L.num_cu) - 1) / size_t(L.num_cu) * ((size_t(g.K) + 127) / 128 + waves - 1) / waves;
+  return ((size_t(g.N) + 15) / 16 + size_t(L.num_cu) - 1) / size_t(L.num_cu) * ((size_t(g.K) + 127) / 128 + 7) / 8;
 }
 template <typename T>
 hipError_t launch_few(const Launch &L, const Q8Args<T> &g) {
-  constexpr int NP = int(sizeof(T)), PACKED = 16 / NP;
   const int steps = (g.K + 127) / 128;
-  auto few = [&](auto rows, auto most, auto depth) {
+  auto few = [&](auto rows, auto most) {
     constexpr int WAVES = decltype(most)::value;
-    hipLaunchKernelGGL((k_q8_few<T, decltype(rows)::value, WAVES, decltype(depth)::value>), dim3(unsigned((g.N + 15) / 16)),
+    hipLaunchKernelGGL((k_q8_few<T, decltype(rows)::value, WAVES>), dim3(unsigned((g.N + 15) / 16)),
                        dim3(64u * unsigned(std::min(steps, WAVES))), 0, L.stream, g);
     return hipGetLastError();
   };
-  std::integral_constant<int, 2> two;
-  std::integral_constant<int, 3> three;
-  std::integral_constant<int, 4> four;
-  std::integral_constant<int, 8> eight;
-  std::integral_constant<int, 16> sixteen;
-  if (g.M <= PACKED) {
-    // Eight waves, so that two workgroups fit a CU, where they have a step each or there are
-    // columns for it: 4096 x 32000 31.7 us and by sixteen 36.2, 8192 x 8192 14.3 and 15.5.
-    std::integral_constant<int, PACKED> packed;
-    return steps <= 8 || g.N > 16 * L.num_cu ? few(packed, eight, two) : few(packed, sixteen, two);
-  }
-  if (g.M <= 8) {
-    if constexpr (NP == 4) return few(eight, eight, three);
-    else return few(eight, eight, two);
-  }
-  if constexpr (NP == 4) return few(sixteen, eight, two);
-  else return few(sixteen, four, two);
+  constexpr std::integral_constant<int, 2> two{};
+  constexpr std::integral_constant<int, 4> four{};
+  constexpr std::integral_constant<int, 8> eight{};
+  constexpr std::integral_constant<int, 16> sixteen{};
+  if (g.M > 4) return g.M <= 8 ? few(eight, eight) : few(sixteen, eight);
+  // Sixteen waves where they have a step each and a workgroup has a CU (us, Z_2^32, by eight
+  // and by sixteen): one row of 4096 x 4096 5.5 and 5.1, of 8192 x 2048 5.5 and 5.2; four of 4096 x
+  // 4096 5.9 and 5.5, of 4096 x 11008 9.8 and 12.3, of 1000 x 4099 3.1 and 4.0.
+  if (steps > 8 && g.N <= 16 * L.num_cu) return g.M <= 2 ? few(two, sixteen) : few(four, sixteen);
+  return g.M <= 2 ? few(two, eight) : few(four, eight);
 }
 
 template <typename T>
@@ -623,10 +603,16 @@ constexpr int kLarge = 16 / int(sizeof(T));  // tiles of 16 words of a large til
 template <typename T>
 hipError_t launch_part(const Launch &L, const Q8Args<T> &g) {
   constexpr int NP = int(sizeof(T));
-  // Few and many (us), 4096 x 4096: Z_2^32 1 row 5.1 and 8.0, 8 rows 7.6 and 9.4, 16 rows 9.0 and
-  // 10.0; Z_2^64 1 row 5.9 and 8.2, 8 rows 11.0 and 10.1, 16 rows 16 and 11.  8192 x 2048: 8 rows
-  // 10.9 and 9.8; Z_2^64 2 rows 8.0 and 9.1.  2048 x 2048, 8 rows: 4.5 and 7.0; Z_2^64 6.1 and 7.0.
-  if (g.M <= 16 / NP || (g.M <= 16 && few_steps(L, g) <= (NP == 4 ? 4 : 2))) return launch_few<T>(L, g);
+  // Few rows while a wave's steps times the square of their digits stay small: its time grows with
+  // their product, the other's slowly.  Few and many (us), Z_2^32: 1 row 4096 x 4096 4.0 and 7.8, 4096 x
+  // 32000 22.7 and 24.6; 4 rows 4.7 and 9.1, 22.8 and 25.6; 8 rows (a step of a wave forms 32
+  // digits a column of k) 4096 x 4096 5.9 and 9.4, 8192 x 8192 (16 steps) 15.2 and 17.4, 20000 x 300 (20) 11.5 and
+  // 8.4; 16 rows (64) 4096 x 4096 (4) 8.0 and 9.9, 8192 x 2048 (8) 11.0 and 10.5.  Z_2^64: 1 row 4096 x
+  // 4096 4.6 and 8.0, 4096 x 32000 26.4 and 25.1; 4 rows (32) 8192 x 8192 14.7 and 18.5, 20000 x 300 10.9 and
+  // 8.5; 8 rows (64) 4096 x 4096 8.0 and 10.2, 8192 x 2048 11.0 and 10.5; 16 rows (128) 1024 x 1024 (1) 4.8
+  // and 7.1, 2048 x 2048 (2) 6.6 and 7.5, 1024 x 8192 (2) 8.8 and 7.3.
+  const size_t digits = size_t(NP) * (g.M <= 2 ? 2 : g.M <= 4 ? 4 : g.M <= 8 ? 8 : 16);
+  if (g.M <= 16 && g.K >= 4 && few_steps(L, g) * digits * digits <= 16384) return launch_few<T>(L, g);
   const int steps = (g.K + 127) / 128, exact = (steps + kExact / 128 - 1) / (kExact / 128);
   // The tile and the parts of K for which a launch takes least: its rounds of one workgroup a
   // CU, each with its start and its steps (two workgroups of the smallest tiles fit a CU, and
