@@ -183,17 +183,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
     __builtin_amdgcn_sched_barrier(0);  // here, not where they are used
   };
 
-  T out[NR] = {};
-  v4i_t acc[PW] = {};
-  auto fold = [&]() __attribute__((always_inline)) {
-    // a register's row of 4: part j % PARTS of a word; of eight parts, the upper four where lg is odd
-#pragma unroll
-    for (int k = 0; k < PW; k++) {
-#pragma unroll
-      for (int j = 0; j < 4; j++) out[j / (4 / NR)] += plane_word<T>(acc[k][j], j % (4 / NR) * PW + k);
-      acc[k] = v4i_t{};
-    }
-  };
+  v4i_t acc[PW] = {};  // of at most 256 steps (launch_part), 2^15 terms
   // Step i of this wave, in x; `later` of its steps have been asked for since; more: x asks for step i + D.
   auto step = [&](int i, Words &x, auto later, auto more) __attribute__((always_inline)) {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(decltype(later)::value * (NW + NB)) : "memory");
@@ -226,7 +216,6 @@ __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
       for (int k = 0; k < PW; k++)
         acc[k] = mfma64(*reinterpret_cast<const v4i_t *>(digits + (from[o] + uint32_t(k * R * 128))), b[o], acc[k]);
     __builtin_amdgcn_sched_barrier(0);  // before the next step's words are waited for
-    if (i % (kExact / 128) == kExact / 128 - 1) fold();
   };
   constexpr std::true_type yes{};
   constexpr std::false_type no{};
@@ -259,7 +248,12 @@ __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
     }
     step(mine - 1, y, none, no);
   }
-  fold();
+  // a register's row of 4: part j % PARTS of a word; of eight parts, the upper four where lg is odd
+  T out[NR] = {};
+#pragma unroll
+  for (int k = 0; k < PW; k++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) out[j / (4 / NR)] += plane_word<T>(acc[k][j], j % (4 / NR) * PW + k);
   __syncthreads();
   T *red = reinterpret_cast<T *>(lds);  // wave, register, lane
 #pragma unroll

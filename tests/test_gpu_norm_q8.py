@@ -184,6 +184,22 @@ def test_q8_rows_far_apart(ctx, M):
     assert np.array_equal(host(ctx.ring_gemm_q8(x, q), ctx.bw), q8_plain(a, w))
 
 
+@pytest.mark.parametrize("M", [5, 16, 20, 40])
+def test_q8_rows_as_far_apart_as_a_workgroup_reaches(ctx, M):
+    """Rows and weights one place nearer than that."""
+    torch = _torch()
+    rng = np.random.default_rng(M)
+    K, N, ld, ldq = 140, 20, (1 << 24) - 1, (1 << 23) - 16
+    a, w = words(rng, (M, K), ctx.bw), rng.integers(-128, 128, (N, K)).astype(np.int8)
+    big = torch.empty(((M - 1) * ld + K,), dtype=torch.int32 if ctx.bw == 32 else torch.int64, device="cuda")
+    wide = torch.empty(((N - 1) * ldq + 144,), dtype=torch.int8, device="cuda")
+    x, q = big.as_strided((M, K), (ld, 1)), wide.as_strided((N, K), (ldq, 1))
+    x.copy_(dev(a))
+    q.copy_(q8_rows(w)[:, :K])
+    torch.cuda.synchronize()
+    assert np.array_equal(host(ctx.ring_gemm_q8(x, q), ctx.bw), q8_plain(a, w))
+
+
 def test_q8_padding_tokens(ctx):
     """A token scale of zero clears its row, the others stay."""
     rng = np.random.default_rng(8)
