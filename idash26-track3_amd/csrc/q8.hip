@@ -183,7 +183,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
     __builtin_amdgcn_sched_barrier(0);  // here, not where they are used
   };
 
-  v4i_t acc[PW] = {};  // of at most 256 steps (launch_part), 2^15 terms
+  v4i_t acc[PW] = {};  // of at most 512 steps (launch_part), 2^16 terms
   // Step i of this wave, in x; `later` of its steps have been asked for since; more: x asks for step i + D.
   auto step = [&](int i, Words &x, auto later, auto more) __attribute__((always_inline)) {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(decltype(later)::value * (NW + NB)) : "memory");
@@ -566,11 +566,6 @@ __global__ __launch_bounds__(256) void k_q8_clear(Q8Args<T> g) {
     g.c[i / g.N * g.ldc + i % g.N] = 0;
 }
 
-// Rounds of one workgroup a CU times the steps of a wave: of a launch of k_q8_few.
-template <typename T>
-size_t few_steps(const Launch &L, const Q8Args<T> &g) {
-  return ((size_t(g.N) + 15) / 16 + size_t(L.num_cu) - 1) / size_t(L.num_cu) * ((size_t(g.K) + 127) / 128 + 7) / 8;
-}
 template <typename T>
 hipError_t launch_few(const Launch &L, const Q8Args<T> &g) {
   const int steps = (g.K + 127) / 128;
@@ -597,17 +592,22 @@ constexpr int kLarge = 16 / int(sizeof(T));  // tiles of 16 words of a large til
 template <typename T>
 hipError_t launch_part(const Launch &L, const Q8Args<T> &g) {
   constexpr int NP = int(sizeof(T));
-  // Few rows while a wave's steps times the square of their digits stay small: its time grows with
-  // their product, the other's slowly.  Few and many (us), Z_2^32: 1 row 4096 x 4096 4.0 and 7.8, 4096 x
-  // 32000 22.7 and 24.6; 4 rows 4.7 and 9.1, 22.8 and 25.6; 8 rows (a step of a wave forms 32
-  // digits a column of k) 4096 x 4096 5.9 and 9.4, 8192 x 8192 (16 steps) 15.2 and 17.4, 20000 x 300 (20) 11.5 and
-  // 8.4; 16 rows (64) 4096 x 4096 (4) 8.0 and 9.9, 8192 x 2048 (8) 11.0 and 10.5.  Z_2^64: 1 row 4096 x
-  // 4096 4.6 and 8.0, 4096 x 32000 26.4 and 25.1; 4 rows (32) 8192 x 8192 14.7 and 18.5, 20000 x 300 10.9 and
-  // 8.5; 8 rows (64) 4096 x 4096 8.0 and 10.2, 8192 x 2048 11.0 and 10.5; 16 rows (128) 1024 x 1024 (1) 4.8
-  // and 7.1, 2048 x 2048 (2) 6.6 and 7.5, 1024 x 8192 (2) 8.8 and 7.3.
-  const size_t digits = size_t(NP) * (g.M <= 2 ? 2 : g.M <= 4 ? 4 : g.M <= 8 ? 8 : 16);
-  if (g.M <= 16 && g.K >= 4 && few_steps(L, g) * digits * digits <= 16384) return launch_few<T>(L, g);
   const int steps = (g.K + 127) / 128, exact = (steps + kExact / 128 - 1) / (kExact / 128);
+  // Few rows while a wave's steps, by the rounds of one workgroup a CU, times the square of their
+  // digits stay small: its time grows with their product, the other's slowly.  Twice as many
+  // where one round has work for half of the CUs and more.
+  // Few and many (us), Z_2^32: 1 row 4096 x 4096 4.0 and 7.8, 4096 x 32000 22.7 and 24.6; 4 rows 4.7 and
+  // 9.1, 22.8 and 25.6; 8 rows (a step of a wave forms 32 digits a column of k) 4096 x 4096 5.9 and
+  // 9.4, 8192 x 8192 (16 steps) 15.2 and 17.4, 20000 x 300 (20) 11.5 and 8.4, 20000 x 4096 16.8 and 20.3, x 2048
+  // 15.7 and 14.5; 16 rows (64) 4096 x 4096 (4) 8.0 and 9.9, 8192 x 300 (8) 9.2 and 7.4, x 2048 11.2 and 10.6, x
+  // 2500 11.0 and 12.6.  Z_2^64: 1 row 4096 x 4096 4.6 and 8.0, 4096 x 32000 26.4 and 25.1; 4 rows (32) 8192 x
+  // 8192 14.7 and 18.5, 20000 x 300 10.9 and 8.5, x 4096 18.5 and 21.6; 8 rows (64) 4096 x 4096 8.0 and 10.2, 8192 x
+  // 2048 11.0 and 10.5, x 2500 10.9 and 11.6; 16 rows (128) 1024 x 1024 (1) 4.8 and 7.1, 2048 x 2048 (2) 6.5 and
+  // 7.4, 1024 x 8192 (2) 8.8 and 7.3.
+  const size_t digits = size_t(NP) * (g.M <= 2 ? 2 : g.M <= 4 ? 4 : g.M <= 8 ? 8 : 16);
+  const size_t wgs16 = (size_t(g.N) + 15) / 16, cus = size_t(L.num_cu), rounds16 = (wgs16 + cus - 1) / cus;
+  const size_t limit = rounds16 == 1 && 2 * wgs16 >= cus ? 32768 : 16384;
+  if (g.M <= 16 && g.K >= 4 && rounds16 * size_t((steps + 7) / 8) * digits * digits <= limit) return launch_few<T>(L, g);
   // The tile and the parts of K for which a launch takes least: its rounds of one workgroup a
   // CU, each with its start and its steps (two workgroups of the smallest tiles fit a CU, and
   // start together), and, where K is split, the output's clearing and the sums' way through
