@@ -695,10 +695,12 @@ class Ctx:
                 (wide > 1 and q.stride(1) != 1) or ldq % 16 or ldq < K:
             raise MpcxError(f"ring_gemm_q8: q: need int8 rows of {K} weights at whole 16 bytes on GPU {self._device}")
         if out is None:
-            out = self._new((M, N))
-        op, ldc = self._rows(out, "ring_gemm_q8: out")
-        if out.shape != (M, N):
-            raise MpcxError(f"ring_gemm_q8: out: shape {tuple(out.shape)}, need {(M, N)}")
+            out = a.new_empty((M, N))
+            op, ldc = out.data_ptr(), N
+        else:
+            op, ldc = self._rows(out, "ring_gemm_q8: out")
+            if out.shape != (M, N):
+                raise MpcxError(f"ring_gemm_q8: out: shape {tuple(out.shape)}, need {(M, N)}")
         sp = self._ints(scale, "ring_gemm_q8: scale", torch.int32, (N,)) if scale is not None else None
         tp = self._ints(tokens, "ring_gemm_q8: tokens", torch.int32, (M,)) if tokens is not None else None
         if M == 0:
@@ -865,6 +867,13 @@ class Ctx:
             raise MpcxError(f"{what}: need int{self.bw} rows of shape {tuple(shape)} on GPU {self._device}")
         return t.data_ptr(), st[0] if shape[0] > 1 else shape[1]
 
+    def _norm_out(self, what, like, out, shape):
+        """An output's tensor, address and row stride: `out`, or a new one like checked rows."""
+        if out is not None:
+            return (out, *self._norm_rows(what, out, shape))
+        out = _torch_module.empty_like(like)
+        return out, out.data_ptr(), out.stride(0) if shape[0] > 1 else shape[1]
+
     def _norm_sums(self, what, x, d, out):
         """The shape of a call, the sum, and x's, d's and the sum's addresses and strides."""
         shape = self._norm_shape(what, x)
@@ -872,10 +881,9 @@ class Ctx:
             if out is not None:
                 raise MpcxError(f"{what}: a sum without a residual")
             return shape, x, (*self._norm_rows(what, x, shape), None, 0, None, 0)
-        if out is None:
-            out = _torch_module.empty_like(x)
-        return shape, out, (*self._norm_rows(what, x, shape), *self._norm_rows(what, d, shape),
-                            *self._norm_rows(what, out, shape))
+        args = (*self._norm_rows(what, x, shape), *self._norm_rows(what, d, shape))
+        out, *place = self._norm_out(what, x, out, shape)
+        return shape, out, (*args, *place)
 
     def norm_sums_keygen(self, rx, rd=None, seed=1, gate=1):
         """Keys of norm_sums_eval from the masks of x and of the residual (rows, dim):
@@ -943,10 +951,8 @@ class Ctx:
 
     def _norm_scale_eval(self, what, party, keys, shares, h, v, gain, out):
         rows, dim = shape = self._norm_shape(what, h)
-        if out is None:
-            out = _torch_module.empty_like(h)
         hp, ldh = self._norm_rows(what, h, shape)
-        yp, ldy = self._norm_rows(what, out, shape)
+        out, yp, ldy = self._norm_out(what, h, out, shape)
         nb, plane = self.lib.mpcx_norm_scale_key_bytes(self.h, rows, dim), rows * dim * self.bw // 8
         ptrs = [self._key(k, nb, what) for k in keys] + [self._key(a, plane, what) for a in shares]
         vp = self._words(v, what, (rows,))

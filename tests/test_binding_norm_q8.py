@@ -16,7 +16,8 @@ KEY = Tensor((1000,), BYTE)
 def c(ctx, monkeypatch):  # noqa: F811
     mpcx._torch_module.int8 = INT8
     mpcx._torch_module.empty_like = lambda t: Tensor(t.shape, t.dtype, t.device_index)
-    monkeypatch.setattr(Tensor, "new_empty", lambda t, n: Tensor((n,), t.dtype, t.device_index), raising=False)
+    monkeypatch.setattr(Tensor, "new_empty", lambda t, n: Tensor(n if isinstance(n, tuple) else (n,), t.dtype, t.device_index),
+                        raising=False)
     return ctx
 
 
