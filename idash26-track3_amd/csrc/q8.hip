@@ -120,14 +120,15 @@ __device__ __forceinline__ int q8_turn(int col) {
 // ---------------------------------------------------------------------------
 template <typename T, int R, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
-  constexpr int NP = int(sizeof(T)), PARTS = 16 / R < NP ? 16 / R : NP, PW = NP / PARTS;  // planes of a part
-  constexpr int NR = PARTS < 4 ? 4 / PARTS : 1;                // a lane's words of the output
+  constexpr int NP = int(sizeof(T)), MT = R > 16 ? R / 16 : 1;  // tiles of 16 rows
+  constexpr int PARTS = MT > 1 ? 1 : 16 / R < NP ? 16 / R : NP, PW = NP / PARTS;  // planes of a part
+  constexpr int NR = PARTS < 4 ? 4 / PARTS : 1;                // a lane's words of a tile of the output
   constexpr int QUADS = R / 2;                                 // a lane's groups of four words of a step
   constexpr int NW = 2, NB = QUADS * NP / 4;                   // loads of a step's weights and words
   constexpr int D = R <= 4 ? 2 : 1;                            // steps asked for ahead
   constexpr int DIGITS = R * NP * 128, OWN = D * NW * 1024 + DIGITS;  // bytes: of a step's digits, of a wave
   __shared__ __align__(16) uint8_t lds[WAVES * OWN];
-  static_assert(sizeof lds >= WAVES * NR * 64 * sizeof(T), "the sums' place");
+  static_assert(sizeof lds >= WAVES * MT * NR * 64 * sizeof(T), "the sums' place");
   const int tid = int(threadIdx.x), lane = tid & 63, waves = int(blockDim.x) >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int li = lane & 15, lg = lane >> 4, n0 = int(blockIdx.x) * 16;
@@ -151,9 +152,9 @@ __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
   }
 #pragma unroll
   for (int i = 0; i < QUADS; i++) ao[i] = uint32_t(min(lane / 32 + 2 * i, g.M - 1)) * uint32_t(g.lda) * uint32_t(NP);
-  // Digits: plane, row, 128 bytes; group j of 16 bytes at j ^ (the plane's part + PARTS (row / 2)).
+  // Digits: plane, row, 128 bytes; group j of 16 bytes at j ^ (the plane's part + PARTS (row / 2)) % 8.
 #pragma unroll
-  for (int i = 0; i < QUADS; i++) to[i] = uint32_t((lane / 32 + 2 * i) * 128 + kq % 4 * 4 + ((kq / 4) ^ (PARTS * i)) * 16);
+  for (int i = 0; i < QUADS; i++) to[i] = uint32_t((lane / 32 + 2 * i) * 128 + kq % 4 * 4 + ((kq / 4) ^ (PARTS * i % 8)) * 16);
   const int row = R * PARTS < 16 ? li / PARTS % R : li / PARTS, part = li % PARTS;
   uint32_t fromw[2], from[2];
 #pragma unroll
@@ -183,7 +184,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
     __builtin_amdgcn_sched_barrier(0);  // here, not where they are used
   };
 
-  v4i_t acc[PW] = {};  // of at most 512 steps (launch_part), 2^16 terms
+  v4i_t acc[MT][PW] = {};  // of at most 512 steps (launch_part), 2^16 terms
   // Step i of this wave, in x; `later` of its steps have been asked for since; more: x asks for step i + D.
   auto step = [&](int i, Words &x, auto later, auto more) __attribute__((always_inline)) {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(decltype(later)::value * (NW + NB)) : "memory");
@@ -214,7 +215,10 @@ __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
     for (int o = 0; o < 2; o++)
 #pragma unroll
       for (int k = 0; k < PW; k++)
-        acc[k] = mfma64(*reinterpret_cast<const v4i_t *>(digits + (from[o] + uint32_t(k * R * 128))), b[o], acc[k]);
+#pragma unroll
+        for (int t = 0; t < MT; t++)
+          acc[t][k] = mfma64(*reinterpret_cast<const v4i_t *>(digits + (from[o] + uint32_t(k * R * 128 + t * 2048))), b[o],
+                             acc[t][k]);
     __builtin_amdgcn_sched_barrier(0);  // before the next step's words are waited for
   };
   constexpr std::true_type yes{};
@@ -249,22 +253,24 @@ __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
     step(mine - 1, y, none, no);
   }
   // a register's row of 4: part j % PARTS of a word; of eight parts, the upper four where lg is odd
-  T out[NR] = {};
+  T out[MT * NR] = {};
 #pragma unroll
-  for (int k = 0; k < PW; k++)
+  for (int t = 0; t < MT; t++)
 #pragma unroll
-    for (int j = 0; j < 4; j++) out[j / (4 / NR)] += plane_word<T>(acc[k][j], j % (4 / NR) * PW + k);
+    for (int k = 0; k < PW; k++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) out[t * NR + j / (4 / NR)] += plane_word<T>(acc[t][k][j], j % (4 / NR) * PW + k);
   __syncthreads();
   T *red = reinterpret_cast<T *>(lds);  // wave, register, lane
 #pragma unroll
-  for (int r = 0; r < NR; r++) red[(wave * NR + r) * 64 + lane] = out[r];
+  for (int r = 0; r < MT * NR; r++) red[(wave * MT * NR + r) * 64 + lane] = out[r];
   __syncthreads();
   for (int e = tid; e < R * 16; e += int(blockDim.x)) {
     const int r = e / 16, c = e % 16, n = n0 + c;
     T v = 0;
     for (int w = 0; w < waves; w++) {
-      const T *z = red + w * NR * 64;
-      if constexpr (PARTS <= 4) v += z[r % NR * 64 + 16 * (r / NR) + c];
+      const T *z = red + w * MT * NR * 64;
+      if constexpr (PARTS <= 4) v += z[(r / 16 * NR + r % NR) * 64 + 16 * (r % 16 / NR) + c];
       else v += z[32 * r + c] + (z[32 * r + 16 + c] << 32);
     }
     if (r < g.M && n < g.N) g.c[size_t(r) * g.ldc + n] = scaled<T>(g, v, r, n);
@@ -566,6 +572,29 @@ __global__ __launch_bounds__(256) void k_q8_clear(Q8Args<T> g) {
     g.c[i / g.N * g.ldc + i % g.N] = 0;
 }
 
+// The weights' way from memory (us), at 6.5 TB/s (in part from the card's cache).
+template <typename T>
+float weights_time(const Q8Args<T> &g) {
+  return float(g.K) * float(g.N) / 6.5e6f;
+}
+// What a launch of k_q8_few takes (us): its start and the larger of the weights' way and its
+// rounds of one workgroup a CU times a wave's steps, each the digits of R rows and, with more
+// than half of the CUs at work, the words' way to them; where but one workgroup fits a CU each
+// round has a start.  Measured beside k_q8_many's by the rule below: Z_2^32 1 row 4096 x
+// 4096 4.0 and 7.8, 4096 x 32000 22.7 and 24.6; 4 rows 4.7 and 9.1, 22.8 and 25.6; 8 rows 4096 x 4096 5.9
+// and 9.4, 8192 x 8192 15.2 and 17.4, 20000 x 300 11.5 and 8.4, 20000 x 4096 16.8 and 20.3; 16 rows 4096 x
+// 4096 8.0 and 9.9, 8192 x 300 9.2 and 7.4, x 2500 11.0 and 12.6; 32 rows 1024 x 1024 4.7 and 7.0, 2048 x
+// 4096 7.5 and 7.8, 4096 x 4096 12.4 and 10.9, 1000 x 4099 9.0 and 7.6.  Z_2^64: 1 row 4096 x 4096 4.6 and
+// 8.0; 4 rows 8192 x 8192 14.7 and 18.5, 20000 x 300 10.9 and 8.5; 8 rows 4096 x 4096 8.0 and 10.2, 8192 x
+// 2500 10.9 and 11.6; 16 rows 1024 x 1024 4.8 and 7.1, 2048 x 2048 6.5 and 7.4, 4096 x 4096 12.5 and 11.2.
+template <typename T>
+float few_time(const Launch &L, const Q8Args<T> &g) {
+  const float digits = float(sizeof(T)) * (g.M <= 2 ? 2.f : g.M <= 4 ? 4.f : g.M <= 8 ? 8.f : g.M <= 16 ? 16.f : 32.f);
+  const float wgs = std::ceil(float(g.N) / 16), cus = float(L.num_cu), rounds = std::ceil(wgs / cus);
+  const float step = 0.15f + 0.0125f * digits + 0.006f * digits * std::max(0.f, 2 * std::min(1.f, wgs / cus) - 1);
+  return 2.5f + std::max(rounds * std::ceil(float(g.K) / 1024) * step, weights_time(g)) +
+         (digits >= 128 ? 2.2f * (rounds - 1) : 0.f);
+}
 template <typename T>
 hipError_t launch_few(const Launch &L, const Q8Args<T> &g) {
   const int steps = (g.K + 127) / 128;
@@ -579,6 +608,9 @@ hipError_t launch_few(const Launch &L, const Q8Args<T> &g) {
   constexpr std::integral_constant<int, 4> four{};
   constexpr std::integral_constant<int, 8> eight{};
   constexpr std::integral_constant<int, 16> sixteen{};
+  if constexpr (sizeof(T) == 4) {
+    if (g.M > 16) return few(std::integral_constant<int, 32>{}, eight);
+  }
   if (g.M > 4) return g.M <= 8 ? few(eight, eight) : few(sixteen, eight);
   // Sixteen waves where they have a step each and a workgroup has a CU (us, Z_2^32, by eight
   // and by sixteen): one row of 4096 x 4096 5.5 and 5.1, of 8192 x 2048 5.5 and 5.2; four of 4096 x
@@ -593,21 +625,6 @@ template <typename T>
 hipError_t launch_part(const Launch &L, const Q8Args<T> &g) {
   constexpr int NP = int(sizeof(T));
   const int steps = (g.K + 127) / 128, exact = (steps + kExact / 128 - 1) / (kExact / 128);
-  // Few rows while a wave's steps, by the rounds of one workgroup a CU, times the square of their
-  // digits stay small: its time grows with their product, the other's slowly.  Twice as many
-  // where one round has work for half of the CUs and more.
-  // Few and many (us), Z_2^32: 1 row 4096 x 4096 4.0 and 7.8, 4096 x 32000 22.7 and 24.6; 4 rows 4.7 and
-  // 9.1, 22.8 and 25.6; 8 rows (a step of a wave forms 32 digits a column of k) 4096 x 4096 5.9 and
-  // 9.4, 8192 x 8192 (16 steps) 15.2 and 17.4, 20000 x 300 (20) 11.5 and 8.4, 20000 x 4096 16.8 and 20.3, x 2048
-  // 15.7 and 14.5; 16 rows (64) 4096 x 4096 (4) 8.0 and 9.9, 8192 x 300 (8) 9.2 and 7.4, x 2048 11.2 and 10.6, x
-  // 2500 11.0 and 12.6.  Z_2^64: 1 row 4096 x 4096 4.6 and 8.0, 4096 x 32000 26.4 and 25.1; 4 rows (32) 8192 x
-  // 8192 14.7 and 18.5, 20000 x 300 10.9 and 8.5, x 4096 18.5 and 21.6; 8 rows (64) 4096 x 4096 8.0 and 10.2, 8192 x
-  // 2048 11.0 and 10.5, x 2500 10.9 and 11.6; 16 rows (128) 1024 x 1024 (1) 4.8 and 7.1, 2048 x 2048 (2) 6.5 and
-  // 7.4, 1024 x 8192 (2) 8.8 and 7.3.
-  const size_t digits = size_t(NP) * (g.M <= 2 ? 2 : g.M <= 4 ? 4 : g.M <= 8 ? 8 : 16);
-  const size_t wgs16 = (size_t(g.N) + 15) / 16, cus = size_t(L.num_cu), rounds16 = (wgs16 + cus - 1) / cus;
-  const size_t limit = rounds16 == 1 && 2 * wgs16 >= cus ? 32768 : 16384;
-  if (g.M <= 16 && g.K >= 4 && rounds16 * size_t((steps + 7) / 8) * digits * digits <= limit) return launch_few<T>(L, g);
   // The tile and the parts of K for which a launch takes least: its rounds of one workgroup a
   // CU, each with its start and its steps (two workgroups of the smallest tiles fit a CU, and
   // start together), and, where K is split, the output's clearing and the sums' way through
@@ -630,6 +647,9 @@ hipError_t launch_part(const Launch &L, const Q8Args<T> &g) {
         if (p > 1) t += 2.5f + 0.1f * float(p) + 0.25e-6f * float(g.M) * float(g.N) * float(p * NP);
         if (best == 0 || t < best) best = t, nt = w, splits = p, large = big != 0;
       }
+  // few rows: four words to load, plane sums in 32 bits
+  if (g.M <= 128 / NP && g.K >= 4 && steps <= 8 * (kExact / 128) && few_time(L, g) <= std::max(best, 4 + weights_time(g)))
+    return launch_few<T>(L, g);
   const int words = large ? kLarge<T> * 16 : kLarge<T> * 8, rows = (g.M + words - 1) / words;
   const int cols = (g.N + 64 * nt - 1) / (64 * nt);
   const size_t wgs = size_t(rows) * size_t(cols) * size_t(splits);

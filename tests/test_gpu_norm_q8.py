@@ -133,7 +133,7 @@ def test_q8_tiles_of_long_rows(ctx, M, K, N):
 
 
 # a few rows by many columns or a long K, by either kernel
-@pytest.mark.parametrize("M", [1, 2, 3, 5, 8, 9, 16])
+@pytest.mark.parametrize("M", [1, 2, 3, 5, 8, 9, 16, 17, 24, 32])
 @pytest.mark.parametrize("K,N", [(2048, 500), (4099, 4096), (8191, 2048), (130, 30001), (20001, 100), (2001, 4200), (3200, 4201), (9000, 2500),
                                  (4099, 4097), (1, 40), (2, 40), (3, 40), (4, 40), (5, 40), (7, 33)])
 def test_q8_few_or_many(ctx, M, K, N):
