@@ -87,13 +87,6 @@ __device__ __forceinline__ T plane_word(int32_t sum, int p) {
 // bytes of a row of weights that may be read: whole 16
 __host__ __device__ __forceinline__ int q8_row(int K) { return (K + 15) & ~15; }
 
-template <typename T>
-__device__ __forceinline__ T scaled(const Q8Args<T> &g, T v, int m, int n) {
-  if (g.scale) v *= T(int64_t(g.scale[n]));
-  if (g.tok) v *= T(int64_t(g.tok[m]));
-  return v;
-}
-
 // Which of a column's 8 groups of 16 weights of a 128-k step lies where in LDS, for the
 // reads' banks: column col of a tile of 16.
 __device__ __forceinline__ int q8_turn(int col) {
@@ -225,6 +218,10 @@ __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
   constexpr std::false_type no{};
   constexpr std::integral_constant<int, 0> none{};
   constexpr std::integral_constant<int, 1> one{};
+  // this thread's word of the output, and its scales
+  const int n = n0 + tid % 16;
+  const int32_t sn = g.scale ? g.scale[min(n, g.N - 1)] : 1;
+  int32_t sm = g.tok ? g.tok[min(tid / 16, g.M - 1)] : 1;
   if constexpr (D == 1) {
     Words x;
     ask(0, x);
@@ -232,8 +229,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
     step(mine - 1, x, none, no);
   } else {  // no branch of fewer loads before a load's use: behind it the compiler would wait for all
     Words x, y;
+    ask(0, x);
     if (mine > 1) {
-      ask(0, x);
       ask(1, y);
       int i = 0;
       for (; i + 3 < mine; i += 2) {
@@ -248,7 +245,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
         step(i, x, one, no);
       }
     } else {
-      ask(0, y);
+      y = x;
     }
     step(mine - 1, y, none, no);
   }
@@ -265,15 +262,15 @@ __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
 #pragma unroll
   for (int r = 0; r < MT * NR; r++) red[(wave * MT * NR + r) * 64 + lane] = out[r];
   __syncthreads();
-  for (int e = tid; e < R * 16; e += int(blockDim.x)) {
-    const int r = e / 16, c = e % 16, n = n0 + c;
+  for (int r = tid / 16; r < min(R, g.M); r += 4 * waves) {
     T v = 0;
     for (int w = 0; w < waves; w++) {
-      const T *z = red + w * MT * NR * 64;
-      if constexpr (PARTS <= 4) v += z[(r / 16 * NR + r % NR) * 64 + 16 * (r % 16 / NR) + c];
-      else v += z[32 * r + c] + (z[32 * r + 16 + c] << 32);
+      const T *z = red + w * MT * NR * 64 + tid % 16;
+      if constexpr (PARTS <= 4) v += z[(r / 16 * NR + r % NR) * 64 + 16 * (r % 16 / NR)];
+      else v += z[32 * r] + (z[32 * r + 16] << 32);
     }
-    if (r < g.M && n < g.N) g.c[size_t(r) * g.ldc + n] = scaled<T>(g, v, r, n);
+    if (n < g.N) g.c[size_t(r) * g.ldc + n] = v * T(int64_t(sn)) * T(int64_t(sm));
+    if (g.tok) sm = g.tok[min(r + 4 * waves, g.M - 1)];
   }
 }
 
