@@ -108,8 +108,9 @@ __device__ __forceinline__ int q8_turn(int col) {
 // Places: a read of 16 bytes serves lanes 0-3, 12-15, 20-27 together, then 4-11, 16-19,
 // 28-31; groups of 16 bytes are turned so that those fall into different banks.
 // Bound by the weights' bytes and, below some 20 MB, by a launch's start and the waves'
-// first loads: in Z_2^32 1 x 4096 x 4096 4.1 us, 1 x 4096 x 11008 9.9 (4.6 TB/s), 1 x 8192 x 8192 13.4; with
-// more rows by the digits, which each workgroup forms: 4096 x 4096, 8 rows 5.9, 16 rows 8.0.
+// first loads: in Z_2^32 1 x 4096 x 4096 3.7 us, 1 x 4096 x 11008 9.6 (4.7 TB/s), 1 x 8192 x 8192 13.3; with
+// more rows by the digits, which each workgroup forms, their way through LDS and the words' way to
+// every CU: 4096 x 4096, 8 rows 5.5, 16 rows 7.7.
 // ---------------------------------------------------------------------------
 template <typename T, int R, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
