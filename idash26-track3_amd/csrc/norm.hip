@@ -28,19 +28,37 @@ struct Words {
   __device__ __forceinline__ void store(T *p) const { __builtin_memcpy(p, w, 16); }
 };
 
+// What a row's sum starts from: the shares of its term that the form adds.
+template <NormForm F, typename T>
+__device__ __forceinline__ T norm_term(const NormSumsArgs<T> &g, size_t t) {
+  T c = 0;
+  if constexpr (F != NormForm::P1) c += g.c0[t];
+  if constexpr (F == NormForm::BOTH || F == NormForm::P1) c += g.c1[t];
+  return c;
+}
+template <NormForm F, typename T>
+__global__ __launch_bounds__(256) void k_norm_terms(NormSumsArgs<T> g) {
+  const size_t t = size_t(blockIdx.x) * 256 + threadIdx.x;
+  if (t < g.rows) g.s[t] = norm_term<F>(g, t);
+}
+
 // ---------------------------------------------------------------------------
 // W waves a row (W a power of two; a workgroup is 4 waves or W).  The bytes are all there is
 // to it: four words in (three without a residual) and one out (none) for one multiplication.
 // 6000 x 4096 in Z_2^32 90 us, 5.5 TB/s (a word a lane instead of 16 bytes: 114); one row of
-// 4096 3.4 (by one wave 17.6).
+// 4096 3.4 (by one wave 17.6).  Long rows, where they are few: PARTS a row, of `len` words
+// (whole turns of the waves), added up in s, which k_norm_terms has begun; sums modulo 2^bw
+// do not depend on their order.
 // ---------------------------------------------------------------------------
-template <NormForm F, typename T, int W, bool RES>
-__global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_norm_sums(NormSumsArgs<T> g) {
+template <NormForm F, typename T, int W, bool RES, bool PARTS>
+__global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_norm_sums(NormSumsArgs<T> g, uint32_t parts, size_t len) {
   constexpr int GROUP = W > 4 ? W : 4, ROWS = GROUP / W, N = Words<T>::N;
   __shared__ T part[GROUP];
   const int wave = int(threadIdx.x) >> 6, at = int(threadIdx.x) % (64 * W);
-  for (size_t t0 = size_t(blockIdx.x) * ROWS; t0 < g.rows; t0 += size_t(gridDim.x) * ROWS) {
-    const size_t t = t0 + wave / W;
+  const size_t units = PARTS ? g.rows * parts : g.rows;
+  for (size_t t0 = size_t(blockIdx.x) * ROWS; t0 < units; t0 += size_t(gridDim.x) * ROWS) {
+    const size_t t = PARTS ? t0 / parts : t0 + wave / W, start = PARTS ? t0 % parts * len : 0;
+    const size_t end = PARTS ? min(start + len, g.dim) : g.dim;
     T sum = 0;
     if (t < g.rows) {
       const T *x = g.x + t * g.ldx, *d = RES ? g.d + t * g.ldd : nullptr;
@@ -53,9 +71,9 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_norm_sums(NormSumsArgs
         return v * v;
       };
       constexpr bool A0 = F == NormForm::BOTH || F == NormForm::P0, A1 = F == NormForm::BOTH || F == NormForm::P1;
-      size_t j = size_t(at) * N;
+      size_t j = start + size_t(at) * N;
 #pragma unroll 2
-      for (; j + N <= g.dim; j += 64 * W * N) {
+      for (; j + N <= end; j += 64 * W * N) {
         Words<T> v, r, b0, b1;
         v.load(x + j);
         if constexpr (RES) r.load(d + j);
@@ -69,7 +87,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_norm_sums(NormSumsArgs
         if constexpr (RES) v.store(h + j);
         if constexpr (F == NormForm::DEAL) v.store(copy + j);
       }
-      for (; j < g.dim; j++) {  // one lane's, fewer than N
+      for (; j < end; j++) {  // one lane's, fewer than N
         T v = x[j];
         if constexpr (RES) v += d[j];
         sum += word(v, A0 ? a0[j] : T(0), A1 ? a1[j] : T(0));
@@ -89,9 +107,12 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_norm_sums(NormSumsArgs
       __syncthreads();
     }
     if (at == 0 && t < g.rows) {
-      if constexpr (F != NormForm::P1) sum += g.c0[t];
-      if constexpr (F == NormForm::BOTH || F == NormForm::P1) sum += g.c1[t];
-      g.s[t] = sum;
+      if constexpr (PARTS) {
+        using A = std::conditional_t<sizeof(T) == 4, unsigned, unsigned long long>;
+        atomicAdd(reinterpret_cast<A *>(g.s + t), A(sum));
+      } else {
+        g.s[t] = sum + norm_term<F>(g, t);
+      }
     }
   }
 }
@@ -149,11 +170,25 @@ hipError_t sums_form(const Launch &L, const NormSumsArgs<T> &g) {
   auto waves = [&](auto w) {
     constexpr int W = decltype(w)::value, ROWS = W > 4 ? 1 : 4 / W;
     const size_t want = (g.rows + ROWS - 1) / ROWS, cap = size_t(L.num_cu) * 16;
-    hipLaunchKernelGGL((k_norm_sums<F, T, W, RES>), dim3(unsigned(std::min(want, cap))), dim3(64 * std::max(W, 4)), 0,
-                       L.stream, g);
+    hipLaunchKernelGGL((k_norm_sums<F, T, W, RES, false>), dim3(unsigned(std::min(want, cap))), dim3(64 * std::max(W, 4)), 0,
+                       L.stream, g, 1u, g.dim);
     return hipGetLastError();
   };
   const size_t turns = (g.dim * sizeof(T) + 1023) / 1024;  // of a wave, to pass a row
+  // Long rows in parts, a workgroup each, where the rows leave CUs idle (us, whole and in parts,
+  // Z_2^32): 1 row of 16384 4.8 and 4.9, of 32768 7.3 and 4.9, of 262144 55 and 5.3; 16 rows of 32768 9.2 and
+  // 6.1; 64 rows 10.8 and 10.6; 128 rows 13.9 and 16.2.
+  const size_t rounds = (turns + 15) / 16, cus = size_t(L.num_cu);  // of 16 waves, to pass a row
+  if (rounds >= 8 && g.rows <= cus / 4) {
+    const size_t most = std::min(rounds, (cus + g.rows - 1) / g.rows), len = (rounds + most - 1) / most * (16384 / sizeof(T));
+    const size_t parts = (g.dim + len - 1) / len;
+    hipLaunchKernelGGL((k_norm_terms<F, T>), dim3(unsigned((g.rows + 255) / 256)), dim3(256), 0, L.stream, g);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((k_norm_sums<F, T, 16, RES, true>), dim3(unsigned(g.rows * parts)), dim3(1024), 0, L.stream, g,
+                       uint32_t(parts), len);
+    return hipGetLastError();
+  }
   // By 16, 4 and 1 waves (us, Z_2^32): 1 x 4096 2.8, 3.1, 4.9; 2000 x 4096 27, 27, 28; 8000 x
   // 4096 117, 124, 131; 700 x 2048 7.5, 6.6, 6.7; 8000 x 1024 34, 27, 27; 8000 x 128 23, 9.4, 5.9.
   if (turns > 8) return waves(std::integral_constant<int, 16>{});

@@ -216,7 +216,7 @@ def test_q8_no_token(ctx):
 
 # ---------------- the norm's gates ----------------
 NORM_SHAPES = [(1, 1), (1, 64), (1, 4096), (1, 70001), (2, 63), (3, 65), (5, 129), (7, 1000), (16, 256), (37, 1279),
-               (64, 312), (130, 2048), (600, 96), (1025, 33), (3000, 4)]
+               (64, 312), (130, 2048), (600, 96), (1025, 33), (3000, 4), (2, 32768), (3, 49155), (64, 32769)]
 
 
 def up(n):
