@@ -177,9 +177,9 @@ hipError_t sums_form(const Launch &L, const NormSumsArgs<T> &g) {
   const size_t turns = (g.dim * sizeof(T) + 1023) / 1024;  // of a wave, to pass a row
   // Long rows in parts, a workgroup each, where the rows leave CUs idle (us, whole and in parts,
   // Z_2^32): 1 row of 16384 4.8 and 4.9, of 32768 7.3 and 4.9, of 262144 55 and 5.3; 16 rows of 32768 9.2 and
-  // 6.1; 64 rows 10.8 and 10.6; 128 rows 13.9 and 16.2.
+  // 6.1; 64 rows 10.8 and 10.6; 128 rows 13.9 and 16.2, of 65536 35 and 29; 256 rows 67 and 69.
   const size_t rounds = (turns + 15) / 16, cus = size_t(L.num_cu);  // of 16 waves, to pass a row
-  if (rounds >= 8 && g.rows <= cus / 4) {
+  if (rounds >= 8 && g.rows <= cus * std::min<size_t>(rounds, 16) / 32) {
     const size_t most = std::min(rounds, (cus + g.rows - 1) / g.rows), len = (rounds + most - 1) / most * (16384 / sizeof(T));
     const size_t parts = (g.dim + len - 1) / len;
     hipLaunchKernelGGL((k_norm_terms<F, T>), dim3(unsigned((g.rows + 255) / 256)), dim3(256), 0, L.stream, g);

@@ -338,6 +338,33 @@ def test_long_rows(ctx):
             assert np.array_equal(host(s, ctx.bw) - host(rs, ctx.bw), np.square(x).sum(1, dtype=ctx.T))
 
 
+@pytest.mark.parametrize("rows,dim", [(1, 40001), (100, 65537)])
+def test_graph_of_long_rows(ctx, rows, dim):
+    """Sums that parts of a row add up: every replay begins them anew."""
+    import torch
+    rng = np.random.default_rng(dim)
+    k0, k1, _, _ = ctx.norm_sums_keygen(dev(words(rng, (rows, dim), ctx.bw)))
+    x = dev(words(rng, (rows, dim), ctx.bw))
+    stream = torch.cuda.Stream()
+    ctx.set_stream(stream)
+    try:
+        with torch.cuda.stream(stream):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                _, s = ctx.norm_sums_eval(k0, k1, x)
+            for i in range(3):
+                x.add_(i)
+                graph.replay()
+                stream.synchronize()
+                assert torch.equal(s, ctx.norm_sums_eval(k0, k1, x)[1])
+        with np.errstate(over="ignore"):
+            v, a = host(x, ctx.bw), sum(key_planes(k, ctx.T, rows * dim, rows)[0].reshape(rows, dim) for k in (k0, k1))
+            c = sum(key_planes(k, ctx.T, rows * dim, rows)[1] for k in (k0, k1))
+            assert np.array_equal(host(s, ctx.bw), (v * (v - ctx.T(2) * a)).sum(1, dtype=ctx.T) + c)
+    finally:
+        ctx.set_stream(None)
+
+
 @pytest.mark.parametrize("value", [0, 1 << 63, (1 << 64) - 1, 0x8000000080000000])
 def test_rows_of_one_value(ctx, value):
     """Zeros, and words at the ends of the ring."""
