@@ -476,7 +476,9 @@ mpcx_status mpcx_attn_mix_message(mpcx_ctx *ctx, int party, const mpcx_attn *a, 
  *
  * Sums (Beaver): h = x + d and s[t] = sum_j h[t, j]^2.  Rows of x, d and h: ldx, ldd,
  * ldh >= dim words apart; d_h may be d_x or d_d.  Without a residual d_d and d_h
- * are NULL and h = x.  Keygen takes the masks of x and d, writes the masks of h (at
+ * are NULL and h = x.  The sum is one modulo 2^bw: as a number it is what a root
+ * needs while it stays below 2^(bw-1), at scale s in Z_2^32 dim * rms^2 < 2^(31-2s)
+ * (scale 12: 128).  Keygen takes the masks of x and d, writes the masks of h (at
  * d_rh, where there is a residual) and s and the parties' keys: the share of
  * h's mask (rows * dim words), then, from the next multiple of 256 bytes on, the
  * share of the sums' term (rows words). */

@@ -13,3 +13,12 @@ def test_decoder(bw, kw):
     lines = []
     assert block.run(bw, say=lines.append, **kw), lines
     assert len(lines) == 4
+
+
+@pytest.mark.parametrize("bw,kw", [(64, dict(blocks=1, model=2560, hidden=96, words=40, prompts=(5,), singles=2)),
+                                   (64, dict(blocks=1, model=6144, hidden=48, words=24, prompts=(3,), singles=2))])
+def test_decoder_of_ordinary_width(bw, kw):
+    """Norms of rows whose width is no power of two, one of them past 4096 (a truncation more)."""
+    import block
+    lines = []
+    assert block.run(bw, say=lines.append, **kw), lines
