@@ -1464,15 +1464,15 @@ template <typename T>
 mpcx_status sums_keygen_t(mpcx_ctx *c, const SumsCall &g, uint64_t seed, uint32_t gate, uint8_t *k0, uint8_t *k1) {
   const size_t n = g.rows * size_t(g.dim), at = attn_key_second(c, n);
   T *A1 = reinterpret_cast<T *>(k1), *C1 = reinterpret_cast<T *>(k1 + at);
-  HIPC(c, launch_prf_ring<T>(c->L, seed, gate, F_ROUT, g.rows, static_cast<T *>(g.s)), "prf");
+  HIPC(c, launch_prf_ring<T>(c->L, seed, gate, F_NSUMS + 1, g.rows, static_cast<T *>(g.s)), "prf");
   NormSumsArgs<T> a = sums_args<T>(g);
   a.c0 = a.s;
   a.s = C1;
   a.copy = A1;
   HIPC(c, launch_norm_sums<T>(c->L, NormForm::DEAL, a), "norm_sums_keygen");
   // a mask and a term are split where party 1's share of them goes
-  HIPC(c, launch_split<T>(c->L, seed, gate, F_SPLIT + 0, n, A1, reinterpret_cast<T *>(k0), A1, nullptr), "split");
-  HIPC(c, launch_split<T>(c->L, seed, gate, F_SPLIT + 2, g.rows, C1, reinterpret_cast<T *>(k0 + at), C1, nullptr),
+  HIPC(c, launch_split<T>(c->L, seed, gate, F_NSUMS + 0, n, A1, reinterpret_cast<T *>(k0), A1, nullptr), "split");
+  HIPC(c, launch_split<T>(c->L, seed, gate, F_NSUMS + 2, g.rows, C1, reinterpret_cast<T *>(k0 + at), C1, nullptr),
        "split");
   HIPC(c, hipStreamSynchronize(c->L.stream), "sync");
   return MPCX_OK;
@@ -1585,16 +1585,16 @@ template <typename T>
 mpcx_status scale_keygen_t(mpcx_ctx *c, const ScaleCall &g, uint64_t seed, uint32_t gate, uint8_t *k0, uint8_t *k1) {
   const size_t n = g.rows * size_t(g.dim), at = attn_key_second(c, g.rows);
   T *C1 = reinterpret_cast<T *>(k1 + at);
-  HIPC(c, launch_split<T>(c->L, seed, gate, F_SPLIT + 0, g.rows, static_cast<const T *>(g.v), reinterpret_cast<T *>(k0),
+  HIPC(c, launch_split<T>(c->L, seed, gate, F_NSCALE + 0, g.rows, static_cast<const T *>(g.v), reinterpret_cast<T *>(k0),
                           reinterpret_cast<T *>(k1), nullptr),
        "split");
-  HIPC(c, launch_prf_ring<T>(c->L, seed, gate, F_ROUT, n, static_cast<T *>(g.y)), "prf");
+  HIPC(c, launch_prf_ring<T>(c->L, seed, gate, F_NSCALE + 1, n, static_cast<T *>(g.y)), "prf");
   NormScaleArgs<T> a = scale_args<T>(c, g, k0, nullptr);
   a.c0 = static_cast<const T *>(g.y);
   a.y = C1;
   a.ldy = size_t(g.dim);
   HIPC(c, launch_norm_scale<T>(c->L, NormForm::DEAL, a), "norm_scale_keygen");
-  HIPC(c, launch_split<T>(c->L, seed, gate, F_SPLIT + 2, n, C1, reinterpret_cast<T *>(k0 + at), C1, nullptr), "split");
+  HIPC(c, launch_split<T>(c->L, seed, gate, F_NSCALE + 2, n, C1, reinterpret_cast<T *>(k0 + at), C1, nullptr), "split");
   HIPC(c, hipStreamSynchronize(c->L.stream), "sync");
   return MPCX_OK;
 }

@@ -495,7 +495,8 @@ mpcx_status mpcx_norm_sums_eval(mpcx_ctx *ctx, size_t rows, int dim, const void 
  * gates.  Keygen takes them and the factors' mask, writes y's mask (rows * dim words)
  * and the keys: the share of the factors' mask (rows words), then, 256-byte
  * aligned, of the product term (rows * dim words).  Rows of h and y: ldh, ldy >=
- * dim words apart; d_yhat may be d_hhat.
+ * dim words apart; d_yhat may be d_hhat.  The two keygens draw from fields of their
+ * own: with one seed they may have one gate id.
  * Any other overlap of an output of these calls with another buffer is refused. */
 size_t mpcx_norm_scale_key_bytes(mpcx_ctx *ctx, size_t rows, int dim);
 mpcx_status mpcx_norm_scale_keygen(mpcx_ctx *ctx, size_t rows, int dim, const void *d_a0, const void *d_a1,

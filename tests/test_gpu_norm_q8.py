@@ -346,3 +346,21 @@ def test_norm_keys_differ_by_gate(ctx):
     r = dev(words(np.random.default_rng(1), (4, 40), ctx.bw))
     keys = [ctx.norm_sums_keygen(r, seed=s, gate=g)[0].cpu().numpy() for s, g in ((1, 1), (1, 2), (2, 1))]
     assert not any(np.array_equal(a[:160], b[:160]) for a, b in ((keys[0], keys[1]), (keys[0], keys[2])))
+
+
+def test_norm_gates_of_one_id(ctx):
+    """The two gates of a norm under one seed and gate id, as the defaults give them, and the other
+    gates' masks and shares under the same: no two draw the same words."""
+    rng = np.random.default_rng(3)
+    rows, dim = 40, 3
+    r, rv = dev(words(rng, (rows, dim), ctx.bw)), dev(words(rng, (rows,), ctx.bw))
+    k0, k1, _, rs = ctx.norm_sums_keygen(r)
+    q0, _, ry = ctx.norm_scale_keygen(k0, k1, rv, dim)
+    drawn = [*key_planes(k0, ctx.T, rows * dim, rows), host(rs, ctx.bw), *key_planes(q0, ctx.T, rows, rows * dim),
+             host(ry, ctx.bw).reshape(-1), host(ctx.split_mask(rv)[0], ctx.bw),
+             host(ctx.gate_keygen(mpcx.TR, rv)[2], ctx.bw)]
+    first = [tuple(d[:rows].tolist()) for d in drawn]
+    assert len(set(first)) == len(first)
+    q0, _, ry = ctx.norm_scale_keygen(k0, k1, rv, dim, gate=2)  # another id, other words
+    again = [host(ry, ctx.bw).reshape(-1), *key_planes(q0, ctx.T, rows, rows * dim)]
+    assert not set(first) & {tuple(d[:rows].tolist()) for d in again}
