@@ -1412,8 +1412,8 @@ mpcx_status mpcx_attn_mix_message(mpcx_ctx *c, int party, const mpcx_attn *a, co
 
 // ---------------- the norm's gates ----------------
 namespace {
-// rows * dim words, countable in 60 bits
-bool norm_sizes(size_t rows, int dim) { return dim >= 1 && rows <= (size_t(1) << 60) / size_t(dim); }
+// rows * dim words, countable in 59 bits: a key's two planes are then in 60, their bytes in 63
+bool norm_sizes(size_t rows, int dim) { return dim >= 1 && rows <= (size_t(1) << 59) / size_t(dim); }
 // The same rows: an output may take an input's place.
 bool same_rows(const ByteRows &a, const ByteRows &b) { return a.p == b.p && (a.rows <= 1 || a.pitch == b.pitch); }
 bool same_or_apart(const ByteRows &a, const ByteRows &b) { return same_rows(a, b) || rows_apart(a, b); }

@@ -379,3 +379,14 @@ def test_rows_of_one_value(ctx, value):
             c0 + c1, host(rs, ctx.bw) + np.square(h).sum(1, dtype=ctx.T))
         hh, s = ctx.norm_sums_eval(k0, k1, z, z)  # masked values that hide zeros
     assert np.array_equal(host(hh, ctx.bw), h) and np.array_equal(host(s, ctx.bw), host(rs, ctx.bw))
+
+
+def test_key_bytes_at_their_end(ctx):
+    """The most rows there are have keys whose bytes can be counted; one row more is refused."""
+    tb, buf, (k0, k1, x, s) = ctx.bw // 8, *places(4)
+    for most, dim in ((1 << 59, 1), ((1 << 59) // 3, 3)):
+        for f in (ctx.lib.mpcx_norm_sums_key_bytes, ctx.lib.mpcx_norm_scale_key_bytes):
+            assert f(ctx.h, most, dim) >= most * (dim + 1) * tb and f(ctx.h, most + 1, dim) == 0
+            assert f(ctx.h, 1 << 60, 1) == 0
+        refused(ctx, lambda rows: ctx.lib.mpcx_norm_sums_eval(ctx.h, rows, dim, k0, k1, x, dim, None, 0, None, 0, s),
+                b"bad argument", [dict(rows=most + 1), dict(rows=1 << 60)])
