@@ -89,6 +89,8 @@ def _up(n):
 
 def prepare(case, seed):
     c, bw = case, case["bw"]
+    if own:
+        _context(bw)  # before the inputs: they are made on its stream
     g = torch.Generator(device="cuda").manual_seed(int(seed))
     s = {"op": c["op"], "bw": bw}
 
@@ -167,28 +169,32 @@ _ctx = {}
 
 
 def _context(bw):
-    """The program's context of this ring and the stream it works on."""
+    """The program's context of this ring.  The program works on a stream of its own: from
+    its first context on it is torch's current one, on which inputs are made, the
+    calls enqueue and outputs are used.  Where a caller has made another stream current
+    the calls wait for that one, and for their own work at their end."""
+    if "stream" not in _ctx:
+        stream = _ctx["stream"] = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        torch.cuda.set_stream(stream)
     if bw not in _ctx:
         if PKG not in sys.path:
             sys.path.insert(0, PKG)
         import mpcx
 
-        stream = torch.cuda.Stream()
-        ctx = mpcx.Ctx(bw=bw, scale=12)
-        ctx.set_stream(stream)
-        _ctx[bw] = (ctx, stream)
+        _ctx[bw] = mpcx.Ctx(bw=bw, scale=12)
+        _ctx[bw].set_stream(_ctx["stream"])
     return _ctx[bw]
 
 
 def _own_run(s):
-    ctx, stream = _context(s["bw"])
-    with torch.cuda.stream(stream):
-        if s["op"] == "q8":
-            return ctx.ring_gemm_q8(s["a"], s["q"], s["scale"], s["tokens"])
-        if s["op"] == "sums":
-            h, total = ctx.norm_sums_eval(*s["key"], s["h"], s["d"])
-            return (h, total) if s["d"] is not None else total
-        return ctx.norm_scale_eval(*s["key"], *s["share"], s["h"], s["v"], s["gain"])
+    ctx = _context(s["bw"])
+    if s["op"] == "q8":
+        return ctx.ring_gemm_q8(s["a"], s["q"], s["scale"], s["tokens"])
+    if s["op"] == "sums":
+        h, total = ctx.norm_sums_eval(*s["key"], s["h"], s["d"])
+        return (h, total) if s["d"] is not None else total
+    return ctx.norm_scale_eval(*s["key"], *s["share"], s["h"], s["v"], s["gain"])
 
 
 def run(state):
