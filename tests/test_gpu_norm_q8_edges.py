@@ -390,3 +390,39 @@ def test_key_bytes_at_their_end(ctx):
             assert f(ctx.h, 1 << 60, 1) == 0
         refused(ctx, lambda rows: ctx.lib.mpcx_norm_sums_eval(ctx.h, rows, dim, k0, k1, x, dim, None, 0, None, 0, s),
                 b"bad argument", [dict(rows=most + 1), dict(rows=1 << 60)])
+
+
+def test_parties_reconstruct_the_norm(ctx):
+    """Each party's messages from its own keys and shares, exchanged over a channel: both hold
+    the gates' outputs."""
+    import threading
+    rng = np.random.default_rng(10)
+    rows, dim = 7, 150
+    x, d, g = (dev(words(rng, s, ctx.bw)) for s in ((rows, dim), (rows, dim), (dim,)))
+    v = dev(words(rng, (rows,), ctx.bw))
+    ks = ctx.norm_sums_keygen(x, d)
+    kv = ctx.norm_scale_keygen(ks[0], ks[1], v, dim, g)
+    h, s = ctx.norm_sums_eval(ks[0], ks[1], x, d)
+    want = [host(s, ctx.bw), host(ctx.norm_scale_eval(kv[0], kv[1], ks[0], ks[1], h, v, g), ctx.bw).reshape(-1)]
+    peers, got, errors = mpcx.Peer.pair(), {}, []
+
+    def party(i):
+        try:
+            c = mpcx.Ctx(bw=ctx.bw, scale=12)
+            hi, s = c.norm_sums_message(i, ks[i], x, d)
+            y = c.norm_scale_message(i, kv[i], ks[i], hi, v, g)
+            got[i] = [c.party_reconstruct(peers[i], host(m, ctx.bw).reshape(-1)) for m in (s, y)]
+            c.close()
+        except Exception as e:  # a thread's failure is the test's
+            errors.append(e)
+
+    threads = [threading.Thread(target=party, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not errors and len(got) == 2, errors
+    for i in (0, 1):
+        assert all(np.array_equal(a, b) for a, b in zip(got[i], want))
+    for peer in peers:
+        peer.close()
