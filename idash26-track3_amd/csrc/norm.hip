@@ -45,8 +45,8 @@ __global__ __launch_bounds__(256) void k_norm_terms(NormSumsArgs<T> g) {
 // ---------------------------------------------------------------------------
 // W waves a row (W a power of two; a workgroup is 4 waves or W).  The bytes are all there is
 // to it: four words in (three without a residual) and one out (none) for one multiplication.
-// 6000 x 4096 in Z_2^32 90 us, 5.5 TB/s (a word a lane instead of 16 bytes: 114); one row of
-// 4096 3.4 (by one wave 17.6).  Long rows, where they are few: PARTS a row, of `len` words
+// 6000 x 4096 in Z_2^32 89 us, 5.5 TB/s (a word a lane instead of 16 bytes: 114); one row of
+// 4096 2.8 (by one wave 4.9).  Long rows, where they are few: PARTS a row, of `len` words
 // (whole turns of the waves), added up in s, which k_norm_terms has begun; sums modulo 2^bw
 // do not depend on their order.
 // ---------------------------------------------------------------------------
@@ -176,8 +176,8 @@ hipError_t sums_form(const Launch &L, const NormSumsArgs<T> &g) {
   };
   const size_t turns = (g.dim * sizeof(T) + 1023) / 1024;  // of a wave, to pass a row
   // Long rows in parts, a workgroup each, where the rows leave CUs idle (us, whole and in parts,
-  // Z_2^32): 1 row of 16384 4.8 and 4.9, of 32768 7.3 and 4.9, of 262144 55 and 5.3; 16 rows of 32768 9.2 and
-  // 6.1; 64 rows 10.8 and 10.6; 128 rows 13.9 and 16.2, of 65536 35 and 29; 256 rows 67 and 69.
+  // Z_2^32): 1 row of 16384 4.6 and 4.8, of 32768 7.3 and 4.8, of 262144 55 and 5.3; 16 rows of 32768 8.6 and
+  // 6.2; 64 rows 10.8 and 10.5; 128 rows 13.8 and 16.2, of 65536 35 and 30; 256 rows 66 and 69.
   const size_t rounds = (turns + 15) / 16, cus = size_t(L.num_cu);  // of 16 waves, to pass a row
   if (rounds >= 8 && g.rows <= cus * std::min<size_t>(rounds, 16) / 32) {
     const size_t most = std::min(rounds, (cus + g.rows - 1) / g.rows), len = (rounds + most - 1) / most * (16384 / sizeof(T));
@@ -189,8 +189,8 @@ hipError_t sums_form(const Launch &L, const NormSumsArgs<T> &g) {
                        uint32_t(parts), len);
     return hipGetLastError();
   }
-  // By 16, 4 and 1 waves (us, Z_2^32): 1 x 4096 2.8, 3.1, 4.9; 2000 x 4096 27, 27, 28; 8000 x
-  // 4096 117, 124, 131; 700 x 2048 7.5, 6.6, 6.7; 8000 x 1024 34, 27, 27; 8000 x 128 23, 9.4, 5.9.
+  // By 16, 4 and 1 waves (us, Z_2^32): 1 x 4096 2.8, 3.0, 4.9; 2000 x 4096 27, 27, 28; 8000 x
+  // 4096 120, 125, 132; 700 x 2048 7.6, 6.7, 6.6; 8000 x 1024 32, 28, 27; 8000 x 128 23, 9.2, 5.4.
   if (turns > 8) return waves(std::integral_constant<int, 16>{});
   if (turns > 2) return waves(std::integral_constant<int, 4>{});
   return waves(std::integral_constant<int, 1>{});

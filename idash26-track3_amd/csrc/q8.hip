@@ -97,20 +97,21 @@ __device__ __forceinline__ int q8_turn(int col) {
 // Few rows, R at most: a workgroup takes 16 columns, its waves the 128-k steps of K in
 // turn, each by itself: it asks for a step's weights, straight into its own part of LDS (in
 // lines of memory; to the lanes' registers, 16 rows of them, they would take four times the
-// cache's accesses), and words, one or, of few rows, two steps ahead (two of 8 rows in Z_2^64
-// leave room for half as many waves: 4096 x 11008 21.9 us, and 16.9; of one row in Z_2^32 9.6, and 10.3
-// by one).  It forms the words' digits, four words a lane at a time, and turns them by its
+// cache's accesses), and words, one or, of few rows, two steps ahead (4096 x 11008: two of 8
+// rows in Z_2^64 leave room for half as many waves, 30% slower; one of one row in Z_2^32 7%
+// slower).  It forms the words' digits, four words a lane at a time, and turns them by its
 // part of LDS into operands (formed in the lanes that need them, each word by as many
-// lanes as there are planes or parts: 4096 x 11008, one row 12.7 us, and 9.6; 8 rows 18.2, and 11.3).
+// lanes as there are planes or parts: 4096 x 11008, one row a third slower, 8 rows 60%).
 // The waves' sums are added up through LDS.
 // The MFMA's 16 rows are the words' by the planes' parts: of 8 words in Z_2^32, say, planes
 // 0 and 1, then 2 and 3, so that a step has 2 R planes / 16 MFMAs.
 // Places: a read of 16 bytes serves lanes 0-3, 12-15, 20-27 together, then 4-11, 16-19,
 // 28-31; groups of 16 bytes are turned so that those fall into different banks.
 // Bound by the weights' bytes and, below some 20 MB, by a launch's start and the waves'
-// first loads: in Z_2^32 1 x 4096 x 4096 3.7 us, 1 x 4096 x 11008 9.6 (4.7 TB/s), 1 x 8192 x 8192 13.3; with
-// more rows by the digits, which each workgroup forms, their way through LDS and the words' way to
-// every CU: 4096 x 4096, 8 rows 5.5, 16 rows 7.7.
+// first loads: in Z_2^32 1 x 4096 x 4096 3.4 us with the weights in the card's cache and 5.3 with
+// them in memory, 1 x 4096 x 11008 9.2 and 10.4, 1 x 8192 x 8192 13.0 and 14.2 (4.7 TB/s), 1 x 4096 x
+// 32000 21.6 and 23.8 (5.5 TB/s); with more rows by the digits, which each workgroup forms, their way
+// through LDS and the words' way to every CU: 4096 x 4096, 8 rows 5.3 and 7.0, 16 rows 7.5 and 8.8.
 // ---------------------------------------------------------------------------
 template <typename T, int R, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
@@ -282,10 +283,12 @@ __global__ __launch_bounds__(64 * WAVES) void k_q8_few(Q8Args<T> g) {
 // It forms the words' digits once, for the next step between the matrix instructions of
 // this one; the weights go straight into LDS (to the lanes' registers they would take four
 // times the cache's accesses: an operand's 16 rows are as many places for 16 lanes, where here
-// 8 lanes take a row's 128 bytes: 94 us, and 73).  1000 x 4096 x 4096 in Z_2^32: 65 to 72 us,
-// 1.9 to 2.1 POP/s of digits (a large int8 library product 2.1), by the card's clock: 62 with words and
-// weights of zeros.  The matrix cores are busy half of the waves' time; 32 steps take 1.8 us
-// each, the start and the output's way to memory 8.
+// 8 lanes take a row's 128 bytes: 29% slower).  1000 x 4096 x 4096 in Z_2^32: 61 to 72 us by
+// the card, 1.9 to 2.2 POP/s of digits (a large int8 library product 2.0 to 2.1).  32 steps take
+// 1.7 us each, the start and the output's way to memory 8.  The matrix cores are busy half of
+// that (the same instructions from registers take 34 to 41 us); the rest is one workgroup of two waves a
+// SIMD that waits at a barrier each step for loads, digits and reads of LDS.  Words or weights of
+// zeros take 54 us where uniform ones take 62: of the rest the card's power is the smaller part.
 // Places in LDS, both such that neither the writes' nor the reads' lanes meet in a bank
 // (a read of 16 bytes serves lanes 0-3, 12-15, 20-27 together, then 4-11, 16-19, 28-31):
 //   digits   plane, tile of 16 words, half of the step o: 64 lanes' 16 bytes, word li of
@@ -578,13 +581,22 @@ float weights_time(const Q8Args<T> &g) {
 // What a launch of k_q8_few takes (us): its start and the larger of the weights' way and its
 // rounds of one workgroup a CU times a wave's steps, each the digits of R rows and, with more
 // than half of the CUs at work, the words' way to them; where but one workgroup fits a CU each
-// round has a start.  Measured beside k_q8_many's by the rule below: Z_2^32 1 row 4096 x
-// 4096 4.0 and 7.8, 4096 x 32000 22.7 and 24.6; 4 rows 4.7 and 9.1, 22.8 and 25.6; 8 rows 4096 x 4096 5.9
-// and 9.4, 8192 x 8192 15.2 and 17.4, 20000 x 300 11.5 and 8.4, 20000 x 4096 16.8 and 20.3; 16 rows 4096 x
-// 4096 8.0 and 9.9, 8192 x 300 9.2 and 7.4, x 2500 11.0 and 12.6; 32 rows 1024 x 1024 4.7 and 7.0, 2048 x
-// 4096 7.5 and 7.8, 4096 x 4096 12.4 and 10.9, 1000 x 4099 9.0 and 7.6.  Z_2^64: 1 row 4096 x 4096 4.6 and
-// 8.0; 4 rows 8192 x 8192 14.7 and 18.5, 20000 x 300 10.9 and 8.5; 8 rows 4096 x 4096 8.0 and 10.2, 8192 x
-// 2500 10.9 and 11.6; 16 rows 1024 x 1024 4.8 and 7.1, 2048 x 2048 6.5 and 7.4, 4096 x 4096 12.5 and 11.2.
+// round has a start.  Fitted to weights in the card's cache, as the rule's other side is.  Both kernels,
+// few and many rows' (us, weights in the cache; then in memory):
+//   Z_2^32   1 row     4096 x 4096 3.4 and 7.6; 5.3, 8.8      4096 x 32000 22.4 and 23.9; 24.7, 28.3
+//            4 rows    4096 x 4096 4.1 and 8.9; 5.7, 10.0     4096 x 32000 23.0 and 25.3; 26.0, 29.8
+//            8 rows    4096 x 4096 5.3 and 9.2; 7.0, 10.0     8192 x 8192 14.5 and 17.3; 18.7, 18.8
+//                      20000 x 300 11.0 and 8.3; 20.7, 9.5    20000 x 4096 16.4 and 20.0; 24.6, 22.8
+//            16 rows   4096 x 4096 7.5 and 9.8; 8.9, 10.4     8192 x 300 8.8 and 7.2; 12.8, 8.0
+//                      8192 x 2500 10.6 and 12.3; 13.4, 12.8
+//            32 rows   1024 x 1024 4.4 and 6.8; 5.3, 7.6      2048 x 4096 7.3 and 7.7; 7.9, 8.5
+//                      4096 x 4096 12.1 and 10.8; 13.5, 11.7  1000 x 4099 8.5 and 7.5; 9.7, 8.8
+//   Z_2^64   1 row     4096 x 4096 4.3 and 7.9; 6.0, 9.1
+//            4 rows    8192 x 8192 14.2 and 18.2; 18.3, 20.2  20000 x 300 10.6 and 8.0; 21.5, 9.3
+//            8 rows    4096 x 4096 7.6 and 9.8; 9.0, 10.4     8192 x 2500 10.6 and 11.3; 13.4, 12.1
+//            16 rows   1024 x 1024 4.4 and 6.9; 5.4, 7.8      2048 x 2048 6.2 and 7.2; 7.6, 8.1
+//                      4096 x 4096 12.2 and 10.9; 13.6, 12.0
+// With them in memory a long K of 6 to 16 rows is up to 11% faster by the other kernel.
 template <typename T>
 float few_time(const Launch &L, const Q8Args<T> &g) {
   const float digits = float(sizeof(T)) * (g.M <= 2 ? 2.f : g.M <= 4 ? 4.f : g.M <= 8 ? 8.f : g.M <= 16 ? 16.f : 32.f);
@@ -611,8 +623,9 @@ hipError_t launch_few(const Launch &L, const Q8Args<T> &g) {
   }
   if (g.M > 4) return g.M <= 8 ? few(eight, eight) : few(sixteen, eight);
   // Sixteen waves where they have a step each and a workgroup has a CU (us, Z_2^32, by eight
-  // and by sixteen): one row of 4096 x 4096 5.5 and 5.1, of 8192 x 2048 5.5 and 5.2; four of 4096 x
-  // 4096 5.9 and 5.5, of 4096 x 11008 9.8 and 12.3, of 1000 x 4099 3.1 and 4.0.
+  // and by sixteen; with the weights in memory): one row of 4096 x 4096 3.6 and 3.4; 5.7, 5.3, of 8192 x
+  // 2048 4.5 and 4.3; 6.2, 6.2; four of 4096 x 4096 4.1 and 4.2; 6.1, 5.7, of 8192 x 4096 8.2 and 7.4; 9.0,
+  // 8.4, of 4096 x 11008 9.3 and 11.3; 11.4, 13.3, of 1000 x 4099 2.7 and 3.5; 3.7, 4.6.
   if (steps > 8 && g.N <= 16 * L.num_cu) return g.M <= 2 ? few(two, sixteen) : few(four, sixteen);
   return g.M <= 2 ? few(two, eight) : few(four, eight);
 }
@@ -628,9 +641,9 @@ hipError_t launch_part(const Launch &L, const Q8Args<T> &g) {
   // start together), and, where K is split, the output's clearing and the sums' way through
   // memory.  Measured (us, one MI355X, all CUs at work): a large tile's step 0.6 + 0.3 nt, its
   // start 6; a small one's 0.27 + 0.19 nt and 4; splitting 2.5, 0.1 a part and 0.25 a MB.  4096 x 4096 in
-  // Z_2^32 by large and by small tiles of width 1, 2, 3, 4: 1000 rows 124, 81, 93, 63 and 115, 81,
-  // 89, 72; 640 89, 75, 48, 54 and 73, 59, 60, 67; 512 64, 41, 45, 53 and 59, 42, 58, 37; 256 32, 37, 44,
-  // 52 and 31, 24, 29, 33; 64 rows by four parts of K 16, 17, 19, 21 and 14, 13, 14, 15.
+  // Z_2^32 by small tiles of width 1, 2, 3, 4 and by large ones of 3, 4: 1000 rows 115, 81, 87, 75 and
+  // 91, 63; 640 75, 58, 59, 66 and 48, 55; 512 59, 42, 57, 38 and 45, 54; 256 31, 25, 29, 33 and 44, 53; 64
+  // rows by four parts of K 13, 13, 14, 14 and 19, 21.
   int nt = 1, splits = exact;
   bool large = false;
   float best = 0;
