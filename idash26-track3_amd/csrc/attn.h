@@ -49,6 +49,10 @@ template <typename T>
 hipError_t launch_gemm_q8(const Launch &L, const Q8Args<T> &g);
 
 // ---------------- the norm's gates ----------------
+// The keygens' PRF fields, beside the enum Field's: share 0 of the rows' (the factors') mask, the
+// output's mask (+1), share 0 of the term (+2).  With fields of their own a norm's two gates
+// may have one gate id.
+constexpr uint32_t F_NSUMS = 0x68, F_NSCALE = 0x6C;
 // What a launch computes: both parties' messages added up, one party's, or the
 // dealer's product term.
 enum class NormForm { BOTH, P0, P1, DEAL };

@@ -70,8 +70,6 @@ enum Field : uint32_t {
   F_SPLIT = 0x40,  // +k: share 0 of plane k
   F_LUTV = 0x58,
   F_RIN = 0x60,    // input masks of reveal gates
-  F_NSUMS = 0x68,  // the norm's gates: +0 share 0 of the rows' mask, +1 output mask, +2 share 0 of the term
-  F_NSCALE = 0x6C, // +0 share 0 of the factors' mask, +1, +2 as above: a norm's two gates may have one id
   F_PARTY = 0x70   // party p's PRF key: dealer PRF block (p, F_PARTY, gate 0xFFFFFFFF)
 };
 
