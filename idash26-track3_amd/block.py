@@ -71,7 +71,7 @@ class Norm:
     BANDS = 3
 
     def __init__(self, ctx, dim, gain=None):
-        s, bits = ctx.s, ctx.bw - 1
+        s, bits, dim = ctx.s, ctx.bw - 1, int(dim)
         if dim < 1:
             raise ValueError(f"Norm: rows of {dim} words")
         wide = bits == 63

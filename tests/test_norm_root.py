@@ -165,3 +165,8 @@ def test_gates(norm):
         Count.calls = 0
         norm(bw, 4096).root(Count(bw, 12), np.array([1 << 24, 0]))
         assert Count.calls <= most
+
+
+def test_widths_of_numpy(norm):
+    """A width as an array's shape or a numpy number holds it."""
+    assert np.array_equal(norm(64, np.int64(1000)).p.values, norm(64, 1000).p.values)
